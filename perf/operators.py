@@ -288,12 +288,16 @@ def _loss_and_gradient(scores, ids, values, lse, weight, temperature):
         grad = mass * q
     else:
         listed_ = torch.zeros_like(e).scatter_add_(1, at, there.to(e.dtype)) > 0
-        rest_e = e.masked_fill(listed_, 0).sum(dim=1, keepdim=True)
-        rest = torch.where(rest_e > 0, (1 - mass).clamp(min=0), torch.zeros_like(mass))
-        some = rest > 0
-        loss = loss + torch.where(some, rest * (rest.log() - rest_e.log() + total.log()), torch.zeros_like(rest))
-        share = torch.where(some, rest * total / rest_e, torch.zeros_like(rest))
-        grad = q * (mass + rest - torch.where(listed_, torch.zeros_like(e), share))
+        rest_x = x.masked_fill(listed_, -math.inf)
+        rest_top = rest_x.amax(dim=1, keepdim=True)
+        some = (rest_top > -math.inf) & (mass < 1)
+        rest_top = torch.where(some, rest_top, top)
+        rest_e = (rest_x - rest_top).exp()
+        rest_total = torch.where(some, rest_e.sum(dim=1, keepdim=True), torch.ones_like(mass))
+        rest = torch.where(some, 1 - mass, torch.zeros_like(mass))
+        log_rest_q = rest_top + rest_total.log() - top - total.log()
+        loss = loss + torch.where(some, rest * (rest.log() - log_rest_q), torch.zeros_like(rest))
+        grad = q * (mass + rest) - rest_e * (rest / rest_total)
     grad = grad.scatter_add(1, at, torch.where(there, -p, torch.zeros_like(p)))
     grad = grad * (weight[:, None].to(x.dtype) / temperature)
     return (torch.where(full, loss, torch.zeros_like(loss))[:, 0],
