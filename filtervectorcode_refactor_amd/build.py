@@ -5,6 +5,7 @@ travels with the repository snapshot to the GPU box:
   * ung_host.cpp    -> g++ (host C++: synthetic inputs, groups, LNG, reorder)
   * ung_runtime.hip -> hipcc --offload-arch=gfx950 (context, planning, launches, C ABI;
                        includes ung_kernels.hip, the device code: one translation unit)
+  * ung_fp8.hip, ung_scores.hip -> hipcc (score operators: kernels and C ABI)
 Packed-FP32 instruction selection is disabled for all device code.
 """
 from __future__ import annotations
@@ -12,11 +13,13 @@ from __future__ import annotations
 import os
 import subprocess
 import sys
+from concurrent.futures import ThreadPoolExecutor
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 ROOT = os.path.dirname(HERE)
 CSRC = os.path.join(HERE, "csrc")
 INCLUDE = os.path.join(ROOT, "include")
+HIP_UNITS = ("ung_runtime", "ung_fp8", "ung_scores")  # translation units with device code
 LIB_NAME = "libung_hip.so"
 LIB_PATH = os.path.join(HERE, LIB_NAME)
 ARCH = os.environ.get("UNG_HIP_ARCH", "gfx950")
@@ -52,11 +55,13 @@ def build(verbose: bool = True) -> str:
     host_obj = os.path.join(obj_dir, "ung_host.o")
     _run([CXX, *HOST_FLAGS, "-I", INCLUDE, "-I", CSRC, "-c",
           os.path.join(CSRC, "ung_host.cpp"), "-o", host_obj], verbose)
-    dev_obj = os.path.join(obj_dir, "ung_runtime.o")
-    _run([HIPCC, *HIP_FLAGS, "-I", INCLUDE, "-I", CSRC, "-c",
-          os.path.join(CSRC, "ung_runtime.hip"), "-o", dev_obj], verbose)
+    dev_objs = [os.path.join(obj_dir, f"{name}.o") for name in HIP_UNITS]
+    steps = [[HIPCC, *HIP_FLAGS, "-I", INCLUDE, "-I", CSRC, "-c", os.path.join(CSRC, f"{name}.hip"), "-o", obj]
+             for name, obj in zip(HIP_UNITS, dev_objs)]
+    with ThreadPoolExecutor(len(steps)) as pool:
+        list(pool.map(lambda cmd: _run(cmd, verbose), steps))
     tmp = LIB_PATH + ".tmp"
-    _run([HIPCC, f"--offload-arch={ARCH}", "-shared", "-fPIC", dev_obj, host_obj,
+    _run([HIPCC, f"--offload-arch={ARCH}", "-shared", "-fPIC", *dev_objs, host_obj,
           "-o", tmp, "-pthread"], verbose)
     os.replace(tmp, LIB_PATH)
     return LIB_PATH
