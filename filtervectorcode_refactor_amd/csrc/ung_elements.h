@@ -6,6 +6,7 @@
 #include <hip/hip_runtime.h>
 
 #include <cstdint>
+#include <type_traits>
 
 #include "ung_hip.h"
 #include "ung_internal.h"
@@ -28,17 +29,62 @@ __device__ inline T from_float(float v)
     return (T)v;
 }
 
-// A 16-byte vector of elements.
+// A 16-byte vector of elements, as the four registers that hold it.
 template <class T>
 struct alignas(16) Vec {
     static constexpr int N = 16 / (int)sizeof(T);
-    T v[N];
+    static constexpr uint32_t NEG_INF_BITS =
+        sizeof(T) == 4 ? 0xFF800000u : std::is_same_v<T, bf16_t> ? 0xFF80FF80u : 0xFC00FC00u;
+    uint32_t w[4];
+
+    __device__ float get(int e) const
+    {
+        if constexpr (sizeof(T) == 4)
+            return __builtin_bit_cast(float, w[e]);
+        else if constexpr (std::is_same_v<T, bf16_t>)
+            return __builtin_bit_cast(float, e & 1 ? w[e / 2] & 0xFFFF0000u : w[e / 2] << 16);
+        else
+            return (float)__builtin_bit_cast(fp16_t, (uint16_t)(e & 1 ? w[e / 2] >> 16 : w[e / 2]));
+    }
+    __device__ T element(int e) const
+    {
+        if constexpr (sizeof(T) == 4)
+            return __builtin_bit_cast(T, w[e]);
+        else
+            return __builtin_bit_cast(T, (uint16_t)(e & 1 ? w[e / 2] >> 16 : w[e / 2]));
+    }
+    __device__ void set(int e, T x)
+    {
+        if constexpr (sizeof(T) == 4)
+            w[e] = __builtin_bit_cast(uint32_t, x);
+        else if (e & 1)
+            w[e / 2] = (w[e / 2] & 0xFFFFu) | (uint32_t)__builtin_bit_cast(uint16_t, x) << 16;
+        else
+            w[e / 2] = (w[e / 2] & 0xFFFF0000u) | __builtin_bit_cast(uint16_t, x);
+    }
+    __device__ void fill_neg_inf()
+    {
+        w[0] = w[1] = w[2] = w[3] = NEG_INF_BITS;
+    }
+    // Elements e and e + 1 (e even) from 32 bits.
+    __device__ void put2(int e, float a, float b)
+    {
+        if constexpr (sizeof(T) == 4) {
+            w[e] = __builtin_bit_cast(uint32_t, a);
+            w[e + 1] = __builtin_bit_cast(uint32_t, b);
+        } else {
+            using Two = T __attribute__((ext_vector_type(2)));
+            const Two two = {from_float<T>(a), from_float<T>(b)};
+            w[e / 2] = __builtin_bit_cast(uint32_t, two);
+        }
+    }
 };
 
-// exp(x) for x <= 0 (weights relative to a maximum): 2^(x log2 e) on the hardware's exp2.
-// Its relative error is that of the rounded product, |x| 2^-24, so the terms that carry a
-// sum (x near 0) are as exact as the library's.
-__device__ inline float exp_neg(float x) { return __builtin_amdgcn_exp2f(x * 1.44269504088896340736f); }
+// exp((s - top) / T) by the hardware's 2^x, c = log2(e) / T.  The difference is taken first:
+// it is exact where s is near top, so the terms that carry a sum are as exact as the library's
+// (the others are off by |exponent| 2^-24 of themselves), and rows of any size are served,
+// rows masked by the type's lowest value among them.
+__device__ inline float weight_of(float s, float top, float c) { return __builtin_amdgcn_exp2f((s - top) * c); }
 
 template <class F>
 __device__ inline float wave_reduce(float v, F f)

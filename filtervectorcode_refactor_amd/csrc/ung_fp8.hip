@@ -64,7 +64,7 @@ __device__ inline void load8(const T *row, uint64_t c, uint64_t cols, float *x)
             const Vec<T> v = *reinterpret_cast<const Vec<T> *>(row + c + h * Vec<T>::N);
 #pragma unroll
             for (int i = 0; i < Vec<T>::N; ++i)
-                x[h * Vec<T>::N + i] = to_float(v.v[i]);
+                x[h * Vec<T>::N + i] = v.get(i);
         }
         return;
     }

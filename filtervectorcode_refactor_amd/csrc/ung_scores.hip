@@ -20,277 +20,369 @@ namespace {
 
 constexpr int MAX_K = UNG_HIP_TOP_SCORES_MAX; // 128
 constexpr float NEG_INF = -__builtin_inff();
+constexpr double LOG2E = 1.4426950408889634;
+
+struct Temperature {
+    float inv, c; // 1 / T, log2(e) / T
+};
+
+__device__ inline float max_of(float a, float b) { return fmaxf(a, b); }
 
 template <class T>
 struct RowRef {
+    static constexpr uint32_t N = Vec<T>::N;
     const T *row;
-    uint32_t shift; // elements between the 16-byte boundary and the row's first one
+    uint32_t shift;        // elements between the 16-byte boundary and the row's first one
     uint32_t len;
+    uint32_t whole, wholes; // the first vector wholly inside the row, and how many there are
+    uint32_t end;          // vectors in all
     __device__ RowRef(const T *r, uint32_t n)
-        : row(r), shift((uint32_t)(((uintptr_t)r & 15) / sizeof(T))), len(n)
+        : row(r), shift((uint32_t)(((uintptr_t)r & 15) / sizeof(T))), len(n), whole(shift ? 1 : 0),
+          wholes((shift + n) / N > whole ? (shift + n) / N - whole : 0), end((shift + n + N - 1) / N)
     {
     }
+    __device__ bool inside(uint32_t i) const { return i - whole < wholes; }
     // Vector i of the row; elements outside the row are -inf.
     __device__ Vec<T> load(uint32_t i) const
     {
-        constexpr int N = Vec<T>::N;
-        const int64_t j = (int64_t)i * N - shift;
-        if (j >= 0 && j + N <= (int64_t)len)
-            return *reinterpret_cast<const Vec<T> *>(row + j);
+        if (inside(i))
+            return reinterpret_cast<const Vec<T> *>(row - shift)[i];
         Vec<T> v;
+        v.fill_neg_inf();
 #pragma unroll
-        for (int e = 0; e < N; ++e)
-            v.v[e] = j + e >= 0 && j + e < (int64_t)len ? row[j + e] : (T)NEG_INF;
+        for (uint32_t e = 0; e < N; ++e) {
+            const uint32_t j = i * N + e - shift; // wraps below the row
+            if (j < len)
+                v.set(e, row[j]);
+        }
         return v;
+    }
+    // Elements of vector i to a row of the same length.
+    __device__ void store_elements(T *to, uint32_t i, const Vec<T> &v) const
+    {
+#pragma unroll
+        for (uint32_t e = 0; e < N; ++e) {
+            const uint32_t j = i * N + e - shift;
+            if (j < len)
+                to[j] = v.element(e);
+        }
     }
 };
 
-// Writes vector i of a row that starts `shift` elements after a 16-byte boundary of the
-// source; `same`: the destination row lies the same way.
-template <class T>
-__device__ inline void store_vec(T *row, uint32_t shift, uint32_t len, uint32_t i, const Vec<T> &v, bool same)
-{
-    constexpr int N = Vec<T>::N;
-    const int64_t j = (int64_t)i * N - shift;
-    if (same && j >= 0 && j + N <= (int64_t)len) {
-        *reinterpret_cast<Vec<T> *>(row + j) = v;
-        return;
-    }
+// A stretch of a row, NT * NV vectors from `begin` on, in a block's registers: a thread holds
+// the vectors begin + thread + i NT that lie wholly inside the row (-inf elsewhere), and its
+// first two threads the vectors across the row's ends, if the stretch has them.
+template <class T, int NT, int NV>
+struct Stretch {
+    Vec<T> v[NV], edge;
+    uint32_t first, edge_at;
+    bool has_edge;
+    __device__ Stretch(const RowRef<T> &ref, uint32_t begin) : first(begin + threadIdx.x)
+    {
+        const Vec<T> *from = reinterpret_cast<const Vec<T> *>(ref.row - ref.shift);
 #pragma unroll
-    for (int e = 0; e < N; ++e)
-        if (j + e >= 0 && j + e < (int64_t)len)
-            row[j + e] = v.v[e];
-}
-
-template <class T>
-__device__ inline uint32_t vectors_of(uint32_t shift, uint32_t len)
-{
-    return (uint32_t)(((uint64_t)shift + len + Vec<T>::N - 1) / Vec<T>::N);
-}
+        for (int i = 0; i < NV; ++i) {
+            v[i].fill_neg_inf();
+            if (ref.inside(first + i * NT))
+                v[i] = from[first + i * NT];
+        }
+        edge_at = threadIdx.x ? ref.end - 1 : 0;
+        has_edge = threadIdx.x < 2 && edge_at - begin < NT * NV && edge_at < ref.end && !ref.inside(edge_at) &&
+                   (threadIdx.x == 0 || edge_at > 0 || ref.end == 0);
+        if (has_edge)
+            edge = ref.load(edge_at);
+    }
+    // f(vector, its place in the row) for every vector of the thread
+    template <class F>
+    __device__ void each(F f)
+    {
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            // keeps the compiler from holding the 32-bit values from pass to pass: 16-bit rows
+            // would take twice the registers
+            if constexpr (sizeof(T) == 2)
+                asm volatile("" : "+v"(v[i].w[0]), "+v"(v[i].w[1]), "+v"(v[i].w[2]), "+v"(v[i].w[3]));
+            f(v[i], first + i * NT);
+        }
+        if (has_edge)
+            f(edge, edge_at);
+    }
+};
 
 // ---- the first k of a row ------------------------------------------------------------
 
-// (score, id) as one whole number that orders like it: larger scores first, of equal ones the
-// lower id; NaN above every score, -0 as 0; 0 = no candidate (-inf).
-__device__ inline uint64_t order_of(float x, uint32_t id)
+// A score as a whole number that orders like it: NaN above every score, -0 as 0, and 0 for no
+// candidate (-inf).  With the id in the lower half, of equal scores the lower id is the larger
+// number.
+__device__ inline uint32_t key_of(float x)
 {
     if (x == NEG_INF)
         return 0;
     const uint32_t b = __float_as_uint(x + 0.0f);
-    uint32_t k = b & 0x80000000u ? ~b : b | 0x80000000u;
-    if (x != x)
-        k = 0xFFFFFFFFu;
-    return (uint64_t)k << 32 | (uint32_t)~id;
+    return x != x ? 0xFFFFFFFFu : b & 0x80000000u ? ~b : b | 0x80000000u;
 }
-
-__device__ inline float score_of(uint64_t o)
+__device__ inline uint64_t order_of(float x, uint32_t id)
 {
-    const uint32_t k = (uint32_t)(o >> 32);
-    return k == 0xFFFFFFFFu ? __builtin_nanf("") : __uint_as_float(k & 0x80000000u ? k & 0x7FFFFFFFu : ~k);
+    const uint32_t k = key_of(x);
+    return k ? (uint64_t)k << 32 | (uint32_t)~id : 0;
+}
+__device__ inline float score_of(uint32_t key)
+{
+    return key == 0xFFFFFFFFu ? __builtin_nanf("") : __uint_as_float(key & 0x80000000u ? key & 0x7FFFFFFFu : ~key);
 }
 
 constexpr int TOP_NT = 256;   // threads of a block
 constexpr int TOP_CAP = 1024; // candidates a block ranks
 
 struct TopShared {
-    uint64_t cand[TOP_CAP];
-    uint64_t most[TOP_NT];
-    float red[TOP_NT / 64];
+    alignas(16) uint64_t cand[TOP_CAP];
+    uint32_t most[TOP_NT];
+    float red[2][TOP_NT / 64];
     uint32_t wave_count[TOP_NT / 64];
     uint32_t count;
-    uint64_t limit;
+    uint32_t limit;
 };
 
-// The k largest of the orders that a block holds (each(f) calls f with those of a thread; 0 =
-// none) to sh.cand in descending order; returns how many there are.  The k-th largest of the threads'
-// maxima is no larger than the k-th largest of all, and few orders lie between the two: those
-// at or above it are collected and ranked by counting.  Where they do not fit (many equal
-// scores, few threads with candidates), the k-th largest is first found bit by bit.
+// The largest key with at least k of the threads' maxima at or above it, found bit by bit by
+// one wave that holds all of them (a count is a ballot); the lowest LOW bits are left 0, which
+// keys of 16-bit scores do not need told apart.  No larger than the k-th largest key of all,
+// and few keys lie between the two.  0: fewer than k threads have a candidate.
+template <int LOW>
+__device__ inline uint32_t limit_of(const uint32_t *most, uint32_t k)
+{
+    uint32_t m[TOP_NT / 64], limit = 0;
+#pragma unroll
+    for (int i = 0; i < TOP_NT / 64; ++i)
+        m[i] = most[i * 64 + (threadIdx.x & 63)];
+#pragma unroll 4
+    for (int bit = 31; bit >= LOW; --bit) {
+        const uint32_t trial = limit | 1u << bit;
+        uint32_t n = 0;
+#pragma unroll
+        for (int i = 0; i < TOP_NT / 64; ++i)
+            n += __popcll(__ballot(m[i] >= trial));
+        limit = n >= k ? trial : limit;
+    }
+    return limit;
+}
+
+// The k-th largest of the orders that a block holds (each(f) calls f with those of a thread; 0
+// = none), bit by bit over the whole block: for rows of many equal scores, where the
+// candidates above the threads' limit do not fit.  There are at least k.
 template <class Each>
-__device__ inline uint32_t select_top(TopShared &sh, uint32_t k, uint64_t thread_most, Each each)
+__device__ inline uint64_t kth_order(TopShared &sh, uint32_t k, Each each)
+{
+    uint64_t limit = 0;
+    for (int bit = 63; bit >= 0; --bit) {
+        const uint64_t trial = limit | 1ull << bit;
+        uint32_t mine = 0;
+        each([&](uint64_t o) { mine += o >= trial; });
+#pragma unroll
+        for (int o = 32; o > 0; o >>= 1)
+            mine += __shfl_xor((int)mine, o);
+        __syncthreads();
+        if ((threadIdx.x & 63) == 0)
+            sh.wave_count[threadIdx.x >> 6] = mine;
+        __syncthreads();
+        uint32_t all = 0;
+#pragma unroll
+        for (int w = 0; w < TOP_NT / 64; ++w)
+            all += sh.wave_count[w];
+        if (all >= k)
+            limit = trial;
+    }
+    return limit;
+}
+
+__device__ inline void add_candidate(TopShared &sh, uint64_t order)
+{
+    const uint32_t at = atomicAdd(&sh.count, 1u);
+    if (at < TOP_CAP)
+        sh.cand[at] = order;
+}
+
+// Results of a row (or of a part of one) whose first k orders are among sh.cand[0..count):
+// each candidate's place is the number of candidates above it.  Where the candidates did not
+// fit, they are collected anew from the k-th order on.
+template <class Each>
+__device__ inline void finish_top(TopShared &sh, uint32_t k, Each each, uint64_t row, bool last, float *values,
+                                  int32_t *ids, float *lse, uint64_t *part, float2 *part_sum, float top, float sum,
+                                  Temperature t)
 {
     const uint32_t tid = threadIdx.x;
-    sh.most[tid] = thread_most;
-    if (tid == 0) {
-        sh.count = 0;
-        sh.limit = 1;
-    }
-    __syncthreads();
-    uint32_t rank = 0;
-    for (uint32_t t = 0; t < TOP_NT; ++t)
-        rank += sh.most[t] > thread_most || (sh.most[t] == thread_most && t < tid);
-    if (rank == k - 1 && thread_most)
-        sh.limit = thread_most;
-    __syncthreads();
-    uint64_t limit = sh.limit;
-    auto collect = [&]() {
-        each([&](uint64_t o) {
-            if (o >= limit) {
-                const uint32_t at = atomicAdd(&sh.count, 1u);
-                if (at < TOP_CAP)
-                    sh.cand[at] = o;
-            }
-        });
-        __syncthreads();
-    };
-    collect();
     uint32_t found = sh.count;
     if (found > TOP_CAP) {
-        // the largest limit with at least k orders at or above it; there are over k of them
-        limit = 0;
-        for (int bit = 63; bit >= 0; --bit) {
-            const uint64_t trial = limit | 1ull << bit;
-            uint32_t mine = 0;
-            each([&](uint64_t o) { mine += o >= trial; });
-#pragma unroll
-            for (int o = 32; o > 0; o >>= 1)
-                mine += __shfl_xor((int)mine, o);
-            __syncthreads();
-            if ((tid & 63) == 0)
-                sh.wave_count[tid >> 6] = mine;
-            __syncthreads();
-            uint32_t all = 0;
-#pragma unroll
-            for (int w = 0; w < TOP_NT / 64; ++w)
-                all += sh.wave_count[w];
-            if (all >= k)
-                limit = trial;
-        }
+        const uint64_t limit = kth_order(sh, k, each);
         if (tid == 0)
             sh.count = 0;
         __syncthreads();
-        collect(); // orders are distinct: k of them
-        found = sh.count;
+        each([&](uint64_t o) {
+            if (o >= limit)
+                add_candidate(sh, o);
+        });
+        __syncthreads();
+        found = sh.count; // k: orders are distinct
     }
-    uint64_t mine[TOP_CAP / TOP_NT];
-    uint32_t place[TOP_CAP / TOP_NT];
-#pragma unroll
-    for (int p = 0; p < TOP_CAP / TOP_NT; ++p) {
-        const uint32_t i = p * TOP_NT + tid;
-        place[p] = k;
-        if (i < found) {
-            mine[p] = sh.cand[i];
-            uint32_t at = 0;
-            for (uint32_t t = 0; t < found; ++t)
-                at += sh.cand[t] > mine[p];
-            place[p] = at;
-        }
+    auto put = [&](uint32_t place, uint64_t o) {
+        if (last) {
+            values[row * k + place] = o ? score_of((uint32_t)(o >> 32)) : NEG_INF;
+            ids[row * k + place] = o ? (int32_t)~(uint32_t)o : -1;
+        } else
+            part[row * k + place] = o;
+    };
+    for (uint32_t i = tid; i < found; i += TOP_NT) {
+        const uint64_t mine = sh.cand[i];
+        uint32_t place = 0;
+#pragma unroll 8
+        for (uint32_t o = 0; o < found; ++o)
+            place += sh.cand[o] > mine;
+        if (place < k)
+            put(place, mine);
     }
-    __syncthreads();
-#pragma unroll
-    for (int p = 0; p < TOP_CAP / TOP_NT; ++p)
-        if (place[p] < k)
-            sh.cand[place[p]] = mine[p];
-    __syncthreads();
-    return found < k ? found : k;
-}
-
-// What a block found: final rows, or partial ones (orders and (maximum, sum) pairs).
-__device__ inline void put_top(const TopShared &sh, uint32_t found, uint32_t k, uint64_t row, bool final_,
-                               float *values, int32_t *ids, float *lse, uint64_t *part, float2 *part_sum, float top,
-                               float sum)
-{
-    const uint32_t tid = threadIdx.x;
-    if (final_) {
-        if (tid < k) {
-            values[row * k + tid] = tid < found ? score_of(sh.cand[tid]) : NEG_INF;
-            ids[row * k + tid] = tid < found ? (int32_t)~(uint32_t)sh.cand[tid] : -1;
-        }
-        if (tid == 0 && lse)
-            lse[row] = fabsf(top) == __builtin_inff() ? top : top + logf(sum);
-    } else {
-        if (tid < k)
-            part[row * k + tid] = tid < found ? sh.cand[tid] : 0;
-        if (tid == 0)
+    if (tid >= found && tid < k)
+        put(tid, 0);
+    if (tid == 0) {
+        if (!last)
             part_sum[row] = make_float2(top, sum);
+        else if (lse)
+            lse[row] = fabsf(top) == __builtin_inff() ? top : top * t.inv + logf(sum);
     }
 }
 
 // The first k of one piece of a row (TOP_NT * NV vectors; the whole row if `pieces` is 1), its
-// values held in registers: one read of the scores, bound by memory.
+// values held in registers: one read of the scores, bound by memory.  While one wave finds
+// the limit from the threads' maxima, the others sum the weights exp((s - maximum) / T).
 template <class T, int NV>
-__global__ __launch_bounds__(TOP_NT) void ung_top_scores_kernel(const T *scores, uint32_t len, uint64_t stride,
-                                                                uint32_t pieces, uint32_t k, float inv_t,
-                                                                float *values, int32_t *ids, float *lse,
-                                                                uint64_t *part, float2 *part_sum)
+__global__ __launch_bounds__(TOP_NT, 4) void ung_top_scores_kernel(const T *scores, uint32_t len, uint64_t stride,
+                                                                   uint32_t pieces, uint32_t k, Temperature t,
+                                                                   float *values, int32_t *ids, float *lse,
+                                                                   uint64_t *part, float2 *part_sum)
 {
     constexpr int N = Vec<T>::N;
+    constexpr int LOW = std::is_same_v<T, bf16_t> ? 16 : std::is_same_v<T, fp16_t> ? 13 : 0;
     __shared__ TopShared sh;
     const uint64_t r = blockIdx.x / pieces;
-    const uint32_t piece = (uint32_t)(blockIdx.x - r * pieces);
+    const uint32_t piece = (uint32_t)(blockIdx.x - r * pieces), tid = threadIdx.x;
     const RowRef<T> ref(scores + r * stride, len);
-    const uint32_t first = piece * (TOP_NT * NV) + threadIdx.x, end = vectors_of<T>(ref.shift, len);
-    Vec<T> v[NV];
+    Stretch<T, TOP_NT, NV> x(ref, piece * (TOP_NT * NV));
+    float most = NEG_INF, most_of[NV + 1];
+    int n = 0;
+    x.each([&](const Vec<T> &v, uint32_t) {
+        float m = v.get(0);
 #pragma unroll
-    for (int i = 0; i < NV; ++i)
-        if (first + i * TOP_NT < end)
-            v[i] = ref.load(first + i * TOP_NT);
-        else
-#pragma unroll
-            for (int e = 0; e < N; ++e)
-                v[i].v[e] = (T)NEG_INF;
-    float most = NEG_INF;
-#pragma unroll
-    for (int i = 0; i < NV; ++i)
-#pragma unroll
-        for (int e = 0; e < N; ++e)
-            most = max_nan(most, to_float(v[i].v[e]));
-    const float top = block_reduce<TOP_NT>(most, sh.red, max_nan);
+        for (int e = 1; e < N; ++e)
+            m = fmaxf(m, v.get(e)); // a NaN shows in the sum
+        most_of[n++] = m;
+        most = fmaxf(most, m);
+    });
+    sh.most[tid] = key_of(most);
+    if (tid == 0)
+        sh.count = 0;
+    const float top = block_reduce<TOP_NT>(most, sh.red[0], max_of);
+    if (tid < 64) {
+        const uint32_t limit = limit_of<LOW>(sh.most, k);
+        if (tid == 0)
+            sh.limit = limit;
+    }
     const float at = top == NEG_INF ? 0.0f : top;
     float sum = 0.0f;
-    uint64_t thread_most = 0;
+    x.each([&](const Vec<T> &v, uint32_t) {
 #pragma unroll
-    for (int i = 0; i < NV; ++i)
-#pragma unroll
-        for (int e = 0; e < N; ++e) {
-            const float x = to_float(v[i].v[e]);
-            sum += exp_neg((x - at) * inv_t);
-            const uint64_t o = order_of(x, (first + i * TOP_NT) * N + e - ref.shift);
-            thread_most = o > thread_most ? o : thread_most;
-        }
-    __syncthreads();
-    sum = block_reduce<TOP_NT>(sum, sh.red, add);
-    auto each = [&](auto f) {
+        for (int e = 0; e < N; ++e)
+            sum += weight_of(v.get(e), at, t.c);
+    });
+    sum = block_reduce<TOP_NT>(sum, sh.red[1], add);
+    // the rest looks at few vectors, and reads those again
+    const T *row = ref.row;
+    const uint32_t shift = ref.shift, first = x.first, edge_at = x.edge_at, slots = NV + (x.has_edge ? 1 : 0);
+    auto scan = [=](uint32_t i, auto f) {
+        const uint32_t from = (i < NV ? first + i * TOP_NT : edge_at) * N - shift;
+#pragma unroll 1
+        for (uint32_t e = 0; e < N; ++e)
+            if (from + e < len)
+                f(to_float(row[from + e]), from + e);
+    };
+    auto each = [=](auto f) {
+        for (uint32_t i = 0; i < slots; ++i)
+            if (i >= NV || ref.inside(first + i * TOP_NT))
+                scan(i, [&](float x, uint32_t id) { f(order_of(x, id)); });
+    };
+    if (sum == sum) {
+        // scores at or above the limit; -inf is below every float
+        const float least = sh.limit ? score_of(sh.limit) : -3.402823466e38f;
+        uint32_t hit = 0;
 #pragma unroll
         for (int i = 0; i < NV; ++i)
-#pragma unroll
-            for (int e = 0; e < N; ++e)
-                f(order_of(to_float(v[i].v[e]), (first + i * TOP_NT) * N + e - ref.shift));
-    };
-    const uint32_t found = select_top(sh, k, thread_most, each);
-    put_top(sh, found, k, blockIdx.x, pieces == 1, values, ids, lse, part, part_sum, top * inv_t, sum);
+            hit |= most_of[i] >= least ? 1u << i : 0u;
+        if (x.has_edge && most_of[NV] >= least)
+            hit |= 1u << NV;
+        for (; hit; hit &= hit - 1)
+            scan((uint32_t)__ffs((int)hit) - 1, [&](float x, uint32_t id) {
+                if (x >= least)
+                    add_candidate(sh, order_of(x, id));
+            });
+    } else if (tid == 0)
+        sh.count = TOP_CAP + 1; // a NaN or +inf: the maxima do not tell
+    __syncthreads();
+    float out_sum = sum, out_top = top;
+    if (sum != sum) { // +inf alone has the log-sum-exp +inf
+        float any = 0.0f;
+        each([&](uint64_t o) { any = (uint32_t)(o >> 32) == 0xFFFFFFFFu ? 1.0f : any; });
+        any = block_reduce<TOP_NT>(any, sh.red[0], add);
+        out_top = any > 0.0f ? sum : __builtin_inff();
+    }
+    finish_top(sh, k, each, blockIdx.x, pieces == 1, values, ids, lse, part, part_sum, out_top, out_sum, t);
 }
 
 constexpr uint32_t MERGE_LISTS = 64; // lists one block merges
 
-// Merges up to MERGE_LISTS partial rows of a row.
+// Merges up to MERGE_LISTS partial rows of a row, NI orders a thread.
+template <int NI>
 __global__ __launch_bounds__(TOP_NT) void ung_top_merge_kernel(const uint64_t *part, const float2 *part_sum,
                                                                uint32_t lists, uint32_t groups, uint32_t k,
                                                                float *values, int32_t *ids, float *lse, uint64_t *out,
-                                                               float2 *out_sum)
+                                                               float2 *out_sum, Temperature t)
 {
     __shared__ TopShared sh;
     const uint64_t r = blockIdx.x / groups;
-    const uint32_t group = (uint32_t)(blockIdx.x - r * groups), first = group * MERGE_LISTS;
-    const uint32_t n = (lists - first < MERGE_LISTS ? lists - first : MERGE_LISTS);
+    const uint32_t tid = threadIdx.x;
+    const uint32_t first = (uint32_t)(blockIdx.x - r * groups) * MERGE_LISTS;
+    const uint32_t n = lists - first < MERGE_LISTS ? lists - first : MERGE_LISTS, items = n * k;
     const uint64_t *mine = part + (r * lists + first) * k;
-    const uint32_t items = n * k;
-    uint64_t thread_most = 0;
-    for (uint32_t i = threadIdx.x; i < items; i += TOP_NT)
-        thread_most = mine[i] > thread_most ? mine[i] : thread_most;
-    auto each = [&](auto f) {
-        for (uint32_t i = threadIdx.x; i < items; i += TOP_NT)
-            f(mine[i]);
-    };
+    uint64_t v[NI];
+#pragma unroll
+    for (int i = 0; i < NI; ++i)
+        v[i] = i * TOP_NT + tid < items ? mine[i * TOP_NT + tid] : 0;
     float2 s = make_float2(NEG_INF, 0.0f);
-    if (threadIdx.x < n)
-        s = part_sum[r * lists + first + threadIdx.x];
-    const float top = block_reduce<TOP_NT>(s.x, sh.red, max_nan);
-    float sum = s.y == 0.0f ? 0.0f : s.y * exp_neg(s.x - (top == NEG_INF ? 0.0f : top));
+    if (tid < n)
+        s = part_sum[r * lists + first + tid];
+    uint32_t most = 0;
+#pragma unroll
+    for (int i = 0; i < NI; ++i)
+        most = max(most, (uint32_t)(v[i] >> 32));
+    sh.most[tid] = most;
+    if (tid == 0)
+        sh.count = 0;
+    const float top = block_reduce<TOP_NT>(s.x, sh.red[0], max_nan);
+    if (tid < 64) {
+        const uint32_t limit = limit_of<0>(sh.most, k);
+        if (tid == 0)
+            sh.limit = limit;
+    }
+    const float sum = block_reduce<TOP_NT>(s.y == 0.0f ? 0.0f : s.y * weight_of(s.x, top == NEG_INF ? 0.0f : top, t.c),
+                                           sh.red[1], add);
+    const uint64_t least = sh.limit ? (uint64_t)sh.limit << 32 : 1;
+    auto each = [&](auto f) {
+#pragma unroll
+        for (int i = 0; i < NI; ++i)
+            f(v[i]);
+    };
+    each([&](uint64_t o) {
+        if (o >= least)
+            add_candidate(sh, o);
+    });
     __syncthreads();
-    sum = block_reduce<TOP_NT>(sum, sh.red, add);
-    const uint32_t found = select_top(sh, k, thread_most, each);
-    put_top(sh, found, k, blockIdx.x, groups == 1, values, ids, lse, out, out_sum, top, sum);
+    finish_top(sh, k, each, blockIdx.x, groups == 1, values, ids, lse, out, out_sum, top, sum, t);
 }
 
 // ---- distillation --------------------------------------------------------------------
@@ -310,34 +402,32 @@ __global__ __launch_bounds__(TOP_NT) void ung_top_merge_kernel(const uint64_t *p
 
 // What the backward pass needs of a row besides its inputs.
 struct alignas(16) Saved {
-    float top;      // largest score / T of the whole row; EMPTY: no loss
-    float inside;   // W / sum exp(s / T - top)
+    float top;      // largest score of the whole row; EMPTY: no loss
+    float inside;   // W / sum exp((s - top) / T)
     float rest_top; // the same two of the columns outside the list: gradient = weight / T *
-    float outside;  // exp(s / T - rest_top) * outside
-    float shift;    // p_k = exp(t_k / T - shift)
-    float unused[3];
+    float outside;  // exp((s - rest_top) / T) * outside
+    float base, log; // p_k = exp((t_k - base) / T - log)
+    float unused[2];
 };
 static_assert(sizeof(Saved) == 4 * UNG_HIP_DISTILL_SAVED, "");
 
 constexpr float EMPTY = __builtin_inff(); // Saved::top of a row without loss
 
 struct DistillShared {
-    float z[MAX_K];  // teacher's score / T; -inf = not there
-    float s[MAX_K];  // the student's there / T
+    float z[MAX_K];  // the teacher's score; -inf = not there
+    float s[MAX_K];  // the student's there
     uint32_t id[MAX_K];
     uint32_t first[MAX_K]; // the entry is the first one to name its column
     float red[2][16];
     Saved saved;
 };
 
-__device__ inline float max_of(float a, float b) { return fmaxf(a, b); }
-
 // The teacher's row: entries into sh by the first k threads, with the student's scores of
 // those whose columns lie in [from, to) (a block that writes the gradient over the scores
 // reads no other block's stretch).
 template <class T>
 __device__ inline void load_entries(DistillShared &sh, const T *row, const int32_t *ids, const float *values,
-                                    uint32_t k, uint32_t len, float inv_t, int64_t from, int64_t to)
+                                    uint32_t k, uint32_t len, int64_t from, int64_t to)
 {
     const uint32_t tid = threadIdx.x;
     if (tid < k) {
@@ -345,16 +435,17 @@ __device__ inline void load_entries(DistillShared &sh, const T *row, const int32
         const float v = values[tid];
         const bool ok = (uint32_t)id < len && v != NEG_INF;
         sh.id[tid] = ok ? (uint32_t)id : 0xFFFFFFFFu;
-        sh.z[tid] = ok ? v * inv_t : NEG_INF;
-        sh.s[tid] = ok && id >= from && id < to ? to_float(row[id]) * inv_t : 0.0f;
+        sh.z[tid] = ok ? v : NEG_INF;
+        sh.s[tid] = ok && id >= from && id < to ? to_float(row[id]) : 0.0f;
         sh.first[tid] = ok;
     }
 }
 
-// Loss and Saved of a row, run by one wave: from its entries and the sums (maximum / T, sum of
-// exp(s / T - maximum)) of its columns, with `lse` of those outside the list.  Returns the
+// Loss and Saved of a row, run by one wave: from its entries and the sums (maximum, sum of
+// exp((s - maximum) / T)) of its columns, with `lse` of those outside the list.  Returns the
 // loss in every lane.
-__device__ inline float finish_row(DistillShared &sh, uint32_t k, const float *lse, float2 sums, Saved &saved)
+__device__ inline float finish_row(DistillShared &sh, uint32_t k, const float *lse, float2 sums, Temperature t,
+                                   Saved &saved)
 {
     const uint32_t lane = threadIdx.x & 63;
     float z[2], s[2], best = NEG_INF, top = sums.x;
@@ -370,7 +461,7 @@ __device__ inline float finish_row(DistillShared &sh, uint32_t k, const float *l
             top = max_of(top, s[h]);
     }
     any = __any(any);
-    saved = Saved{EMPTY, 0.0f, 0.0f, 0.0f, 0.0f, {}};
+    saved = Saved{EMPTY, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, {}};
     best = wave_reduce(best, max_nan);
     top = wave_reduce(top, max_of);
     const float at = top == NEG_INF ? 0.0f : top;
@@ -380,44 +471,45 @@ __device__ inline float finish_row(DistillShared &sh, uint32_t k, const float *l
 #pragma unroll
         for (int h = 0; h < 2; ++h)
             if (h * 64 + lane < k && sh.first[h * 64 + lane])
-                in += expf(s[h] - at);
-        total = wave_reduce(in, add) + (sums.y == 0.0f ? 0.0f : sums.y * expf(sums.x - at));
+                in += weight_of(s[h], at, t.c);
+        total = wave_reduce(in, add) + (sums.y == 0.0f ? 0.0f : sums.y * weight_of(sums.x, at, t.c));
     }
     if (total != total) // a NaN among the scores, or +inf: the whole row is NaN
         top = total;
     if (!any || top == NEG_INF)
         return 0.0f;
-    float shift;
+    float base = 0.0f, log_base = 0.0f;
     if (lse)
-        shift = *lse;
+        log_base = *lse;
     else {
         float sum = 0.0f;
 #pragma unroll
         for (int h = 0; h < 2; ++h)
-            sum += z[h] == NEG_INF ? 0.0f : expf(z[h] - best);
-        shift = best + logf(wave_reduce(sum, add));
+            sum += z[h] == NEG_INF ? 0.0f : expf((z[h] - best) * t.inv);
+        base = best;
+        log_base = logf(wave_reduce(sum, add));
     }
     const float log_total = logf(total);
     float mass = 0.0f, loss = 0.0f;
 #pragma unroll
     for (int h = 0; h < 2; ++h)
         if (z[h] != NEG_INF) {
-            const float log_p = z[h] - shift, p = expf(log_p);
+            const float log_p = (z[h] - base) * t.inv - log_base, p = expf(log_p);
             mass += p;
             if (!(p <= 0.0f))
-                loss += p * (log_p - (s[h] - top - log_total));
+                loss += p * (log_p - ((s[h] - top) * t.inv - log_total));
         }
     mass = wave_reduce(mass, add);
     loss = wave_reduce(loss, add);
-    saved = Saved{top, mass / total, top, mass / total, shift, {}};
+    saved = Saved{top, mass / total, top, mass / total, base, log_base, {}};
     if (lse && !(sums.y <= 0.0f)) {
         const float rest = 1.0f - mass < 0.0f ? 0.0f : 1.0f - mass;
         saved.rest_top = sums.x;
         if (!(rest <= 0.0f)) {
-            loss += rest * (logf(rest) - (sums.x - top + logf(sums.y) - log_total));
+            loss += rest * (logf(rest) - ((sums.x - top) * t.inv + logf(sums.y) - log_total));
             saved.inside = (mass + rest) / total;
         }
-        saved.outside = expf(sums.x - top) * saved.inside - rest / sums.y;
+        saved.outside = weight_of(sums.x, top, t.c) * saved.inside - rest / sums.y;
     }
     return loss;
 }
@@ -425,45 +517,50 @@ __device__ inline float finish_row(DistillShared &sh, uint32_t k, const float *l
 // Gradient of a stretch of a row whose vectors are in registers, then of the listed columns
 // that lie in it (in one more write: their scores were read before the first one).
 template <class T, int NT, int NV>
-__device__ inline void write_gradient(DistillShared &sh, const Vec<T> (&v)[NV], uint32_t begin, uint32_t shift,
-                                      uint32_t len, uint32_t end, uint32_t k, float inv_t, const Saved &saved,
-                                      float weight, T *grad)
+__device__ inline void write_gradient(DistillShared &sh, const RowRef<T> &ref, Stretch<T, NT, NV> &x, uint32_t begin, uint32_t k,
+                                      Temperature t, const Saved saved, float weight, T *grad)
 {
     constexpr int N = Vec<T>::N;
-    const bool same = ((uintptr_t)grad & 15) == shift * sizeof(T);
-    const bool empty = saved.top == EMPTY;
-    const float w = weight * inv_t, out = saved.outside * w;
-#pragma unroll
-    for (int i = 0; i < NV; ++i) {
-        const uint32_t at = begin + threadIdx.x + i * NT;
-        if (at >= end)
-            break;
+    const bool same = ((uintptr_t)grad & 15) == ref.shift * sizeof(T);
+    const float c = t.c, w = weight * t.inv, out = saved.outside * w;
+    const float rest_top = saved.rest_top;
+    auto put = [&](const Vec<T> &g, uint32_t at) {
+        const bool inside = ref.inside(at);
+        if (same && inside)
+            reinterpret_cast<Vec<T> *>(grad - ref.shift)[at] = g;
+        else if (inside || (x.has_edge && at == x.edge_at)) // an end is written by its holder alone
+            ref.store_elements(grad, at, g);
+    };
+    if (saved.top == EMPTY) {
+        x.each([&](const Vec<T> &, uint32_t at) { put(Vec<T>{}, at); });
+        return;
+    }
+    x.each([&](const Vec<T> &v, uint32_t at) {
         Vec<T> g;
 #pragma unroll
-        for (int e = 0; e < N; ++e)
-            g.v[e] = from_float<T>(empty ? 0.0f : exp_neg(to_float(v[i].v[e]) * inv_t - saved.rest_top) * out);
-        store_vec(grad, shift, len, at, g, same);
-    }
-    if (empty)
-        return;
+        for (int e = 0; e < N; e += 2)
+            g.put2(e, weight_of(v.get(e), rest_top, c) * out, weight_of(v.get(e + 1), rest_top, c) * out);
+        put(g, at);
+    });
     __syncthreads();
     if (threadIdx.x < k) {
         const uint32_t id = sh.id[threadIdx.x];
-        const uint32_t at = (id + shift) / N;
+        const uint32_t at = (id + ref.shift) / N;
         if (id != 0xFFFFFFFFu && at >= begin && at < begin + NT * NV) {
             float p = 0.0f; // of every entry that names this column
-            for (uint32_t t = 0; t < k; ++t)
-                p += sh.id[t] == id ? expf(sh.z[t] - saved.shift) : 0.0f;
-            grad[id] = from_float<T>((exp_neg(sh.s[threadIdx.x] - saved.top) * saved.inside - p) * w);
+            for (uint32_t o = 0; o < k; ++o)
+                p += sh.id[o] == id ? expf((sh.z[o] - saved.base) * t.inv - saved.log) : 0.0f;
+            const float e = weight_of(sh.s[threadIdx.x], saved.top, t.c);
+            grad[id] = from_float<T>((e * saved.inside - p) * w);
         }
     }
 }
 
-// Sums of a stretch of a row in registers, in every thread: its maximum / T and the sum of
-// exp(s / T - maximum).  With `tail` listed columns become -inf first.
+// Sums of a stretch of a row in registers, in every thread: its maximum and the sum of
+// exp((s - maximum) / T).  With `tail` listed columns become -inf first.
 template <class T, int NT, int NV>
-__device__ inline float2 stretch_sums(DistillShared &sh, uint32_t *bits, Vec<T> (&v)[NV], uint32_t begin,
-                                      uint32_t shift, uint32_t k, bool tail, float inv_t)
+__device__ inline float2 stretch_sums(DistillShared &sh, uint32_t *bits, Stretch<T, NT, NV> &x, uint32_t begin,
+                                      uint32_t shift, uint32_t k, bool tail, float c)
 {
     constexpr int N = Vec<T>::N;
     const uint32_t tid = threadIdx.x;
@@ -479,53 +576,39 @@ __device__ inline float2 stretch_sums(DistillShared &sh, uint32_t *bits, Vec<T> 
             }
         }
         __syncthreads();
-#pragma unroll
-        for (int i = 0; i < NV; ++i) {
-            const uint32_t b = (tid + i * NT) * N;
+        x.each([&](Vec<T> &v, uint32_t at) {
+            const uint32_t b = (at - begin) * N;
             const uint32_t listed = bits[b >> 5] >> (b & 31) & ((1u << N) - 1);
             if (listed)
 #pragma unroll
                 for (int e = 0; e < N; ++e)
                     if (listed >> e & 1)
-                        v[i].v[e] = (T)NEG_INF;
-        }
+                        v.set(e, (T)NEG_INF);
+        });
     }
     float most = NEG_INF;
-#pragma unroll
-    for (int i = 0; i < NV; ++i)
+    x.each([&](const Vec<T> &v, uint32_t) {
 #pragma unroll
         for (int e = 0; e < N; ++e)
-            most = max_of(most, to_float(v[i].v[e])); // a NaN shows in the sum
-    const float top = block_reduce<NT>(most, sh.red[0], max_of) * inv_t;
+            most = max_of(most, v.get(e)); // a NaN shows in the sum
+    });
+    const float top = block_reduce<NT>(most, sh.red[0], max_of);
     const float at = top == NEG_INF ? 0.0f : top;
     float sum = 0.0f;
-#pragma unroll
-    for (int i = 0; i < NV; ++i)
+    x.each([&](const Vec<T> &v, uint32_t) {
 #pragma unroll
         for (int e = 0; e < N; ++e)
-            sum += exp_neg(to_float(v[i].v[e]) * inv_t - at);
+            sum += weight_of(v.get(e), at, c);
+    });
     return make_float2(top, block_reduce<NT>(sum, sh.red[1], add));
-}
-
-template <class T, int NT, int NV>
-__device__ inline void load_stretch(const RowRef<T> &ref, uint32_t first, uint32_t end, Vec<T> (&v)[NV])
-{
-#pragma unroll
-    for (int i = 0; i < NV; ++i)
-        if (first + i * NT < end)
-            v[i] = ref.load(first + i * NT);
-        else
-#pragma unroll
-            for (int e = 0; e < Vec<T>::N; ++e)
-                v[i].v[e] = (T)NEG_INF;
 }
 
 // A row by one block, its scores in registers: loss, and the gradient with `grad`.  One read
 // of the scores and one write of the gradient, bound by memory.  `grad` may be the scores.
 template <class T, int NT, int NV>
-__global__ __launch_bounds__(NT) void ung_distill_row_kernel(const T *scores, uint32_t len, uint64_t stride,
+__global__ __launch_bounds__(NT, NV <= 8 ? 8 : 4) void ung_distill_row_kernel(const T *scores, uint32_t len, uint64_t stride,
                                                              const int32_t *ids, const float *values, uint32_t k,
-                                                             const float *lse, const float *weight, float inv_t,
+                                                             const float *lse, const float *weight, Temperature t,
                                                              float *loss, Saved *saved_out, T *grad,
                                                              uint64_t grad_stride)
 {
@@ -533,15 +616,13 @@ __global__ __launch_bounds__(NT) void ung_distill_row_kernel(const T *scores, ui
     __shared__ uint32_t bits[NT * NV * Vec<T>::N / 32];
     const uint64_t r = blockIdx.x;
     const RowRef<T> ref(scores + r * stride, len);
-    const uint32_t end = vectors_of<T>(ref.shift, len);
-    Vec<T> v[NV];
-    load_stretch<T, NT, NV>(ref, threadIdx.x, end, v);
-    load_entries(sh, ref.row, ids + r * k, values + r * k, k, len, inv_t, 0, len);
-    const float2 sums = stretch_sums<T, NT, NV>(sh, bits, v, 0, ref.shift, k, lse != nullptr, inv_t);
+    Stretch<T, NT, NV> x(ref, 0);
+    load_entries(sh, ref.row, ids + r * k, values + r * k, k, len, 0, len);
+    const float2 sums = stretch_sums<T, NT, NV>(sh, bits, x, 0, ref.shift, k, lse != nullptr, t.c);
     __syncthreads();
     if (threadIdx.x < 64) {
         Saved saved;
-        const float l = finish_row(sh, k, lse ? lse + r : nullptr, sums, saved);
+        const float l = finish_row(sh, k, lse ? lse + r : nullptr, sums, t, saved);
         if (threadIdx.x == 0) {
             loss[r] = l;
             if (saved_out)
@@ -552,26 +633,24 @@ __global__ __launch_bounds__(NT) void ung_distill_row_kernel(const T *scores, ui
     if (!grad)
         return;
     __syncthreads();
-    write_gradient<T, NT, NV>(sh, v, 0, ref.shift, len, end, k, inv_t, sh.saved, weight ? weight[r] : 1.0f,
-                              grad + r * grad_stride);
+    write_gradient<T, NT, NV>(sh, ref, x, 0, k, t, sh.saved, weight ? weight[r] : 1.0f, grad + r * grad_stride);
 }
 
 // Sums of one piece of a row (NT * NV vectors).
 template <class T, int NT, int NV>
 __global__ __launch_bounds__(NT) void ung_distill_part_kernel(const T *scores, uint32_t len, uint64_t stride,
                                                               const int32_t *ids, const float *values, uint32_t k,
-                                                              int tail, float inv_t, uint32_t pieces, float2 *part)
+                                                              int tail, Temperature t, uint32_t pieces, float2 *part)
 {
     __shared__ DistillShared sh;
     __shared__ uint32_t bits[NT * NV * Vec<T>::N / 32];
     const uint64_t r = blockIdx.x / pieces;
     const uint32_t begin = (uint32_t)(blockIdx.x - r * pieces) * (NT * NV);
     const RowRef<T> ref(scores + r * stride, len);
-    Vec<T> v[NV];
-    load_stretch<T, NT, NV>(ref, begin + threadIdx.x, vectors_of<T>(ref.shift, len), v);
+    Stretch<T, NT, NV> x(ref, begin);
     if (tail)
-        load_entries(sh, ref.row, ids + r * k, values + r * k, k, len, inv_t, 0, 0);
-    const float2 sums = stretch_sums<T, NT, NV>(sh, bits, v, begin, ref.shift, k, tail, inv_t);
+        load_entries(sh, ref.row, ids + r * k, values + r * k, k, len, 0, 0);
+    const float2 sums = stretch_sums<T, NT, NV>(sh, bits, x, begin, ref.shift, k, tail, t.c);
     if (threadIdx.x == 0)
         part[blockIdx.x] = sums;
 }
@@ -580,17 +659,17 @@ __global__ __launch_bounds__(NT) void ung_distill_part_kernel(const T *scores, u
 template <class T>
 __global__ __launch_bounds__(128) void ung_distill_join_kernel(const T *scores, uint32_t len, uint64_t stride,
                                                                const int32_t *ids, const float *values, uint32_t k,
-                                                               const float *lse, float inv_t, uint32_t pieces,
+                                                               const float *lse, Temperature t, uint32_t pieces,
                                                                const float2 *part, float *loss, Saved *saved_out)
 {
     __shared__ DistillShared sh;
     const uint64_t r = blockIdx.x;
-    load_entries(sh, scores + r * stride, ids + r * k, values + r * k, k, len, inv_t, 0, len);
+    load_entries(sh, scores + r * stride, ids + r * k, values + r * k, k, len, 0, len);
     __syncthreads();
     if (lse && threadIdx.x < k) {
         const uint32_t id = sh.id[threadIdx.x];
-        for (uint32_t t = 0; t < threadIdx.x; ++t)
-            if (sh.id[t] == id)
+        for (uint32_t o = 0; o < threadIdx.x; ++o)
+            if (sh.id[o] == id)
                 sh.first[threadIdx.x] = 0;
     }
     __syncthreads();
@@ -603,10 +682,10 @@ __global__ __launch_bounds__(128) void ung_distill_join_kernel(const T *scores, 
     top = wave_reduce(top, max_of);
     const float at = top == NEG_INF ? 0.0f : top;
     for (uint32_t i = threadIdx.x; i < pieces; i += 64)
-        sum += mine[i].y == 0.0f ? 0.0f : mine[i].x == NEG_INF ? mine[i].y : mine[i].y * expf(mine[i].x - at);
+        sum += mine[i].y == 0.0f ? 0.0f : mine[i].x == NEG_INF ? mine[i].y : mine[i].y * weight_of(mine[i].x, at, t.c);
     sum = wave_reduce(sum, add);
     Saved saved;
-    const float l = finish_row(sh, k, lse ? lse + r : nullptr, make_float2(top, sum), saved);
+    const float l = finish_row(sh, k, lse ? lse + r : nullptr, make_float2(top, sum), t, saved);
     if (threadIdx.x == 0) {
         loss[r] = l;
         saved_out[r] = saved;
@@ -617,21 +696,18 @@ __global__ __launch_bounds__(128) void ung_distill_join_kernel(const T *scores, 
 template <class T, int NT, int NV>
 __global__ __launch_bounds__(NT) void ung_distill_grad_kernel(const T *scores, uint32_t len, uint64_t stride,
                                                               const int32_t *ids, const float *values, uint32_t k,
-                                                              const Saved *saved, const float *weight, float inv_t,
+                                                              const Saved *saved, const float *weight, Temperature t,
                                                               uint32_t pieces, T *grad, uint64_t grad_stride)
 {
     __shared__ DistillShared sh;
     const uint64_t r = blockIdx.x / pieces;
     const uint32_t begin = (uint32_t)(blockIdx.x - r * pieces) * (NT * NV);
     const RowRef<T> ref(scores + r * stride, len);
-    const uint32_t end = vectors_of<T>(ref.shift, len);
-    Vec<T> v[NV];
-    load_stretch<T, NT, NV>(ref, begin + threadIdx.x, end, v);
+    Stretch<T, NT, NV> x(ref, begin);
     const int64_t from = (int64_t)begin * Vec<T>::N - ref.shift;
-    load_entries(sh, ref.row, ids + r * k, values + r * k, k, len, inv_t, from, from + NT * NV * Vec<T>::N);
+    load_entries(sh, ref.row, ids + r * k, values + r * k, k, len, from, from + NT * NV * Vec<T>::N);
     __syncthreads(); // the entries' scores are read before this block writes
-    write_gradient<T, NT, NV>(sh, v, begin, ref.shift, len, end, k, inv_t, saved[r],
-                              weight ? weight[r] : 1.0f, grad + r * grad_stride);
+    write_gradient<T, NT, NV>(sh, ref, x, begin, k, t, saved[r], weight ? weight[r] : 1.0f, grad + r * grad_stride);
 }
 
 } // namespace
@@ -679,6 +755,8 @@ int check_temperature(const char *what, float t)
     set_error("%s: temperature %g is not a positive number", what, (double)t);
     return UNG_HIP_EINVAL;
 }
+
+Temperature temperature_of(float t) { return Temperature{1.0f / t, (float)(LOG2E / t)}; }
 
 int check_k(const char *what, uint32_t k, uint32_t least)
 {
@@ -807,13 +885,13 @@ int distill(const char *what, const void *scores, int type, uint64_t rows, uint6
     return with_type(type, [&](auto zero) {
         using T = decltype(zero);
         const T *p = (const T *)scores;
-        const float inv_t = 1.0f / temperature;
+        const Temperature t = temperature_of(temperature);
         const uint32_t vectors = vectors_at_most<T>(scores, rows, stride, len);
         int rc;
         if (whole_rows(rows, vectors)) {
             with_nv(row_cut(vectors).nv, [&](auto nv) {
                 ung_distill_row_kernel<T, ROW_NT, nv.value><<<(uint32_t)rows, ROW_NT, 0, st>>>(
-                    p, (uint32_t)len, stride, ids, values, k, lse, weight, inv_t, loss, saved, (T *)grad, grad_stride);
+                    p, (uint32_t)len, stride, ids, values, k, lse, weight, t, loss, saved, (T *)grad, grad_stride);
             });
             return launched(what);
         }
@@ -826,14 +904,14 @@ int distill(const char *what, const void *scores, int type, uint64_t rows, uint6
         Saved *kept = saved ? saved : (Saved *)((char *)workspace + parts);
         with_nv(cut.nv, [&](auto nv) {
             ung_distill_part_kernel<T, PIECE_NT, nv.value><<<(uint32_t)blocks, PIECE_NT, 0, st>>>(
-                p, (uint32_t)len, stride, ids, values, k, lse != nullptr, inv_t, cut.pieces, part);
+                p, (uint32_t)len, stride, ids, values, k, lse != nullptr, t, cut.pieces, part);
         });
         ung_distill_join_kernel<T><<<(uint32_t)rows, 128, 0, st>>>(p, (uint32_t)len, stride, ids, values, k, lse,
-                                                                   inv_t, cut.pieces, part, loss, kept);
+                                                                   t, cut.pieces, part, loss, kept);
         if (grad)
             with_nv(cut.nv, [&](auto nv) {
                 ung_distill_grad_kernel<T, PIECE_NT, nv.value><<<(uint32_t)blocks, PIECE_NT, 0, st>>>(
-                    p, (uint32_t)len, stride, ids, values, k, kept, weight, inv_t, cut.pieces, (T *)grad, grad_stride);
+                    p, (uint32_t)len, stride, ids, values, k, kept, weight, t, cut.pieces, (T *)grad, grad_stride);
             });
         return launched(what);
     });
@@ -886,6 +964,7 @@ int ung_hip_top_scores(const void *scores, int type, uint64_t rows, uint64_t len
         if ((rc = check_grid(what, rows * cut.pieces)) ||
             (rc = check_workspace(what, workspace, workspace_bytes, top_bytes(rows, cut.pieces, k))))
             return rc;
+        const Temperature t = temperature_of(temperature);
         char *at = (char *)workspace;
         auto take = [&](uint64_t bytes) {
             void *p = at;
@@ -901,7 +980,7 @@ int ung_hip_top_scores(const void *scores, int type, uint64_t rows, uint64_t len
         }
         with_nv(cut.nv, [&](auto nv) {
             ung_top_scores_kernel<T, nv.value><<<(uint32_t)(rows * lists), TOP_NT, 0, st>>>(
-                (const T *)scores, (uint32_t)len, row_stride, (uint32_t)lists, k, 1.0f / temperature, values, ids, lse,
+                (const T *)scores, (uint32_t)len, row_stride, (uint32_t)lists, k, t, values, ids, lse,
                 part, sums);
         });
         while (lists > 1) {
@@ -912,8 +991,17 @@ int ung_hip_top_scores(const void *scores, int type, uint64_t rows, uint64_t len
                 out = (uint64_t *)take(rows * groups * k * 8);
                 out_sums = (float2 *)take(rows * groups * 8);
             }
-            ung_top_merge_kernel<<<(uint32_t)(rows * groups), TOP_NT, 0, st>>>(
-                part, sums, (uint32_t)lists, (uint32_t)groups, k, values, ids, lse, out, out_sums);
+            auto merge = [&](auto kernel) {
+                kernel<<<(uint32_t)(rows * groups), TOP_NT, 0, st>>>(part, sums, (uint32_t)lists, (uint32_t)groups, k,
+                                                                     values, ids, lse, out, out_sums, t);
+            };
+            const uint64_t items = (lists < MERGE_LISTS ? lists : MERGE_LISTS) * k;
+            if (items <= TOP_NT * 4)
+                merge(ung_top_merge_kernel<4>);
+            else if (items <= TOP_NT * 12)
+                merge(ung_top_merge_kernel<12>);
+            else
+                merge(ung_top_merge_kernel<MERGE_LISTS * MAX_K / TOP_NT>);
             part = out;
             sums = out_sums;
             lists = groups;
@@ -987,7 +1075,7 @@ int ung_hip_distill_backward(const void *scores, int type, uint64_t rows, uint64
             ung_distill_grad_kernel<T, PIECE_NT, nv.value><<<(uint32_t)(rows * cut.pieces), PIECE_NT, 0,
                                                              (hipStream_t)stream>>>(
                 (const T *)scores, (uint32_t)len, row_stride, ids, values, k, (const Saved *)saved, weight,
-                1.0f / temperature, cut.pieces, (T *)grad, grad_stride);
+                temperature_of(temperature), cut.pieces, (T *)grad, grad_stride);
         });
         return launched(what);
     });
