@@ -275,71 +275,99 @@ __device__ inline f32x4 block_product(const Wide &x, const Wide &y)
     return p;
 }
 
-// 16 bytes a lane from global memory straight into LDS, at `lds` + 16 * lane.
-__device__ inline void to_lds(const uint8_t *src, uint8_t *lds)
+// 16 (or 4) bytes a lane from global memory straight into LDS, at `lds` + 16 (4) * lane.
+using lds_ptr = __attribute__((address_space(3))) void *;
+__device__ inline void to_lds16(__amdgpu_buffer_rsrc_t from, uint32_t offset, uint32_t advance, void *lds)
 {
-    __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) uint32_t *)src,
-                                     (__attribute__((address_space(3))) uint32_t *)lds, 16, 0, 0);
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(from, (lds_ptr)lds, 16, offset, advance, 0, 0);
+}
+__device__ inline void to_lds4(__amdgpu_buffer_rsrc_t from, uint32_t offset, uint32_t advance, void *lds)
+{
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(from, (lds_ptr)lds, 4, offset, advance, 0, 0);
 }
 
-// A block of 4 waves makes a BM x BN tile of the product, each wave a quarter of it.  Per
-// 128-byte block of the inner length both tiles are staged in LDS, 16-byte pieces of a row
-// rotated by exclusive-or with the row so that eight lanes read eight rows without a bank
-// conflict; the staged loads are rotated on the global side, as they land in lane order.
-// Block products start from zero and enter the running sums by one multiply-add with the
-// scales' product, so sums and scales stay in 32 bits.  The table side (b) is the matrix
-// instruction's row side: a lane holds four neighbouring columns of one row of c, with one
-// scale of a.
-template <int BM, int BN, bool SQUARE, class OT>
-__global__ __launch_bounds__(256, 2) void ung_fp8_tile_product_kernel(const uint8_t *a, const float *a_scale,
-                                                                      const uint8_t *b, const float *b_scale,
-                                                                      uint64_t m, uint64_t n, uint32_t kblocks, OT *c,
-                                                                      uint64_t c_stride, uint32_t m_tiles,
-                                                                      uint32_t n_tiles, int vector_stores)
+__device__ inline __amdgpu_buffer_rsrc_t buffer_of(const void *p)
 {
-    constexpr int WM = BM / 2, WN = BN / 2, TM = WM / 16, TN = WN / 16;
-    __shared__ alignas(16) uint8_t as[2][BM * KB];
-    __shared__ alignas(16) uint8_t bs[2][BN * KB];
-    __shared__ float sa[2][BM], sb[2][BN];
-    const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const uint32_t wm = (wave & 1) * WM, wn = (wave >> 1) * WN;
-    const uint32_t tm = blockIdx.x % m_tiles, tn = blockIdx.x / m_tiles;
-    const uint64_t m0 = (uint64_t)tm * BM, n0 = (uint64_t)tn * BN, kp = (uint64_t)kblocks * KB;
-    (void)n_tiles;
+    return __builtin_amdgcn_make_buffer_rsrc(const_cast<void *>(p), 0, 0xFFFFFFFFu, 0x00020000);
+}
 
+// Tile of the product that block `id` of `total` makes.  Blocks go to the eight XCDs in turn;
+// each XCD takes a contiguous run of the tiles, in bands of 8 tiles of m, so that the tiles it
+// works on at a time share their panels in its L2.
+__device__ inline void tile_of(uint32_t id, uint32_t m_tiles, uint32_t n_tiles, uint32_t &tm, uint32_t &tn)
+{
+    const uint32_t total = m_tiles * n_tiles, xcd = id & 7, each = total >> 3, extra = total & 7;
+    const uint32_t t = xcd * each + (xcd < extra ? xcd : extra) + (id >> 3);
+    const uint32_t band = t / (8 * n_tiles), in = t - band * 8 * n_tiles;
+    const uint32_t high = m_tiles - band * 8 < 8 ? m_tiles - band * 8 : 8;
+    tm = band * 8 + in % high;
+    tn = in / high;
+}
+
+// A block of WM x WN waves makes a BM x BN tile of the product, each wave BM / WM x 64 of it.
+// Per 128-byte block of the inner length both tiles are staged in LDS by loads that bypass the
+// registers, one block ahead of the matrix instructions.  A row's eight 16-byte pieces are
+// rotated by exclusive-or with a number of the row so that any eight lanes that read eight
+// rows meet all banks; the rotation is made on the global side, as such loads land in lane
+// order.  Block products start from zero and enter the running sums by one multiply-add with
+// the scales, so sums and scales stay in 32 bits.  The table side (b) is the matrix
+// instruction's row side, its 64 rows spread over four instructions so that a lane ends with
+// 16 neighbouring columns of one row of c, and with one scale of a.
+template <int BM, int BN, int WM, int WN, bool SQUARE, class OT>
+__global__ __launch_bounds__(WM * WN * 64, 2) void ung_fp8_product_kernel(const uint8_t *a, const float *a_scale,
+                                                                          const uint8_t *b, const float *b_scale,
+                                                                          uint64_t m, uint64_t n, uint32_t kblocks,
+                                                                          OT *c, uint64_t c_stride, uint32_t m_tiles,
+                                                                          uint32_t n_tiles, int vector_stores)
+{
+    constexpr int WAVES = WM * WN, TM = BM / WM / 16, TN = 4, DEEP = 3;
+    static_assert(BN / WN == 64 && BM / 8 % WAVES == 0 && BN / 8 % WAVES == 0 && (BM + BN) / 64 <= WAVES, "");
+    struct Panels {
+        alignas(16) uint8_t a[BM * KB], b[BN * KB];
+        float sa[BM], sb[BN];
+    };
+    __shared__ Panels even, odd;
+    const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const uint32_t wm = (wave % WM) * (BM / WM), wn = (wave / WM) * 64;
+    uint32_t tm, tn;
+    tile_of(blockIdx.x, m_tiles, n_tiles, tm, tn);
+    const uint64_t m0 = (uint64_t)tm * BM, n0 = (uint64_t)tn * BN, kp = (uint64_t)kblocks * KB;
     // rows past the end repeat the last one; their results are not stored
-    auto stage = [&](uint32_t kb, int buf) {
-        const uint32_t piece = (lane & 7) ^ (lane >> 3);
+    const uint32_t last_m = (uint32_t)min(m - m0, (uint64_t)BM) - 1, last_n = (uint32_t)min(n - n0, (uint64_t)BN) - 1;
+
+    // staging: each wave loads every WAVES-th group of 8 rows, then 64 scales of a or b
+    const __amdgpu_buffer_rsrc_t a_from = buffer_of(a + m0 * kp), b_from = buffer_of(b + n0 * kp);
+    static_assert(8 * WAVES % 32 == 0, ""); // a lane's rotation is the same in all its groups
+    const uint32_t line = wave * 8 + (lane >> 3);
+    const uint32_t a_piece = ((lane & 7) ^ (line & 7)) * 16;
+    const uint32_t b_piece = ((lane & 7) ^ ((line & 3) | (line >> 2 & 4))) * 16;
+    const bool of_a = wave < BM / 64, of_b = !of_a && wave < (BM + BN) / 64;
+    const __amdgpu_buffer_rsrc_t s_from =
+        buffer_of(of_a ? a_scale + m0 * kblocks : b_scale + (SQUARE ? n0 / KB : n0) * kblocks);
+    const uint32_t s_row = (of_a ? wave : wave - BM / 64) * 64;
+    const uint32_t s_line = min(s_row + lane, of_a ? last_m : last_n);
+    const uint32_t s_at = (SQUARE && !of_a ? s_line / KB : s_line) * kblocks * 4;
+    auto stage = [&](Panels &to, uint32_t kb) {
+        uint32_t l = line;
+        asm volatile("" : "+v"(l)); // offsets are made anew: the sums need the registers
 #pragma unroll
-        for (int i = 0; i < BM / 32; ++i) {
-            const uint32_t r = (wave * (BM / 32) + i) * 8 + (lane >> 3);
-            const uint64_t row = min(m0 + r, m - 1);
-            to_lds(a + row * kp + (uint64_t)kb * KB + piece * 16, &as[buf][(wave * (BM / 32) + i) * 1024]);
-        }
+        for (int i = 0; i < BM / 8 / WAVES; ++i)
+            to_lds16(a_from, min(l + i * WAVES * 8, last_m) * (uint32_t)kp + a_piece, kb * KB,
+                     to.a + (i * WAVES + wave) * 1024);
 #pragma unroll
-        for (int i = 0; i < BN / 32; ++i) {
-            const uint32_t r = (wave * (BN / 32) + i) * 8 + (lane >> 3);
-            const uint64_t row = min(n0 + r, n - 1);
-            to_lds(b + row * kp + (uint64_t)kb * KB + piece * 16, &bs[buf][(wave * (BN / 32) + i) * 1024]);
-        }
-        for (uint32_t t = threadIdx.x; t < BM; t += 256)
-            sa[buf][t] = a_scale[min(m0 + t, m - 1) * kblocks + kb];
-        for (uint32_t t = threadIdx.x; t < BN; t += 256) {
-            const uint64_t row = min(n0 + t, n - 1);
-            sb[buf][t] = b_scale[(SQUARE ? row / KB : row) * kblocks + kb];
-        }
+        for (int i = 0; i < BN / 8 / WAVES; ++i)
+            to_lds16(b_from, min(l + i * WAVES * 8, last_n) * (uint32_t)kp + b_piece, kb * KB,
+                     to.b + (i * WAVES + wave) * 1024);
+        if (of_a)
+            to_lds4(s_from, s_at, kb * 4, to.sa + s_row);
+        else if (of_b)
+            to_lds4(s_from, s_at, kb * 4, to.sb + s_row);
     };
-    auto fragment = [&](const uint8_t *tile, uint32_t row0) {
-        const uint32_t r = row0 + (lane & 15), g = lane >> 4;
-        Frag f;
-        f.h[0] = *reinterpret_cast<const uint4 *>(tile + r * KB + ((g ^ (r & 7)) * 16));
-        f.h[1] = *reinterpret_cast<const uint4 *>(tile + r * KB + (((g + 4) ^ (r & 7)) * 16));
-        if constexpr (sizeof(OT) == 4)
-            return widen(f);
-        else
-            return f;
-    };
-    using Part = decltype(fragment(nullptr, 0));
+
+    // a lane's place in the panels: pieces g and g + 4 of its row (they differ in bit 6)
+    const uint32_t r = lane & 15, g = lane >> 4, b_row = wn + (r >> 2) * 16 + (r & 3);
+    const uint32_t a_lane = (wm + r) * KB + (g ^ (r & 7)) * 16, b_lane = b_row * KB + (g ^ (r & 7)) * 16;
+    using Part = std::conditional_t<sizeof(OT) == 4, Wide, Frag>;
 
     f32x4 acc[TM][TN];
 #pragma unroll
@@ -348,62 +376,95 @@ __global__ __launch_bounds__(256, 2) void ung_fp8_tile_product_kernel(const uint
         for (int j = 0; j < TN; ++j)
             acc[i][j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 
-    if (kblocks)
-        stage(0, 0);
-    for (uint32_t kb = 0; kb < kblocks; ++kb) {
-        const int buf = kb & 1;
-        // loads into LDS are counted as memory loads, which a barrier alone does not await
-        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-        __syncthreads(); // this block's tiles have landed; the other buffer is free
-        if (kb + 1 < kblocks)
-            stage(kb + 1, buf ^ 1);
-        Part af[TM], bf[TN];
-        float s[TM];
-        f32x4 sn[TN];
-#pragma unroll
-        for (int i = 0; i < TM; ++i) {
-            af[i] = fragment(as[buf], wm + i * 16);
-            s[i] = sa[buf][wm + i * 16 + (lane & 15)];
-        }
+    auto multiply = [&](const Panels &p) {
+        uint32_t a_at = a_lane, b_at = b_lane, sa_at = wm + r, sb_at = wn + g * 16;
+        // one address each, not one for every fragment of both panels
+        asm volatile("" : "+v"(a_at), "+v"(b_at), "+v"(sa_at), "+v"(sb_at));
+        const uint8_t *pa = p.a + a_at, *pa4 = p.a + (a_at ^ 64), *pb = p.b + b_at, *pb4 = p.b + (b_at ^ 64);
+        auto fragment = [&](const uint8_t *lo, const uint8_t *hi) {
+            Frag f;
+            f.h[0] = *reinterpret_cast<const uint4 *>(lo);
+            f.h[1] = *reinterpret_cast<const uint4 *>(hi);
+            if constexpr (sizeof(OT) == 4)
+                return widen(f);
+            else
+                return f;
+        };
+        Part bf[TN], af[2];
+        f32x4 sn[TN], q[DEEP + 1];
+        float s[2];
+        auto load_a = [&](int i) {
+            af[i & 1] = fragment(pa + i * 16 * KB, pa4 + i * 16 * KB);
+            s[i & 1] = p.sa[sa_at + i * 16];
+        };
+        load_a(0);
 #pragma unroll
         for (int j = 0; j < TN; ++j) {
-            bf[j] = fragment(bs[buf], wn + j * 16);
-            sn[j] = *reinterpret_cast<const f32x4 *>(&sb[buf][wn + j * 16 + (lane >> 4) * 4]);
+            bf[j] = fragment(pb + j * 4 * KB, pb4 + j * 4 * KB);
+            if (!SQUARE)
+                sn[j] = *reinterpret_cast<const f32x4 *>(&p.sb[sb_at + j * 4]);
         }
+        const float s_all = SQUARE ? p.sb[sb_at] : 1.0f;
+        float scale = 0.0f;
+        // a result enters its sum DEEP products after it was begun
 #pragma unroll
-        for (int i = 0; i < TM; ++i)
-#pragma unroll
-            for (int j = 0; j < TN; ++j) {
-                const f32x4 p = block_product(bf[j], af[i]);
+        for (int t = 0; t < TM * TN + DEEP; ++t) {
+            if (t < TM * TN) {
+                if (t % TN == 1 && t / TN + 1 < TM)
+                    load_a(t / TN + 1);
+                q[t % (DEEP + 1)] = block_product(bf[t % TN], af[t / TN & 1]);
+            }
+            const int o = t - DEEP, i = o / TN, j = o % TN;
+            if (o >= 0) {
+                if (j == 0)
+                    scale = SQUARE ? s[i & 1] * s_all : s[i & 1];
 #pragma unroll
                 for (int e = 0; e < 4; ++e)
-                    acc[i][j][e] = __builtin_fmaf(p[e], s[i] * sn[j][e], acc[i][j][e]);
+                    acc[i][j][e] =
+                        __builtin_fmaf(q[o % (DEEP + 1)][e], SQUARE ? scale : scale * sn[j][e], acc[i][j][e]);
             }
+            __builtin_amdgcn_sched_barrier(0);
+        }
+    };
+    auto step = [&](const Panels &now, Panels &next, uint32_t kb) {
+        // loads into LDS are counted as memory loads, which a barrier alone does not await
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        __syncthreads(); // `now` has landed; every wave is done with `next`
+        if (kb + 1 < kblocks)
+            stage(next, kb + 1);
+        multiply(now);
+    };
+
+    if (kblocks)
+        stage(even, 0);
+    for (uint32_t kb = 0; kb < kblocks; kb += 2) {
+        step(even, odd, kb);
+        if (kb + 1 < kblocks)
+            step(odd, even, kb + 1);
     }
+
+    const uint64_t col = n0 + wn + (lane >> 4) * 16;
+    if (col >= n)
+        return;
 #pragma unroll
     for (int i = 0; i < TM; ++i) {
         const uint64_t row = m0 + wm + i * 16 + (lane & 15);
         if (row >= m)
-            continue;
+            break;
+        OT *to = c + row * c_stride + col;
+        Vec<OT> o[16 / Vec<OT>::N];
 #pragma unroll
-        for (int j = 0; j < TN; ++j) {
-            const uint64_t col = n0 + wn + j * 16 + (lane >> 4) * 4;
-            OT o[4];
+        for (int e = 0; e < 16; e += 2)
+            o[e / Vec<OT>::N].put2(e % Vec<OT>::N, acc[i][e / 4][e % 4], acc[i][e / 4][e % 4 + 1]);
+        if (vector_stores && col + 16 <= n) {
 #pragma unroll
-            for (int e = 0; e < 4; ++e)
-                o[e] = from_float<OT>(acc[i][j][e]);
-            OT *to = c + row * c_stride + col;
-            if (vector_stores && col + 4 <= n) {
-                if constexpr (sizeof(OT) == 2)
-                    *reinterpret_cast<uint2 *>(to) = *reinterpret_cast<const uint2 *>(o);
-                else
-                    *reinterpret_cast<uint4 *>(to) = *reinterpret_cast<const uint4 *>(o);
-            } else {
+            for (int h = 0; h < 16 / Vec<OT>::N; ++h)
+                reinterpret_cast<Vec<OT> *>(to)[h] = o[h];
+        } else {
 #pragma unroll
-                for (int e = 0; e < 4; ++e)
-                    if (col + e < n)
-                        to[e] = o[e];
-            }
+            for (int e = 0; e < 16; ++e)
+                if (col + e < n)
+                    to[e] = o[e / Vec<OT>::N].element(e % Vec<OT>::N);
         }
     }
 }
@@ -511,7 +572,7 @@ int ung_hip_fp8_matmul(const uint8_t *a, const float *a_scale, const uint8_t *b,
         return UNG_HIP_EINVAL;
     }
     const uint64_t mt = ceil_div(m, 128), nt = ceil_div(n, 128);
-    if (m > UINT32_MAX || n > UINT32_MAX || kp / KB > UINT32_MAX || mt * nt > INT32_MAX) {
+    if (m > UINT32_MAX || n > UINT32_MAX || kp > UINT32_MAX / 256 || mt * nt > INT32_MAX) {
         set_error("ung_hip_fp8_matmul: a %llu x %llu x %llu product is too large", (unsigned long long)m,
                   (unsigned long long)n, (unsigned long long)kp);
         return UNG_HIP_EINVAL;
@@ -521,13 +582,22 @@ int ung_hip_fp8_matmul(const uint8_t *a, const float *a_scale, const uint8_t *b,
     const hipStream_t st = (hipStream_t)stream;
     return with_type(type, [&](auto zero) {
         using T = decltype(zero);
-        const int vec = (uintptr_t)c % (4 * sizeof(T)) == 0 && (m == 1 || c_stride % 4 == 0);
-        auto go = [&](auto kernel) {
-            kernel<<<(uint32_t)(mt * nt), 256, 0, st>>>(a, a_scale, b, b_scale, m, n, (uint32_t)(kp / KB), (T *)c,
-                                                        c_stride, (uint32_t)mt, (uint32_t)nt, vec);
+        const int vec = (uintptr_t)c % 16 == 0 && (m == 1 || c_stride * sizeof(T) % 16 == 0);
+        auto go = [&](auto kernel, uint32_t bm, uint32_t bn, uint32_t threads) {
+            const uint32_t mt = (uint32_t)ceil_div(m, bm), nt = (uint32_t)ceil_div(n, bn);
+            kernel<<<mt * nt, threads, 0, st>>>(a, a_scale, b, b_scale, m, n, (uint32_t)(kp / KB), (T *)c, c_stride,
+                                                mt, nt, vec);
         };
-        b_square ? go(ung_fp8_tile_product_kernel<128, 128, true, T>)
-                 : go(ung_fp8_tile_product_kernel<128, 128, false, T>);
+        if constexpr (sizeof(T) == 2) {
+            if (m > 128 && n > 128)
+                b_square ? go(ung_fp8_product_kernel<256, 256, 2, 4, true, T>, 256, 256, 512)
+                         : go(ung_fp8_product_kernel<256, 256, 2, 4, false, T>, 256, 256, 512);
+            else
+                b_square ? go(ung_fp8_product_kernel<128, 128, 2, 2, true, T>, 128, 128, 256)
+                         : go(ung_fp8_product_kernel<128, 128, 2, 2, false, T>, 128, 128, 256);
+        } else
+            b_square ? go(ung_fp8_product_kernel<128, 128, 2, 2, true, T>, 128, 128, 256)
+                     : go(ung_fp8_product_kernel<128, 128, 2, 2, false, T>, 128, 128, 256);
         return launched("ung_hip_fp8_matmul");
     });
 }
