@@ -90,7 +90,7 @@ SIGNATURES = {
     "ung_hip_debug_error_bound": (_int, [_vp, C.POINTER(_dbl), C.POINTER(_dbl), C.POINTER(_dbl), C.POINTER(_int)]),
     "ung_hip_debug_partial_bounds": (_int, [_vp, _u64, _vp, _vp, _vp, _vp, C.POINTER(_u64)]),
     "ung_hip_fp8_quantize": (_int, [_vp, _int, _u64, _u64, _u64, _int, _vp, _vp, _vp, _vp, _vp]),
-    "ung_hip_fp8_matmul_workspace": (_int, [_u64, _u64, _u64, C.POINTER(_u64)]),
+    "ung_hip_fp8_matmul_workspace": (_int, [_u64, _u64, _u64, _int, C.POINTER(_u64)]),
     "ung_hip_fp8_matmul": (_int, [_vp, _vp, _vp, _vp, _int, _u64, _u64, _u64, _vp, _int, _u64, _vp, _u64, _vp]),
     "ung_hip_top_scores_workspace": (_int, [_vp, _int, _u64, _u64, _u64, _u32, C.POINTER(_u64)]),
     "ung_hip_top_scores": (_int, [_vp, _int, _u64, _u64, _u64, _u32, C.c_float, _vp, _vp, _vp, _vp, _u64, _vp]),

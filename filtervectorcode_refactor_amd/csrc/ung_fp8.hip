@@ -7,6 +7,7 @@
 // block's scale, s = max(largest magnitude, 2^-64) * (1 / 448), rounded to 32 bits.
 #include <hip/hip_runtime.h>
 
+#include <atomic>
 #include <cstdint>
 
 #include "ung_elements.h"
@@ -286,9 +287,9 @@ __device__ inline void to_lds4(__amdgpu_buffer_rsrc_t from, uint32_t offset, uin
     __builtin_amdgcn_raw_ptr_buffer_load_lds(from, (lds_ptr)lds, 4, offset, advance, 0, 0);
 }
 
-__device__ inline __amdgpu_buffer_rsrc_t buffer_of(const void *p)
+__device__ inline __amdgpu_buffer_rsrc_t buffer_of(const void *p, uint32_t bytes = 0xFFFFFFFFu)
 {
-    return __builtin_amdgcn_make_buffer_rsrc(const_cast<void *>(p), 0, 0xFFFFFFFFu, 0x00020000);
+    return __builtin_amdgcn_make_buffer_rsrc(const_cast<void *>(p), 0, bytes, 0x00020000);
 }
 
 // Tile of the product that block `id` of `total` makes.  Blocks go to the eight XCDs in turn;
@@ -469,6 +470,419 @@ __global__ __launch_bounds__(WM * WN * 64, 2) void ung_fp8_product_kernel(const 
     }
 }
 
+// ---- large 16-bit products -------------------------------------------------------------
+
+using f32x16 = __attribute__((ext_vector_type(16))) float;
+using u32x4 = __attribute__((ext_vector_type(4))) uint32_t;
+
+template <int N>
+__device__ inline void await_loads()
+{
+    // at most N of the wave's memory operations are still under way; loads into LDS count
+    asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
+}
+
+constexpr int BIG = 256; // a tile is BIG x BIG
+
+// Work of one block: every so-manieth of its XCD's (tile, share of the inner length) items.
+struct Items {
+    uint32_t at, end, by;
+    __device__ Items(uint32_t total)
+    {
+        const uint32_t xcd = blockIdx.x & 7, each = total >> 3, extra = total & 7;
+        at = xcd * each + (xcd < extra ? xcd : extra);
+        end = at + each + (xcd < extra ? 1 : 0);
+        at += blockIdx.x >> 3;
+        by = (gridDim.x - xcd + 7) >> 3;
+    }
+};
+
+// One item: where its tile lies and which blocks of the inner length it sums.
+struct Item {
+    uint32_t m0, n0, kb, kb_end, split;
+    uint32_t live = 1; // 0: past the last item, row 0 of this one alone is loaded
+    __device__ Item(uint32_t id, uint32_t m_tiles, uint32_t n_tiles, uint32_t kblocks, uint32_t splits)
+    {
+        // shares of one tile lie far apart, tiles of one share side by side
+        const uint32_t tiles = m_tiles * n_tiles;
+        split = id / tiles;
+        const uint32_t t = id - split * tiles, band = t / (8 * n_tiles), in = t - band * 8 * n_tiles;
+        const uint32_t high = m_tiles - band * 8 < 8 ? m_tiles - band * 8 : 8;
+        m0 = one((band * 8 + in % high) * BIG);
+        n0 = one(in / high * BIG);
+        const uint32_t each = kblocks / splits, extra = kblocks - each * splits;
+        kb = one(split * each + min(split, extra));
+        kb_end = one(kb + each + (split < extra ? 1 : 0));
+        split = one(split);
+    }
+    // divisions leave a block's numbers in vector registers
+    static __device__ uint32_t one(uint32_t v) { return __builtin_amdgcn_readfirstlane(v); }
+};
+
+// A lane's 16 results (columns h * 16 + 0..15 of row r, lane = 32 h + r) among the lanes, so
+// that a store writes 64 (32-bit results: 128) neighbouring bytes of a row, not 16 each here
+// and there: halves of the wave, then quarters of it, trade the vectors that are not theirs.
+// place(): row and column of vector x after it.
+__device__ inline void trade32(uint32_t &a, uint32_t &b)
+{
+    const auto t = __builtin_amdgcn_permlane32_swap(a, b, false, false);
+    a = t[0];
+    b = t[1];
+}
+__device__ inline void trade16(uint32_t &a, uint32_t &b)
+{
+    const auto t = __builtin_amdgcn_permlane16_swap(a, b, false, false);
+    a = t[0];
+    b = t[1];
+}
+template <class T, int N>
+__device__ inline void spread(Vec<T> (&o)[N])
+{
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+        if constexpr (N == 2) {
+            trade32(o[0].w[w], o[1].w[w]); // 0: columns 0..15 (8 by half), 1: 16..31
+            trade16(o[0].w[w], o[1].w[w]); // 0: rows 0..15, 1: rows 16..31
+        } else {
+            // to pairs (0, 1), (2, 3): the wave's halves side by side
+            trade32(o[0].w[w], o[2].w[w]); // 0: columns 0..3 | 8..11, 2: 16..19 | 24..27
+            trade32(o[1].w[w], o[3].w[w]);
+            trade16(o[0].w[w], o[2].w[w]);
+            trade16(o[1].w[w], o[3].w[w]);
+        }
+    }
+}
+template <class T>
+__device__ inline void place(uint32_t lane, int x, uint32_t &row, uint32_t &col)
+{
+    const uint32_t quarter = lane >> 4 & 1, half = lane >> 5;
+    if constexpr (sizeof(T) == 2) {
+        row = (lane & 15) + x * 16;
+        col = quarter * 16 + half * 8;
+    } else {
+        row = (lane & 15) + (x >> 1) * 16;
+        col = quarter * 16 + half * 8 + (x & 1) * 4;
+    }
+}
+
+// Blocks that stay: one for each CU, eight waves, a 128 x 64 part of a 256 x 256 tile each.
+// The blocks of the inner length of all their items form one sequence of stages.  A stage is
+// worked on in two phases: b's panel (then kept in registers) with one half of a's rows, and
+// the other half.  Panels are staged in LDS by loads past the registers: what a phase frees is
+// loaded anew at the start of the next one, b and a's first half for the stage after the next,
+// a's second half for the next stage.  A phase waits only for the loads that it needs, so
+// loads flow across phases, stages and tiles, and a tile's results are stored while the next
+// one's loads are under way.
+//   32 x 32 x 64 matrix instructions: half the operand reads of the 16 x 16 x 128 ones for
+// the same work, which leaves the register file to the multiply-adds that scale one tile
+// while the next one is made.
+//   Panels lie in LDS variables of their own, and every path makes the same loads and stores
+// (at the end, loads of one row that nobody reads): so the compiler knows which loads a read
+// of LDS depends on, and adds no wait of its own.
+// SQUARE: b's scales by square.  WHOLE: results go out in groups of 16 columns, n and the
+// rows' alignment allow it; else one by one.
+template <bool SQUARE, bool WHOLE, class OT>
+__global__ __launch_bounds__(512, 2) void ung_fp8_big_product_kernel(const uint8_t *a, const float *a_scale,
+                                                                     const uint8_t *b, const float *b_scale,
+                                                                     uint32_t m, uint32_t n, uint32_t kblocks, OT *c,
+                                                                     uint64_t c_stride, uint32_t m_tiles,
+                                                                     uint32_t n_tiles, uint32_t splits)
+{
+    __shared__ alignas(16) uint8_t b_even[BIG * KB], b_odd[BIG * KB];
+    __shared__ alignas(16) uint8_t a0_even[BIG / 2 * KB], a0_odd[BIG / 2 * KB];
+    __shared__ alignas(16) uint8_t a1_even[BIG / 2 * KB], a1_odd[BIG / 2 * KB];
+    __shared__ alignas(16) float s_even[2 * BIG], s_odd[2 * BIG]; // scales of a, then of b
+    const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const uint32_t wm = wave & 1, wn = wave >> 1; // halves of m, quarters of n
+    const uint32_t kp = kblocks * KB;
+
+    // ---- loads: a wave loads rows (i * 8 + wave) * 8 + lane / 8 of a panel ----
+    const uint32_t line = wave * 8 + (lane >> 3);
+    // a row's pieces are rotated so that the 16 lanes that LDS serves at a time (4 n + 0..3 for n
+    // = 0, 3, 5, 6 or 1, 2, 4, 7 of each half wave) read 16 different groups of four banks
+    const uint32_t a_piece = ((lane & 7) ^ (line >> 1 & 7)) * 16;
+    const uint32_t b_piece = ((lane & 7) ^ ((line >> 1 & 1) | (line >> 3 & 2) | (line & 4))) * 16;
+    Items items(m_tiles * n_tiles * splits), ahead_items = items;
+    if (items.at >= items.end)
+        return;
+    Item now(items.at, m_tiles, n_tiles, kblocks, splits);
+    Item ahead = now; // the stage whose b and first half of a are loaded next
+    auto rows_of = [&](uint32_t all, uint32_t first, uint32_t live) {
+        return live ? min(all - first, (uint32_t)BIG) - 1 : 0u;
+    };
+    auto load_b = [&](uint8_t *to, int first, int end) {
+        const __amdgpu_buffer_rsrc_t from = buffer_of(b + (uint64_t)ahead.n0 * kp);
+        const uint32_t last = rows_of(n, ahead.n0, ahead.live);
+        for (int i = first; i < end; ++i)
+            to_lds16(from, min(line + i * 64, last) * kp + b_piece, ahead.kb * KB, to + (i * 8 + wave) * 1024);
+        __builtin_amdgcn_sched_barrier(0); // the waits count on the loads' order
+    };
+    auto load_a = [&](uint8_t *to, uint32_t half, const Item &of, int first, int end) {
+        const __amdgpu_buffer_rsrc_t from = buffer_of(a + (uint64_t)of.m0 * kp);
+        const uint32_t last = rows_of(m, of.m0, of.live);
+        for (int i = first; i < end; ++i)
+            to_lds16(from, min(half * 64 + line + i * 128, last) * kp + a_piece, of.kb * KB,
+                     to + (i * 8 + wave) * 1024);
+        __builtin_amdgcn_sched_barrier(0);
+    };
+    auto load_scales = [&](float *to, const Item &of) {
+        const bool of_a = wave < 4;
+        const uint32_t first = of_a ? of.m0 : SQUARE ? of.n0 / KB : of.n0;
+        const uint32_t row = min((wave & 3) * 64 + lane, of_a ? rows_of(m, of.m0, of.live) : rows_of(n, of.n0, of.live));
+        to_lds4(buffer_of((of_a ? a_scale : b_scale) + (uint64_t)first * kblocks),
+                (SQUARE && !of_a ? row / KB : row) * kblocks * 4, of.kb * 4, to + wave * 64);
+        __builtin_amdgcn_sched_barrier(0);
+    };
+    auto advance = [&]() {
+        if (ahead.live && ++ahead.kb == ahead.kb_end) {
+            ahead_items.at += ahead_items.by;
+            if (ahead_items.at < ahead_items.end)
+                ahead = Item(ahead_items.at, m_tiles, n_tiles, kblocks, splits);
+            else
+                ahead.live = ahead.kb = 0;
+        }
+    };
+
+    // ---- fragments: row lane % 32, 32 of 64 bytes by lane / 32, two halves of a block ----
+    const uint32_t r = lane & 31, h = lane >> 5, turn = ((h * 2) ^ (r >> 1 & 7)) * 16;
+    const uint32_t a_lane = (wm * 64 + r) * KB + turn;
+    const uint32_t b_lane = (wn * 64 + (r >> 2 & 1) * 16 + (r >> 3) * 4 + (r & 3)) * KB + turn;
+    struct Half {
+        Frag k[2];
+    };
+    auto fragment = [&](const uint8_t *panel, uint32_t at, uint32_t tile) {
+        Half f;
+#pragma unroll
+        for (int s = 0; s < 2; ++s)
+#pragma unroll
+            for (int x = 0; x < 2; ++x)
+                f.k[s].h[x] = *reinterpret_cast<const uint4 *>(panel + (at ^ (s * 64) ^ (x * 16)) + tile * 32 * KB);
+        return f;
+    };
+    f32x16 acc[4][2];
+    auto clear = [&]() {
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+            for (int j = 0; j < 2; ++j)
+#pragma unroll
+                for (int e = 0; e < 16; ++e)
+                    acc[i][j][e] = 0.0f;
+    };
+    Half bf[2];
+    auto phase = [&](auto which, const uint8_t *pa, const uint8_t *pb, const float *scales, auto load) {
+        constexpr int P = decltype(which)::value;
+        uint32_t a_at = a_lane, b_at = b_lane, s_at = wm * 128 + P * 64 + r, sb_at = BIG + wn * 64 + h * 16;
+        asm volatile("" : "+v"(a_at), "+v"(b_at), "+v"(s_at), "+v"(sb_at)); // made anew, not kept for every panel
+        if constexpr (P == 0) {
+#pragma unroll
+            for (int j = 0; j < 2; ++j)
+                bf[j] = fragment(pb, b_at, j);
+        }
+        Half af = fragment(pa, a_at, 0);
+        const float s_all = SQUARE ? scales[sb_at] : 1.0f;
+        float s[2];
+        s[0] = scales[s_at] * s_all;
+        s[1] = scales[s_at + 32] * s_all;
+        f32x16 q[2];
+        auto add = [&](int o) {
+            const int i = P * 2 + o / 2, j = o % 2;
+#pragma unroll
+            for (int g = 0; g < 4; ++g) {
+                f32x4 sn;
+                if (!SQUARE)
+                    sn = *reinterpret_cast<const f32x4 *>(&scales[sb_at + j * 32 + g * 4]);
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    acc[i][j][g * 4 + e] = __builtin_fmaf(q[o & 1][g * 4 + e], SQUARE ? s[o / 2] : s[o / 2] * sn[e],
+                                                          acc[i][j][g * 4 + e]);
+                if (!SQUARE)
+                    __builtin_amdgcn_sched_barrier(0); // four scales at a time: the sums need the registers
+            }
+            asm volatile("" : "+v"(acc[i][j])); // here, not after the waits and loads that follow
+        };
+#pragma unroll
+        for (int t = 0; t < 4; ++t) {
+            f32x16 z;
+#pragma unroll
+            for (int e = 0; e < 16; ++e)
+                z[e] = 0.0f;
+#pragma unroll
+            for (int k = 0; k < 2; ++k)
+                z = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(bf[t % 2].k[k].v, af.k[k].v, z, 0, 0, 0, 0x7F7F7F7F,
+                                                                     0, 0x7F7F7F7F);
+            q[t & 1] = z;
+            load(t); // a few at a time: a wave that waits for the loads' queue starts no products
+            if (t == 1)
+                af = fragment(pa, a_at, 1);
+            if (t)
+                add(t - 1);
+            __builtin_amdgcn_sched_barrier(0);
+        }
+        add(3);
+        __builtin_amdgcn_sched_barrier(0);
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); // the panels are read
+    };
+
+    auto store = [&]() {
+        const uint32_t row0 = wm * 128 + r, col0 = wn * 64 + h * 16;
+        const uint32_t rows = min(m - now.m0, (uint32_t)BIG), cols = min(n - now.n0, (uint32_t)BIG);
+        OT *tile = c + ((uint64_t)now.split * m + now.m0) * c_stride + now.n0;
+        const __amdgpu_buffer_rsrc_t to = buffer_of(tile, 0x7FFFFFFFu);
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+                const uint32_t row = row0 + i * 32, col = col0 + j * 32;
+                Vec<OT> o[16 / Vec<OT>::N];
+#pragma unroll
+                for (int e = 0; e < 16; e += 2)
+                    o[e / Vec<OT>::N].put2(e % Vec<OT>::N, acc[i][j][e], acc[i][j][e + 1]);
+                if (WHOLE) {
+                    spread(o);
+#pragma unroll
+                    for (int x = 0; x < 16 / Vec<OT>::N; ++x) {
+                        uint32_t row_x, col_x;
+                        place<OT>(lane, x, row_x, col_x);
+                        row_x += wm * 128 + i * 32;
+                        col_x += wn * 64 + j * 32;
+                        // out of range: the store is dropped
+                        const uint32_t at = row_x < rows && col_x < cols
+                                                ? (row_x * (uint32_t)c_stride + col_x) * (uint32_t)sizeof(OT)
+                                                : 0x80000000u;
+                        __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, o[x]), to, at, 0, 0);
+                    }
+                } else if (row < rows) {
+                    OT *out = tile + row * c_stride + col;
+#pragma unroll
+                    for (int e = 0; e < 16; ++e)
+                        if (col + e < cols)
+                            out[e] = o[e / Vec<OT>::N].element(e % Vec<OT>::N);
+                }
+            }
+    };
+
+    // A wave's loads in order, for a stage k: b and a's first half 6 (in the second phase of
+    // k - 2), scales 1 and a's second half 2 (in the first phase of k - 1).
+    auto stage = [&](uint8_t *pb, uint8_t *pa0, uint8_t *pa1, float *ps, uint8_t *pa1_next, float *ps_next, Item &mid) {
+        await_loads<8>(); // all but the stage's second half of a and the next one's first 6 loads
+        __builtin_amdgcn_s_barrier();
+        __builtin_amdgcn_sched_barrier(0);
+        phase(std::integral_constant<int, 0>{}, pa0, pb, ps, [&](int t) {
+            if (t == 0)
+                load_scales(ps_next, mid);
+            else if (t < 3)
+                load_a(pa1_next, 1, mid, t - 1, t);
+        });
+        await_loads<9>(); // all but the next stage's
+        __builtin_amdgcn_s_barrier();
+        __builtin_amdgcn_sched_barrier(0);
+        phase(std::integral_constant<int, 1>{}, pa1, pb, ps, [&](int t) {
+            if (t < 2)
+                load_b(pb, t * 2, t * 2 + 2);
+            else
+                load_a(pa0, 0, ahead, t - 2, t - 1);
+        });
+        mid = ahead;
+        advance();
+        if (++now.kb == now.kb_end) {
+            store();
+            items.at += items.by;
+            if (items.at < items.end) {
+                now = Item(items.at, m_tiles, n_tiles, kblocks, splits);
+                clear();
+            }
+        }
+    };
+
+    clear();
+    load_b(b_even, 0, 4);
+    load_a(a0_even, 0, ahead, 0, 2);
+    load_scales(s_even, ahead);
+    load_a(a1_even, 1, ahead, 0, 2);
+    advance();
+    load_b(b_odd, 0, 4);
+    load_a(a0_odd, 0, ahead, 0, 2);
+    Item mid = ahead;
+    advance();
+    // the number of stages ends the loop: a flag would have the two panels' stages follow
+    // themselves in the compiler's eyes
+    uint32_t left = 0;
+    for (uint32_t i = items.at; i < items.end; i += items.by) {
+        const Item item(i, m_tiles, n_tiles, kblocks, splits);
+        left += item.kb_end - item.kb;
+    }
+    for (;;) {
+        stage(b_even, a0_even, a1_even, s_even, a1_odd, s_odd, mid);
+        if (--left == 0)
+            break;
+        stage(b_odd, a0_odd, a1_odd, s_odd, a1_even, s_even, mid);
+        if (--left == 0)
+            break;
+    }
+    await_loads<0>(); // nothing may land in LDS that is another block's by then
+}
+
+// c = the sum of `splits` sets of 32-bit sums, in their order.
+template <class OT>
+__global__ __launch_bounds__(256) void ung_fp8_join_kernel(const float *part, uint32_t splits, uint64_t rows,
+                                                           uint64_t cols, uint64_t part_stride, OT *c,
+                                                           uint64_t c_stride)
+{
+    const uint64_t chunks = part_stride / 4;
+    for (uint64_t at = blockIdx.x * 256ull + threadIdx.x; at < rows * chunks; at += gridDim.x * 256ull) {
+        const uint64_t row = at / chunks, col = (at - row * chunks) * 4;
+        f32x4 sum = {0.0f, 0.0f, 0.0f, 0.0f};
+        for (uint32_t s = 0; s < splits; ++s)
+            sum += *reinterpret_cast<const f32x4 *>(part + (s * rows + row) * part_stride + col);
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+            if (col + e < cols)
+                c[row * c_stride + col + e] = from_float<OT>(sum[e]);
+    }
+}
+
+// ---- choice of the kernel ----------------------------------------------------------------
+
+// CUs of the current device, asked for once.
+uint32_t cu_count()
+{
+    static std::atomic<uint32_t> known[64];
+    int device = 0, n = 0;
+    if (hipGetDevice(&device) != hipSuccess || device < 0 || device >= 64) {
+        (void)hipGetLastError();
+        return 256;
+    }
+    uint32_t got = known[device].load(std::memory_order_relaxed);
+    if (!got) {
+        if (hipDeviceGetAttribute(&n, hipDeviceAttributeMultiprocessorCount, device) != hipSuccess || n < 8) {
+            (void)hipGetLastError();
+            n = 256;
+        }
+        known[device].store(got = (uint32_t)n, std::memory_order_relaxed);
+    }
+    return got;
+}
+
+bool big_product(uint64_t m, uint64_t n, int type) { return type != UNG_HIP_F32 && m > 128 && n > 128; }
+
+// Shares of the inner length: where the tiles do not fill the CUs, as many as fill them, each
+// of at least 8 blocks.
+uint32_t splits_of(uint64_t m, uint64_t n, uint64_t kp, int type)
+{
+    if (!big_product(m, n, type))
+        return 1;
+    const uint64_t tiles = ceil_div(m, BIG) * ceil_div(n, BIG), by_cu = cu_count() / tiles, by_k = kp / KB / 8;
+    const uint64_t splits = by_cu < by_k ? by_cu : by_k;
+    return splits > 1 ? (uint32_t)splits : 1;
+}
+
+uint64_t split_stride(uint64_t n) { return ceil_div(n, 4) * 4; }
+uint64_t split_bytes(uint64_t m, uint64_t n, uint32_t splits)
+{
+    return splits > 1 ? (uint64_t)splits * m * split_stride(n) * 4 : 0;
+}
+
 } // namespace
 
 extern "C" {
@@ -528,17 +942,14 @@ int ung_hip_fp8_quantize(const void *x, int type, uint64_t rows, uint64_t cols, 
     });
 }
 
-int ung_hip_fp8_matmul_workspace(uint64_t m, uint64_t n, uint64_t kp, uint64_t *bytes)
+int ung_hip_fp8_matmul_workspace(uint64_t m, uint64_t n, uint64_t kp, int type, uint64_t *bytes)
 {
     clear_error();
-    if (!bytes) {
-        set_error("ung_hip_fp8_matmul_workspace: null bytes");
+    if (!bytes || !known_type(type)) {
+        set_error("ung_hip_fp8_matmul_workspace: null bytes or unknown element type %d", type);
         return UNG_HIP_EINVAL;
     }
-    (void)m;
-    (void)n;
-    (void)kp;
-    *bytes = 0;
+    *bytes = split_bytes(m, n, splits_of(m, n, kp, type));
     return UNG_HIP_OK;
 }
 
@@ -572,13 +983,18 @@ int ung_hip_fp8_matmul(const uint8_t *a, const float *a_scale, const uint8_t *b,
         return UNG_HIP_EINVAL;
     }
     const uint64_t mt = ceil_div(m, 128), nt = ceil_div(n, 128);
-    if (m > UINT32_MAX || n > UINT32_MAX || kp > UINT32_MAX / 256 || mt * nt > INT32_MAX) {
+    if (m > INT32_MAX || n > INT32_MAX || kp > UINT32_MAX / 256 || mt * nt > INT32_MAX) {
         set_error("ung_hip_fp8_matmul: a %llu x %llu x %llu product is too large", (unsigned long long)m,
                   (unsigned long long)n, (unsigned long long)kp);
         return UNG_HIP_EINVAL;
     }
-    (void)workspace;
-    (void)workspace_bytes;
+    const uint32_t splits = splits_of(m, n, kp, type);
+    const uint64_t needed = split_bytes(m, n, splits);
+    if (needed && (!workspace || workspace_bytes < needed || (uintptr_t)workspace % 16)) {
+        set_error("ung_hip_fp8_matmul: needs %llu bytes of workspace at a 16-byte boundary (got %llu)",
+                  (unsigned long long)needed, (unsigned long long)(workspace ? workspace_bytes : 0));
+        return UNG_HIP_EINVAL;
+    }
     const hipStream_t st = (hipStream_t)stream;
     return with_type(type, [&](auto zero) {
         using T = decltype(zero);
@@ -589,9 +1005,35 @@ int ung_hip_fp8_matmul(const uint8_t *a, const float *a_scale, const uint8_t *b,
                                                 mt, nt, vec);
         };
         if constexpr (sizeof(T) == 2) {
-            if (m > 128 && n > 128)
-                b_square ? go(ung_fp8_product_kernel<256, 256, 2, 4, true, T>, 256, 256, 512)
-                         : go(ung_fp8_product_kernel<256, 256, 2, 4, false, T>, 256, 256, 512);
+            if (big_product(m, n, type)) {
+                const uint32_t tm = (uint32_t)ceil_div(m, BIG), tn = (uint32_t)ceil_div(n, BIG);
+                const uint32_t items = tm * tn * splits, grid = items < cu_count() ? items : cu_count();
+                auto run = [&](auto kernel, auto *to, uint64_t stride) {
+                    kernel<<<grid, 512, 0, st>>>(a, a_scale, b, b_scale, (uint32_t)m, (uint32_t)n, (uint32_t)(kp / KB),
+                                                 to, stride, tm, tn, splits);
+                };
+                const bool whole = vec && n % 16 == 0 && c_stride < (1u << 21);
+                if (splits == 1) {
+                    if (b_square)
+                        whole ? run(ung_fp8_big_product_kernel<true, true, T>, (T *)c, c_stride)
+                              : run(ung_fp8_big_product_kernel<true, false, T>, (T *)c, c_stride);
+                    else
+                        whole ? run(ung_fp8_big_product_kernel<false, true, T>, (T *)c, c_stride)
+                              : run(ung_fp8_big_product_kernel<false, false, T>, (T *)c, c_stride);
+                } else {
+                    const uint64_t stride = split_stride(n);
+                    float *part = (float *)workspace;
+                    if (n % 16 == 0 && stride < (1u << 21))
+                        b_square ? run(ung_fp8_big_product_kernel<true, true, float>, part, stride)
+                                 : run(ung_fp8_big_product_kernel<false, true, float>, part, stride);
+                    else
+                        b_square ? run(ung_fp8_big_product_kernel<true, false, float>, part, stride)
+                                 : run(ung_fp8_big_product_kernel<false, false, float>, part, stride);
+                    const uint64_t blocks = ceil_div(m * (stride / 4), 256);
+                    ung_fp8_join_kernel<T><<<(uint32_t)(blocks < 4096 ? blocks : 4096), 256, 0, st>>>(
+                        part, splits, m, n, stride, (T *)c, c_stride);
+                }
+            }
             else
                 b_square ? go(ung_fp8_product_kernel<128, 128, 2, 2, true, T>, 128, 128, 256)
                          : go(ung_fp8_product_kernel<128, 128, 2, 2, false, T>, 128, 128, 256);

@@ -161,7 +161,7 @@ def matmul_fp8(a, a_scale, b, b_scale, dtype=torch.bfloat16):
     c = torch.empty(m, n, dtype=dtype, device=a.device)
     lib = _library()
     with _On(a) as stream:
-        keep, at, size = _workspace(lib.ung_hip_fp8_matmul_workspace, m, n, kp, device=a.device)
+        keep, at, size = _workspace(lib.ung_hip_fp8_matmul_workspace, m, n, kp, _TYPES[dtype], device=a.device)
         check(lib.ung_hip_fp8_matmul(a.data_ptr(), a_scale.data_ptr(), b.data_ptr(), b_scale.data_ptr(), square, m, n,
                                      kp, c.data_ptr(), _TYPES[dtype], n, at, size, stream))
     return c

@@ -350,7 +350,7 @@ int ung_hip_fp8_quantize(const void *x, int type, uint64_t rows, uint64_t cols, 
  * scales (b_square = 0) or square ones (b_square = 1: b_scale[j / 128][t]).  Gradients of the
  * product are products of the same kind: with the upstream gradient g quantised both ways,
  * da = g (b^T)^T by the turned b, db = g^T (a^T)^T by the turned g and a. */
-int ung_hip_fp8_matmul_workspace(uint64_t m, uint64_t n, uint64_t kp, uint64_t *bytes);
+int ung_hip_fp8_matmul_workspace(uint64_t m, uint64_t n, uint64_t kp, int type, uint64_t *bytes);
 int ung_hip_fp8_matmul(const uint8_t *a, const float *a_scale, const uint8_t *b, const float *b_scale, int b_square,
                        uint64_t m, uint64_t n, uint64_t kp, void *c, int type, uint64_t c_stride, void *workspace,
                        uint64_t workspace_bytes, void *stream);

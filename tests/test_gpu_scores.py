@@ -170,7 +170,7 @@ def test_product_into_wider_rows(m, n, pad):
     qb, sb, b = _operand(n, 256, "square", g)
     c = torch.full((m, n + pad), -5.0, device="cuda")
     lib = F.load()
-    keep, at, size = S._workspace(lib.ung_hip_fp8_matmul_workspace, m, n, 256, device="cuda")
+    keep, at, size = S._workspace(lib.ung_hip_fp8_matmul_workspace, m, n, 256, 0, device="cuda")
     rc = lib.ung_hip_fp8_matmul(qa.data_ptr(), sa.data_ptr(), qb.data_ptr(), sb.data_ptr(), 1, m, n, 256, c.data_ptr(),
                                 0, n + pad, at, size, torch.cuda.current_stream().cuda_stream)
     assert rc == 0

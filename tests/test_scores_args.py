@@ -43,7 +43,7 @@ def test_matmul():
     _refused(f(P + 1, P, P, P, 0, 4, 4, 128, P, 0, 4, None, 0, None), "alignment")
     _refused(f(P, P, P, P, 0, 1 << 33, 4, 128, P, 0, 4, None, 0, None), "too large")
     assert f(None, None, None, None, 0, 0, 4, 128, None, 0, 4, None, 0, None) == 0
-    _refused(F.load().ung_hip_fp8_matmul_workspace(4, 4, 128, None), "null")
+    _refused(F.load().ung_hip_fp8_matmul_workspace(4, 4, 128, 0, None), "null")
 
 
 def test_top_scores():
