@@ -483,17 +483,45 @@ __device__ inline void await_loads()
 }
 
 constexpr int BIG = 256; // a tile is BIG x BIG
+// Tiles of m that follow each other before the next one of n.  The tiles that an XCD works on
+// at a time share their panels in its L2, best in a square; but wide rows of c a power of two
+// apart lie in the same few memory channels, so these tiles should span many columns.  4096 x
+// 32768 x 768: 16: 209, 8: 218, 4: 150, 2: 144, 1: 152 us; 8192 x 8192 x 8192: 520, 502, 497,
+// 515, 553 us.
+constexpr uint32_t BAND = 4;
 
-// Work of one block: every so-manieth of its XCD's (tile, share of the inner length) items.
+// Divisions leave a block's numbers in vector registers.
+__device__ inline uint32_t uniform(uint32_t v) { return __builtin_amdgcn_readfirstlane(v); }
+
+// Work of one block: one (tile, share of the inner length) item in each round of its XCD's
+// run of items.  XCDs begin in different rounds: in the same one they would write columns a
+// power of two apart at a time, which lie in the same few memory channels.
 struct Items {
-    uint32_t at, end, by;
+    uint32_t first, count, by, local, rounds, round, left, id;
     __device__ Items(uint32_t total)
     {
         const uint32_t xcd = blockIdx.x & 7, each = total >> 3, extra = total & 7;
-        at = xcd * each + (xcd < extra ? xcd : extra);
-        end = at + each + (xcd < extra ? 1 : 0);
-        at += blockIdx.x >> 3;
+        first = xcd * each + (xcd < extra ? xcd : extra);
+        count = each + (xcd < extra ? 1 : 0);
         by = (gridDim.x - xcd + 7) >> 3;
+        local = blockIdx.x >> 3;
+        rounds = uniform((count + by - 1) / by);
+        left = local < count ? uniform((count - local + by - 1) / by) : 0;
+        round = left ? uniform(xcd % rounds) : 0;
+        settle();
+    }
+    __device__ void settle() // past a last round that has no item for this block
+    {
+        if (local + round * by >= count)
+            round = 0;
+        id = first + local + round * by;
+    }
+    __device__ void next()
+    {
+        if (--left) {
+            round = round + 1 == rounds ? 0 : round + 1;
+            settle();
+        }
     }
 };
 
@@ -506,17 +534,15 @@ struct Item {
         // shares of one tile lie far apart, tiles of one share side by side
         const uint32_t tiles = m_tiles * n_tiles;
         split = id / tiles;
-        const uint32_t t = id - split * tiles, band = t / (8 * n_tiles), in = t - band * 8 * n_tiles;
-        const uint32_t high = m_tiles - band * 8 < 8 ? m_tiles - band * 8 : 8;
-        m0 = one((band * 8 + in % high) * BIG);
-        n0 = one(in / high * BIG);
+        const uint32_t t = id - split * tiles, band = t / (BAND * n_tiles), in = t - band * BAND * n_tiles;
+        const uint32_t high = m_tiles - band * BAND < BAND ? m_tiles - band * BAND : BAND;
+        m0 = uniform((band * BAND + in % high) * BIG);
+        n0 = uniform(in / high * BIG);
         const uint32_t each = kblocks / splits, extra = kblocks - each * splits;
-        kb = one(split * each + min(split, extra));
-        kb_end = one(kb + each + (split < extra ? 1 : 0));
-        split = one(split);
+        kb = uniform(split * each + min(split, extra));
+        kb_end = uniform(kb + each + (split < extra ? 1 : 0));
+        split = uniform(split);
     }
-    // divisions leave a block's numbers in vector registers
-    static __device__ uint32_t one(uint32_t v) { return __builtin_amdgcn_readfirstlane(v); }
 };
 
 // A lane's 16 results (columns h * 16 + 0..15 of row r, lane = 32 h + r) among the lanes, so
@@ -603,9 +629,9 @@ __global__ __launch_bounds__(512, 2) void ung_fp8_big_product_kernel(const uint8
     const uint32_t a_piece = ((lane & 7) ^ (line >> 1 & 7)) * 16;
     const uint32_t b_piece = ((lane & 7) ^ ((line >> 1 & 1) | (line >> 3 & 2) | (line & 4))) * 16;
     Items items(m_tiles * n_tiles * splits), ahead_items = items;
-    if (items.at >= items.end)
+    if (!items.left)
         return;
-    Item now(items.at, m_tiles, n_tiles, kblocks, splits);
+    Item now(items.id, m_tiles, n_tiles, kblocks, splits);
     Item ahead = now; // the stage whose b and first half of a are loaded next
     auto rows_of = [&](uint32_t all, uint32_t first, uint32_t live) {
         return live ? min(all - first, (uint32_t)BIG) - 1 : 0u;
@@ -635,9 +661,9 @@ __global__ __launch_bounds__(512, 2) void ung_fp8_big_product_kernel(const uint8
     };
     auto advance = [&]() {
         if (ahead.live && ++ahead.kb == ahead.kb_end) {
-            ahead_items.at += ahead_items.by;
-            if (ahead_items.at < ahead_items.end)
-                ahead = Item(ahead_items.at, m_tiles, n_tiles, kblocks, splits);
+            ahead_items.next();
+            if (ahead_items.left)
+                ahead = Item(ahead_items.id, m_tiles, n_tiles, kblocks, splits);
             else
                 ahead.live = ahead.kb = 0;
         }
@@ -787,9 +813,9 @@ __global__ __launch_bounds__(512, 2) void ung_fp8_big_product_kernel(const uint8
         advance();
         if (++now.kb == now.kb_end) {
             store();
-            items.at += items.by;
-            if (items.at < items.end) {
-                now = Item(items.at, m_tiles, n_tiles, kblocks, splits);
+            items.next();
+            if (items.left) {
+                now = Item(items.id, m_tiles, n_tiles, kblocks, splits);
                 clear();
             }
         }
@@ -808,8 +834,8 @@ __global__ __launch_bounds__(512, 2) void ung_fp8_big_product_kernel(const uint8
     // the number of stages ends the loop: a flag would have the two panels' stages follow
     // themselves in the compiler's eyes
     uint32_t left = 0;
-    for (uint32_t i = items.at; i < items.end; i += items.by) {
-        const Item item(i, m_tiles, n_tiles, kblocks, splits);
+    for (Items i = items; i.left; i.next()) {
+        const Item item(i.id, m_tiles, n_tiles, kblocks, splits);
         left += item.kb_end - item.kb;
     }
     for (;;) {
