@@ -292,18 +292,25 @@ __device__ inline __amdgpu_buffer_rsrc_t buffer_of(const void *p, uint32_t bytes
     return __builtin_amdgcn_make_buffer_rsrc(const_cast<void *>(p), 0, bytes, 0x00020000);
 }
 
-// Tile of the product that block `id` of `total` makes.  Blocks go to the eight XCDs in turn;
-// each XCD takes a contiguous run of the tiles, in bands of 8 tiles of m, so that the tiles it
-// works on at a time share their panels in its L2.
-__device__ inline void tile_of(uint32_t id, uint32_t m_tiles, uint32_t n_tiles, uint32_t &tm, uint32_t &tn)
-{
-    const uint32_t total = m_tiles * n_tiles, xcd = id & 7, each = total >> 3, extra = total & 7;
-    const uint32_t t = xcd * each + (xcd < extra ? xcd : extra) + (id >> 3);
-    const uint32_t band = t / (8 * n_tiles), in = t - band * 8 * n_tiles;
-    const uint32_t high = m_tiles - band * 8 < 8 ? m_tiles - band * 8 : 8;
-    tm = band * 8 + in % high;
-    tn = in / high;
-}
+// What block `id` makes: a tile of the product, and which share of the inner length's blocks it
+// sums.  Blocks go to the eight XCDs in turn; each XCD takes a contiguous run of them, in bands
+// of 8 tiles of m, so that the tiles it works on at a time share their panels in its L2.
+struct Place {
+    uint32_t tm, tn, split, kb, kb_end;
+    __device__ Place(uint32_t id, uint32_t m_tiles, uint32_t n_tiles, uint32_t kblocks, uint32_t splits)
+    {
+        const uint32_t tiles = m_tiles * n_tiles, total = tiles * splits, xcd = id & 7, each = total >> 3;
+        const uint32_t extra = total & 7, item = xcd * each + (xcd < extra ? xcd : extra) + (id >> 3);
+        split = item / tiles;
+        const uint32_t t = item - split * tiles, band = t / (8 * n_tiles), in = t - band * 8 * n_tiles;
+        const uint32_t high = m_tiles - band * 8 < 8 ? m_tiles - band * 8 : 8;
+        tm = band * 8 + in % high;
+        tn = in / high;
+        const uint32_t share = kblocks / splits, longer = kblocks - share * splits;
+        kb = split * share + min(split, longer);
+        kb_end = kb + share + (split < longer ? 1 : 0);
+    }
+};
 
 // A block of WM x WN waves makes a BM x BN tile of the product, each wave BM / WM x 64 of it.
 // Per 128-byte block of the inner length both tiles are staged in LDS by loads that bypass the
@@ -314,61 +321,61 @@ __device__ inline void tile_of(uint32_t id, uint32_t m_tiles, uint32_t n_tiles, 
 // the scales, so sums and scales stay in 32 bits.  The table side (b) is the matrix
 // instruction's row side, its 64 rows spread over four instructions so that a lane ends with
 // 16 neighbouring columns of one row of c, and with one scale of a.
-template <int BM, int BN, int WM, int WN, bool SQUARE, class OT>
+//   EXACT: products in 32 bits.  The sums of a share go to its own m rows of c.
+template <int BM, int BN, int WM, int WN, bool EXACT, bool SQUARE, class OT>
 __global__ __launch_bounds__(WM * WN * 64, 2) void ung_fp8_product_kernel(const uint8_t *a, const float *a_scale,
                                                                           const uint8_t *b, const float *b_scale,
                                                                           uint64_t m, uint64_t n, uint32_t kblocks,
                                                                           OT *c, uint64_t c_stride, uint32_t m_tiles,
-                                                                          uint32_t n_tiles, int vector_stores)
+                                                                          uint32_t n_tiles, uint32_t splits,
+                                                                          int vector_stores)
 {
-    constexpr int WAVES = WM * WN, TM = BM / WM / 16, TN = 4, DEEP = 3;
-    static_assert(BN / WN == 64 && BM / 8 % WAVES == 0 && BN / 8 % WAVES == 0 && (BM + BN) / 64 <= WAVES, "");
+    constexpr int WAVES = WM * WN, TM = BM / WM / 16, TN = 4, DEEP = 3, SA = (BM + 63) / 64, SB = BN / 64;
+    static_assert(BN / WN == 64 && BM / 8 % WAVES == 0 && BN / 8 % WAVES == 0 && BM % (16 * WM) == 0, "");
     struct Panels {
         alignas(16) uint8_t a[BM * KB], b[BN * KB];
-        float sa[BM], sb[BN];
+        float sa[SA * 64], sb[BN];
     };
     __shared__ Panels even, odd;
     const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const uint32_t wm = (wave % WM) * (BM / WM), wn = (wave / WM) * 64;
-    uint32_t tm, tn;
-    tile_of(blockIdx.x, m_tiles, n_tiles, tm, tn);
-    const uint64_t m0 = (uint64_t)tm * BM, n0 = (uint64_t)tn * BN, kp = (uint64_t)kblocks * KB;
+    const Place at(blockIdx.x, m_tiles, n_tiles, kblocks, splits);
+    const uint64_t m0 = (uint64_t)at.tm * BM, n0 = (uint64_t)at.tn * BN, kp = (uint64_t)kblocks * KB;
     // rows past the end repeat the last one; their results are not stored
     const uint32_t last_m = (uint32_t)min(m - m0, (uint64_t)BM) - 1, last_n = (uint32_t)min(n - n0, (uint64_t)BN) - 1;
 
-    // staging: each wave loads every WAVES-th group of 8 rows, then 64 scales of a or b
+    // staging: each wave loads every WAVES-th group of 8 rows, and of 64 scales of a, then of b
     const __amdgpu_buffer_rsrc_t a_from = buffer_of(a + m0 * kp), b_from = buffer_of(b + n0 * kp);
-    static_assert(8 * WAVES % 32 == 0, ""); // a lane's rotation is the same in all its groups
     const uint32_t line = wave * 8 + (lane >> 3);
-    const uint32_t a_piece = ((lane & 7) ^ (line & 7)) * 16;
-    const uint32_t b_piece = ((lane & 7) ^ ((line & 3) | (line >> 2 & 4))) * 16;
-    const bool of_a = wave < BM / 64, of_b = !of_a && wave < (BM + BN) / 64;
-    const __amdgpu_buffer_rsrc_t s_from =
-        buffer_of(of_a ? a_scale + m0 * kblocks : b_scale + (SQUARE ? n0 / KB : n0) * kblocks);
-    const uint32_t s_row = (of_a ? wave : wave - BM / 64) * 64;
-    const uint32_t s_line = min(s_row + lane, of_a ? last_m : last_n);
-    const uint32_t s_at = (SQUARE && !of_a ? s_line / KB : s_line) * kblocks * 4;
+    auto a_piece = [&](uint32_t row) { return ((lane & 7) ^ (row & 7)) * 16; };
+    auto b_piece = [&](uint32_t row) { return ((lane & 7) ^ ((row & 3) | (row >> 2 & 4))) * 16; };
+    const __amdgpu_buffer_rsrc_t sa_from = buffer_of(a_scale + m0 * kblocks);
+    const __amdgpu_buffer_rsrc_t sb_from = buffer_of(b_scale + (SQUARE ? n0 / KB : n0) * kblocks);
     auto stage = [&](Panels &to, uint32_t kb) {
         uint32_t l = line;
         asm volatile("" : "+v"(l)); // offsets are made anew: the sums need the registers
 #pragma unroll
-        for (int i = 0; i < BM / 8 / WAVES; ++i)
-            to_lds16(a_from, min(l + i * WAVES * 8, last_m) * (uint32_t)kp + a_piece, kb * KB,
-                     to.a + (i * WAVES + wave) * 1024);
+        for (int i = 0; i < BM / 8 / WAVES; ++i) {
+            const uint32_t row = l + i * WAVES * 8;
+            to_lds16(a_from, min(row, last_m) * (uint32_t)kp + a_piece(row), kb * KB, to.a + (i * WAVES + wave) * 1024);
+        }
 #pragma unroll
-        for (int i = 0; i < BN / 8 / WAVES; ++i)
-            to_lds16(b_from, min(l + i * WAVES * 8, last_n) * (uint32_t)kp + b_piece, kb * KB,
-                     to.b + (i * WAVES + wave) * 1024);
-        if (of_a)
-            to_lds4(s_from, s_at, kb * 4, to.sa + s_row);
-        else if (of_b)
-            to_lds4(s_from, s_at, kb * 4, to.sb + s_row);
+        for (int i = 0; i < BN / 8 / WAVES; ++i) {
+            const uint32_t row = l + i * WAVES * 8;
+            to_lds16(b_from, min(row, last_n) * (uint32_t)kp + b_piece(row), kb * KB, to.b + (i * WAVES + wave) * 1024);
+        }
+        for (uint32_t i = wave; i < SA + SB; i += WAVES) {
+            const bool of_a = i < SA;
+            const uint32_t first = (of_a ? i : i - SA) * 64, row = min(first + lane, of_a ? last_m : last_n);
+            to_lds4(of_a ? sa_from : sb_from, (SQUARE && !of_a ? row / KB : row) * kblocks * 4, kb * 4,
+                    (of_a ? to.sa : to.sb) + first);
+        }
     };
 
     // a lane's place in the panels: pieces g and g + 4 of its row (they differ in bit 6)
     const uint32_t r = lane & 15, g = lane >> 4, b_row = wn + (r >> 2) * 16 + (r & 3);
     const uint32_t a_lane = (wm + r) * KB + (g ^ (r & 7)) * 16, b_lane = b_row * KB + (g ^ (r & 7)) * 16;
-    using Part = std::conditional_t<sizeof(OT) == 4, Wide, Frag>;
+    using Part = std::conditional_t<EXACT, Wide, Frag>;
 
     f32x4 acc[TM][TN];
 #pragma unroll
@@ -386,7 +393,7 @@ __global__ __launch_bounds__(WM * WN * 64, 2) void ung_fp8_product_kernel(const 
             Frag f;
             f.h[0] = *reinterpret_cast<const uint4 *>(lo);
             f.h[1] = *reinterpret_cast<const uint4 *>(hi);
-            if constexpr (sizeof(OT) == 4)
+            if constexpr (EXACT)
                 return widen(f);
             else
                 return f;
@@ -431,16 +438,16 @@ __global__ __launch_bounds__(WM * WN * 64, 2) void ung_fp8_product_kernel(const 
         // loads into LDS are counted as memory loads, which a barrier alone does not await
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
         __syncthreads(); // `now` has landed; every wave is done with `next`
-        if (kb + 1 < kblocks)
+        if (kb + 1 < at.kb_end)
             stage(next, kb + 1);
         multiply(now);
     };
 
-    if (kblocks)
-        stage(even, 0);
-    for (uint32_t kb = 0; kb < kblocks; kb += 2) {
+    if (at.kb < at.kb_end)
+        stage(even, at.kb);
+    for (uint32_t kb = at.kb; kb < at.kb_end; kb += 2) {
         step(even, odd, kb);
-        if (kb + 1 < kblocks)
+        if (kb + 1 < at.kb_end)
             step(odd, even, kb + 1);
     }
 
@@ -452,7 +459,7 @@ __global__ __launch_bounds__(WM * WN * 64, 2) void ung_fp8_product_kernel(const 
         const uint64_t row = m0 + wm + i * 16 + (lane & 15);
         if (row >= m)
             break;
-        OT *to = c + row * c_stride + col;
+        OT *to = c + (at.split * m + row) * c_stride + col;
         Vec<OT> o[16 / Vec<OT>::N];
 #pragma unroll
         for (int e = 0; e < 16; e += 2)
@@ -605,8 +612,8 @@ __device__ inline void place(uint32_t lane, int x, uint32_t &row, uint32_t &col)
 //   Panels lie in LDS variables of their own, and every path makes the same loads and stores
 // (at the end, loads of one row that nobody reads): so the compiler knows which loads a read
 // of LDS depends on, and adds no wait of its own.
-// SQUARE: b's scales by square.  WHOLE: results go out in groups of 16 columns, n and the
-// rows' alignment allow it; else one by one.
+// SQUARE: b's scales by square.  WHOLE: results go out in vectors of 16 bytes, n and the rows'
+// alignment allow it; else one by one.
 template <bool SQUARE, bool WHOLE, class OT>
 __global__ __launch_bounds__(512, 2) void ung_fp8_big_product_kernel(const uint8_t *a, const float *a_scale,
                                                                      const uint8_t *b, const float *b_scale,
@@ -752,7 +759,9 @@ __global__ __launch_bounds__(512, 2) void ung_fp8_big_product_kernel(const uint8
 
     auto store = [&]() {
         const uint32_t row0 = wm * 128 + r, col0 = wn * 64 + h * 16;
-        const uint32_t rows = min(m - now.m0, (uint32_t)BIG), cols = min(n - now.n0, (uint32_t)BIG);
+        const uint32_t rows = min(m - now.m0, (uint32_t)BIG);
+        // rows of shares are whole vectors long: what lies past n is not read again
+        const uint32_t cols = min((sizeof(OT) == 4 ? (n + 3) / 4 * 4 : n) - now.n0, (uint32_t)BIG);
         OT *tile = c + ((uint64_t)now.split * m + now.m0) * c_stride + now.n0;
         const __amdgpu_buffer_rsrc_t to = buffer_of(tile, 0x7FFFFFFFu);
 #pragma unroll
@@ -890,17 +899,45 @@ uint32_t cu_count()
     return got;
 }
 
-bool big_product(uint64_t m, uint64_t n, int type) { return type != UNG_HIP_F32 && m > 128 && n > 128; }
+// How a product is made: by tiles of BIG x BIG, of 128 x 128, or (few rows) of 32 x 128, and
+// from how many shares of the inner length.
+struct Plan {
+    bool big, few;
+    uint32_t splits;
+};
 
-// Shares of the inner length: where the tiles do not fill the CUs, as many as fill them, each
-// of at least 8 blocks.
-uint32_t splits_of(uint64_t m, uint64_t n, uint64_t kp, int type)
+// BIG tiles where they keep five of eight CUs busy over all rounds: their kernel reaches 2200
+// TFLOP/s, the 128 x 128 one 1400 with four times as many tiles to spread.  Measured both ways,
+// us: 4096 x 32768 x 768 134 against 155, 4096 x 4096 x 768 21.5, 24.3, 5120 x 5120 x 1024 40.2,
+// 43.4; below the bound 2500 x 3500 x 4096 (55 %) 94, 84, 2048 x 2048 x 2048 (25 %) 37, 16,
+// 300 x 1000 x 128 6.7, 4.8.
+// Tiles of 32 rows for up to 32 rows: 1 x 1000000 x 384 in 32 bits 84 against 135, 16 x 32768
+// x 768 5.6, 6.9, 1 x 10000 x 128 3.5, 3.9.
+// Shares where tiles leave CUs free: at least four, or the pass that joins them costs what they
+// save (1024 x 1024 x 2048 in two 18.5 against 14.0), of at least 8 blocks (BIG: 32, 4096 x 768
+// x 8192 in shares of 16 54 against 49).  150 x 150 x 65536 33 against 328 in one, 4096 x 768 x
+// 32768 129 against 175.
+Plan plan_of(uint64_t m, uint64_t n, uint64_t kp, int type)
 {
-    if (!big_product(m, n, type))
-        return 1;
-    const uint64_t tiles = ceil_div(m, BIG) * ceil_div(n, BIG), by_cu = cu_count() / tiles, by_k = kp / KB / 8;
-    const uint64_t splits = by_cu < by_k ? by_cu : by_k;
-    return splits > 1 ? (uint32_t)splits : 1;
+    const uint64_t kblocks = kp / KB, cus = cu_count();
+    auto shares = [&](uint64_t tiles, uint64_t places, uint64_t least) {
+        const uint64_t by_place = places / tiles, by_k = kblocks / least, s = by_place < by_k ? by_place : by_k;
+        return s >= 4 ? (uint32_t)s : 1u;
+    };
+    Plan p = {false, false, 1};
+    if (m == 0 || n == 0 || kblocks == 0) // (a product of no length: 128 x 128 tiles of zeros)
+        return p;
+    if (type != UNG_HIP_F32 && m > 128 && n > 128) {
+        const uint64_t tiles = ceil_div(m, BIG) * ceil_div(n, BIG);
+        p.splits = shares(tiles, cus, 32);
+        const uint64_t items = tiles * p.splits;
+        p.big = items * 8 > ceil_div(items, cus) * cus * 5;
+        if (p.big)
+            return p;
+    }
+    p.few = m <= 32;
+    p.splits = shares(ceil_div(m, p.few ? 32 : 128) * ceil_div(n, 128), 2 * cus, 8);
+    return p;
 }
 
 uint64_t split_stride(uint64_t n) { return ceil_div(n, 4) * 4; }
@@ -975,7 +1012,7 @@ int ung_hip_fp8_matmul_workspace(uint64_t m, uint64_t n, uint64_t kp, int type, 
         set_error("ung_hip_fp8_matmul_workspace: null bytes or unknown element type %d", type);
         return UNG_HIP_EINVAL;
     }
-    *bytes = split_bytes(m, n, splits_of(m, n, kp, type));
+    *bytes = split_bytes(m, n, plan_of(m, n, kp, type).splits);
     return UNG_HIP_OK;
 }
 
@@ -1014,7 +1051,8 @@ int ung_hip_fp8_matmul(const uint8_t *a, const float *a_scale, const uint8_t *b,
                   (unsigned long long)n, (unsigned long long)kp);
         return UNG_HIP_EINVAL;
     }
-    const uint32_t splits = splits_of(m, n, kp, type);
+    const Plan plan = plan_of(m, n, kp, type);
+    const uint32_t splits = plan.splits;
     const uint64_t needed = split_bytes(m, n, splits);
     if (needed && (!workspace || workspace_bytes < needed || (uintptr_t)workspace % 16)) {
         set_error("ung_hip_fp8_matmul: needs %llu bytes of workspace at a 16-byte boundary (got %llu)",
@@ -1024,48 +1062,47 @@ int ung_hip_fp8_matmul(const uint8_t *a, const float *a_scale, const uint8_t *b,
     const hipStream_t st = (hipStream_t)stream;
     return with_type(type, [&](auto zero) {
         using T = decltype(zero);
-        const int vec = (uintptr_t)c % 16 == 0 && (m == 1 || c_stride * sizeof(T) % 16 == 0);
-        auto go = [&](auto kernel, uint32_t bm, uint32_t bn, uint32_t threads) {
-            const uint32_t mt = (uint32_t)ceil_div(m, bm), nt = (uint32_t)ceil_div(n, bn);
-            kernel<<<mt * nt, threads, 0, st>>>(a, a_scale, b, b_scale, m, n, (uint32_t)(kp / KB), (T *)c, c_stride,
-                                                mt, nt, vec);
-        };
-        if constexpr (sizeof(T) == 2) {
-            if (big_product(m, n, type)) {
-                const uint32_t tm = (uint32_t)ceil_div(m, BIG), tn = (uint32_t)ceil_div(n, BIG);
-                const uint32_t items = tm * tn * splits, grid = items < cu_count() ? items : cu_count();
-                auto run = [&](auto kernel, auto *to, uint64_t stride) {
-                    kernel<<<grid, 512, 0, st>>>(a, a_scale, b, b_scale, (uint32_t)m, (uint32_t)n, (uint32_t)(kp / KB),
-                                                 to, stride, tm, tn, splits);
-                };
-                const bool whole = vec && n % 16 == 0 && c_stride < (1u << 21);
-                if (splits == 1) {
-                    if (b_square)
-                        whole ? run(ung_fp8_big_product_kernel<true, true, T>, (T *)c, c_stride)
-                              : run(ung_fp8_big_product_kernel<true, false, T>, (T *)c, c_stride);
-                    else
-                        whole ? run(ung_fp8_big_product_kernel<false, true, T>, (T *)c, c_stride)
-                              : run(ung_fp8_big_product_kernel<false, false, T>, (T *)c, c_stride);
-                } else {
-                    const uint64_t stride = split_stride(n);
-                    float *part = (float *)workspace;
-                    if (n % 16 == 0 && stride < (1u << 21))
-                        b_square ? run(ung_fp8_big_product_kernel<true, true, float>, part, stride)
-                                 : run(ung_fp8_big_product_kernel<false, true, float>, part, stride);
-                    else
-                        b_square ? run(ung_fp8_big_product_kernel<true, false, float>, part, stride)
-                                 : run(ung_fp8_big_product_kernel<false, false, float>, part, stride);
-                    const uint64_t blocks = ceil_div(m * (stride / 4), 256);
-                    ung_fp8_join_kernel<T><<<(uint32_t)(blocks < 4096 ? blocks : 4096), 256, 0, st>>>(
-                        part, splits, m, n, stride, (T *)c, c_stride);
+        const bool vec = (uintptr_t)c % 16 == 0 && (m == 1 || c_stride * sizeof(T) % 16 == 0);
+        // `to` is c, or (splits > 1) the shares' sums
+        auto make = [&](auto *to, uint64_t stride, bool vectors) {
+            using OT = std::remove_reference_t<decltype(*to)>;
+            constexpr bool EXACT = sizeof(T) == 4;
+            auto run = [&](auto kernel, uint32_t bm, uint32_t bn, uint32_t grid, uint32_t threads, auto... last) {
+                const uint32_t tm = (uint32_t)ceil_div(m, bm), tn = (uint32_t)ceil_div(n, bn), items = tm * tn * splits;
+                kernel<<<items < grid ? items : grid, threads, 0, st>>>(a, a_scale, b, b_scale, m, n,
+                                                                        (uint32_t)(kp / KB), to, stride, tm, tn, splits,
+                                                                        last...);
+            };
+            if constexpr (!EXACT) {
+                if (plan.big) {
+                    auto big = [&](auto kernel) { run(kernel, BIG, BIG, cu_count(), 512); };
+                    bool whole = true; // shares' sums: rows of whole vectors, and not that many columns
+                    if constexpr (sizeof(OT) == 2)
+                        whole = vectors && n % Vec<T>::N == 0 && stride < (1u << 21);
+                    if (whole)
+                        b_square ? big(ung_fp8_big_product_kernel<true, true, OT>)
+                                 : big(ung_fp8_big_product_kernel<false, true, OT>);
+                    else if constexpr (sizeof(OT) == 2)
+                        b_square ? big(ung_fp8_big_product_kernel<true, false, OT>)
+                                 : big(ung_fp8_big_product_kernel<false, false, OT>);
+                    return;
                 }
             }
+            if (plan.few)
+                b_square ? run(ung_fp8_product_kernel<32, 128, 1, 2, EXACT, true, OT>, 32, 128, ~0u, 128, vectors)
+                         : run(ung_fp8_product_kernel<32, 128, 1, 2, EXACT, false, OT>, 32, 128, ~0u, 128, vectors);
             else
-                b_square ? go(ung_fp8_product_kernel<128, 128, 2, 2, true, T>, 128, 128, 256)
-                         : go(ung_fp8_product_kernel<128, 128, 2, 2, false, T>, 128, 128, 256);
-        } else
-            b_square ? go(ung_fp8_product_kernel<128, 128, 2, 2, true, T>, 128, 128, 256)
-                     : go(ung_fp8_product_kernel<128, 128, 2, 2, false, T>, 128, 128, 256);
+                b_square ? run(ung_fp8_product_kernel<128, 128, 2, 2, EXACT, true, OT>, 128, 128, ~0u, 256, vectors)
+                         : run(ung_fp8_product_kernel<128, 128, 2, 2, EXACT, false, OT>, 128, 128, ~0u, 256, vectors);
+        };
+        if (splits == 1) {
+            make((T *)c, c_stride, vec);
+        } else {
+            const uint64_t stride = split_stride(n), blocks = ceil_div(m * (stride / 4), 256);
+            make((float *)workspace, stride, true);
+            ung_fp8_join_kernel<T><<<(uint32_t)(blocks < 4096 ? blocks : 4096), 256, 0, st>>>(
+                (const float *)workspace, splits, m, n, stride, (T *)c, c_stride);
+        }
         return launched("ung_hip_fp8_matmul");
     });
 }

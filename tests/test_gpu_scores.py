@@ -162,6 +162,83 @@ def test_product_spoilt_rows_stay_apart():
     assert torch.equal(~torch.isfinite(c), bad)
 
 
+def _operand_there(n, d, block, seed):
+    """An operand and its values in 64 bits, all on the GPU."""
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    x = torch.randn(n, d, generator=g, device="cuda") * torch.exp(torch.randn(n, 1, generator=g, device="cuda"))
+    q, scale = S.quantize_fp8(x, block=block)
+    rows = torch.arange(n, device="cuda") // (1 if block == "row" else 128)
+    return q, scale, q.double() * scale.double()[rows].repeat_interleave(128, dim=1)
+
+
+# one and several rounds of large tiles, ragged both ways; rows of c that allow vectors and not;
+# sums in shares, of large tiles, of small ones and of few rows
+LARGE = [(2300, 5000, 130, "square"), (2304, 5003, 100, "row"), (5000, 4504, 260, "row"), (6400, 7001, 128, "square"),
+         (4000, 708, 20500, "square"), (4000, 703, 20500, "row"), (150, 150, 9000, "square"), (33, 1030, 6000, "row"),
+         (20, 3000, 5000, "square"), (1, 65, 8192, "row")]
+
+
+@pytest.mark.parametrize("m,n,d,block", LARGE)
+def test_large_product(m, n, d, block):
+    qa, sa, a = _operand_there(m, d, "row", m + d)
+    qb, sb, b = _operand_there(n, d, block, n + d)
+    want, wide = a @ b.t(), a.abs() @ b.abs().t()
+    kp = a.shape[1]
+    for kind in ("bf16", "fp32"):
+        bound = ((kp + 2 * kp // 128 + 2) * EPS + (2.0 ** -10 if kind != "fp32" else 0.0)) * wide
+        bound += HALF_ULP[kind] * want.abs() * 1.001 + TINY[kind]
+        got = S.matmul_fp8(qa, sa, qb, sb, dtype=TYPES[kind])
+        assert ((got.double() - want).abs() <= bound).all(), kind
+        assert torch.equal(got, S.matmul_fp8(qa, sa, qb, sb, dtype=TYPES[kind])), kind
+
+
+@pytest.mark.parametrize("pad", [8, 3])
+def test_large_product_into_wider_rows(pad):
+    """c_stride above n, large tiles: what lies between the rows is left alone."""
+    m, n, d = 2400, 4808, 256
+    qa, sa, _ = _operand_there(m, d, "row", 1)
+    qb, sb, _ = _operand_there(n, d, "square", 2)
+    c = torch.full((m, n + pad), -5.0, device="cuda", dtype=torch.bfloat16)
+    lib = F.load()
+    rc = lib.ung_hip_fp8_matmul(qa.data_ptr(), sa.data_ptr(), qb.data_ptr(), sb.data_ptr(), 1, m, n, d, c.data_ptr(),
+                                2, n + pad, None, 0, torch.cuda.current_stream().cuda_stream)
+    assert rc == 0
+    assert (c[:, n:] == -5.0).all() and torch.equal(c[:, :n], S.matmul_fp8(qa, sa, qb, sb))
+
+
+def test_large_product_spoilt_rows_stay_apart():
+    g = torch.Generator(device="cuda").manual_seed(3)
+    x, y = (torch.randn(n, 300, generator=g, device="cuda") for n in (3000, 4500))
+    x[2999, 200], x[7, 0], y[140, 3] = math.inf, math.nan, math.nan
+    c = S.matmul_fp8(*S.quantize_fp8(x), *S.quantize_fp8(y))
+    bad = torch.zeros(3000, 4500, dtype=torch.bool, device="cuda")
+    bad[2999], bad[7], bad[:, 140] = True, True, True
+    assert torch.equal(~torch.isfinite(c), bad)
+
+
+@pytest.mark.parametrize("kind", ["fp32", "fp16", "bf16"])
+def test_products_of_no_length(kind):
+    for m, n in ((1, 1), (40, 300), (300, 400), (2500, 4500)):
+        a, b = (S.quantize_fp8(torch.empty(r, 0, device="cuda")) for r in (m, n))
+        c = S.matmul_fp8(*a, *b, dtype=TYPES[kind])
+        assert tuple(c.shape) == (m, n) and not c.any()
+
+
+def test_product_needs_its_workspace():
+    qa, sa, _ = _operand_there(150, 9000, "row", 1)
+    qb, sb, _ = _operand_there(150, 9000, "row", 2)
+    c = torch.full((150, 150), -5.0, device="cuda")
+    lib = F.load()
+    keep, at, size = S._workspace(lib.ung_hip_fp8_matmul_workspace, 150, 150, qa.shape[1], 0, device="cuda")
+    assert size > 0
+    for where, bytes_ in ((None, size), (at, size - 1), (at + 4, size)):
+        rc = lib.ung_hip_fp8_matmul(qa.data_ptr(), sa.data_ptr(), qb.data_ptr(), sb.data_ptr(), 0, 150, 150,
+                                    qa.shape[1], c.data_ptr(), 0, 150, where, bytes_,
+                                    torch.cuda.current_stream().cuda_stream)
+        assert rc == -1 and b"workspace" in lib.ung_hip_last_error()
+    assert (c == -5.0).all()
+
+
 @pytest.mark.parametrize("m,n,pad", [(5, 33, 3), (130, 129, 8), (20, 2000, 1)])
 def test_product_into_wider_rows(m, n, pad):
     """c_stride above n: what lies between the rows is left alone."""
