@@ -26,6 +26,7 @@ from ._lib import check
 BLOCK = 128      # columns a scale stands for
 MAX_K = 128      # longest list of top_scores and of the distillation
 FP8 = torch.float8_e4m3fn
+_BYTES = (FP8, torch.uint8)
 _SAVED = 8       # floats a row that the backward pass of the distillation needs
 
 _TYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
@@ -47,19 +48,25 @@ def _library():
     return _ready
 
 
+# The raw handle of a device's current stream, without making a torch.cuda.Stream of it (0.1
+# against 2.6 us, a fifth of a small call).
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
+    lambda index: torch.cuda.current_stream(index).cuda_stream)
+
+
 class _On:
     """The device of a tensor made current for a call (HIP calls go to the current device)."""
 
     __slots__ = ("index", "before")
 
     def __init__(self, t):
-        self.index = t.device.index
+        self.index = t.get_device()
 
     def __enter__(self):
         self.before = torch.cuda.current_device()
         if self.before != self.index:
             torch.cuda.set_device(self.index)
-        return torch.cuda.current_stream().cuda_stream
+        return _raw_stream(self.index)
 
     def __exit__(self, *exc):
         if self.before != self.index:
@@ -71,26 +78,36 @@ def _need(ok, message):
         raise ValueError(message)
 
 
+# Messages are made only for an error: making one costs more than its check.
 def _on_gpu(name, t, like=None):
-    _need(isinstance(t, torch.Tensor) and t.is_cuda, f"{name}: a tensor on the GPU is needed")
-    _need(like is None or t.device == like.device, f"{name} is on another GPU")
+    if not (isinstance(t, torch.Tensor) and t.is_cuda):
+        raise ValueError(f"{name}: a tensor on the GPU is needed")
+    if like is not None and t.get_device() != like.get_device():
+        raise ValueError(f"{name} is on another GPU")
 
 
 def _matrix(name, t, like=None):
     """Checks a matrix of scores or rows; returns its type code and row stride."""
     _on_gpu(name, t, like)
-    _need(t.dim() == 2, f"{name}: a matrix is needed, got {t.dim()} dimensions")
-    _need(t.dtype in _TYPES, f"{name}: float32, float16 or bfloat16 is needed, got {t.dtype}")
-    _need(t.shape[1] <= 1 or t.stride(1) == 1, f"{name}: elements of a row have to lie side by side")
-    _need(t.shape[0] <= 1 or t.stride(0) >= t.shape[1], f"{name}: rows overlap")
-    return _TYPES[t.dtype], max(t.stride(0), t.shape[1])
+    kind = _TYPES.get(t.dtype)
+    if kind is None:
+        raise ValueError(f"{name}: float32, float16 or bfloat16 is needed, got {t.dtype}")
+    if t.dim() != 2:
+        raise ValueError(f"{name}: a matrix is needed, got {t.dim()} dimensions")
+    rows, cols = t.shape
+    stride, side = t.stride()
+    if cols > 1 and side != 1:
+        raise ValueError(f"{name}: elements of a row have to lie side by side")
+    if rows > 1 and stride < cols:
+        raise ValueError(f"{name}: rows overlap")
+    return kind, max(stride, cols)
 
 
 def _vector(name, t, n, like):
     """A row-wise float32 vector; one value for all rows (an expanded scalar) is laid out."""
     _on_gpu(name, t, like)
-    _need(t.dtype == torch.float32 and tuple(t.shape) == (n,), f"{name}: {n} float32 values are needed, got "
-                                                               f"{tuple(t.shape)} of {t.dtype}")
+    if t.dtype != torch.float32 or tuple(t.shape) != (n,):
+        raise ValueError(f"{name}: {n} float32 values are needed, got {tuple(t.shape)} of {t.dtype}")
     return t if t.is_contiguous() else t.contiguous()
 
 
@@ -117,7 +134,8 @@ def quantize_fp8(x, block="row", transpose=False):
     blocks] for ``"square"`` (128 x 128).  qt [columns, n rounded up] is the transposed operand:
     quantised along its own rows (``"row"``), or the same values turned (``"square"``)."""
     kind, stride = _matrix("x", x)
-    _need(block in ("row", "square"), f'block: "row" or "square" is needed, got {block!r}')
+    if block not in ("row", "square"):
+        raise ValueError(f'block: "row" or "square" is needed, got {block!r}')
     square = block == "square"
     n, d = x.shape
     nb, db = _blocks(n), _blocks(d)
@@ -135,35 +153,42 @@ def quantize_fp8(x, block="row", transpose=False):
 
 
 def _operand(name, q, scale, like=None):
+    """Checks an operand; returns its rows, their length and whether its scales are by square."""
     _on_gpu(name, q, like)
-    _need(q.dtype in (FP8, torch.uint8) and q.dim() == 2 and q.is_contiguous() and q.shape[1] % BLOCK == 0,
-          f"{name}: contiguous float8_e4m3fn rows of a multiple of {BLOCK} bytes are needed, got {tuple(q.shape)} of "
-          f"{q.dtype}")
+    if q.dim() != 2 or q.dtype not in _BYTES or q.shape[1] % BLOCK or not q.is_contiguous():
+        raise ValueError(f"{name}: contiguous float8_e4m3fn rows of a multiple of {BLOCK} bytes are needed, got "
+                         f"{tuple(q.shape)} of {q.dtype}")
     _on_gpu(f"{name}_scale", scale, q)
-    _need(scale.dtype == torch.float32 and scale.is_contiguous(), f"{name}_scale: contiguous float32 is needed")
-    rows, blocks = q.shape[0], q.shape[1] // BLOCK
-    if tuple(scale.shape) == (rows, blocks):
-        return False
-    _need(tuple(scale.shape) == (_blocks(rows), blocks),
-          f"{name}_scale: ({rows}, {blocks}) or ({_blocks(rows)}, {blocks}) is needed, got {tuple(scale.shape)}")
-    return True
+    if scale.dtype != torch.float32 or not scale.is_contiguous():
+        raise ValueError(f"{name}_scale: contiguous float32 is needed")
+    (rows, kp), shape = q.shape, tuple(scale.shape)
+    if shape == (rows, kp // BLOCK):
+        return rows, kp, False
+    if shape != (_blocks(rows), kp // BLOCK):
+        raise ValueError(f"{name}_scale: ({rows}, {kp // BLOCK}) or ({_blocks(rows)}, {kp // BLOCK}) is needed, got "
+                         f"{shape}")
+    return rows, kp, True
 
 
 def matmul_fp8(a, a_scale, b, b_scale, dtype=torch.bfloat16):
     """a b^T of two 8-bit operands (quantize_fp8) in ``dtype``; a with row scales, b with row
     or square ones.  Results are rounded once; float32 ones are summed in 32 bits throughout,
     16-bit ones by the 8-bit matrix instruction (errors of 1.4e-5 of their norm)."""
-    _need(not _operand("a", a, a_scale), "a: row scales are needed")
-    square = _operand("b", b, b_scale, a)
-    _need(dtype in _TYPES, f"dtype: float32, float16 or bfloat16 is needed, got {dtype}")
-    (m, kp), n = a.shape, b.shape[0]
-    _need(b.shape[1] == kp, f"a and b: rows of {kp} and {b.shape[1]} bytes do not go together")
+    m, kp, a_square = _operand("a", a, a_scale)
+    n, b_kp, square = _operand("b", b, b_scale, a)
+    kind = _TYPES.get(dtype)
+    if a_square:
+        raise ValueError("a: row scales are needed")
+    if kind is None:
+        raise ValueError(f"dtype: float32, float16 or bfloat16 is needed, got {dtype}")
+    if b_kp != kp:
+        raise ValueError(f"a and b: rows of {kp} and {b_kp} bytes do not go together")
     c = torch.empty(m, n, dtype=dtype, device=a.device)
     lib = _library()
     with _On(a) as stream:
-        keep, at, size = _workspace(lib.ung_hip_fp8_matmul_workspace, m, n, kp, _TYPES[dtype], device=a.device)
+        keep, at, size = _workspace(lib.ung_hip_fp8_matmul_workspace, m, n, kp, kind, device=a.device)
         check(lib.ung_hip_fp8_matmul(a.data_ptr(), a_scale.data_ptr(), b.data_ptr(), b_scale.data_ptr(), square, m, n,
-                                     kp, c.data_ptr(), _TYPES[dtype], n, at, size, stream))
+                                     kp, c.data_ptr(), kind, n, at, size, stream))
     return c
 
 
@@ -225,7 +250,8 @@ def top_scores(scores, k, temperature=1.0):
     the whole row.  Columns at -inf are not listed; missing entries are (-inf, -1)."""
     kind, stride = _matrix("scores", scores)
     n, v = scores.shape
-    _need(1 <= k <= MAX_K, f"k={k} outside 1..{MAX_K}")
+    if not 1 <= k <= MAX_K:
+        raise ValueError(f"k={k} outside 1..{MAX_K}")
     values = torch.empty(n, k, device=scores.device)
     ids = torch.empty(n, k, dtype=torch.int32, device=scores.device)
     lse = torch.empty(n, device=scores.device)
@@ -253,12 +279,13 @@ def entries_of_neighbors(ids, distances):
 def _teacher(scores, ids, values, lse):
     _on_gpu("ids", ids, scores)
     _on_gpu("values", values, scores)
-    n = scores.shape[0]
-    _need(ids.dim() == 2 and ids.shape[0] == n and ids.dtype == torch.int32,
-          f"ids: int32 [{n}, k] is needed, got {tuple(ids.shape)} of {ids.dtype}")
-    _need(values.shape == ids.shape and values.dtype == torch.float32,
-          f"values: float32 {tuple(ids.shape)} is needed, got {tuple(values.shape)} of {values.dtype}")
-    _need(ids.shape[1] <= MAX_K, f"k={ids.shape[1]} outside 0..{MAX_K}")
+    n, shape = scores.shape[0], ids.shape
+    if len(shape) != 2 or shape[0] != n or ids.dtype != torch.int32:
+        raise ValueError(f"ids: int32 [{n}, k] is needed, got {tuple(shape)} of {ids.dtype}")
+    if values.shape != shape or values.dtype != torch.float32:
+        raise ValueError(f"values: float32 {tuple(shape)} is needed, got {tuple(values.shape)} of {values.dtype}")
+    if shape[1] > MAX_K:
+        raise ValueError(f"k={shape[1]} outside 0..{MAX_K}")
     ids = ids if ids.is_contiguous() else ids.contiguous()
     values = values if values.is_contiguous() else values.contiguous()
     return ids, values, lse if lse is None else _vector("teacher_lse", lse, n, scores)
