@@ -57,13 +57,13 @@ struct RowRef {
         }
         return v;
     }
-    // Elements of vector i to a row of the same length.
-    __device__ void store_elements(T *to, uint32_t i, const Vec<T> &v) const
+    // Elements of vector i to a row of the same length, but for those whose bits are in `skip`.
+    __device__ void store_elements(T *to, uint32_t i, const Vec<T> &v, uint32_t skip) const
     {
 #pragma unroll
         for (uint32_t e = 0; e < N; ++e) {
             const uint32_t j = i * N + e - shift;
-            if (j < len)
+            if (j < len && !(skip >> e & 1))
                 to[j] = v.element(e);
         }
     }
@@ -397,8 +397,9 @@ __global__ __launch_bounds__(TOP_NT) void ung_top_merge_kernel(const uint64_t *p
 // taken as 1 - sum q_k: that would cancel where the student's mass lies in the list, and
 // vanish where its other scores are far below.  A bit for each column of the block's stretch,
 // in LDS, tells them apart; where Q_r counts, listed columns leave the stretch's sums and
-// enter the row's from the entries.  A row without a valid entry, or without a score above
-// -inf, has loss and gradient 0.
+// enter the row's from the entries.  Their gradients come from the entries too, and the
+// vectors that hold them go out without them, so that no store waits for another.  A row
+// without a valid entry, or without a score above -inf, has loss and gradient 0.
 
 // What the backward pass needs of a row besides its inputs.
 struct alignas(16) Saved {
@@ -414,59 +415,150 @@ static_assert(sizeof(Saved) == 4 * UNG_HIP_DISTILL_SAVED, "");
 constexpr float EMPTY = __builtin_inff(); // Saved::top of a row without loss
 
 struct DistillShared {
-    float z[MAX_K];  // the teacher's score; -inf = not there
-    float s[MAX_K];  // the student's there
+    float z[MAX_K]; // the teacher's score; -inf = not there
+    float s[MAX_K]; // the student's there
+    float p[MAX_K]; // p_k
     uint32_t id[MAX_K];
     uint32_t first[MAX_K]; // the entry is the first one to name its column
     float red[2][16];
+    float base, log, mass; // as in Saved; sum of p_k
+    uint32_t any, twice;   // entries there are; a column that several of them name
     Saved saved;
 };
 
-// The teacher's row: entries into sh by the first k threads, with the student's scores of
-// those whose columns lie in [from, to) (a block that writes the gradient over the scores
-// reads no other block's stretch).
+// One entry of the teacher's row, loaded by each of the first k threads: ahead of the scores,
+// which it would else have to wait for.
+struct Entry {
+    int32_t id;
+    float value;
+    __device__ Entry(const int32_t *ids, const float *values, uint32_t k)
+        : id(threadIdx.x < k ? ids[threadIdx.x] : -1), value(threadIdx.x < k ? values[threadIdx.x] : NEG_INF)
+    {
+    }
+};
+
+// Entries into sh, with the student's scores of those whose columns lie in [from, to) (a block
+// that writes the gradient over the scores reads no other block's stretch).
 template <class T>
-__device__ inline void load_entries(DistillShared &sh, const T *row, const int32_t *ids, const float *values,
-                                    uint32_t k, uint32_t len, int64_t from, int64_t to)
+__device__ inline void keep_entries(DistillShared &sh, const Entry &e, const T *row, uint32_t k, uint32_t len,
+                                    int64_t from, int64_t to)
 {
     const uint32_t tid = threadIdx.x;
+    if (tid == 0)
+        sh.twice = 0;
     if (tid < k) {
-        const int32_t id = ids[tid];
-        const float v = values[tid];
-        const bool ok = (uint32_t)id < len && v != NEG_INF;
-        sh.id[tid] = ok ? (uint32_t)id : 0xFFFFFFFFu;
-        sh.z[tid] = ok ? v : NEG_INF;
-        sh.s[tid] = ok && id >= from && id < to ? to_float(row[id]) : 0.0f;
+        const bool ok = (uint32_t)e.id < len && e.value != NEG_INF;
+        sh.id[tid] = ok ? (uint32_t)e.id : 0xFFFFFFFFu;
+        sh.z[tid] = ok ? e.value : NEG_INF;
+        sh.s[tid] = ok && e.id >= from && e.id < to ? to_float(row[e.id]) : 0.0f;
         sh.first[tid] = ok;
     }
 }
 
-// Loss and Saved of a row, run by one wave: from its entries and the sums (maximum, sum of
-// exp((s - maximum) / T)) of its columns, with `lse` of those outside the list.  Returns the
-// loss in every lane.
-__device__ inline float finish_row(DistillShared &sh, uint32_t k, const float *lse, float2 sums, Temperature t,
-                                   Saved &saved)
+// sh.first by the order of the entries (of equal ones a fixed one, whichever thread came first).
+__device__ inline void find_first(DistillShared &sh, uint32_t k)
+{
+    const uint32_t tid = threadIdx.x;
+    if (tid < k) {
+        const uint32_t id = sh.id[tid];
+        bool first = id != 0xFFFFFFFFu;
+        for (uint32_t o = 0; o < tid; ++o)
+            first &= sh.id[o] != id;
+        sh.first[tid] = first;
+    }
+    __syncthreads();
+}
+
+// Bits of the listed columns among the `vectors` vectors from `begin` on, and sh.first and
+// sh.twice of the entries there.  Begins and ends with the block together.
+template <int N, int NT>
+__device__ inline void mark_listed(DistillShared &sh, uint32_t *bits, uint32_t begin, uint32_t vectors,
+                                   uint32_t shift, uint32_t k)
+{
+    const uint32_t tid = threadIdx.x;
+    for (uint32_t i = tid; i < vectors * N / 32; i += NT)
+        bits[i] = 0;
+    __syncthreads();
+    if (tid < k && sh.id[tid] != 0xFFFFFFFFu) {
+        const uint64_t at = (uint64_t)sh.id[tid] + shift, from = (uint64_t)begin * N;
+        if (at >= from && at < from + (uint64_t)vectors * N) {
+            const uint32_t bit = 1u << ((at - from) & 31);
+            if (atomicOr(&bits[(at - from) >> 5], bit) & bit)
+                sh.twice = 1;
+        }
+    }
+    __syncthreads();
+    if (sh.twice)
+        find_first(sh, k);
+}
+
+// Listed columns of one vector, a bit for each.
+template <int N>
+__device__ inline uint32_t listed_of(const uint32_t *bits, uint32_t begin, uint32_t at)
+{
+    const uint32_t b = (at - begin) * N;
+    return bits[b >> 5] >> (b & 31) & ((1u << N) - 1);
+}
+
+// The teacher's side of a row, run by one wave.
+__device__ inline void teacher_row(DistillShared &sh, uint32_t k, const float *lse, Temperature t)
 {
     const uint32_t lane = threadIdx.x & 63;
-    float z[2], s[2], best = NEG_INF, top = sums.x;
+    float z[2], best = NEG_INF, base = 0.0f, log_base = 0.0f;
     bool any = false;
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-        const uint32_t i = h * 64 + lane;
-        z[h] = i < k ? sh.z[i] : NEG_INF;
-        s[h] = i < k ? sh.s[i] : 0.0f;
+        z[h] = h * 64 + lane < k ? sh.z[h * 64 + lane] : NEG_INF;
         any |= z[h] != NEG_INF;
         best = max_nan(best, z[h]);
-        if (lse && i < k && sh.first[i])
-            top = max_of(top, s[h]);
     }
     any = __any(any);
+    if (lse)
+        log_base = *lse;
+    else if (any) {
+        float sum = 0.0f;
+        base = wave_reduce(best, max_nan);
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+            sum += z[h] == NEG_INF ? 0.0f : expf((z[h] - base) * t.inv);
+        log_base = logf(wave_reduce(sum, add));
+    }
+    float mass = 0.0f;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        const float p = z[h] == NEG_INF ? 0.0f : expf((z[h] - base) * t.inv - log_base);
+        mass += p;
+        if (h * 64 + lane < k)
+            sh.p[h * 64 + lane] = p;
+    }
+    mass = wave_reduce(mass, add);
+    if (lane == 0) {
+        sh.any = any;
+        sh.base = base;
+        sh.log = log_base;
+        sh.mass = mass;
+    }
+}
+
+// Loss and Saved of a row, run by the wave that made the teacher's side: from that, the entries
+// and the sums (maximum, sum of exp((s - maximum) / T)) of the row's columns, with `lse` of
+// those outside the list.  Returns the loss in every lane.
+__device__ inline float finish_row(DistillShared &sh, uint32_t k, bool tail, float2 sums, Temperature t, Saved &saved)
+{
+    const uint32_t lane = threadIdx.x & 63;
+    float s[2], top = sums.x;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        const uint32_t i = h * 64 + lane;
+        s[h] = i < k ? sh.s[i] : 0.0f;
+        if (tail && i < k && sh.first[i])
+            top = max_of(top, s[h]);
+    }
     saved = Saved{EMPTY, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, {}};
-    best = wave_reduce(best, max_nan);
     top = wave_reduce(top, max_of);
     const float at = top == NEG_INF ? 0.0f : top;
     float total = sums.y;
-    if (lse) {
+    if (tail) {
         float in = 0.0f;
 #pragma unroll
         for (int h = 0; h < 2; ++h)
@@ -476,33 +568,22 @@ __device__ inline float finish_row(DistillShared &sh, uint32_t k, const float *l
     }
     if (total != total) // a NaN among the scores, or +inf: the whole row is NaN
         top = total;
-    if (!any || top == NEG_INF)
+    if (!sh.any || top == NEG_INF)
         return 0.0f;
-    float base = 0.0f, log_base = 0.0f;
-    if (lse)
-        log_base = *lse;
-    else {
-        float sum = 0.0f;
+    const float log_total = logf(total), mass = sh.mass;
+    float loss = 0.0f;
 #pragma unroll
-        for (int h = 0; h < 2; ++h)
-            sum += z[h] == NEG_INF ? 0.0f : expf((z[h] - best) * t.inv);
-        base = best;
-        log_base = logf(wave_reduce(sum, add));
-    }
-    const float log_total = logf(total);
-    float mass = 0.0f, loss = 0.0f;
-#pragma unroll
-    for (int h = 0; h < 2; ++h)
-        if (z[h] != NEG_INF) {
-            const float log_p = (z[h] - base) * t.inv - log_base, p = expf(log_p);
-            mass += p;
+    for (int h = 0; h < 2; ++h) {
+        const uint32_t i = h * 64 + lane;
+        if (i < k && sh.z[i] != NEG_INF) {
+            const float p = sh.p[i], log_p = (sh.z[i] - sh.base) * t.inv - sh.log;
             if (!(p <= 0.0f))
                 loss += p * (log_p - ((s[h] - top) * t.inv - log_total));
         }
-    mass = wave_reduce(mass, add);
+    }
     loss = wave_reduce(loss, add);
-    saved = Saved{top, mass / total, top, mass / total, base, log_base, {}};
-    if (lse && !(sums.y <= 0.0f)) {
+    saved = Saved{top, mass / total, top, mass / total, sh.base, sh.log, {}};
+    if (tail && !(sums.y <= 0.0f)) {
         const float rest = 1.0f - mass < 0.0f ? 0.0f : 1.0f - mass;
         saved.rest_top = sums.x;
         if (!(rest <= 0.0f)) {
@@ -514,78 +595,65 @@ __device__ inline float finish_row(DistillShared &sh, uint32_t k, const float *l
     return loss;
 }
 
-// Gradient of a stretch of a row whose vectors are in registers, then of the listed columns
-// that lie in it (in one more write: their scores were read before the first one).
+// Gradient of a stretch of a row whose vectors are in registers: of the listed columns (marked
+// in `bits`) from their entries, of the others from the vectors.
 template <class T, int NT, int NV>
-__device__ inline void write_gradient(DistillShared &sh, const RowRef<T> &ref, Stretch<T, NT, NV> &x, uint32_t begin, uint32_t k,
-                                      Temperature t, const Saved saved, float weight, T *grad)
+__device__ inline void write_gradient(DistillShared &sh, const uint32_t *bits, const RowRef<T> &ref,
+                                      Stretch<T, NT, NV> &x, uint32_t begin, uint32_t k, Temperature t,
+                                      const Saved saved, float weight, T *grad)
 {
     constexpr int N = Vec<T>::N;
     const bool same = ((uintptr_t)grad & 15) == ref.shift * sizeof(T);
     const float c = t.c, w = weight * t.inv, out = saved.outside * w;
     const float rest_top = saved.rest_top;
-    auto put = [&](const Vec<T> &g, uint32_t at) {
+    auto put = [&](const Vec<T> &g, uint32_t at, uint32_t skip) {
         const bool inside = ref.inside(at);
-        if (same && inside)
+        if (same && inside && !skip)
             reinterpret_cast<Vec<T> *>(grad - ref.shift)[at] = g;
         else if (inside || (x.has_edge && at == x.edge_at)) // an end is written by its holder alone
-            ref.store_elements(grad, at, g);
+            ref.store_elements(grad, at, g, skip);
     };
     if (saved.top == EMPTY) {
-        x.each([&](const Vec<T> &, uint32_t at) { put(Vec<T>{}, at); });
+        x.each([&](const Vec<T> &, uint32_t at) { put(Vec<T>{}, at, 0); });
         return;
+    }
+    const uint32_t id = threadIdx.x < k && sh.first[threadIdx.x] ? sh.id[threadIdx.x] : 0xFFFFFFFFu;
+    const uint32_t at = (id + ref.shift) / N;
+    if (id != 0xFFFFFFFFu && at >= begin && at < begin + NT * NV) {
+        float p = sh.p[threadIdx.x];
+        if (sh.twice) { // of every entry that names this column
+            p = 0.0f;
+            for (uint32_t o = 0; o < k; ++o)
+                p += sh.id[o] == id ? sh.p[o] : 0.0f;
+        }
+        const float e = weight_of(sh.s[threadIdx.x], saved.top, t.c);
+        grad[id] = from_float<T>((e * saved.inside - p) * w);
     }
     x.each([&](const Vec<T> &v, uint32_t at) {
         Vec<T> g;
 #pragma unroll
         for (int e = 0; e < N; e += 2)
             g.put2(e, weight_of(v.get(e), rest_top, c) * out, weight_of(v.get(e + 1), rest_top, c) * out);
-        put(g, at);
+        put(g, at, listed_of<N>(bits, begin, at));
     });
-    __syncthreads();
-    if (threadIdx.x < k) {
-        const uint32_t id = sh.id[threadIdx.x];
-        const uint32_t at = (id + ref.shift) / N;
-        if (id != 0xFFFFFFFFu && at >= begin && at < begin + NT * NV) {
-            float p = 0.0f; // of every entry that names this column
-            for (uint32_t o = 0; o < k; ++o)
-                p += sh.id[o] == id ? expf((sh.z[o] - saved.base) * t.inv - saved.log) : 0.0f;
-            const float e = weight_of(sh.s[threadIdx.x], saved.top, t.c);
-            grad[id] = from_float<T>((e * saved.inside - p) * w);
-        }
-    }
 }
 
 // Sums of a stretch of a row in registers, in every thread: its maximum and the sum of
 // exp((s - maximum) / T).  With `tail` listed columns become -inf first.
 template <class T, int NT, int NV>
-__device__ inline float2 stretch_sums(DistillShared &sh, uint32_t *bits, Stretch<T, NT, NV> &x, uint32_t begin,
-                                      uint32_t shift, uint32_t k, bool tail, float c)
+__device__ inline float2 stretch_sums(DistillShared &sh, const uint32_t *bits, Stretch<T, NT, NV> &x, uint32_t begin,
+                                      bool tail, float c)
 {
     constexpr int N = Vec<T>::N;
-    const uint32_t tid = threadIdx.x;
-    if (tail) {
-        for (uint32_t i = tid; i < NT * NV * N / 32; i += NT)
-            bits[i] = 0;
-        __syncthreads();
-        if (tid < k && sh.id[tid] != 0xFFFFFFFFu) {
-            const uint64_t at = (uint64_t)sh.id[tid] + shift, from = (uint64_t)begin * N;
-            if (at >= from && at < from + NT * NV * N) {
-                const uint32_t bit = 1u << ((at - from) & 31);
-                sh.first[tid] = !(atomicOr(&bits[(at - from) >> 5], bit) & bit);
-            }
-        }
-        __syncthreads();
+    if (tail)
         x.each([&](Vec<T> &v, uint32_t at) {
-            const uint32_t b = (at - begin) * N;
-            const uint32_t listed = bits[b >> 5] >> (b & 31) & ((1u << N) - 1);
+            const uint32_t listed = listed_of<N>(bits, begin, at);
             if (listed)
 #pragma unroll
                 for (int e = 0; e < N; ++e)
                     if (listed >> e & 1)
                         v.set(e, (T)NEG_INF);
         });
-    }
     float most = NEG_INF;
     x.each([&](const Vec<T> &v, uint32_t) {
 #pragma unroll
@@ -604,7 +672,9 @@ __device__ inline float2 stretch_sums(DistillShared &sh, uint32_t *bits, Stretch
 }
 
 // A row by one block, its scores in registers: loss, and the gradient with `grad`.  One read
-// of the scores and one write of the gradient, bound by memory.  `grad` may be the scores.
+// of the scores and one write of the gradient, bound by memory: 4096 x 32768, k = 64, bf16 130
+// us (4.1 TB/s), float32 214 (5.0; a copy of it 4.9); 64 x 10000 8.2.  `grad` may be the scores.
+// One wave makes the teacher's side while the others await the scores.
 template <class T, int NT, int NV>
 __global__ __launch_bounds__(NT, NV <= 8 ? 8 : 4) void ung_distill_row_kernel(const T *scores, uint32_t len, uint64_t stride,
                                                              const int32_t *ids, const float *values, uint32_t k,
@@ -616,13 +686,16 @@ __global__ __launch_bounds__(NT, NV <= 8 ? 8 : 4) void ung_distill_row_kernel(co
     __shared__ uint32_t bits[NT * NV * Vec<T>::N / 32];
     const uint64_t r = blockIdx.x;
     const RowRef<T> ref(scores + r * stride, len);
+    const Entry entry(ids + r * k, values + r * k, k);
     Stretch<T, NT, NV> x(ref, 0);
-    load_entries(sh, ref.row, ids + r * k, values + r * k, k, len, 0, len);
-    const float2 sums = stretch_sums<T, NT, NV>(sh, bits, x, 0, ref.shift, k, lse != nullptr, t.c);
-    __syncthreads();
+    keep_entries(sh, entry, ref.row, k, len, 0, len);
+    mark_listed<Vec<T>::N, NT>(sh, bits, 0, NT * NV, ref.shift, k);
+    if (threadIdx.x < 64)
+        teacher_row(sh, k, lse ? lse + r : nullptr, t);
+    const float2 sums = stretch_sums<T, NT, NV>(sh, bits, x, 0, lse != nullptr, t.c);
     if (threadIdx.x < 64) {
         Saved saved;
-        const float l = finish_row(sh, k, lse ? lse + r : nullptr, sums, t, saved);
+        const float l = finish_row(sh, k, lse != nullptr, sums, t, saved);
         if (threadIdx.x == 0) {
             loss[r] = l;
             if (saved_out)
@@ -633,7 +706,7 @@ __global__ __launch_bounds__(NT, NV <= 8 ? 8 : 4) void ung_distill_row_kernel(co
     if (!grad)
         return;
     __syncthreads();
-    write_gradient<T, NT, NV>(sh, ref, x, 0, k, t, sh.saved, weight ? weight[r] : 1.0f, grad + r * grad_stride);
+    write_gradient<T, NT, NV>(sh, bits, ref, x, 0, k, t, sh.saved, weight ? weight[r] : 1.0f, grad + r * grad_stride);
 }
 
 // Sums of one piece of a row (NT * NV vectors).
@@ -647,10 +720,13 @@ __global__ __launch_bounds__(NT) void ung_distill_part_kernel(const T *scores, u
     const uint64_t r = blockIdx.x / pieces;
     const uint32_t begin = (uint32_t)(blockIdx.x - r * pieces) * (NT * NV);
     const RowRef<T> ref(scores + r * stride, len);
+    const Entry entry(ids + r * k, values + r * k, tail ? k : 0);
     Stretch<T, NT, NV> x(ref, begin);
-    if (tail)
-        load_entries(sh, ref.row, ids + r * k, values + r * k, k, len, 0, 0);
-    const float2 sums = stretch_sums<T, NT, NV>(sh, bits, x, begin, ref.shift, k, tail, t.c);
+    if (tail) {
+        keep_entries(sh, entry, ref.row, k, len, 0, 0);
+        mark_listed<Vec<T>::N, NT>(sh, bits, begin, NT * NV, ref.shift, k);
+    }
+    const float2 sums = stretch_sums<T, NT, NV>(sh, bits, x, begin, tail, t.c);
     if (threadIdx.x == 0)
         part[blockIdx.x] = sums;
 }
@@ -664,14 +740,12 @@ __global__ __launch_bounds__(128) void ung_distill_join_kernel(const T *scores, 
 {
     __shared__ DistillShared sh;
     const uint64_t r = blockIdx.x;
-    load_entries(sh, scores + r * stride, ids + r * k, values + r * k, k, len, 0, len);
+    keep_entries(sh, Entry(ids + r * k, values + r * k, k), scores + r * stride, k, len, 0, len);
     __syncthreads();
-    if (lse && threadIdx.x < k) {
-        const uint32_t id = sh.id[threadIdx.x];
-        for (uint32_t o = 0; o < threadIdx.x; ++o)
-            if (sh.id[o] == id)
-                sh.first[threadIdx.x] = 0;
-    }
+    if (lse)
+        find_first(sh, k);
+    if (threadIdx.x < 64)
+        teacher_row(sh, k, lse ? lse + r : nullptr, t);
     __syncthreads();
     if (threadIdx.x >= 64)
         return;
@@ -685,7 +759,7 @@ __global__ __launch_bounds__(128) void ung_distill_join_kernel(const T *scores, 
         sum += mine[i].y == 0.0f ? 0.0f : mine[i].x == NEG_INF ? mine[i].y : mine[i].y * weight_of(mine[i].x, at, t.c);
     sum = wave_reduce(sum, add);
     Saved saved;
-    const float l = finish_row(sh, k, lse ? lse + r : nullptr, make_float2(top, sum), t, saved);
+    const float l = finish_row(sh, k, lse != nullptr, make_float2(top, sum), t, saved);
     if (threadIdx.x == 0) {
         loss[r] = l;
         saved_out[r] = saved;
@@ -700,14 +774,20 @@ __global__ __launch_bounds__(NT) void ung_distill_grad_kernel(const T *scores, u
                                                               uint32_t pieces, T *grad, uint64_t grad_stride)
 {
     __shared__ DistillShared sh;
+    __shared__ uint32_t bits[NT * NV * Vec<T>::N / 32];
     const uint64_t r = blockIdx.x / pieces;
     const uint32_t begin = (uint32_t)(blockIdx.x - r * pieces) * (NT * NV);
     const RowRef<T> ref(scores + r * stride, len);
+    const Entry entry(ids + r * k, values + r * k, k);
+    const Saved row = saved[r];
     Stretch<T, NT, NV> x(ref, begin);
     const int64_t from = (int64_t)begin * Vec<T>::N - ref.shift;
-    load_entries(sh, ref.row, ids + r * k, values + r * k, k, len, from, from + NT * NV * Vec<T>::N);
-    __syncthreads(); // the entries' scores are read before this block writes
-    write_gradient<T, NT, NV>(sh, ref, x, begin, k, t, saved[r], weight ? weight[r] : 1.0f, grad + r * grad_stride);
+    keep_entries(sh, entry, ref.row, k, len, from, from + NT * NV * Vec<T>::N);
+    if (threadIdx.x < k)
+        sh.p[threadIdx.x] = sh.z[threadIdx.x] == NEG_INF ? 0.0f : expf((sh.z[threadIdx.x] - row.base) * t.inv - row.log);
+    // and the entries' scores are read before this block writes
+    mark_listed<Vec<T>::N, NT>(sh, bits, begin, NT * NV, ref.shift, k);
+    write_gradient<T, NT, NV>(sh, bits, ref, x, begin, k, t, row, weight ? weight[r] : 1.0f, grad + r * grad_stride);
 }
 
 } // namespace
@@ -805,7 +885,8 @@ uint64_t top_bytes(uint64_t rows, uint32_t pieces, uint32_t k)
     return bytes;
 }
 
-template <class F>
+// f with nv, one of 1, 2, 4 .. MOST, as a constant.
+template <int MOST, class F>
 void with_nv(uint32_t nv, F f)
 {
     if (nv == 1)
@@ -814,16 +895,22 @@ void with_nv(uint32_t nv, F f)
         f(std::integral_constant<int, 2>{});
     else if (nv == 4)
         f(std::integral_constant<int, 4>{});
-    else if (nv == 8)
+    else if (MOST == 8 || nv == 8)
         f(std::integral_constant<int, 8>{});
     else
-        f(std::integral_constant<int, 16>{});
+        f(std::integral_constant<int, MOST>{});
 }
 
 constexpr int ROW_NT = 512;   // threads of a block that holds a whole row
 constexpr int PIECE_NT = 256; // ... a piece of one
 
-bool whole_rows(uint64_t rows, uint32_t vectors) { return vectors <= ROW_NT * 16 && (rows >= 128 || vectors <= ROW_NT * 2); }
+// A row by one block if it fits a block's registers, unless few long rows would leave most CUs
+// without work: then pieces of rows, in three launches.  Loss and gradient, us, whole against in
+// pieces: 64 x 10000 bf16 8.2, 13; 64 x 32768 12.6, 15; 120 x 65000 21.4, 22; 64 x 65000 18.7, 15.9.
+bool whole_rows(uint64_t rows, uint32_t vectors)
+{
+    return vectors <= ROW_NT * 8 || (vectors <= ROW_NT * 16 && rows >= 128);
+}
 
 Cut row_cut(uint32_t vectors)
 {
@@ -889,7 +976,7 @@ int distill(const char *what, const void *scores, int type, uint64_t rows, uint6
         const uint32_t vectors = vectors_at_most<T>(scores, rows, stride, len);
         int rc;
         if (whole_rows(rows, vectors)) {
-            with_nv(row_cut(vectors).nv, [&](auto nv) {
+            with_nv<16>(row_cut(vectors).nv, [&](auto nv) {
                 ung_distill_row_kernel<T, ROW_NT, nv.value><<<(uint32_t)rows, ROW_NT, 0, st>>>(
                     p, (uint32_t)len, stride, ids, values, k, lse, weight, t, loss, saved, (T *)grad, grad_stride);
             });
@@ -902,14 +989,14 @@ int distill(const char *what, const void *scores, int type, uint64_t rows, uint6
             return rc;
         float2 *part = (float2 *)workspace;
         Saved *kept = saved ? saved : (Saved *)((char *)workspace + parts);
-        with_nv(cut.nv, [&](auto nv) {
+        with_nv<8>(cut.nv, [&](auto nv) {
             ung_distill_part_kernel<T, PIECE_NT, nv.value><<<(uint32_t)blocks, PIECE_NT, 0, st>>>(
                 p, (uint32_t)len, stride, ids, values, k, lse != nullptr, t, cut.pieces, part);
         });
         ung_distill_join_kernel<T><<<(uint32_t)rows, 128, 0, st>>>(p, (uint32_t)len, stride, ids, values, k, lse,
                                                                    t, cut.pieces, part, loss, kept);
         if (grad)
-            with_nv(cut.nv, [&](auto nv) {
+            with_nv<8>(cut.nv, [&](auto nv) {
                 ung_distill_grad_kernel<T, PIECE_NT, nv.value><<<(uint32_t)blocks, PIECE_NT, 0, st>>>(
                     p, (uint32_t)len, stride, ids, values, k, kept, weight, t, cut.pieces, (T *)grad, grad_stride);
             });
@@ -978,7 +1065,7 @@ int ung_hip_top_scores(const void *scores, int type, uint64_t rows, uint64_t len
             part = (uint64_t *)take(rows * lists * k * 8);
             sums = (float2 *)take(rows * lists * 8);
         }
-        with_nv(cut.nv, [&](auto nv) {
+        with_nv<16>(cut.nv, [&](auto nv) {
             ung_top_scores_kernel<T, nv.value><<<(uint32_t)(rows * lists), TOP_NT, 0, st>>>(
                 (const T *)scores, (uint32_t)len, row_stride, (uint32_t)lists, k, t, values, ids, lse,
                 part, sums);
@@ -1071,7 +1158,7 @@ int ung_hip_distill_backward(const void *scores, int type, uint64_t rows, uint64
         int rc;
         if ((rc = check_grid(what, rows * cut.pieces)))
             return rc;
-        with_nv(cut.nv, [&](auto nv) {
+        with_nv<8>(cut.nv, [&](auto nv) {
             ung_distill_grad_kernel<T, PIECE_NT, nv.value><<<(uint32_t)(rows * cut.pieces), PIECE_NT, 0,
                                                              (hipStream_t)stream>>>(
                 (const T *)scores, (uint32_t)len, row_stride, ids, values, k, (const Saved *)saved, weight,

@@ -536,6 +536,22 @@ def test_distill(n, v, k, kind, tail):
         _check_distill(x, view, ids, val, lse if tail else None, t, kind, n)
 
 
+@pytest.mark.parametrize("v", [300, 5000, 70000])
+def test_distill_is_the_same_every_time(v):
+    """Columns named many times over: sums keep their order whichever entry is seen first."""
+    g = _gen(v)
+    x = torch.randn(9, v, generator=g).cuda()
+    ids = torch.randint(0, 20, (9, 100), generator=g, dtype=torch.int32).cuda()
+    val = torch.randn(9, 100, generator=g).cuda()
+    lse = torch.logsumexp(val, 1) + 0.3
+    loss, grad = S.distill_step(x, ids, val, teacher_lse=lse)
+    saved = S.distill_forward(x, ids, val, teacher_lse=lse)[1]
+    for _ in range(10):
+        again = S.distill_step(x, ids, val, teacher_lse=lse)
+        assert torch.equal(loss, again[0]) and torch.equal(grad, again[1])
+        assert torch.equal(saved[:, :6], S.distill_forward(x, ids, val, teacher_lse=lse)[1][:, :6])
+
+
 @pytest.mark.parametrize("tail", [False, True])
 def test_distill_columns_named_twice(tail):
     x, _, view = _scores(6, 40, "fp32", 0, 3)
