@@ -350,9 +350,15 @@ __global__ __launch_bounds__(TOP_NT) void ung_top_merge_kernel(const uint64_t *p
     const uint32_t n = lists - first < MERGE_LISTS ? lists - first : MERGE_LISTS, items = n * k;
     const uint64_t *mine = part + (r * lists + first) * k;
     uint64_t v[NI];
+    // lists are sorted: each is turned by its own amount, or some threads would hold all the
+    // large orders and their maxima tell little (k = 128: 55 us)
+    const float per_k = 1.0f / (float)k;
 #pragma unroll
-    for (int i = 0; i < NI; ++i)
-        v[i] = i * TOP_NT + tid < items ? mine[i * TOP_NT + tid] : 0;
+    for (int i = 0; i < NI; ++i) {
+        const uint32_t j = i * TOP_NT + tid, list = (uint32_t)(((float)j + 0.5f) * per_k);
+        const uint32_t turned = j - list * k + __umulhi(list * 0x9E3779B1u, k);
+        v[i] = j < items ? mine[list * k + (turned < k ? turned : turned - k)] : 0;
+    }
     float2 s = make_float2(NEG_INF, 0.0f);
     if (tid < n)
         s = part_sum[r * lists + first + tid];
@@ -868,13 +874,21 @@ struct Cut {
     uint32_t nv, pieces;
 };
 
+// A row by one block where it fits one (64 x 10000 float32 8.9 us, in pieces 12.2; 1 x 10000 6.7,
+// 10.1; 256 x 16000 9.5, 14.3).  Longer rows in pieces, shorter ones where blocks are few, but
+// no more than one pass merges (1 x 100000 in 49 pieces 13.6, in 98 18.5).
 Cut top_cut(uint64_t rows, uint32_t vectors)
 {
     uint32_t nv = 16;
-    while (nv > 1 && (TOP_NT * (nv / 2) >= vectors || rows * ceil_div(vectors, TOP_NT * nv) < 512))
+    if (vectors <= TOP_NT * 16) {
+        while (nv > 1 && TOP_NT * (nv / 2) >= vectors)
+            nv /= 2;
+        return Cut{nv, 1};
+    }
+    while (nv > 1 && rows * ceil_div(vectors, TOP_NT * nv) < 512 &&
+           ceil_div(vectors, TOP_NT * (nv / 2)) <= MERGE_LISTS)
         nv /= 2;
-    const uint64_t pieces = ceil_div(vectors, TOP_NT * nv);
-    return Cut{nv, (uint32_t)(pieces ? pieces : 1)};
+    return Cut{nv, (uint32_t)ceil_div(vectors, TOP_NT * nv)};
 }
 
 uint64_t top_bytes(uint64_t rows, uint32_t pieces, uint32_t k)
