@@ -276,6 +276,14 @@ __device__ inline f32x4 block_product(const Wide &x, const Wide &y)
     return p;
 }
 
+// What lanes of a wave wrote to LDS is read by others after this, and the other way round (a
+// wave's LDS operations are done in order).
+__device__ inline void wave_lds_fence()
+{
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+}
+
 // 16 (or 4) bytes a lane from global memory straight into LDS, at `lds` + 16 (4) * lane.
 using lds_ptr = __attribute__((address_space(3))) void *;
 __device__ inline void to_lds16(__amdgpu_buffer_rsrc_t from, uint32_t offset, uint32_t advance, void *lds)
@@ -451,29 +459,58 @@ __global__ __launch_bounds__(WM * WN * 64, 2) void ung_fp8_product_kernel(const 
             step(odd, even, kb + 1);
     }
 
-    const uint64_t col = n0 + wn + (lane >> 4) * 16;
-    if (col >= n)
+    // A lane holds 16 columns of a row.  16-bit results go out as they lie if rows of c allow
+    // vectors (1000 x 100000 x 128 49 us, turned 53).  Else 16 rows at a time are turned in LDS, so
+    // that a store's lanes write neighbouring elements: 1000 x 30000 x 384 in 32 bits 40 us, as
+    // they lie 58; 1000 x 100001 x 128 in 16 bits 83, 387.
+    constexpr uint32_t PITCH = 64 * sizeof(OT) + 16, N = Vec<OT>::N;
+    static_assert(16 * PITCH * WAVES <= sizeof(Panels), "");
+    const bool turned = sizeof(OT) == 4 || !vector_stores || n0 + BN > n;
+    if (turned)
+        __syncthreads(); // every wave is done with the panels
+    if (n0 + wn >= n)
         return;
+    uint8_t *own = reinterpret_cast<uint8_t *>(&even) + wave * (16 * PITCH);
+    const bool vectors = vector_stores && n0 + wn + 64 <= n;
 #pragma unroll
     for (int i = 0; i < TM; ++i) {
-        const uint64_t row = m0 + wm + i * 16 + (lane & 15);
-        if (row >= m)
-            break;
-        OT *to = c + (at.split * m + row) * c_stride + col;
-        Vec<OT> o[16 / Vec<OT>::N];
+        const uint64_t row0 = m0 + wm + i * 16;
+        const uint32_t rows = (uint32_t)min(m > row0 ? m - row0 : 0, (uint64_t)16);
+        OT *to = c + (at.split * m + row0) * c_stride + n0 + wn;
+        Vec<OT> o[16 / N];
 #pragma unroll
         for (int e = 0; e < 16; e += 2)
-            o[e / Vec<OT>::N].put2(e % Vec<OT>::N, acc[i][e / 4][e % 4], acc[i][e / 4][e % 4 + 1]);
-        if (vector_stores && col + 16 <= n) {
+            o[e / N].put2(e % N, acc[i][e / 4][e % 4], acc[i][e / 4][e % 4 + 1]);
+        if (!turned) {
+            if (r < rows)
 #pragma unroll
-            for (int h = 0; h < 16 / Vec<OT>::N; ++h)
-                reinterpret_cast<Vec<OT> *>(to)[h] = o[h];
-        } else {
-#pragma unroll
-            for (int e = 0; e < 16; ++e)
-                if (col + e < n)
-                    to[e] = o[e / Vec<OT>::N].element(e % Vec<OT>::N);
+                for (int x = 0; x < 16 / N; ++x)
+                    *reinterpret_cast<Vec<OT> *>(to + r * c_stride + g * 16 + x * N) = o[x];
+            continue;
         }
+#pragma unroll
+        for (int x = 0; x < 16 / N; ++x)
+            *reinterpret_cast<Vec<OT> *>(own + r * PITCH + (g * 16 + x * N) * sizeof(OT)) = o[x];
+        wave_lds_fence();
+        if (vectors) {
+            constexpr uint32_t LANES = 64 / N; // that hold a row
+            const uint32_t y0 = lane / LANES, x = lane % LANES * N;
+#pragma unroll
+            for (uint32_t y = 0; y < 16; y += N)
+                if (y + y0 < rows)
+                    *reinterpret_cast<Vec<OT> *>(to + (y + y0) * c_stride + x) =
+                        *reinterpret_cast<const Vec<OT> *>(own + (y + y0) * PITCH + x * sizeof(OT));
+        } else if (n0 + wn + lane < n) {
+            OT v[16];
+#pragma unroll
+            for (uint32_t y = 0; y < 16; ++y)
+                v[y] = *reinterpret_cast<const OT *>(own + y * PITCH + lane * sizeof(OT));
+#pragma unroll
+            for (uint32_t y = 0; y < 16; ++y)
+                if (y < rows)
+                    to[y * c_stride + lane] = v[y];
+        }
+        wave_lds_fence();
     }
 }
 
@@ -613,7 +650,8 @@ __device__ inline void place(uint32_t lane, int x, uint32_t &row, uint32_t &col)
 // (at the end, loads of one row that nobody reads): so the compiler knows which loads a read
 // of LDS depends on, and adds no wait of its own.
 // SQUARE: b's scales by square.  WHOLE: results go out in vectors of 16 bytes, n and the rows'
-// alignment allow it; else one by one.
+// alignment allow it; else they are turned in LDS first (4096 x 32767 x 768, row scales: 195 us;
+// one by one as they lie 559; 4096 x 32768 164).
 template <bool SQUARE, bool WHOLE, class OT>
 __global__ __launch_bounds__(512, 2) void ung_fp8_big_product_kernel(const uint8_t *a, const float *a_scale,
                                                                      const uint8_t *b, const float *b_scale,
@@ -625,9 +663,12 @@ __global__ __launch_bounds__(512, 2) void ung_fp8_big_product_kernel(const uint8
     __shared__ alignas(16) uint8_t a0_even[BIG / 2 * KB], a0_odd[BIG / 2 * KB];
     __shared__ alignas(16) uint8_t a1_even[BIG / 2 * KB], a1_odd[BIG / 2 * KB];
     __shared__ alignas(16) float s_even[2 * BIG], s_odd[2 * BIG]; // scales of a, then of b
+    constexpr uint32_t PITCH = 32 * sizeof(OT) + 16; // results of 32 x 32, for rows that allow no vectors
+    __shared__ alignas(16) uint8_t turn_area[WHOLE ? 16 : 8 * 32 * PITCH];
     const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const uint32_t wm = wave & 1, wn = wave >> 1; // halves of m, quarters of n
     const uint32_t kp = kblocks * KB;
+    uint8_t *const own = turn_area + (WHOLE ? 0 : wave * (32 * PITCH));
 
     // ---- loads: a wave loads rows (i * 8 + wave) * 8 + lane / 8 of a panel ----
     const uint32_t line = wave * 8 + (lane >> 3);
@@ -758,7 +799,9 @@ __global__ __launch_bounds__(512, 2) void ung_fp8_big_product_kernel(const uint8
     };
 
     auto store = [&]() {
-        const uint32_t row0 = wm * 128 + r, col0 = wn * 64 + h * 16;
+        uint32_t l = lane;
+        asm volatile("" : "+v"(l)); // places are made here, not kept from tile to tile
+        const uint32_t r = l & 31, h = l >> 5;
         const uint32_t rows = min(m - now.m0, (uint32_t)BIG);
         // rows of shares are whole vectors long: what lies past n is not read again
         const uint32_t cols = min((sizeof(OT) == 4 ? (n + 3) / 4 * 4 : n) - now.n0, (uint32_t)BIG);
@@ -768,7 +811,6 @@ __global__ __launch_bounds__(512, 2) void ung_fp8_big_product_kernel(const uint8
         for (int i = 0; i < 4; ++i)
 #pragma unroll
             for (int j = 0; j < 2; ++j) {
-                const uint32_t row = row0 + i * 32, col = col0 + j * 32;
                 Vec<OT> o[16 / Vec<OT>::N];
 #pragma unroll
                 for (int e = 0; e < 16; e += 2)
@@ -778,7 +820,7 @@ __global__ __launch_bounds__(512, 2) void ung_fp8_big_product_kernel(const uint8
 #pragma unroll
                     for (int x = 0; x < 16 / Vec<OT>::N; ++x) {
                         uint32_t row_x, col_x;
-                        place<OT>(lane, x, row_x, col_x);
+                        place<OT>(l, x, row_x, col_x);
                         row_x += wm * 128 + i * 32;
                         col_x += wn * 64 + j * 32;
                         // out of range: the store is dropped
@@ -787,12 +829,18 @@ __global__ __launch_bounds__(512, 2) void ung_fp8_big_product_kernel(const uint8
                                                 : 0x80000000u;
                         __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, o[x]), to, at, 0, 0);
                     }
-                } else if (row < rows) {
-                    OT *out = tile + row * c_stride + col;
+                } else { // turned in LDS: a store's lanes write neighbouring elements of two rows
 #pragma unroll
-                    for (int e = 0; e < 16; ++e)
-                        if (col + e < cols)
-                            out[e] = o[e / Vec<OT>::N].element(e % Vec<OT>::N);
+                    for (int x = 0; x < 16 / Vec<OT>::N; ++x)
+                        *reinterpret_cast<Vec<OT> *>(own + r * PITCH + h * 16 * sizeof(OT) + x * 16) = o[x];
+                    wave_lds_fence();
+                    const uint32_t row = wm * 128 + i * 32 + h, col = wn * 64 + j * 32 + r;
+#pragma unroll 4
+                    for (uint32_t y = 0; y < 32; y += 2)
+                        if (row + y < rows && col < cols)
+                            tile[(row + y) * c_stride + col] =
+                                *reinterpret_cast<const OT *>(own + (y + h) * PITCH + r * sizeof(OT));
+                    wave_lds_fence();
                 }
             }
     };
@@ -868,6 +916,7 @@ __global__ __launch_bounds__(256) void ung_fp8_join_kernel(const float *part, ui
     for (uint64_t at = blockIdx.x * 256ull + threadIdx.x; at < rows * chunks; at += gridDim.x * 256ull) {
         const uint64_t row = at / chunks, col = (at - row * chunks) * 4;
         f32x4 sum = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll 8
         for (uint32_t s = 0; s < splits; ++s)
             sum += *reinterpret_cast<const f32x4 *>(part + (s * rows + row) * part_stride + col);
 #pragma unroll
@@ -913,30 +962,37 @@ struct Plan {
 // 300 x 1000 x 128 6.7, 4.8.
 // Tiles of 32 rows for up to 32 rows: 1 x 1000000 x 384 in 32 bits 84 against 135, 16 x 32768
 // x 768 5.6, 6.9, 1 x 10000 x 128 3.5, 3.9.
-// Shares where tiles leave CUs free: at least four, or the pass that joins them costs what they
-// save (1024 x 1024 x 2048 in two 18.5 against 14.0), of at least 8 blocks (BIG: 32, 4096 x 768
-// x 8192 in shares of 16 54 against 49).  150 x 150 x 65536 33 against 328 in one, 4096 x 768 x
-// 32768 129 against 175.
+// Shares of the inner length where tiles leave CUs free.  BIG: at least four of at least 32
+// blocks (4096 x 768 x 32768 129 us, 128 x 128 tiles 175; 4096 x 768 x 8192 in shares of 16 54, 49).
+// Else as many as make the sum of the stages one share takes (0.6 us each; in 32 bits 1.4) and
+// of the joining pass (4 us, and its traffic at 3 TB/s) least: XXX
 Plan plan_of(uint64_t m, uint64_t n, uint64_t kp, int type)
 {
     const uint64_t kblocks = kp / KB, cus = cu_count();
-    auto shares = [&](uint64_t tiles, uint64_t places, uint64_t least) {
-        const uint64_t by_place = places / tiles, by_k = kblocks / least, s = by_place < by_k ? by_place : by_k;
-        return s >= 4 ? (uint32_t)s : 1u;
-    };
     Plan p = {false, false, 1};
     if (m == 0 || n == 0 || kblocks == 0) // (a product of no length: 128 x 128 tiles of zeros)
         return p;
     if (type != UNG_HIP_F32 && m > 128 && n > 128) {
         const uint64_t tiles = ceil_div(m, BIG) * ceil_div(n, BIG);
-        p.splits = shares(tiles, cus, 32);
+        const uint64_t by_cu = cus / tiles, by_k = kblocks / 32, s = by_cu < by_k ? by_cu : by_k;
+        p.splits = s >= 4 ? (uint32_t)s : 1;
         const uint64_t items = tiles * p.splits;
         p.big = items * 8 > ceil_div(items, cus) * cus * 5;
         if (p.big)
             return p;
     }
     p.few = m <= 32;
-    p.splits = shares(ceil_div(m, p.few ? 32 : 128) * ceil_div(n, 128), 2 * cus, 8);
+    p.splits = 1;
+    const uint64_t tiles = ceil_div(m, p.few ? 32 : 128) * ceil_div(n, 128);
+    const double stage = type == UNG_HIP_F32 ? 1.4 : 0.6, traffic = (double)m * (double)n * 8 / 3e6;
+    double best = stage * (double)kblocks;
+    for (uint64_t s = 2; s * tiles <= 2 * cus && s * 2 <= kblocks; ++s) {
+        const double cost = stage * (double)ceil_div(kblocks, s) + 4.0 + (0.1 + traffic) * (double)s;
+        if (cost < best) {
+            best = cost;
+            p.splits = (uint32_t)s;
+        }
+    }
     return p;
 }
 

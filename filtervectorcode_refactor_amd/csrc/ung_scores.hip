@@ -168,7 +168,7 @@ __device__ inline uint32_t limit_of(const uint32_t *most, uint32_t k)
 
 // The k-th largest of the orders that a block holds (each(f) calls f with those of a thread; 0
 // = none), bit by bit over the whole block: for rows of many equal scores, where the
-// candidates above the threads' limit do not fit.  There are at least k.
+// candidates above the threads' limit do not fit.  0: there are fewer than k.
 template <class Each>
 __device__ inline uint64_t kth_order(TopShared &sh, uint32_t k, Each each)
 {
@@ -194,6 +194,26 @@ __device__ inline uint64_t kth_order(TopShared &sh, uint32_t k, Each each)
     return limit;
 }
 
+// The k-th largest key of up to TOP_CAP candidates, by one wave as in limit_of; 0 if there are
+// fewer than k.
+template <int LOW>
+__device__ inline uint32_t kth_key(const uint64_t *cand, uint32_t found, uint32_t k)
+{
+    uint32_t m[TOP_CAP / 64], limit = 0;
+#pragma unroll
+    for (int i = 0; i < TOP_CAP / 64; ++i)
+        m[i] = i * 64 + (threadIdx.x & 63) < found ? (uint32_t)(cand[i * 64 + (threadIdx.x & 63)] >> 32) : 0;
+    for (int bit = 31; bit >= LOW; --bit) {
+        const uint32_t trial = limit | 1u << bit;
+        uint32_t n = 0;
+#pragma unroll
+        for (int i = 0; i < TOP_CAP / 64; ++i)
+            n += __popcll(__ballot(m[i] >= trial));
+        limit = n >= k ? trial : limit;
+    }
+    return limit;
+}
+
 __device__ inline void add_candidate(TopShared &sh, uint64_t order)
 {
     const uint32_t at = atomicAdd(&sh.count, 1u);
@@ -204,7 +224,7 @@ __device__ inline void add_candidate(TopShared &sh, uint64_t order)
 // Results of a row (or of a part of one) whose first k orders are among sh.cand[0..count):
 // each candidate's place is the number of candidates above it.  Where the candidates did not
 // fit, they are collected anew from the k-th order on.
-template <class Each>
+template <int LOW, class Each>
 __device__ inline void finish_top(TopShared &sh, uint32_t k, Each each, uint64_t row, bool last, float *values,
                                   int32_t *ids, float *lse, uint64_t *part, float2 *part_sum, float top, float sum,
                                   Temperature t)
@@ -217,11 +237,32 @@ __device__ inline void finish_top(TopShared &sh, uint32_t k, Each each, uint64_t
             sh.count = 0;
         __syncthreads();
         each([&](uint64_t o) {
-            if (o >= limit)
+            if (o && o >= limit) // limit 0: fewer than k
                 add_candidate(sh, o);
         });
         __syncthreads();
-        found = sh.count; // k: orders are distinct
+        found = sh.count; // k at most: orders are distinct
+    } else if (found > 320) {
+        // ranking compares every two candidates: with the k-th key of them, few are left
+        uint64_t mine[TOP_CAP / TOP_NT];
+#pragma unroll
+        for (int i = 0; i < TOP_CAP / TOP_NT; ++i)
+            mine[i] = i * TOP_NT + tid < found ? sh.cand[i * TOP_NT + tid] : 0;
+        if (tid < 64) {
+            const uint32_t limit = kth_key<LOW>(sh.cand, found, k);
+            if (tid == 0) {
+                sh.limit = limit;
+                sh.count = 0;
+            }
+        }
+        __syncthreads();
+        const uint64_t least = sh.limit ? (uint64_t)sh.limit << 32 : 1;
+#pragma unroll
+        for (int i = 0; i < TOP_CAP / TOP_NT; ++i)
+            if (mine[i] >= least)
+                add_candidate(sh, mine[i]);
+        __syncthreads();
+        found = sh.count;
     }
     auto put = [&](uint32_t place, uint64_t o) {
         if (last) {
@@ -293,14 +334,13 @@ __global__ __launch_bounds__(TOP_NT, 4) void ung_top_scores_kernel(const T *scor
     });
     sum = block_reduce<TOP_NT>(sum, sh.red[1], add);
     // the rest looks at few vectors, and reads those again
-    const T *row = ref.row;
     const uint32_t shift = ref.shift, first = x.first, edge_at = x.edge_at, slots = NV + (x.has_edge ? 1 : 0);
     auto scan = [=](uint32_t i, auto f) {
-        const uint32_t from = (i < NV ? first + i * TOP_NT : edge_at) * N - shift;
-#pragma unroll 1
-        for (uint32_t e = 0; e < N; ++e)
-            if (from + e < len)
-                f(to_float(row[from + e]), from + e);
+        const uint32_t at = i < NV ? first + i * TOP_NT : edge_at;
+        const Vec<T> v = ref.load(at); // -inf outside the row
+#pragma unroll
+        for (int e = 0; e < N; ++e)
+            f(v.get(e), at * N + e - shift);
     };
     auto each = [=](auto f) {
         for (uint32_t i = 0; i < slots; ++i)
@@ -331,7 +371,7 @@ __global__ __launch_bounds__(TOP_NT, 4) void ung_top_scores_kernel(const T *scor
         any = block_reduce<TOP_NT>(any, sh.red[0], add);
         out_top = any > 0.0f ? sum : __builtin_inff();
     }
-    finish_top(sh, k, each, blockIdx.x, pieces == 1, values, ids, lse, part, part_sum, out_top, out_sum, t);
+    finish_top<LOW>(sh, k, each, blockIdx.x, pieces == 1, values, ids, lse, part, part_sum, out_top, out_sum, t);
 }
 
 constexpr uint32_t MERGE_LISTS = 64; // lists one block merges
@@ -388,7 +428,7 @@ __global__ __launch_bounds__(TOP_NT) void ung_top_merge_kernel(const uint64_t *p
             add_candidate(sh, o);
     });
     __syncthreads();
-    finish_top(sh, k, each, blockIdx.x, groups == 1, values, ids, lse, out, out_sum, top, sum, t);
+    finish_top<0>(sh, k, each, blockIdx.x, groups == 1, values, ids, lse, out, out_sum, top, sum, t);
 }
 
 // ---- distillation --------------------------------------------------------------------

@@ -536,6 +536,31 @@ def test_distill(n, v, k, kind, tail):
         _check_distill(x, view, ids, val, lse if tail else None, t, kind, n)
 
 
+@pytest.mark.parametrize("kind", ["fp32", "bf16"])
+@pytest.mark.parametrize("v", [200, 5000, 40000])
+def test_top_of_a_row_with_nan_and_few_scores(v, kind):
+    """A NaN, two scores and nothing else: NaN is first, the rest of a long list is missing."""
+    x = torch.full((3, v), -math.inf)
+    x[1, v // 2], x[1, 3], x[1, v - 1] = math.nan, -2.0, 5.0
+    x[2, 7] = math.nan
+    values, ids, lse = (t.cpu() for t in S.top_scores(x.to(TYPES[kind]).cuda(), 128))
+    assert ids[1, :3].tolist() == [v // 2, v - 1, 3] and values[1, 1:3].tolist() == [5.0, -2.0]
+    assert ids[2, 0] == 7 and torch.isnan(values[1:, 0]).all() and torch.isnan(lse[1:]).all()
+    assert (ids[0] == -1).all() and (ids[1, 3:] == -1).all() and (ids[2, 1:] == -1).all() and lse[0] == -math.inf
+    assert (values[0] == -math.inf).all() and (values[1, 3:] == -math.inf).all()
+
+
+@pytest.mark.parametrize("kind", ["fp32", "bf16"])
+@pytest.mark.parametrize("n,v,k", [(40, 849, 100), (9, 1000, 128), (5, 130, 128), (3, 100000, 128), (70, 3000, 128)])
+def test_long_lists_of_short_rows(n, v, k, kind):
+    """k close to the number of a block's threads that hold scores: nearly all are candidates."""
+    x = torch.randn(n, v, generator=_gen(n + v)).to(TYPES[kind])
+    values, ids, _ = S.top_scores(x.cuda(), k)
+    order = np.lexsort((np.broadcast_to(np.arange(v), (n, v)), -x.double().numpy()))[:, :k]
+    assert (ids.cpu().numpy() == order).all()
+    assert torch.equal(values.cpu(), torch.gather(x.float(), 1, torch.from_numpy(order)))
+
+
 @pytest.mark.parametrize("v", [300, 5000, 70000])
 def test_distill_is_the_same_every_time(v):
     """Columns named many times over: sums keep their order whichever entry is seen first."""
