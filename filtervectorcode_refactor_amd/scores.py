@@ -136,20 +136,24 @@ def quantize_fp8(x, block="row", transpose=False):
     kind, stride = _matrix("x", x)
     if block not in ("row", "square"):
         raise ValueError(f'block: "row" or "square" is needed, got {block!r}')
-    square = block == "square"
-    n, d = x.shape
-    nb, db = _blocks(n), _blocks(d)
-    q = torch.empty(n, db * BLOCK, dtype=FP8, device=x.device)
-    scale = torch.empty(nb if square else n, db, device=x.device)
-    qt = scale_t = None
-    if transpose:
-        qt = torch.empty(d, nb * BLOCK, dtype=FP8, device=x.device)
-        scale_t = torch.empty(db if square else d, nb, device=x.device)
     with _On(x) as stream:
-        check(_library().ung_hip_fp8_quantize(x.data_ptr(), kind, n, d, stride, square, q.data_ptr(), scale.data_ptr(),
-                                              qt.data_ptr() if transpose else None,
-                                              scale_t.data_ptr() if transpose else None, stream))
-    return (q, scale, qt, scale_t) if transpose else (q, scale)
+        return _quantize(x, kind, stride, block == "square", transpose, _library(), stream)
+
+
+def _quantize(x, kind, row_stride, square, transpose, lib, stream):
+    n, d = x.shape
+    nb, db, device = _blocks(n), _blocks(d), x.device
+    q = torch.empty(n, db * BLOCK, dtype=FP8, device=device)
+    scale = torch.empty(nb if square else n, db, device=device)
+    if not transpose:
+        check(lib.ung_hip_fp8_quantize(x.data_ptr(), kind, n, d, row_stride, square, q.data_ptr(), scale.data_ptr(),
+                                       None, None, stream))
+        return q, scale
+    qt = torch.empty(d, nb * BLOCK, dtype=FP8, device=device)
+    scale_t = torch.empty(db if square else d, nb, device=device)
+    check(lib.ung_hip_fp8_quantize(x.data_ptr(), kind, n, d, row_stride, square, q.data_ptr(), scale.data_ptr(),
+                                   qt.data_ptr(), scale_t.data_ptr(), stream))
+    return q, scale, qt, scale_t
 
 
 def _operand(name, q, scale, like=None):
@@ -176,19 +180,22 @@ def matmul_fp8(a, a_scale, b, b_scale, dtype=torch.bfloat16):
     16-bit ones by the 8-bit matrix instruction (errors of 1.4e-5 of their norm)."""
     m, kp, a_square = _operand("a", a, a_scale)
     n, b_kp, square = _operand("b", b, b_scale, a)
-    kind = _TYPES.get(dtype)
     if a_square:
         raise ValueError("a: row scales are needed")
-    if kind is None:
+    if dtype not in _TYPES:
         raise ValueError(f"dtype: float32, float16 or bfloat16 is needed, got {dtype}")
     if b_kp != kp:
         raise ValueError(f"a and b: rows of {kp} and {b_kp} bytes do not go together")
-    c = torch.empty(m, n, dtype=dtype, device=a.device)
-    lib = _library()
     with _On(a) as stream:
-        keep, at, size = _workspace(lib.ung_hip_fp8_matmul_workspace, m, n, kp, kind, device=a.device)
-        check(lib.ung_hip_fp8_matmul(a.data_ptr(), a_scale.data_ptr(), b.data_ptr(), b_scale.data_ptr(), square, m, n,
-                                     kp, c.data_ptr(), kind, n, at, size, stream))
+        return _product(a, a_scale, b, b_scale, square, m, n, kp, dtype, _library(), stream)
+
+
+def _product(a, a_scale, b, b_scale, square, m, n, kp, dtype, lib, stream):
+    kind, device = _TYPES[dtype], a.device
+    c = torch.empty(m, n, dtype=dtype, device=device)
+    keep, at, size = _workspace(lib.ung_hip_fp8_matmul_workspace, m, n, kp, kind, device=device)
+    check(lib.ung_hip_fp8_matmul(a.data_ptr(), a_scale.data_ptr(), b.data_ptr(), b_scale.data_ptr(), square, m, n, kp,
+                                 c.data_ptr(), kind, n, at, size, stream))
     return c
 
 
@@ -196,14 +203,21 @@ def matmul_fp8_grad(g, xt, xt_scale, wt, wt_scale):
     """Gradients of y = x w^T from g = dy: (dx in g's type, dw in float32).  xt, wt: the
     transposed operands of x (row scales along its rows) and of w (square or row scales), as
     quantize_fp8 gives them; g is brought to 8 bits both ways round in one pass."""
-    _matrix("g", g)
-    (m, n), d = g.shape, wt.shape[0]
-    _need(xt.dim() == 2 and wt.dim() == 2 and xt.shape[0] == d, "xt and wt: the same number of rows is needed")
-    _need(xt.shape[1] == _blocks(m) * BLOCK, f"xt: rows of {_blocks(m) * BLOCK} bytes are needed for {m} rows of g")
-    _need(wt.shape[1] == _blocks(n) * BLOCK, f"wt: rows of {_blocks(n) * BLOCK} bytes are needed for {n} columns of g")
-    q, scale, qt, scale_t = quantize_fp8(g, transpose=True)
-    return (matmul_fp8(q, scale, wt, wt_scale, dtype=g.dtype),
-            matmul_fp8(qt, scale_t, xt, xt_scale, dtype=torch.float32))
+    kind, stride = _matrix("g", g)
+    d, xt_len, xt_square = _operand("xt", xt, xt_scale, g)
+    wt_rows, wt_len, wt_square = _operand("wt", wt, wt_scale, g)
+    m, n = g.shape
+    if wt_rows != d:
+        raise ValueError("xt and wt: the same number of rows is needed")
+    if xt_len != _blocks(m) * BLOCK:
+        raise ValueError(f"xt: rows of {_blocks(m) * BLOCK} bytes are needed for {m} rows of g")
+    if wt_len != _blocks(n) * BLOCK:
+        raise ValueError(f"wt: rows of {_blocks(n) * BLOCK} bytes are needed for {n} columns of g")
+    lib = _library()
+    with _On(g) as stream:
+        q, scale, qt, scale_t = _quantize(g, kind, stride, False, True, lib, stream)
+        return (_product(q, scale, wt, wt_scale, wt_square, m, d, wt_len, g.dtype, lib, stream),
+                _product(qt, scale_t, xt, xt_scale, xt_square, n, d, xt_len, torch.float32, lib, stream))
 
 
 class _LinearFp8(torch.autograd.Function):
