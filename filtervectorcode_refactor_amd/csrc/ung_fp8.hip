@@ -997,21 +997,19 @@ __global__ __launch_bounds__(512, 2) void ung_fp8_big_product_kernel(const uint8
     load_a(a0_odd, 0, ahead, 0, 2);
     Item mid = ahead;
     advance();
-    // the number of stages ends the loop: a flag would have the two panels' stages follow
-    // themselves in the compiler's eyes
+    // the number of stages ends the loop, in pairs: with a flag, or an exit between the two, the
+    // compiler takes the other panels' loads for these
     uint32_t left = 0;
     for (Items i = items; i.left; i.next()) {
         const Item item(i.id, m_tiles, n_tiles, kblocks, splits);
         left += item.kb_end - item.kb;
     }
-    for (;;) {
+    for (uint32_t pairs = left / 2; pairs; --pairs) {
         stage(b_even, a0_even, a1_even, s_even, a1_odd, s_odd, mid);
-        if (--left == 0)
-            break;
         stage(b_odd, a0_odd, a1_odd, s_odd, a1_even, s_even, mid);
-        if (--left == 0)
-            break;
     }
+    if (left & 1)
+        stage(b_even, a0_even, a1_even, s_even, a1_odd, s_odd, mid);
     await_loads<0>(); // nothing may land in LDS that is another block's by then
 }
 
