@@ -91,6 +91,12 @@ __device__ inline Vec<T> load_loose(const T *p)
     return v;
 }
 
+template <class T>
+__device__ inline void store_loose(T *p, const Vec<T> &v)
+{
+    __builtin_memcpy(p, &v, sizeof v);
+}
+
 // Eight consecutive elements of a row from column c; those at or past `cols` are 0.
 template <class T>
 __device__ inline void load8(const T *row, uint64_t c, uint64_t cols, float *x)
@@ -577,10 +583,11 @@ __global__ __launch_bounds__(WM * WN * 64, 2) void ung_fp8_product_kernel(const 
             step(odd, even, kb + 1);
     }
 
-    // A lane holds 16 columns of a row.  16-bit results go out as they lie if rows of c allow
-    // vectors (1000 x 100000 x 128 49 us, turned 53).  Else 16 rows at a time are turned in LDS, so
-    // that a store's lanes write neighbouring elements: 1000 x 30000 x 384 in 32 bits 40 us, as
-    // they lie 58; 1000 x 100001 x 128 in 16 bits 83, 387.
+    // A lane holds 16 columns of a row.  16-bit results go out as they lie if rows of c lie at
+    // 4-byte boundaries (1000 x 100000 x 128 49 us, turned 53; 1000 x 100004 54, one by one 83).  Else
+    // 16 rows at a time are turned in LDS, so that a store's lanes write neighbouring elements:
+    // 1000 x 30000 x 384 in 32 bits 40 us, as they lie 58; 1000 x 100001 x 128 in 16 bits 83, as they
+    // lie 387, in vectors off 4-byte boundaries 100.
     constexpr int N = Vec<OT>::N, PITCH = 64 * sizeof(OT) + 16;
     static_assert(16 * PITCH * WAVES <= sizeof(Panels), "");
     const bool turned = sizeof(OT) == 4 || !vector_stores || n0 + BN > n;
@@ -603,7 +610,7 @@ __global__ __launch_bounds__(WM * WN * 64, 2) void ung_fp8_product_kernel(const 
             if (r < rows)
 #pragma unroll
                 for (int x = 0; x < 16 / N; ++x)
-                    *reinterpret_cast<Vec<OT> *>(to + r * c_stride + g * 16 + x * N) = o[x];
+                    store_loose(to + r * c_stride + g * 16 + x * N, o[x]);
             continue;
         }
 #pragma unroll
@@ -616,8 +623,8 @@ __global__ __launch_bounds__(WM * WN * 64, 2) void ung_fp8_product_kernel(const 
 #pragma unroll
             for (uint32_t y = 0; y < 16; y += N)
                 if (y + y0 < rows)
-                    *reinterpret_cast<Vec<OT> *>(to + (y + y0) * c_stride + x) =
-                        *reinterpret_cast<const Vec<OT> *>(own + (y + y0) * PITCH + x * sizeof(OT));
+                    store_loose(to + (y + y0) * c_stride + x,
+                                *reinterpret_cast<const Vec<OT> *>(own + (y + y0) * PITCH + x * sizeof(OT)));
         } else if (n0 + wn + lane < n) {
             OT v[16];
 #pragma unroll
@@ -767,15 +774,16 @@ __device__ inline void place(uint32_t lane, int x, uint32_t &row, uint32_t &col)
 //   Panels lie in LDS variables of their own, and every path makes the same loads and stores
 // (at the end, loads of one row that nobody reads): so the compiler knows which loads a read
 // of LDS depends on, and adds no wait of its own.
-// SQUARE: b's scales by square.  WHOLE: results go out in vectors of 16 bytes, n and the rows'
-// alignment allow it; else they are turned in LDS first (4096 x 32767 x 768, row scales: 195 us;
-// one by one as they lie 559; 4096 x 32768 164).
+// SQUARE: b's scales by square.  WHOLE: n is whole vectors of 16 bytes and rows of c lie at
+// 4-byte boundaries, so results go out in vectors; with `vector_stores` all but the last
+// columns; else they are turned in LDS first.  4096 x 32768 x 768 140 us, 32764 142 (turned 170),
+// 32767 170 (in vectors 194; one by one as they lie 559 by rows' scales, turned 189).
 template <bool SQUARE, bool WHOLE, class OT>
 __global__ __launch_bounds__(512, 2) void ung_fp8_big_product_kernel(const uint8_t *a, const float *a_scale,
                                                                      const uint8_t *b, const float *b_scale,
                                                                      uint32_t m, uint32_t n, uint32_t kblocks, OT *c,
                                                                      uint64_t c_stride, uint32_t m_tiles,
-                                                                     uint32_t n_tiles, uint32_t splits)
+                                                                     uint32_t n_tiles, uint32_t splits, int vector_stores)
 {
     __shared__ alignas(16) uint8_t b_even[BIG * KB], b_odd[BIG * KB];
     __shared__ alignas(16) uint8_t a0_even[BIG / 2 * KB], a0_odd[BIG / 2 * KB];
@@ -946,6 +954,24 @@ __global__ __launch_bounds__(512, 2) void ung_fp8_big_product_kernel(const uint8
                                                 ? (row_x * (uint32_t)c_stride + col_x) * (uint32_t)sizeof(OT)
                                                 : 0x80000000u;
                         __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, o[x]), to, at, 0, 0);
+                    }
+                } else if (vector_stores) { // the last columns one by one
+                    spread(o);
+#pragma unroll
+                    for (int x = 0; x < 16 / Vec<OT>::N; ++x) {
+                        uint32_t row_x, col_x;
+                        place<OT>(l, x, row_x, col_x);
+                        row_x += wm * 128 + i * 32;
+                        col_x += wn * 64 + j * 32;
+                        OT *out = tile + row_x * c_stride + col_x;
+                        if (row_x < rows && col_x + Vec<OT>::N <= cols)
+                            store_loose(out, o[x]);
+                        else if (row_x < rows) {
+#pragma unroll
+                            for (int e = 0; e < Vec<OT>::N; ++e)
+                                if (col_x + e < cols)
+                                    out[e] = o[x].element(e);
+                        }
                     }
                 } else { // turned in LDS: a store's lanes write neighbouring elements of two rows
 #pragma unroll
@@ -1229,7 +1255,7 @@ int ung_hip_fp8_matmul(const uint8_t *a, const float *a_scale, const uint8_t *b,
     const hipStream_t st = (hipStream_t)stream;
     return with_type(type, [&](auto zero) {
         using T = decltype(zero);
-        const bool vec = (uintptr_t)c % 16 == 0 && (m == 1 || c_stride * sizeof(T) % 16 == 0);
+        const bool vec = (uintptr_t)c % 4 == 0 && (m == 1 || c_stride * sizeof(T) % 4 == 0);
         // `to` is c, or (splits > 1) the shares' sums
         auto make = [&](auto *to, uint64_t stride, bool vectors) {
             using OT = std::remove_reference_t<decltype(*to)>;
@@ -1242,7 +1268,7 @@ int ung_hip_fp8_matmul(const uint8_t *a, const float *a_scale, const uint8_t *b,
             };
             if constexpr (!EXACT) {
                 if (plan.big) {
-                    auto big = [&](auto kernel) { run(kernel, BIG, BIG, cu_count(), 512); };
+                    auto big = [&](auto kernel) { run(kernel, BIG, BIG, cu_count(), 512, vectors); };
                     bool whole = true; // shares' sums: rows of whole vectors, and not that many columns
                     if constexpr (sizeof(OT) == 2)
                         whole = vectors && n % Vec<T>::N == 0 && stride < (1u << 21);

@@ -347,8 +347,8 @@ int ung_hip_fp8_quantize(const void *x, int type, uint64_t rows, uint64_t cols, 
  * are summed in 32 bits throughout; 16-bit ones by the 8-bit matrix instruction, which keeps
  * 13 bits below the largest of each eight neighbouring products (1.4e-5 of the result's norm
  * on normal values).  a has row scales; b's are row scales (b_square = 0) or square ones
- * (b_square = 1: b_scale[j / 128][t]).  Rows of c may have any stride and alignment; from
- * 16-byte boundaries on, with n a multiple of 16 bytes, they are written fastest.  Gradients
+ * (b_square = 1: b_scale[j / 128][t]).  Rows of c may have any stride and alignment; at
+ * 4-byte boundaries they are written fastest.  Gradients
  * of the product are products of the same kind: with the upstream gradient g quantised both
  * ways, da = g (b^T)^T by the turned b, db = g^T (a^T)^T by the turned g and a. */
 int ung_hip_fp8_matmul_workspace(uint64_t m, uint64_t n, uint64_t kp, int type, uint64_t *bytes);

@@ -173,7 +173,7 @@ def _operand_there(n, d, block, seed):
 
 # one and several rounds of large tiles, ragged both ways; rows of c that allow vectors and not;
 # sums in shares, of large tiles, of small ones and of few rows
-LARGE = [(2300, 5000, 130, "square"), (2304, 5003, 100, "row"), (5000, 4504, 260, "row"), (6400, 7001, 128, "square"),
+LARGE = [(2300, 5000, 130, "square"), (2300, 5002, 130, "row"), (130, 1002, 256, "row"), (2304, 5003, 100, "row"), (5000, 4504, 260, "row"), (6400, 7001, 128, "square"),
          (4000, 708, 20500, "square"), (4000, 703, 20500, "row"), (150, 150, 9000, "square"), (33, 1030, 6000, "row"),
          (20, 3000, 5000, "square"), (1, 65, 8192, "row")]
 
@@ -192,7 +192,7 @@ def test_large_product(m, n, d, block):
         assert torch.equal(got, S.matmul_fp8(qa, sa, qb, sb, dtype=TYPES[kind])), kind
 
 
-@pytest.mark.parametrize("pad", [8, 3])
+@pytest.mark.parametrize("pad", [8, 2, 3])
 def test_large_product_into_wider_rows(pad):
     """c_stride above n, large tiles: what lies between the rows is left alone."""
     m, n, d = 2400, 4808, 256
