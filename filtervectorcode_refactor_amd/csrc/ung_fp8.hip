@@ -57,8 +57,9 @@ __device__ inline float scale_of(uint32_t most)
 // product's remainder, exact in a fused multiply-add, corrects it (Markstein's step; r is
 // itself correctly rounded, s is a normal number).  A block with an infinity has s = inf,
 // r = 0, where the step would make a NaN of every value: with s = 0 there it adds nothing.
-struct Divisor {
+struct alignas(8) Divisor {
     float s, r;
+    Divisor() = default;
     __device__ explicit Divisor(float scale) : s(scale), r(1.0f / scale)
     {
         if (r == 0.0f)
@@ -71,15 +72,12 @@ __device__ inline float quotient(float x, Divisor d)
     return __builtin_fmaf(__builtin_fmaf(-d.s, q, x), d.r, q);
 }
 
-__device__ inline uint2 pack8(const float *y)
+__device__ inline uint32_t pack4(const float *y)
 {
-    int lo = 0, hi = 0;
-    lo = __builtin_amdgcn_cvt_pk_fp8_f32(y[0], y[1], lo, false);
-    lo = __builtin_amdgcn_cvt_pk_fp8_f32(y[2], y[3], lo, true);
-    hi = __builtin_amdgcn_cvt_pk_fp8_f32(y[4], y[5], hi, false);
-    hi = __builtin_amdgcn_cvt_pk_fp8_f32(y[6], y[7], hi, true);
-    return make_uint2((uint32_t)lo, (uint32_t)hi);
+    int w = __builtin_amdgcn_cvt_pk_fp8_f32(y[0], y[1], 0, false);
+    return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(y[2], y[3], w, true);
 }
+__device__ inline uint2 pack8(const float *y) { return make_uint2(pack4(y), pack4(y + 4)); }
 
 // 16 bytes from an address that is aligned to its elements alone; global memory takes such
 // loads whole (300000 x 203 bf16 44 us, by elements 67).
@@ -148,45 +146,48 @@ __global__ __launch_bounds__(256) void ung_fp8_rows_kernel(const T *x, uint64_t 
     }
 }
 
-// 8 x 8 elements; those at or past `rows` or `cols` are 0.  All loads are under way before the
+constexpr int PR = 4;        // rows of a thread's patch
+constexpr int TILE_NT = 512; // threads of a tile: 128 / PR * 16
+
+// PR x 8 elements; those at or past `rows` or `cols` are 0.  All loads are under way before the
 // first value is used: those outside read the last row or column instead.
 template <class T>
 __device__ inline void load_patch(const T *x, uint64_t stride, uint64_t r0, uint64_t rows, uint64_t c0, uint64_t cols,
-                                  float (&v)[8][8])
+                                  float (&v)[PR][8])
 {
     constexpr int N = Vec<T>::N;
-    const T *row[8];
+    const T *row[PR];
 #pragma unroll
-    for (int i = 0; i < 8; ++i)
+    for (int i = 0; i < PR; ++i)
         row[i] = x + min(r0 + i, rows - 1) * stride;
     if (c0 + 8 <= cols) {
-        Vec<T> raw[8][8 / N];
+        Vec<T> raw[PR][8 / N];
 #pragma unroll
-        for (int i = 0; i < 8; ++i)
+        for (int i = 0; i < PR; ++i)
 #pragma unroll
             for (int h = 0; h < 8 / N; ++h)
                 raw[i][h] = load_loose(row[i] + c0 + h * N);
 #pragma unroll
-        for (int i = 0; i < 8; ++i)
+        for (int i = 0; i < PR; ++i)
 #pragma unroll
             for (int j = 0; j < 8; ++j)
                 v[i][j] = raw[i][j / N].get(j % N);
-        if (r0 + 8 > rows)
+        if (r0 + PR > rows)
 #pragma unroll
-            for (int i = 0; i < 8; ++i)
+            for (int i = 0; i < PR; ++i)
 #pragma unroll
                 for (int j = 0; j < 8; ++j)
                     v[i][j] = r0 + i < rows ? v[i][j] : 0.0f;
         return;
     }
-    T raw[8][8];
+    T raw[PR][8];
 #pragma unroll
-    for (int i = 0; i < 8; ++i)
+    for (int i = 0; i < PR; ++i)
 #pragma unroll
         for (int j = 0; j < 8; ++j)
             raw[i][j] = row[i][min(c0 + j, cols - 1)];
 #pragma unroll
-    for (int i = 0; i < 8; ++i)
+    for (int i = 0; i < PR; ++i)
 #pragma unroll
         for (int j = 0; j < 8; ++j)
             v[i][j] = r0 + i < rows && c0 + j < cols ? to_float(raw[i][j]) : 0.0f;
@@ -195,7 +196,7 @@ __device__ inline void load_patch(const T *x, uint64_t stride, uint64_t r0, uint
 // Largest magnitudes of a patch's rows and columns.  16-bit values are compared as such, in
 // pairs: v holds them in its upper halves (bf16), or they are made again (fp16), exactly.
 template <class T>
-__device__ inline void patch_magnitudes(const float (&v)[8][8], uint32_t (&row)[8], uint32_t (&col)[8])
+__device__ inline void patch_magnitudes(const float (&v)[PR][8], uint32_t (&row)[PR], uint32_t (&col)[8])
 {
     if constexpr (sizeof(T) == 2) {
         using u16x2 = __attribute__((ext_vector_type(2))) unsigned short;
@@ -215,7 +216,7 @@ __device__ inline void patch_magnitudes(const float (&v)[8][8], uint32_t (&row)[
         };
         u16x2 down[4] = {};
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
+        for (int i = 0; i < PR; ++i) {
             u16x2 across = {};
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
@@ -233,7 +234,7 @@ __device__ inline void patch_magnitudes(const float (&v)[8][8], uint32_t (&row)[
         for (int j = 0; j < 8; ++j)
             col[j] = 0;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
+        for (int i = 0; i < PR; ++i) {
             row[i] = 0;
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
@@ -246,34 +247,38 @@ __device__ inline void patch_magnitudes(const float (&v)[8][8], uint32_t (&row)[
 }
 
 // A 128 x 128 tile to 8 bits, both ways round: q with scales of its rows' blocks or of the
-// whole square, and (qt) the transposed rows with scales of theirs.  A thread holds an 8 x 8
-// patch, so a transposed row's eight bytes are packed in registers; they cross the block
-// through LDS and leave as whole 128-byte runs.  Bound by memory where rows are no power of two
-// apart, with about as much work for the vector units: 32768 x 768 bf16 with squares 23.5 us
-// (4.3 TB/s), 4096 x 32768 by rows 134 (4.0).
-//   Tiles that an XCD works on at a time lie side by side, two rows of them: rows a power of
-// two apart lie in the same few memory channels, and scales fill lines of the same L2 (4096 x
-// 32768 by rows, bands of 16, 4, 2, 1: 149, 141, 134, 135 us).
+// whole square, and (qt) the transposed rows with scales of theirs.  A thread holds a 4 x 8
+// patch, so four bytes of a transposed row are packed in registers; they cross the block
+// through LDS, 16-byte pieces rotated by their row against conflicts, and leave as whole
+// 128-byte runs.  A tile alone is bound by its threads' instructions (8 x 8 patches and each
+// thread with divisors of its own: 300 x 1000 bf16 9.0 us, this 6.2), many by memory: 32768 x 768
+// with squares 20.6 (4.9 TB/s; 23.4), 3740 x 5946 by rows 23.2 (3.8; 26.7), and rows a power of two
+// apart by its channels: 4096 x 32768 130 (4.1; 129).
+//   Tiles that an XCD works on at a time lie side by side, two rows of them, against that and
+// so that scales fill lines of the same L2 (8 x 8 patches, 4096 x 32768 by rows, bands of 16, 4,
+// 2, 1: 149, 141, 134, 135 us).
 template <class T, bool SQUARE>
-__global__ __launch_bounds__(256) void ung_fp8_tile_kernel(const T *x, uint64_t rows, uint64_t cols, uint64_t stride,
+__global__ __launch_bounds__(TILE_NT) void ung_fp8_tile_kernel(const T *x, uint64_t rows, uint64_t cols, uint64_t stride,
                                                            uint32_t col_blocks, uint32_t row_blocks, uint8_t *q,
                                                            float *scale, uint8_t *qt, float *scale_t)
 {
-    __shared__ uint32_t most_of[4][KB];
-    __shared__ alignas(16) uint8_t turned[KB][KB + 16];
+    constexpr int WAVES = TILE_NT / 64;
+    __shared__ uint32_t most_of[WAVES][KB];
+    __shared__ Divisor by_col[KB];
+    __shared__ alignas(16) uint8_t turned[KB][KB];
     uint32_t rb, cb;
     tile_of(xcd_run(blockIdx.x, row_blocks * col_blocks), 2, row_blocks, col_blocks, rb, cb);
     const uint32_t tr = threadIdx.x >> 4, tc = threadIdx.x & 15;
-    const uint64_t r0 = (uint64_t)rb * KB + tr * 8, c0 = (uint64_t)cb * KB + tc * 8;
-    float v[8][8], y[8];
+    const uint64_t r0 = (uint64_t)rb * KB + tr * PR, c0 = (uint64_t)cb * KB + tc * 8;
+    float v[PR][8], y[8];
     load_patch<T>(x, stride, r0, rows, c0, cols, v);
-    uint32_t row_most[8], col_most[8];
+    uint32_t row_most[PR], col_most[8];
     patch_magnitudes<T>(v, row_most, col_most);
     Divisor by_all(1.0f);
     if (SQUARE) {
         uint32_t most = 0;
 #pragma unroll
-        for (int i = 0; i < 8; ++i)
+        for (int i = 0; i < PR; ++i)
             most = max(most, row_most[i]);
 #pragma unroll
         for (int o = 32; o > 0; o >>= 1)
@@ -281,7 +286,9 @@ __global__ __launch_bounds__(256) void ung_fp8_tile_kernel(const T *x, uint64_t 
         if ((threadIdx.x & 63) == 0)
             most_of[0][threadIdx.x >> 6] = most;
         __syncthreads();
-        most = max(max(most_of[0][0], most_of[0][1]), max(most_of[0][2], most_of[0][3]));
+#pragma unroll
+        for (int w = 0; w < WAVES; ++w)
+            most = max(most, most_of[0][w]);
         const float s = scale_of(most);
         by_all = Divisor(s);
         if (threadIdx.x == 0) {
@@ -292,7 +299,7 @@ __global__ __launch_bounds__(256) void ung_fp8_tile_kernel(const T *x, uint64_t 
     }
     if (q) {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
+        for (int i = 0; i < PR; ++i) {
             Divisor by = by_all;
             if (!SQUARE) {
                 uint32_t most = row_most[i];
@@ -323,29 +330,34 @@ __global__ __launch_bounds__(256) void ung_fp8_tile_kernel(const T *x, uint64_t 
                 most_of[threadIdx.x >> 6][tc * 8 + j] = most;
         }
         __syncthreads();
+        if (threadIdx.x < KB) { // a column's divisor once, not by each of the threads that hold it
+            const uint32_t c = threadIdx.x;
+            uint32_t most = 0;
+#pragma unroll
+            for (int w = 0; w < WAVES; ++w)
+                most = max(most, most_of[w][c]);
+            const float s = scale_of(most);
+            by_col[c] = Divisor(s);
+            if ((uint64_t)cb * KB + c < cols)
+                scale_t[((uint64_t)cb * KB + c) * row_blocks + rb] = s;
+        }
+        __syncthreads();
     }
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
-        Divisor by = by_all;
-        if (!SQUARE) {
-            const uint32_t c = tc * 8 + j;
-            const float s = scale_of(max(max(most_of[0][c], most_of[1][c]), max(most_of[2][c], most_of[3][c])));
-            by = Divisor(s);
-            if (tr == 0 && c0 + j < cols)
-                scale_t[(c0 + j) * row_blocks + rb] = s;
-        }
+        const Divisor by = SQUARE ? by_all : by_col[tc * 8 + j];
 #pragma unroll
-        for (int i = 0; i < 8; ++i)
+        for (int i = 0; i < PR; ++i)
             y[i] = quotient(v[i][j], by);
-        *reinterpret_cast<uint2 *>(&turned[tc * 8 + j][tr * 8]) = pack8(y);
+        *reinterpret_cast<uint32_t *>(&turned[tc * 8 + j][((tr >> 2) ^ (tc & 7)) * 16 + (tr & 3) * 4]) = pack4(y);
     }
     __syncthreads();
 #pragma unroll
-    for (int p = 0; p < 4; ++p) {
-        const uint32_t c = p * 32 + (threadIdx.x >> 3), at = (threadIdx.x & 7) * 16;
+    for (int p = 0; p < KB * 8 / TILE_NT; ++p) {
+        const uint32_t c = p * (TILE_NT / 8) + (threadIdx.x >> 3), at = (threadIdx.x & 7) * 16;
         if ((uint64_t)cb * KB + c < cols)
             *reinterpret_cast<uint4 *>(qt + (((uint64_t)cb * KB + c) * row_blocks + rb) * KB + at) =
-                *reinterpret_cast<const uint4 *>(&turned[c][at]);
+                *reinterpret_cast<const uint4 *>(&turned[c][at ^ ((c >> 3 & 7) * 16)]);
     }
 }
 
@@ -1189,7 +1201,7 @@ int ung_hip_fp8_quantize(const void *x, int type, uint64_t rows, uint64_t cols, 
             ung_fp8_rows_kernel<T><<<grid, 256, 0, st>>>(p, rows, cols, row_stride, (uint32_t)cb, q, scale);
         } else {
             auto go = [&](auto kernel) {
-                kernel<<<(uint32_t)(cb * rb), 256, 0, st>>>(p, rows, cols, row_stride, (uint32_t)cb, (uint32_t)rb, q,
+                kernel<<<(uint32_t)(cb * rb), TILE_NT, 0, st>>>(p, rows, cols, row_stride, (uint32_t)cb, (uint32_t)rb, q,
                                                             scale, qt, scale_t);
             };
             square ? go(ung_fp8_tile_kernel<T, true>) : go(ung_fp8_tile_kernel<T, false>);
