@@ -121,6 +121,9 @@ inline bool known_type(int t) { return t == UNG_HIP_F32 || t == UNG_HIP_F16 || t
 inline uint64_t type_size(int t) { return t == UNG_HIP_F32 ? 4 : 2; }
 inline uint64_t ceil_div(uint64_t a, uint64_t b) { return (a + b - 1) / b; }
 
+// A launch's threads are counted in 32 bits along each axis.
+inline uint64_t most_blocks(uint32_t threads) { return UINT32_MAX / threads; }
+
 // The launch's own error, as a return code.
 inline int launched(const char *what)
 {

@@ -1182,7 +1182,8 @@ int ung_hip_fp8_quantize(const void *x, int type, uint64_t rows, uint64_t cols, 
         return UNG_HIP_EINVAL;
     }
     const uint64_t cb = ceil_div(cols, KB), rb = ceil_div(rows, KB);
-    if (rows > UINT32_MAX || cols > UINT32_MAX || cb * rb > INT32_MAX) {
+    const uint64_t tiles = square || qt ? cb * rb : 0; // rows alone are looped over
+    if (rows > UINT32_MAX || cols > UINT32_MAX || tiles > most_blocks(TILE_NT)) {
         set_error("ung_hip_fp8_quantize: %llu x %llu elements are too many", (unsigned long long)rows,
                   (unsigned long long)cols);
         return UNG_HIP_EINVAL;
@@ -1251,7 +1252,7 @@ int ung_hip_fp8_matmul(const uint8_t *a, const float *a_scale, const uint8_t *b,
         return UNG_HIP_EINVAL;
     }
     const uint64_t mt = ceil_div(m, 128), nt = ceil_div(n, 128);
-    if (m > INT32_MAX || n > INT32_MAX || kp > UINT32_MAX / 256 || mt * nt > INT32_MAX) {
+    if (m > INT32_MAX || n > INT32_MAX || kp > UINT32_MAX / 256 || mt * nt > most_blocks(256)) {
         set_error("ung_hip_fp8_matmul: a %llu x %llu x %llu product is too large", (unsigned long long)m,
                   (unsigned long long)n, (unsigned long long)kp);
         return UNG_HIP_EINVAL;

@@ -892,9 +892,9 @@ int check_k(const char *what, uint32_t k, uint32_t least)
     return UNG_HIP_EINVAL;
 }
 
-int check_grid(const char *what, uint64_t blocks)
+int check_grid(const char *what, uint64_t blocks, uint32_t threads)
 {
-    if (blocks <= INT32_MAX)
+    if (blocks <= most_blocks(threads))
         return UNG_HIP_OK;
     set_error("%s: too many scores (%llu blocks)", what, (unsigned long long)blocks);
     return UNG_HIP_EINVAL;
@@ -1030,6 +1030,8 @@ int distill(const char *what, const void *scores, int type, uint64_t rows, uint6
         const uint32_t vectors = vectors_at_most<T>(scores, rows, stride, len);
         int rc;
         if (whole_rows(rows, vectors)) {
+            if ((rc = check_grid(what, rows, ROW_NT)))
+                return rc;
             with_nv<16>(row_cut(vectors).nv, [&](auto nv) {
                 ung_distill_row_kernel<T, ROW_NT, nv.value><<<(uint32_t)rows, ROW_NT, 0, st>>>(
                     p, (uint32_t)len, stride, ids, values, k, lse, weight, t, loss, saved, (T *)grad, grad_stride);
@@ -1038,7 +1040,7 @@ int distill(const char *what, const void *scores, int type, uint64_t rows, uint6
         }
         const Cut cut = piece_cut(rows, vectors);
         const uint64_t parts = part_bytes(rows, cut.pieces), blocks = rows * cut.pieces;
-        if ((rc = check_grid(what, blocks)) ||
+        if ((rc = check_grid(what, blocks, PIECE_NT)) ||
             (rc = check_workspace(what, workspace, workspace_bytes, parts + (saved ? 0 : rows * sizeof(Saved)))))
             return rc;
         float2 *part = (float2 *)workspace;
@@ -1102,7 +1104,7 @@ int ung_hip_top_scores(const void *scores, int type, uint64_t rows, uint64_t len
         using T = decltype(zero);
         const Cut cut = top_cut(rows, vectors_at_most<T>(scores, rows, row_stride, len));
         int rc;
-        if ((rc = check_grid(what, rows * cut.pieces)) ||
+        if ((rc = check_grid(what, rows * cut.pieces, TOP_NT)) ||
             (rc = check_workspace(what, workspace, workspace_bytes, top_bytes(rows, cut.pieces, k))))
             return rc;
         const Temperature t = temperature_of(temperature);
@@ -1210,7 +1212,7 @@ int ung_hip_distill_backward(const void *scores, int type, uint64_t rows, uint64
         using T = decltype(zero);
         const Cut cut = piece_cut(rows, vectors_at_most<T>(scores, rows, row_stride, len));
         int rc;
-        if ((rc = check_grid(what, rows * cut.pieces)))
+        if ((rc = check_grid(what, rows * cut.pieces, PIECE_NT)))
             return rc;
         with_nv<8>(cut.nv, [&](auto nv) {
             ung_distill_grad_kernel<T, PIECE_NT, nv.value><<<(uint32_t)(rows * cut.pieces), PIECE_NT, 0,

@@ -87,3 +87,15 @@ def test_distill(k):
     assert lib.ung_hip_distill_workspace(P, 0, 1, 1_000_000, 1_000_000, C.byref(need)) == 0 and need.value > 0
     _refused(step(P, 0, 1, 1_000_000, 1_000_000, P, P, k, None, None, 1.0, P, P, 1_000_000, None, 0, None), "workspace")
     assert step(None, 0, 0, 4, 4, None, None, k, None, None, 1.0, None, None, 4, None, 0, None) == 0
+
+
+def test_more_blocks_than_a_launch_takes():
+    """A launch counts its threads in 32 bits: more are refused by name, not by the launch."""
+    lib, rows = F.load(), 1 << 25
+    _refused(lib.ung_hip_fp8_quantize(P, 0, 1 << 31, 1, 1, 0, P, P, P, P, None), "too many")
+    _refused(lib.ung_hip_fp8_quantize(P, 0, 1 << 31, 1, 1, 1, P, P, None, None, None), "too many")
+    _refused(lib.ung_hip_fp8_matmul(P, P, P, P, 0, 128, (1 << 31) - 1, 0, P, 0, 1 << 31, None, 0, None), "too large")
+    _refused(lib.ung_hip_top_scores(P, 0, rows, 4, 4, 2, 1.0, P, P, P, None, 0, None), "too many")
+    _refused(lib.ung_hip_distill_forward(P, 0, rows, 4, 4, P, P, 4, None, 1.0, P, P, None, 0, None), "too many")
+    _refused(lib.ung_hip_distill_backward(P, 0, rows, 4, 4, P, P, 4, P, None, 1.0, P, 4, None), "too many")
+    _refused(lib.ung_hip_distill_step(P, 0, rows, 4, 4, P, P, 4, None, None, 1.0, P, P, 4, None, 0, None), "too many")
