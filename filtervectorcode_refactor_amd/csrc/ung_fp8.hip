@@ -1102,11 +1102,11 @@ uint32_t cu_count()
     return got;
 }
 
-// How a product is made: by tiles of BIG x BIG, of 128 x 128, or (few rows) of 32 x 128, and
-// from how many shares of the inner length.
+// How a product is made: by tiles of BIG x BIG, or of `high` x 128, and from how many shares of
+// the inner length.
 struct Plan {
-    bool big, few;
-    uint32_t splits;
+    bool big;
+    uint32_t high, splits;
 };
 
 // BIG tiles where they keep five of eight CUs busy over all rounds: their kernel reaches 2200
@@ -1114,8 +1114,10 @@ struct Plan {
 // us: 4096 x 32768 x 768 134 against 155, 4096 x 4096 x 768 21.5, 24.3, 5120 x 5120 x 1024 40.2,
 // 43.4; below the bound 2500 x 3500 x 4096 (55 %) 94, 84, 2048 x 2048 x 2048 (25 %) 37, 16,
 // 300 x 1000 x 128 6.7, 4.8.
-// Tiles of 32 rows for up to 32 rows: 1 x 1000000 x 384 in 32 bits 84 against 135, 16 x 32768
-// x 768 5.6, 6.9, 1 x 10000 x 128 3.5, 3.9.
+// Else up to 128 rows by the least of 32, 64, 96 and 128 that holds them: 1 x 1000000 x 384 in 32
+// bits 84 against 135 by 128 rows, 16 x 32768 x 768 5.6, 6.9, 1 x 10000 x 128 3.5, 3.9; 64 x 100000
+// x 384 in 16 bits 11.8, 14.3, in 32 bits 14.5, 20.0, 64 x 1000 x 768 5.9, 8.6; 77 x 100000 x 384 13.1,
+// 14.5, in 32 bits 18.1, 20.4.
 // Shares of the inner length where tiles leave CUs free.  BIG: at least four of at least 32
 // blocks (4096 x 768 x 32768 129 us, 128 x 128 tiles 175; 4096 x 768 x 8192 in shares of 16 54, 49).
 // Else as many as make the sum of the stages one share takes (0.6 us each; in 32 bits 1.4) and
@@ -1125,7 +1127,7 @@ struct Plan {
 Plan plan_of(uint64_t m, uint64_t n, uint64_t kp, int type)
 {
     const uint64_t kblocks = kp / KB, cus = cu_count();
-    Plan p = {false, false, 1};
+    Plan p = {false, 128, 1};
     if (m == 0 || n == 0 || kblocks == 0) // (a product of no length: 128 x 128 tiles of zeros)
         return p;
     if (type != UNG_HIP_F32 && m > 128 && n > 128) {
@@ -1137,9 +1139,9 @@ Plan plan_of(uint64_t m, uint64_t n, uint64_t kp, int type)
         if (p.big)
             return p;
     }
-    p.few = m <= 32;
+    p.high = m <= 32 ? 32 : m <= 64 ? 64 : m <= 96 ? 96 : 128;
     p.splits = 1;
-    const uint64_t tiles = ceil_div(m, p.few ? 32 : 128) * ceil_div(n, 128);
+    const uint64_t tiles = ceil_div(m, p.high) * ceil_div(n, 128);
     const double stage = type == UNG_HIP_F32 ? 1.4 : 0.6, traffic = (double)m * (double)n * 8 / 3e6;
     double best = stage * (double)kblocks;
     for (uint64_t s = 2; s * tiles <= 2 * cus && s * 2 <= kblocks; ++s) {
@@ -1294,12 +1296,21 @@ int ung_hip_fp8_matmul(const uint8_t *a, const float *a_scale, const uint8_t *b,
                     return;
                 }
             }
-            if (plan.few)
-                b_square ? run(ung_fp8_product_kernel<32, 128, 1, 2, EXACT, true, OT>, 32, 128, ~0u, 128, vectors)
-                         : run(ung_fp8_product_kernel<32, 128, 1, 2, EXACT, false, OT>, 32, 128, ~0u, 128, vectors);
+            auto tiles = [&](auto high, auto wm, auto wn) {
+                constexpr int BM = decltype(high)::value, WM = decltype(wm)::value, WN = decltype(wn)::value;
+                b_square ? run(ung_fp8_product_kernel<BM, 128, WM, WN, EXACT, true, OT>, BM, 128, ~0u, WM * WN * 64, vectors)
+                         : run(ung_fp8_product_kernel<BM, 128, WM, WN, EXACT, false, OT>, BM, 128, ~0u, WM * WN * 64, vectors);
+            };
+            constexpr std::integral_constant<int, 1> one;
+            constexpr std::integral_constant<int, 2> two;
+            if (plan.high == 32)
+                tiles(std::integral_constant<int, 32>{}, one, two);
+            else if (plan.high == 64)
+                tiles(std::integral_constant<int, 64>{}, two, two);
+            else if (plan.high == 96)
+                tiles(std::integral_constant<int, 96>{}, two, two);
             else
-                b_square ? run(ung_fp8_product_kernel<128, 128, 2, 2, EXACT, true, OT>, 128, 128, ~0u, 256, vectors)
-                         : run(ung_fp8_product_kernel<128, 128, 2, 2, EXACT, false, OT>, 128, 128, ~0u, 256, vectors);
+                tiles(std::integral_constant<int, 128>{}, two, two);
         };
         if (splits == 1) {
             make((T *)c, c_stride, vec);

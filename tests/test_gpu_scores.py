@@ -747,3 +747,18 @@ def test_refusals():
         with pytest.raises((ValueError, F.UngHipError)):
             f()
             _say("not refused:", i)
+
+
+@pytest.mark.parametrize("m", [32, 33, 63, 64, 65, 95, 96, 97, 128, 129, 192, 193, 385])
+@pytest.mark.parametrize("n,d,block", [(257, 300, "row"), (1003, 4000, "square")])
+def test_product_at_the_tiles_heights(m, n, d, block):
+    """Tiles of 32, 64, 96 and 128 rows, at and beside their bounds, sums in shares too."""
+    qa, sa, a = _operand_there(m, d, "row", m)
+    qb, sb, b = _operand_there(n, d, block, n)
+    want, wide = a @ b.t(), a.abs() @ b.abs().t()
+    kp = a.shape[1]
+    for kind in ("bf16", "fp32"):
+        bound = ((kp + 2 * kp // 128 + 2) * EPS + (2.0 ** -10 if kind != "fp32" else 0.0)) * wide
+        bound += HALF_ULP[kind] * want.abs() * 1.001 + TINY[kind]
+        got = S.matmul_fp8(qa, sa, qb, sb, dtype=TYPES[kind])
+        assert ((got.double() - want).abs() <= bound).all(), kind
