@@ -1118,6 +1118,10 @@ struct Plan {
 // bits 84 against 135 by 128 rows, 16 x 32768 x 768 5.6, 6.9, 1 x 10000 x 128 3.5, 3.9; 64 x 100000
 // x 384 in 16 bits 11.8, 14.3, in 32 bits 14.5, 20.0, 64 x 1000 x 768 5.9, 8.6; 77 x 100000 x 384 13.1,
 // 14.5, in 32 bits 18.1, 20.4.
+// Of 64 rows for more rows too where there are at most two such tiles for a CU: three blocks fit
+// one instead of two, and a stage takes 0.4 us instead of 0.6: 300 x 1000 x 384 4.7 against 6.8, in
+// 32 bits 5.7, 8.1, 1000 x 2000 x 1024 8.1, 10.8, 300 x 10000 x 4096 22.9, 26.4; 2048 x 2000 x 4096
+// (two a CU) 25.2, 28.3.
 // Shares of the inner length where tiles leave CUs free.  BIG: at least four of at least 32
 // blocks (4096 x 768 x 32768 129 us, 128 x 128 tiles 175; 4096 x 768 x 8192 in shares of 16 54, 49).
 // Else as many as make the sum of the stages one share takes (0.6 us each; in 32 bits 1.4) and
@@ -1139,7 +1143,8 @@ Plan plan_of(uint64_t m, uint64_t n, uint64_t kp, int type)
         if (p.big)
             return p;
     }
-    p.high = m <= 32 ? 32 : m <= 64 ? 64 : m <= 96 ? 96 : 128;
+    const bool few_tiles = ceil_div(m, 64) * ceil_div(n, 128) <= 2 * cus;
+    p.high = m <= 32 ? 32 : m <= 64 || few_tiles ? 64 : m <= 96 ? 96 : 128;
     p.splits = 1;
     const uint64_t tiles = ceil_div(m, p.high) * ceil_div(n, 128);
     const double stage = type == UNG_HIP_F32 ? 1.4 : 0.6, traffic = (double)m * (double)n * 8 / 3e6;
