@@ -1118,13 +1118,13 @@ struct Plan {
 // bits 84 against 135 by 128 rows, 16 x 32768 x 768 5.6, 6.9, 1 x 10000 x 128 3.5, 3.9; 64 x 100000
 // x 384 in 16 bits 11.8, 14.3, in 32 bits 14.5, 20.0, 64 x 1000 x 768 5.9, 8.6; 77 x 100000 x 384 13.1,
 // 14.5, in 32 bits 18.1, 20.4.
-// Of 64 rows for more rows too where there are at most two such tiles for a CU: three blocks fit
-// one instead of two, and a stage takes 0.4 us instead of 0.6: 300 x 1000 x 384 4.7 against 6.8, in
-// 32 bits 5.7, 8.1, 1000 x 2000 x 1024 8.1, 10.8, 300 x 10000 x 4096 22.9, 26.4; 2048 x 2000 x 4096
-// (two a CU) 25.2, 28.3.
+// Of 64 rows for more rows too where all such tiles are under way at a time: three blocks fit a
+// CU instead of two, and a stage takes less: 300 x 1000 x 384 4.7 against 6.8, in 32 bits 5.7, 8.1,
+// 1000 x 2000 x 1024 8.1, 10.8, 1100 x 4096 x 2048 19.2, 20.9, in 32 bits 30.3, 34.5, 450 x 10000 x 768
+// 10.6, 12.7; past three a CU 2500 x 2500 x 2048 26.8, 22.3, 700 x 10000 x 4096 50.1, 40.2.
 // Shares of the inner length where tiles leave CUs free.  BIG: at least four of at least 32
 // blocks (4096 x 768 x 32768 129 us, 128 x 128 tiles 175; 4096 x 768 x 8192 in shares of 16 54, 49).
-// Else as many as make the sum of the stages one share takes (0.6 us each; in 32 bits 1.4) and
+// Else as many as make the sum of the stages one share takes (0.6 us each; in 32 bits 1.4, of 64 rows 1.0) and
 // of the joining pass (4 us, 0.1 a share and its traffic at 3 TB/s) least: 1000 x 100 x 4096 in 32
 // bits 14 us, in one 45; 150 x 150 x 65536 21, 328; 512 x 512 x 2048 10.9, 13.7; 1024 x 1024 x 2048
 // stays in one, 14.0, in two 18.5.
@@ -1143,11 +1143,11 @@ Plan plan_of(uint64_t m, uint64_t n, uint64_t kp, int type)
         if (p.big)
             return p;
     }
-    const bool few_tiles = ceil_div(m, 64) * ceil_div(n, 128) <= 2 * cus;
+    const bool few_tiles = ceil_div(m, 64) * ceil_div(n, 128) <= 3 * cus;
     p.high = m <= 32 ? 32 : m <= 64 || few_tiles ? 64 : m <= 96 ? 96 : 128;
     p.splits = 1;
     const uint64_t tiles = ceil_div(m, p.high) * ceil_div(n, 128);
-    const double stage = type == UNG_HIP_F32 ? 1.4 : 0.6, traffic = (double)m * (double)n * 8 / 3e6;
+    const double stage = type != UNG_HIP_F32 ? 0.6 : p.high == 64 ? 1.0 : 1.4, traffic = (double)m * (double)n * 8 / 3e6;
     double best = stage * (double)kblocks;
     for (uint64_t s = 2; s * tiles <= 2 * cus && s * 2 <= kblocks; ++s) {
         const double cost = stage * (double)ceil_div(kblocks, s) + 4.0 + (0.1 + traffic) * (double)s;
