@@ -248,6 +248,7 @@ __device__ inline void finish_top(TopShared &sh, uint32_t k, Each each, uint64_t
 #pragma unroll
         for (int i = 0; i < TOP_CAP / TOP_NT; ++i)
             mine[i] = i * TOP_NT + tid < found ? sh.cand[i * TOP_NT + tid] : 0;
+        __syncthreads(); // every wave has read the count, or a late one would find it reset
         if (tid < 64) {
             const uint32_t limit = kth_key<LOW>(sh.cand, found, k);
             if (tid == 0) {

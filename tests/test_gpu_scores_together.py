@@ -1,0 +1,54 @@
+"""GPU tests of the score operators where waves, blocks, autograd and memory meet: candidates that
+a block ranks, shortens or searches, gradients taken twice or in place, rows of wide buffers.
+Results are compared with what the inputs say by construction or with plain 64-bit forms."""
+import pytest
+import torch
+
+import filtervectorcode_refactor_amd as F
+from filtervectorcode_refactor_amd import scores as S
+
+pytestmark = pytest.mark.gpu
+
+TYPES = {"fp32": torch.float32, "fp16": torch.float16, "bf16": torch.bfloat16}
+
+
+def _gen(seed):
+    return torch.Generator().manual_seed(seed)
+
+
+# ---- candidates of the first scores -------------------------------------------------------------
+def _equal_scores(ties, n, v, k, kind):
+    """`ties` scores of a row share the largest value, so all of them are candidates.  Rows
+    enough that blocks start and end beside each other, and the same lists every time."""
+    g = _gen(ties)
+    x = torch.randint(-40, 0, (n, v), generator=g).float()
+    at = torch.rand(n, v, generator=g).argsort(dim=1)[:, :ties]
+    x.scatter_(1, at, 1.0)
+    view = x.to(TYPES[kind]).cuda()
+    want = at.sort(dim=1).values[:, :k].int()
+    first = S.top_scores(view, k)
+    assert torch.equal(first[1].cpu(), want) and (first[0] == 1.0).all()
+    for _ in range(5):
+        assert all(torch.equal(a, b) for a, b in zip(first, S.top_scores(view, k)))
+
+
+@pytest.mark.parametrize("ties", [319, 320, 321, 640, 1023, 1024])
+@pytest.mark.parametrize("kind", ["fp32", "bf16"])
+def test_top_scores_of_as_many_equal_scores(ties, kind):
+    """Candidates that are ranked as they are, or shortened by their k-th key first."""
+    _equal_scores(ties, 600, 2047, 48, kind)
+
+
+@pytest.mark.parametrize("holders", [21, 40, 60])
+def test_merged_top_scores_of_equal_scores(holders):
+    """The same where a row's pieces are merged: `holders` pieces of 2048 scores bring 16 equal
+    ones each (336 and more candidates; their lists are 16 long)."""
+    v, k = 125_000, 16
+    x = torch.zeros(3, v)
+    for p in range(holders):
+        x[:, p * 2048 + 100:p * 2048 + 116] = 7.0
+    want = (torch.arange(k) + 100).int()
+    view = x.bfloat16().cuda()
+    for _ in range(5):
+        values, ids, _ = S.top_scores(view, k)
+        assert torch.equal(ids.cpu(), want.expand(3, k)) and (values == 7.0).all()
