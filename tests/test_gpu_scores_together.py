@@ -39,6 +39,13 @@ def test_top_scores_of_as_many_equal_scores(ties, kind):
     _equal_scores(ties, 600, 2047, 48, kind)
 
 
+@pytest.mark.parametrize("ties,v", [(1025, 1100), (1025, 2047), (1500, 2047), (1025, 3000), (4000, 4090), (1025, 8000), (9000, 16000), (20000, 30000)])
+@pytest.mark.parametrize("kind", ["fp32", "fp16", "bf16"])
+def test_top_scores_of_more_equal_scores_than_a_block_ranks(ties, v, kind):
+    """The k-th of them is searched bit by bit, in kernels of every number of vectors a thread."""
+    _equal_scores(ties, 600, v, 48, kind)
+
+
 @pytest.mark.parametrize("holders", [21, 40, 60])
 def test_merged_top_scores_of_equal_scores(holders):
     """The same where a row's pieces are merged: `holders` pieces of 2048 scores bring 16 equal
