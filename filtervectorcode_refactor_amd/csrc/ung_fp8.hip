@@ -1166,6 +1166,26 @@ uint64_t split_bytes(uint64_t m, uint64_t n, uint32_t splits)
     return splits > 1 ? (uint64_t)splits * m * split_stride(n) * 4 : 0;
 }
 
+// Sizes and type of a product; plan_of counts on it.
+int check_product(const char *what, uint64_t m, uint64_t n, uint64_t kp, int type)
+{
+    if (!known_type(type)) {
+        set_error("%s: unknown element type %d", what, type);
+        return UNG_HIP_EINVAL;
+    }
+    if (kp % KB) {
+        set_error("%s: inner length %llu is no multiple of %d", what, (unsigned long long)kp, KB);
+        return UNG_HIP_EINVAL;
+    }
+    if (m && n && (m > INT32_MAX || n > INT32_MAX || kp > UINT32_MAX / 256 ||
+                   ceil_div(m, 128) * ceil_div(n, 128) > most_blocks(256))) {
+        set_error("%s: a %llu x %llu x %llu product is too large", what, (unsigned long long)m,
+                  (unsigned long long)n, (unsigned long long)kp);
+        return UNG_HIP_EINVAL;
+    }
+    return UNG_HIP_OK;
+}
+
 } // namespace
 
 extern "C" {
@@ -1221,11 +1241,14 @@ int ung_hip_fp8_quantize(const void *x, int type, uint64_t rows, uint64_t cols, 
 
 int ung_hip_fp8_matmul_workspace(uint64_t m, uint64_t n, uint64_t kp, int type, uint64_t *bytes)
 {
+    static const char what[] = "ung_hip_fp8_matmul_workspace";
     clear_error();
-    if (!bytes || !known_type(type)) {
-        set_error("ung_hip_fp8_matmul_workspace: null bytes or unknown element type %d", type);
+    if (!bytes) {
+        set_error("%s: null bytes", what);
         return UNG_HIP_EINVAL;
     }
+    if (const int rc = check_product(what, m, n, kp, type))
+        return rc;
     *bytes = split_bytes(m, n, plan_of(m, n, kp, type).splits);
     return UNG_HIP_OK;
 }
@@ -1235,14 +1258,8 @@ int ung_hip_fp8_matmul(const uint8_t *a, const float *a_scale, const uint8_t *b,
                        uint64_t workspace_bytes, void *stream)
 {
     clear_error();
-    if (!known_type(type)) {
-        set_error("ung_hip_fp8_matmul: unknown element type %d", type);
-        return UNG_HIP_EINVAL;
-    }
-    if (kp % KB) {
-        set_error("ung_hip_fp8_matmul: inner length %llu is no multiple of %d", (unsigned long long)kp, KB);
-        return UNG_HIP_EINVAL;
-    }
+    if (const int rc = check_product("ung_hip_fp8_matmul", m, n, kp, type))
+        return rc;
     if (m == 0 || n == 0)
         return UNG_HIP_OK;
     if (!c || (kp && (!a || !a_scale || !b || !b_scale))) {
@@ -1257,12 +1274,6 @@ int ung_hip_fp8_matmul(const uint8_t *a, const float *a_scale, const uint8_t *b,
     if ((uintptr_t)a % 16 || (uintptr_t)b % 16 || (uintptr_t)a_scale % 4 || (uintptr_t)b_scale % 4 ||
         (uintptr_t)c % type_size(type)) {
         set_error("ung_hip_fp8_matmul: a and b need 16-byte alignment, the rest that of its elements");
-        return UNG_HIP_EINVAL;
-    }
-    const uint64_t mt = ceil_div(m, 128), nt = ceil_div(n, 128);
-    if (m > INT32_MAX || n > INT32_MAX || kp > UINT32_MAX / 256 || mt * nt > most_blocks(256)) {
-        set_error("ung_hip_fp8_matmul: a %llu x %llu x %llu product is too large", (unsigned long long)m,
-                  (unsigned long long)n, (unsigned long long)kp);
         return UNG_HIP_EINVAL;
     }
     const Plan plan = plan_of(m, n, kp, type);
