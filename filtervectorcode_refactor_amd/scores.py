@@ -125,6 +125,27 @@ def _workspace(fn, *args, device):
     return t, t.data_ptr(), need.value
 
 
+class _Underivable(torch.autograd.Function):
+    """Results that depend on `of` by kernels that autograd does not see: whoever differentiates
+    them gets an error instead of a gradient without that part."""
+
+    @staticmethod
+    def forward(ctx, message, of, *results):
+        ctx.message = message
+        return results
+
+    @staticmethod
+    def backward(ctx, *_):
+        raise RuntimeError(ctx.message)
+
+
+def _once(name, *grads):
+    """Gradients out of a backward pass; with create_graph they are marked as underivable."""
+    if not torch.is_grad_enabled():
+        return grads
+    return _Underivable.apply(f"{name} has no second derivative", torch.zeros((), requires_grad=True), *grads)
+
+
 # ---- 8-bit operands and their product -----------------------------------------------------
 def quantize_fp8(x, block="row", transpose=False):
     """Rows as an 8-bit operand: (q, scale), with ``transpose`` (q, scale, qt, scale_t).
@@ -245,12 +266,12 @@ class _LinearFp8(torch.autograd.Function):
         elif need_w:
             _, _, qt, scale_t = quantize_fp8(g, transpose=True)
             dw = matmul_fp8(qt, scale_t, *saved, dtype=torch.float32)
-        return (dx.to(x_type) if need_x else None), (dw.to(w_type) if need_w else None), None
+        return *_once("linear_fp8", dx.to(x_type) if need_x else None, dw.to(w_type) if need_w else None), None
 
 
 def linear_fp8(x, w, dtype=torch.bfloat16):
     """x w^T with both brought to 8 bits (x by rows, w by 128 x 128 squares), differentiable in
-    both; its gradients are products in 8 bits too."""
+    both, once; its gradients are products in 8 bits too."""
     _matrix("x", x)
     _matrix("w", w, x)
     _need(x.shape[1] == w.shape[1], f"x and w: rows of {x.shape[1]} and {w.shape[1]} do not go together")
@@ -397,9 +418,11 @@ class _DistillLoss(torch.autograd.Function):
     @staticmethod
     def backward(ctx, g):
         scores, ids, values, saved = ctx.saved_tensors
-        return distill_backward(g, scores, ids, values, saved, temperature=ctx.temperature), None, None, None, None
+        grad = distill_backward(g, scores, ids, values, saved, temperature=ctx.temperature)
+        return *_once("distill_loss", grad), None, None, None, None
 
 
 def distill_loss(scores, ids, values, teacher_lse=None, temperature=1.0):
-    """The loss of each row (distill_forward), differentiable in the scores."""
+    """The loss of each row (distill_forward), differentiable in the scores, once; the teacher's
+    side is taken as given."""
     return _DistillLoss.apply(scores, ids, values, teacher_lse, temperature)

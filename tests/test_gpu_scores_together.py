@@ -59,3 +59,20 @@ def test_merged_top_scores_of_equal_scores(holders):
     for _ in range(5):
         values, ids, _ = S.top_scores(view, k)
         assert torch.equal(ids.cpu(), want.expand(3, k)) and (values == 7.0).all()
+
+
+# ---- gradients --------------------------------------------------------------------------------------
+def test_second_derivatives_are_refused():
+    x, w = torch.randn(40, 200, device="cuda", requires_grad=True), torch.randn(300, 200, device="cuda", requires_grad=True)
+    ids, values = torch.zeros(40, 2, dtype=torch.int32, device="cuda"), torch.zeros(40, 2, device="cuda")
+    plain = torch.autograd.grad(S.distill_loss(S.linear_fp8(x, w), ids, values).sum(), (x, w))
+    again = torch.autograd.grad(S.distill_loss(S.linear_fp8(x, w), ids, values).sum(), (x, w), create_graph=True)
+    assert all(torch.equal(a, b) for a, b in zip(plain, again))
+    for g in again:
+        with pytest.raises(RuntimeError, match="no second derivative"):
+            g.square().sum().backward(retain_graph=True)
+    s = torch.randn(40, 300, device="cuda", requires_grad=True)
+    (g,) = torch.autograd.grad(S.distill_loss(s, ids, values).sum(), s, create_graph=True)
+    with pytest.raises(RuntimeError, match="distill_loss has no second derivative"):
+        g.square().sum().backward()
+    assert x.grad is None and w.grad is None and s.grad is None
