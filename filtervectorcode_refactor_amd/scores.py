@@ -359,6 +359,12 @@ def distill_forward(scores, ids, values, teacher_lse=None, temperature=1.0):
     return loss, saved
 
 
+def _written(out):
+    """Tells autograd that a caller's tensor has been written: what was saved of it before is stale."""
+    if out is not None and not out.is_inference():
+        torch.autograd.graph.increment_version(out)
+
+
 def _gradient(scores, stride, out):
     if out is None:
         return _like_rows(scores, stride), stride
@@ -385,6 +391,7 @@ def distill_backward(weight, scores, ids, values, saved, teacher_lse=None, tempe
         check(_library().ung_hip_distill_backward(scores.data_ptr(), kind, n, v, stride, ids.data_ptr(),
                                                   values.data_ptr(), ids.shape[1], saved.data_ptr(), _address(weight),
                                                   temperature, grad.data_ptr(), grad_stride, stream))
+    _written(out)
     return grad
 
 
@@ -404,6 +411,7 @@ def distill_step(scores, ids, values, weight=None, teacher_lse=None, temperature
         check(lib.ung_hip_distill_step(scores.data_ptr(), kind, n, v, stride, ids.data_ptr(), values.data_ptr(),
                                        ids.shape[1], _address(lse), _address(weight), temperature, loss.data_ptr(),
                                        grad.data_ptr(), grad_stride, at, size, stream))
+    _written(out)
     return loss, grad
 
 

@@ -76,3 +76,44 @@ def test_second_derivatives_are_refused():
     with pytest.raises(RuntimeError, match="distill_loss has no second derivative"):
         g.square().sum().backward()
     assert x.grad is None and w.grad is None and s.grad is None
+
+
+def _student(n, v, k=4):
+    g = torch.Generator(device="cuda").manual_seed(n + v)
+    s = torch.randn(n, v, device="cuda", generator=g)
+    ids = torch.randint(0, v, (n, k), device="cuda", generator=g, dtype=torch.int32)
+    return s, ids, torch.randn(n, k, device="cuda", generator=g)
+
+
+@pytest.mark.parametrize("apart", [False, True])
+def test_autograd_sees_scores_replaced_in_place(apart):
+    """What another function saved of the scores is gone once the gradient has replaced them: its
+    backward pass is refused, as after any operation in place."""
+    s, ids, values = _student(20, 500)
+
+    def replace(t):
+        if not apart:
+            return S.distill_step(t, ids, values, out=t)[1]
+        saved = S.distill_forward(t, ids, values)[1]
+        return S.distill_backward(None, t, ids, values, saved, out=t)
+
+    want = S.distill_step(s, ids, values)[1]
+    leaf = s.clone().requires_grad_()
+    for later in (lambda t: t.square().sum(), lambda t: S.distill_loss(t, ids, values).sum()):
+        t = leaf * 1.0
+        loss = later(t)
+        with torch.no_grad():
+            assert torch.equal(replace(t), want)
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            loss.backward()
+    t = leaf * 1.0  # nobody needs the scores again: their gradient may take their place
+    with torch.no_grad():
+        grad = replace(t)
+    t.backward(grad)
+    assert torch.equal(leaf.grad, want) and grad.data_ptr() == t.data_ptr()
+    other = torch.empty_like(s)
+    assert other._version == 0
+    assert S.distill_step(s, ids, values, out=other)[1] is other and other._version == 1 and s._version == 0
+    with torch.inference_mode():
+        t = s.clone()
+    assert torch.equal(replace(t), want)
