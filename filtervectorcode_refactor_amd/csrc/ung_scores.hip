@@ -1004,7 +1004,33 @@ int check_distill(const char *what, const void *scores, int type, uint64_t rows,
     return UNG_HIP_OK;
 }
 
-int check_grad(const char *what, const void *grad, int type, uint64_t rows, uint64_t len, uint64_t grad_stride)
+// Whether an element of `rows` rows of len elements at a is one of such rows at b, by their
+// addresses in elements; strides are len at least where there are several rows.
+bool rows_meet(uint64_t a, uint64_t a_stride, uint64_t b, uint64_t b_stride, uint64_t rows, uint64_t len)
+{
+    const uint64_t a_end = a + (rows - 1) * a_stride + len, b_end = b + (rows - 1) * b_stride + len;
+    if (a >= b_end || b >= a_end)
+        return false;
+    if (rows == 1)
+        return true;
+    if (a_stride == b_stride) { // rows i of the later ones begin `in` after rows i + `by` of the earlier
+        const uint64_t from = a < b ? b - a : a - b, by = from / a_stride, in = from % a_stride;
+        return (in < len && by < rows) || (in + len > a_stride && by + 1 < rows);
+    }
+    for (uint64_t i = 0, j = 0; i < rows && j < rows;) {
+        const uint64_t x = a + i * a_stride, y = b + j * b_stride;
+        if (x + len <= y)
+            ++i;
+        else if (y + len <= x)
+            ++j;
+        else
+            return true;
+    }
+    return false;
+}
+
+int check_grad(const char *what, const void *scores, uint64_t stride, const void *grad, int type, uint64_t rows,
+               uint64_t len, uint64_t grad_stride)
 {
     if (rows && len && !grad) {
         set_error("%s: null gradient", what);
@@ -1017,6 +1043,13 @@ int check_grad(const char *what, const void *grad, int type, uint64_t rows, uint
     }
     if ((uintptr_t)grad % type_size(type)) {
         set_error("%s: the gradient is not aligned to its elements", what);
+        return UNG_HIP_EINVAL;
+    }
+    // in place a block writes what it alone reads; elsewhere among the scores others still read
+    const bool in_place = grad == scores && (rows == 1 || grad_stride == stride);
+    if (rows && len && !in_place &&
+        rows_meet((uintptr_t)scores / type_size(type), stride, (uintptr_t)grad / type_size(type), grad_stride, rows, len)) {
+        set_error("%s: the gradient overlaps the scores without being in their place", what);
         return UNG_HIP_EINVAL;
     }
     return UNG_HIP_OK;
@@ -1205,7 +1238,7 @@ int ung_hip_distill_backward(const void *scores, int type, uint64_t rows, uint64
     clear_error();
     int rc;
     if ((rc = check_distill(what, scores, type, rows, len, row_stride, ids, values, k, temperature)) ||
-        (rc = check_grad(what, grad, type, rows, len, grad_stride)))
+        (rc = check_grad(what, scores, row_stride, grad, type, rows, len, grad_stride)))
         return rc;
     if (rows == 0 || len == 0)
         return UNG_HIP_OK;
@@ -1238,7 +1271,7 @@ int ung_hip_distill_step(const void *scores, int type, uint64_t rows, uint64_t l
     clear_error();
     int rc;
     if ((rc = check_distill(what, scores, type, rows, len, row_stride, ids, values, k, temperature)) ||
-        (rc = check_grad(what, grad, type, rows, len, grad_stride)))
+        (rc = check_grad(what, scores, row_stride, grad, type, rows, len, grad_stride)))
         return rc;
     if (rows == 0)
         return UNG_HIP_OK;

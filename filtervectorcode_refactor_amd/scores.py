@@ -377,8 +377,8 @@ def _gradient(scores, stride, out):
 def distill_backward(weight, scores, ids, values, saved, teacher_lse=None, temperature=1.0, out=None):
     """Gradient of sum(weight * loss) by the scores, in their type; the arguments are those of
     the forward call (teacher_lse is part of ``saved`` already).  ``out`` may be the scores
-    themselves, which the gradient then replaces; by default it is a new tensor whose rows lie
-    as theirs."""
+    themselves, which the gradient then replaces, but not overlap them otherwise; by default it is
+    a new tensor whose rows lie as theirs."""
     kind, stride = _matrix("scores", scores)
     ids, values, _ = _teacher(scores, ids, values, teacher_lse)
     n, v = scores.shape

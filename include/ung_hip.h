@@ -385,7 +385,8 @@ int ung_hip_top_scores(const void *scores, int type, uint64_t rows, uint64_t len
  *             backward pass needs
  *   backward  grad of sum(weight[i] * loss[i]) (weight NULL: ones) for the forward call's inputs
  *   step      both: loss and grad
- * grad may be the scores themselves (same stride), which it then replaces. */
+ * grad may be the scores themselves (same stride), which it then replaces; rows that overlap the
+ * scores' otherwise are refused. */
 #define UNG_HIP_DISTILL_SAVED 8
 int ung_hip_distill_workspace(const void *scores, int type, uint64_t rows, uint64_t len, uint64_t row_stride,
                               uint64_t *bytes);

@@ -5,6 +5,7 @@ import pytest
 import torch
 
 import filtervectorcode_refactor_amd as F
+import filtervectorcode_refactor_amd as F
 from filtervectorcode_refactor_amd import scores as S
 
 pytestmark = pytest.mark.gpu
@@ -117,3 +118,23 @@ def test_autograd_sees_scores_replaced_in_place(apart):
     with torch.inference_mode():
         t = s.clone()
     assert torch.equal(replace(t), want)
+
+
+def test_gradients_beside_and_over_the_scores():
+    """Rows of one buffer: the gradient between the scores' rows, in their place, and refused over
+    a part of them."""
+    s, ids, values = _student(30, 400)
+    want = S.distill_step(s, ids, values)[1]
+    wide = torch.zeros(30, 1000, device="cuda")
+    wide[:, :400] = s
+    scores, beside, over = wide[:, :400], wide[:, 500:900], wide[:, 300:700]
+    _, saved = S.distill_forward(scores, ids, values)
+    for call in (lambda out: S.distill_step(scores, ids, values, out=out)[1],
+                 lambda out: S.distill_backward(None, scores, ids, values, saved, out=out)):
+        assert torch.equal(call(beside), want) and torch.equal(scores, s)
+        for out in (over, wide.view(-1)[16:].as_strided((30, 400), (1000, 1)), wide.view(-1)[:12_000].view(30, 400)):
+            with pytest.raises((ValueError, F.UngHipError)):
+                call(out)
+        assert torch.equal(scores, s)
+    assert torch.equal(S.distill_step(scores, ids, values, out=scores)[1], want)
+    assert torch.equal(wide[:, :400], want) and torch.equal(wide[:, 500:900], want)

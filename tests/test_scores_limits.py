@@ -33,3 +33,52 @@ def test_matmul_workspace_of_what_no_product_takes(m, n, kp, word, type):
         if kp % 128 == 0:
             assert F.load().ung_hip_fp8_matmul_workspace(*empty, kp, type, C.byref(need)) == 0 and need.value == 0
             need.value = 7
+
+
+F32, BF16 = 0, 2
+
+
+def _grad_calls(lib, scores, type, rows, len_, stride, grad, grad_stride):
+    """Messages of the two entry points that write a gradient; a null argument that is looked at
+    later refuses what the gradient's place does not."""
+    for rc in (lambda: lib.ung_hip_distill_backward(scores, type, rows, len_, stride, P, P, 2, None, None, 1.0, grad,
+                                                    grad_stride, None),
+               lambda: lib.ung_hip_distill_step(scores, type, rows, len_, stride, P, P, 2, None, None, 1.0, None, grad,
+                                                grad_stride, None, 0, None)):
+        assert rc() == _lib.UNG_HIP_EINVAL
+        yield _lib.last_error()
+
+
+def _meet(rows, len_, stride, at, grad_stride):
+    """Whether an element of the rows at 0 and one of the rows at `at` are the same."""
+    if rows == 1:
+        return abs(at) < len_
+    a = np.arange(rows)[:, None] * stride + np.arange(len_)
+    b = at + np.arange(rows)[:, None] * grad_stride + np.arange(len_)
+    return bool(np.isin(a, b).any())
+
+
+@pytest.mark.parametrize("type,size", [(F32, 4), (BF16, 2)])
+@pytest.mark.parametrize("rows,len_,stride,grad_stride", [
+    (4, 10, 10, 10), (4, 10, 12, 12), (4, 10, 20, 20), (4, 10, 25, 25), (4, 10, 31, 31), (1, 10, 10, 10),
+    (4, 10, 20, 40), (4, 10, 40, 20), (5, 3, 7, 11), (5, 3, 11, 7), (7, 2, 5, 2), (3, 1, 4, 6)])
+def test_gradients_that_overlap_the_scores_in_part(type, size, rows, len_, stride, grad_stride):
+    """A gradient over some of the scores that other blocks still read: refused.  Over all of them
+    in place, between their rows or beside them: not refused."""
+    lib = F.load()
+    middle = P + (1 << 14)
+    far = rows * max(stride, grad_stride) + 3
+    for at in range(-far, far + 1):
+        in_place = at == 0 and (stride == grad_stride or rows == 1)
+        refused = not in_place and _meet(rows, len_, stride, at, grad_stride)
+        for message in _grad_calls(lib, middle, type, rows, len_, stride, middle + at * size, grad_stride):
+            assert ("overlaps" in message) == refused, (at, message)
+
+
+def test_wide_rows_beside_each_other_are_looked_at_quickly():
+    """Halves of one buffer's rows, many of them: decided by the strides, not row by row."""
+    lib, rows, len_ = F.load(), 10_000_000, 50
+    for at, refused in ((50, False), (49, True), (150, False), (151, True), (-50, False), (-49, True), (-150, False),
+                        (-151, True)):
+        for message in _grad_calls(lib, 1 << 40, F32, rows, len_, 200, (1 << 40) + at * 4, 200):
+            assert ("overlaps" in message) == refused, (at, message)
