@@ -331,9 +331,13 @@ def _address(t):
 
 
 def _like_rows(scores, stride):
-    """A tensor for the gradient whose rows lie as the scores' do."""
+    """A tensor for the gradient whose rows lie as the scores' do; where those are slices of much
+    wider ones (more than an eighth of a row lies between them), as close together as rows that
+    begin at the same places of 16-byte vectors can."""
     n, v = scores.shape
-    return torch.empty_strided((n, v), (stride, 1), dtype=scores.dtype, device=scores.device)
+    if stride - v > v // 8:
+        stride = v + (stride - v) % (16 // scores.element_size())
+    return torch.empty_strided((n, v), (stride, 1), dtype=scores.dtype, device=scores.device), stride
 
 
 def distill_forward(scores, ids, values, teacher_lse=None, temperature=1.0):
@@ -367,7 +371,7 @@ def _written(out):
 
 def _gradient(scores, stride, out):
     if out is None:
-        return _like_rows(scores, stride), stride
+        return _like_rows(scores, stride)
     _need(out.dtype == scores.dtype and out.shape == scores.shape, "out: the scores' shape and type are needed")
     _, out_stride = _matrix("out", out, scores)
     _need(out.data_ptr() != scores.data_ptr() or out_stride == stride, "out: in place, the scores' rows are needed")
@@ -378,7 +382,7 @@ def distill_backward(weight, scores, ids, values, saved, teacher_lse=None, tempe
     """Gradient of sum(weight * loss) by the scores, in their type; the arguments are those of
     the forward call (teacher_lse is part of ``saved`` already).  ``out`` may be the scores
     themselves, which the gradient then replaces, but not overlap them otherwise; by default it is
-    a new tensor whose rows lie as theirs."""
+    a new tensor whose rows lie as theirs, but without wide gaps."""
     kind, stride = _matrix("scores", scores)
     ids, values, _ = _teacher(scores, ids, values, teacher_lse)
     n, v = scores.shape

@@ -138,3 +138,32 @@ def test_gradients_beside_and_over_the_scores():
         assert torch.equal(scores, s)
     assert torch.equal(S.distill_step(scores, ids, values, out=scores)[1], want)
     assert torch.equal(wide[:, :400], want) and torch.equal(wide[:, 500:900], want)
+
+
+@pytest.mark.parametrize("kind", ["fp32", "fp16", "bf16"])
+@pytest.mark.parametrize("n,v,width,first", [(64, 50, 100_000, 0), (64, 50, 100_003, 3), (40, 999, 8 * 999, 999), (16, 1000, 1 << 16, 5),
+                                             (9, 3, 70, 1), (1, 30, 500, 7), (4, 0, 100, 0)])
+def test_gradients_of_slices_of_wide_rows(n, v, width, first, kind):
+    """A gradient takes the room of its own elements, not of the buffer that the scores lie in."""
+    g = torch.Generator(device="cuda").manual_seed(n + v + width)
+    wide = torch.randn(n, width, device="cuda", generator=g).to(TYPES[kind])
+    s = wide[:, first:first + v]
+    ids = torch.randint(0, max(v, 1), (n, 3), device="cuda", generator=g, dtype=torch.int32)
+    values = torch.randn(n, 3, device="cuda", generator=g)
+    # the same scores' gradients into rows that lie as theirs
+    as_wide = torch.zeros_like(wide)
+    want_loss, want = S.distill_step(s, ids, values, out=as_wide[:, first:first + v])
+    loss, grad = S.distill_step(s, ids, values)
+    assert torch.equal(grad, want) and torch.equal(loss, want_loss)
+    saved = S.distill_forward(s, ids, values)[1]
+    want = S.distill_backward(None, s, ids, values, saved, out=as_wide[:, first:first + v])
+    apart = S.distill_backward(None, s, ids, values, saved)
+    assert torch.equal(apart, want)
+    for got in (grad, apart):
+        assert got.dtype == s.dtype and got.untyped_storage().nbytes() <= n * (v + 16) * s.element_size()
+    leaf = wide.clone().requires_grad_()
+    S.distill_loss(leaf[:, first:first + v], ids, values).sum().backward()
+    assert torch.equal(leaf.grad, as_wide)
+    padded = torch.randn(n, v + 8, device="cuda", generator=g).to(TYPES[kind])[:, :v]
+    if v > 64 and n > 1:  # little lies between these: their gradient's rows lie as theirs
+        assert S.distill_step(padded, ids, values)[1].stride() == padded.stride()
