@@ -132,11 +132,14 @@ class _Underivable(torch.autograd.Function):
     @staticmethod
     def forward(ctx, message, of, *results):
         ctx.message = message
-        return results
+        ctx.set_materialize_grads(False)
+        return tuple(r if r is None else r.detach() for r in results)  # as themselves they could not be changed in place
 
     @staticmethod
-    def backward(ctx, *_):
-        raise RuntimeError(ctx.message)
+    def backward(ctx, *grads):
+        if any(g is not None for g in grads):
+            raise RuntimeError(ctx.message)
+        return (None,) * (len(grads) + 2)
 
 
 def _once(name, *grads):
@@ -282,7 +285,8 @@ def linear_fp8(x, w, dtype=torch.bfloat16):
 def top_scores(scores, k, temperature=1.0):
     """(values [n, k] float32, ids [n, k] int32, lse [n] float32): the first k scores of each
     row, larger first and of equal ones the lower id, and log sum exp(score / temperature) of
-    the whole row.  Columns at -inf are not listed; missing entries are (-inf, -1)."""
+    the whole row.  Columns at -inf are not listed; missing entries are (-inf, -1).  There is no
+    gradient: of scores that require one, differentiating values or lse raises."""
     kind, stride = _matrix("scores", scores)
     n, v = scores.shape
     if not 1 <= k <= MAX_K:
@@ -296,6 +300,9 @@ def top_scores(scores, k, temperature=1.0):
                                     device=scores.device)
         check(lib.ung_hip_top_scores(scores.data_ptr(), kind, n, v, stride, k, temperature, values.data_ptr(),
                                      ids.data_ptr(), lse.data_ptr(), at, size, stream))
+    if scores.requires_grad and torch.is_grad_enabled():
+        values, lse = _Underivable.apply("top_scores has no gradient: detach its values and log-sum-exp", scores,
+                                         values, lse)
     return values, ids, lse
 
 

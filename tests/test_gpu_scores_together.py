@@ -167,3 +167,27 @@ def test_gradients_of_slices_of_wide_rows(n, v, width, first, kind):
     padded = torch.randn(n, v + 8, device="cuda", generator=g).to(TYPES[kind])[:, :v]
     if v > 64 and n > 1:  # little lies between these: their gradient's rows lie as theirs
         assert S.distill_step(padded, ids, values)[1].stride() == padded.stride()
+
+
+def test_top_scores_of_a_model_in_training():
+    """Lists of scores that require a gradient are made as before; only differentiating their
+    values or log-sum-exp, which have no gradient, is refused."""
+    s, _, _ = _student(20, 700)
+    want = S.top_scores(s, 8)
+    leaf = s.clone().requires_grad_()
+    values, ids, lse = got = S.top_scores(leaf, 8)
+    assert all(torch.equal(a, b) for a, b in zip(got, want)) and not ids.requires_grad
+    for loss in (values.sum(), lse.sum(), leaf.sum() + lse.sum(), (leaf.gather(1, ids.long()) - values).sum()):
+        with pytest.raises(RuntimeError, match="top_scores"):
+            loss.backward()
+    leaf.grad = None
+    leaf.gather(1, ids.long()).sum().backward()
+    assert torch.equal(leaf.grad.sum(dim=1), torch.full((20,), 8.0, device="cuda"))
+    loss = S.distill_loss(leaf, ids, values.detach(), teacher_lse=lse.detach())
+    assert torch.isfinite(torch.autograd.grad(loss.sum(), leaf)[0]).all()
+    # a teacher's side is taken as given, however it was made
+    assert torch.isfinite(torch.autograd.grad(S.distill_loss(leaf, ids, values, teacher_lse=lse).sum(), leaf)[0]).all()
+    with torch.no_grad():
+        assert not any(t.requires_grad for t in S.top_scores(leaf, 8))
+    assert not any(t.requires_grad for t in S.top_scores(s, 8))
+    assert torch.equal(S.top_scores(leaf, 8)[0].neg_(), -want[0])
