@@ -260,3 +260,35 @@ def test_errors_of_the_8_bit_matrix_instruction(m, n, d, kind):
     ulp = 2 * HALF_ULP[kind] * torch.exp2(torch.floor(torch.log2(want.abs().clamp(min=2.0 ** -14))))
     bound = 1.5 * (ulp * (0.8 * 1.4e-5 * share)).mean()
     assert (got.double() - rounded.double()).square().mean() <= bound
+
+
+# ---- what a layer needs of its operands ----------------------------------------------------------------
+@pytest.mark.parametrize("kind", ["fp32", "fp16", "bf16"])
+@pytest.mark.parametrize("n,d,pad", [(1, 1, 0), (3, 130, 5), (300, 1000, 0), (129, 257, 3)])
+def test_transposed_operand_alone(n, d, pad, kind):
+    """Without the rows' own operand (q NULL) the transposed one is the same."""
+    x = torch.randn(n, d + pad, generator=_gen(n + d)).to(TYPES[kind]).cuda()[:, :d]
+    _, _, qt, scale_t = S.quantize_fp8(x, transpose=True)
+    qt2, scale_t2 = S._transposed(x)
+    assert torch.equal(qt2.view(torch.uint8), qt.view(torch.uint8)) and torch.equal(scale_t2, scale_t)
+
+
+def test_weight_gradient_alone_makes_no_rows_operand(monkeypatch):
+    """Of a layer whose input needs no gradient: the upstream gradient is brought to 8 bits along
+    the rows of its transpose alone, and the result is the same."""
+    x, w = torch.randn(200, 300, device="cuda"), torch.randn(500, 300, device="cuda", requires_grad=True)
+    up = torch.randn(200, 500, device="cuda", dtype=torch.bfloat16)
+    (want,) = torch.autograd.grad(S.linear_fp8(x.clone().requires_grad_(), w), w, up)
+    y = S.linear_fp8(x, w)
+    lib, calls = S._library(), []
+
+    class Seen:
+        def __getattr__(self, name):
+            if name == "ung_hip_fp8_quantize":
+                return lambda *a: calls.append(a[6:10]) or lib.ung_hip_fp8_quantize(*a)
+            return getattr(lib, name)
+
+    monkeypatch.setattr(S, "_ready", Seen())
+    (got,) = torch.autograd.grad(y, w, up)
+    assert torch.equal(got, want)
+    assert len(calls) == 1 and calls[0][:2] == (None, None) and all(calls[0][2:])

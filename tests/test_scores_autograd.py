@@ -15,6 +15,7 @@ def plain(monkeypatch):
         return torch.logsumexp(scores, dim=1), scores
 
     monkeypatch.setattr(S, "quantize_fp8", quantize_fp8)
+    monkeypatch.setattr(S, "_transposed", lambda x: (x.t(), None))
     monkeypatch.setattr(S, "matmul_fp8", lambda a, _, b, __, dtype=None: a @ b.t())
     monkeypatch.setattr(S, "matmul_fp8_grad", lambda g, xt, _, wt, __: (g @ wt.t(), g.t() @ xt.t()))
     monkeypatch.setattr(S, "distill_forward", distill_forward)
