@@ -879,15 +879,15 @@ int check_scores(const char *what, const void *scores, int type, uint64_t rows, 
     return UNG_HIP_OK;
 }
 
+Temperature temperature_of(float t) { return Temperature{1.0f / t, (float)(LOG2E / t)}; }
+
 int check_temperature(const char *what, float t)
 {
-    if (t > 0.0f && t < __builtin_inff())
+    if (t > 0.0f && t < __builtin_inff() && temperature_of(t).c < __builtin_inff())
         return UNG_HIP_OK;
-    set_error("%s: temperature %g is not a positive number", what, (double)t);
+    set_error("%s: temperature %g is not a positive number with a reciprocal in 32 bits", what, (double)t);
     return UNG_HIP_EINVAL;
 }
-
-Temperature temperature_of(float t) { return Temperature{1.0f / t, (float)(LOG2E / t)}; }
 
 int check_k(const char *what, uint32_t k, uint32_t least)
 {

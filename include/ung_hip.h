@@ -356,14 +356,15 @@ int ung_hip_fp8_matmul(const uint8_t *a, const float *a_scale, const uint8_t *b,
                        uint64_t m, uint64_t n, uint64_t kp, void *c, int type, uint64_t c_stride, void *workspace,
                        uint64_t workspace_bytes, void *stream);
 
-/* Largest k of the two operators below. */
+/* Largest k of the two operators below.  Their temperature T is a positive number with 1 / T and
+ * log2(e) / T in the range of 32 bits. */
 #define UNG_HIP_TOP_SCORES_MAX 128
 
 /* The first k scores of each row in (score descending, id ascending) order: values [rows x k]
  * in 32 bits, ids [rows x k], and lse [rows] (nullable) = log sum exp(score / temperature)
  * over the whole row.  NaN counts as larger than every score; -inf marks a column filtered
  * out and is never listed: missing entries have id -1 (UINT32_MAX as in the rows of
- * ung_hip_cross_topk) and value -inf.  1 <= k <= UNG_HIP_TOP_SCORES_MAX, len < 2^31 - 64. */
+ * ung_hip_cross_topk) and value -inf.  1 <= k <= UNG_HIP_TOP_SCORES_MAX, len <= 2^31 - 64. */
 int ung_hip_top_scores_workspace(const void *scores, int type, uint64_t rows, uint64_t len, uint64_t row_stride,
                                  uint32_t k, uint64_t *bytes);
 int ung_hip_top_scores(const void *scores, int type, uint64_t rows, uint64_t len, uint64_t row_stride, uint32_t k,

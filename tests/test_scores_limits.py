@@ -82,3 +82,18 @@ def test_wide_rows_beside_each_other_are_looked_at_quickly():
                         (-151, True)):
         for message in _grad_calls(lib, 1 << 40, F32, rows, len_, 200, (1 << 40) + at * 4, 200):
             assert ("overlaps" in message) == refused, (at, message)
+
+
+@pytest.mark.parametrize("t", [1e-45, 1e-40, 1e-39, 2.9e-39, 4.2e-39])
+def test_temperatures_whose_reciprocal_overflows(t):
+    """log2(e) / T past float32 makes 0 * inf of a row's largest score: refused, not NaN."""
+    lib = F.load()
+    _refused(lib.ung_hip_top_scores(P, 0, 4, 4, 4, 2, t, None, P, P, None, 0, None), "temperature")
+    _refused(lib.ung_hip_distill_forward(P, 0, 4, 4, 4, P, P, 2, None, t, None, P, None, 0, None), "temperature")
+    _refused(lib.ung_hip_distill_backward(P, 0, 4, 4, 4, P, P, 2, None, None, t, P, 4, None), "temperature")
+    _refused(lib.ung_hip_distill_step(P, 0, 4, 4, 4, P, P, 2, None, None, t, None, P, 4, None, 0, None), "temperature")
+
+
+@pytest.mark.parametrize("t", [4.3e-39, 1e-38, 1e-3, 1.0, 1e30, 3e38])
+def test_temperatures_that_are_served(t):
+    _refused(F.load().ung_hip_top_scores(P, 0, 4, 4, 4, 2, t, None, P, P, None, 0, None), "null values")
