@@ -322,10 +322,9 @@ def top_scores(scores, k, temperature=1.0):
 def entries_of_neighbors(ids, distances):
     """Neighbour rows (ids uint32/int32, missing ones UINT32_MAX / -1; squared distances, missing
     ones +inf) as a teacher's top scores: (ids int32, -distance float32)."""
-    if isinstance(ids, torch.Tensor):
-        ids = ids.view(torch.int32) if ids.dtype != torch.int32 else ids
-    else:
-        ids = torch.from_numpy(ids.view("int32"))
+    if str(ids.dtype).split(".")[-1] not in ("uint32", "int32"):
+        raise ValueError(f"ids: uint32 or int32 is needed, got {ids.dtype}")
+    ids = ids.view(torch.int32) if isinstance(ids, torch.Tensor) else torch.from_numpy(ids.view("int32"))
     distances = distances if isinstance(distances, torch.Tensor) else torch.from_numpy(distances)
     return ids, -distances.float()
 
