@@ -292,3 +292,71 @@ def test_weight_gradient_alone_makes_no_rows_operand(monkeypatch):
     (got,) = torch.autograd.grad(y, w, up)
     assert torch.equal(got, want)
     assert len(calls) == 1 and calls[0][:2] == (None, None) and all(calls[0][2:])
+
+
+def _stands_for(q, scale, block="row"):
+    scale = scale if block == "row" else scale.repeat_interleave(128, dim=0)[:q.shape[0]]
+    return q.double() * scale.double().repeat_interleave(128, dim=1)
+
+
+@pytest.mark.parametrize("kind", ["bf16", "fp16", "fp32"])
+@pytest.mark.parametrize("m,n,d", [(40, 300, 200), (300, 1000, 100), (1, 129, 128)])
+def test_layer_against_64_bits(m, n, d, kind):
+    """linear_fp8 and its gradients (bfloat16 is its default type) against the products of the
+    operands that the formulas name: y = x w^T, dx = g w, dw = g^T x, each side in 8 bits along
+    the inner length."""
+    g = torch.Generator(device="cuda").manual_seed(m + n + d)
+    x = torch.randn(m, d, device="cuda", generator=g).requires_grad_()
+    w = torch.randn(n, d, device="cuda", generator=g).requires_grad_()
+    y = S.linear_fp8(x, w) if kind == "bf16" else S.linear_fp8(x, w, dtype=TYPES[kind])
+    up = torch.randn(m, n, device="cuda", generator=g).to(TYPES[kind])
+    assert y.dtype == TYPES[kind]
+    y.backward(up)
+    xq, xs, xt, xts = S.quantize_fp8(x.detach(), transpose=True)
+    wq, ws, wt, wts = S.quantize_fp8(w.detach(), block="square", transpose=True)
+    gq, gs, gt, gts = S.quantize_fp8(up, transpose=True)
+    for got, a, b, type in ((y, _stands_for(xq, xs), _stands_for(wq, ws, "square"), kind),
+                            (x.grad, _stands_for(gq, gs), _stands_for(wt, wts, "square"), kind),
+                            (w.grad, _stands_for(gt, gts), _stands_for(xt, xts), "fp32")):
+        want, kp = a @ b.t(), a.shape[1]
+        bound = ((kp + 2 * kp // 128 + 2) * EPS + (2.0 ** -10 if type != "fp32" else 0.0)) * (a.abs() @ b.abs().t())
+        bound += HALF_ULP[type] * want.abs() * 1.001 + 2.0 ** -25
+        assert ((got.detach().double() - want).abs() <= bound).all()
+
+
+def test_zeros_of_either_sign_have_the_byte_0():
+    x = torch.tensor([[-0.0, 0.0, 1.0, -2.0]], device="cuda")
+    for kind in TYPES:
+        q, _ = S.quantize_fp8(x.to(TYPES[kind]))
+        assert q.view(torch.uint8)[0, :2].tolist() == [0, 0] and not q.view(torch.uint8)[0, 4:].any()
+
+
+def test_threads_and_streams_at_once():
+    """Four threads, each on a stream of its own with its own sizes: what each gets alone."""
+    from concurrent.futures import ThreadPoolExecutor
+
+    def work(seed):
+        g = torch.Generator(device="cuda").manual_seed(seed)
+        m, n, d = 60 + 70 * seed, 900 + 300 * seed, 130 + 100 * seed
+        x, w = torch.randn(m, d, device="cuda", generator=g), torch.randn(n, d, device="cuda", generator=g)
+        long = torch.randn(2, 90_000 + seed, device="cuda", generator=g)
+        out = []
+        for _ in range(5):
+            y = S.matmul_fp8(*S.quantize_fp8(x), *S.quantize_fp8(w, block="square"))
+            values, ids, lse = S.top_scores(y, 20)
+            loss, grad = S.distill_step(y, ids, values, teacher_lse=lse + 0.1)
+            out += [y, values, ids, lse, loss, grad, *S.top_scores(long, 32),
+                    *S.distill_step(long, ids[:2], values[:2])]
+        torch.cuda.current_stream().synchronize()
+        return [t.cpu() for t in out]
+
+    alone = [work(i) for i in range(4)]
+
+    def on_a_stream(seed):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            return work(seed)
+
+    with ThreadPoolExecutor(4) as pool:
+        together = list(pool.map(on_a_stream, range(4)))
+    for a, b in zip(alone, together):
+        assert all(torch.equal(s, t) for s, t in zip(a, b))
