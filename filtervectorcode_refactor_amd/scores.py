@@ -115,10 +115,6 @@ def _blocks(n):
     return -(-n // BLOCK)
 
 
-def _address(t):
-    return None if t is None else t.data_ptr()
-
-
 def _workspace(fn, *args, device):
     """(tensor, address, bytes) of a call's workspace, from torch's allocator on its stream."""
     need = C.c_uint64()
@@ -168,29 +164,32 @@ def quantize_fp8(x, block="row", transpose=False):
         return _quantize(x, kind, stride, block == "square", transpose, _library(), stream)
 
 
-def _quantize(x, kind, row_stride, square, transpose, lib, stream, rows=True):
-    """(q, scale) with ``rows``, and (qt, scale_t) with ``transpose``."""
+def _quantize(x, kind, row_stride, square, transpose, lib, stream):
     n, d = x.shape
     nb, db, device = _blocks(n), _blocks(d), x.device
-    q = scale = qt = scale_t = None
-    if rows:
-        q = torch.empty(n, db * BLOCK, dtype=FP8, device=device)
-        scale = torch.empty(nb if square else n, db, device=device)
-    if transpose:
-        qt = torch.empty(d, nb * BLOCK, dtype=FP8, device=device)
-        scale_t = torch.empty(db if square else d, nb, device=device)
-    check(lib.ung_hip_fp8_quantize(x.data_ptr(), kind, n, d, row_stride, square, _address(q), _address(scale),
-                                   _address(qt), _address(scale_t), stream))
+    q = torch.empty(n, db * BLOCK, dtype=FP8, device=device)
+    scale = torch.empty(nb if square else n, db, device=device)
     if not transpose:
+        check(lib.ung_hip_fp8_quantize(x.data_ptr(), kind, n, d, row_stride, square, q.data_ptr(), scale.data_ptr(),
+                                       None, None, stream))
         return q, scale
-    return (q, scale, qt, scale_t) if rows else (qt, scale_t)
+    qt = torch.empty(d, nb * BLOCK, dtype=FP8, device=device)
+    scale_t = torch.empty(db if square else d, nb, device=device)
+    check(lib.ung_hip_fp8_quantize(x.data_ptr(), kind, n, d, row_stride, square, q.data_ptr(), scale.data_ptr(),
+                                   qt.data_ptr(), scale_t.data_ptr(), stream))
+    return q, scale, qt, scale_t
 
 
 def _transposed(x):
     """(qt, scale_t) of quantize_fp8(x, transpose=True) alone: the rows' own bytes are not written."""
     kind, stride = _matrix("x", x)
+    n, d = x.shape
+    qt = torch.empty(d, _blocks(n) * BLOCK, dtype=FP8, device=x.device)
+    scale_t = torch.empty(d, _blocks(n), device=x.device)
     with _On(x) as stream:
-        return _quantize(x, kind, stride, False, True, _library(), stream, rows=False)
+        check(_library().ung_hip_fp8_quantize(x.data_ptr(), kind, n, d, stride, False, None, None, qt.data_ptr(),
+                                              scale_t.data_ptr(), stream))
+    return qt, scale_t
 
 
 def _operand(name, q, scale, like=None):
@@ -342,6 +341,10 @@ def _teacher(scores, ids, values, lse):
     ids = ids if ids.is_contiguous() else ids.contiguous()
     values = values if values.is_contiguous() else values.contiguous()
     return ids, values, lse if lse is None else _vector("teacher_lse", lse, n, scores)
+
+
+def _address(t):
+    return None if t is None else t.data_ptr()
 
 
 def _like_rows(scores, stride):
