@@ -1124,11 +1124,14 @@ struct Plan {
 // 10.6, 12.7; past three a CU 2500 x 2500 x 2048 26.8, 22.3, 700 x 10000 x 4096 50.1, 40.2.
 // Shares of the inner length where tiles leave CUs free.  BIG: at least four of at least 32
 // blocks (4096 x 768 x 32768 129 us, 128 x 128 tiles 175; 4096 x 768 x 8192 in shares of 16 54, 49).
-// Else as many as make the sum of the stages one share takes (0.6 us each; in 32 bits 1.4, of 64
-// rows 1.0) and of the joining pass (4 us, 0.1 a share and its traffic at 3 TB/s) least, with 128 x
-// 128 tiles: 1000 x 100 x 4096 in 32 bits 14 us (64 rows 10.6), in one 45; 150 x 150 x 65536 21, 328;
-// 512 x 512 x 2048 10.9, 13.7; 1024 x 1024 x 2048 stayed in one, 14.0, in two 18.5.  Shares of 64 rows
-// by 0.42 us a stage in 16 bits were fewer and slower: 64 x 10000 x 4096 21.2, by 0.6 14.8.
+// Else as many as make a cost least: 0.6 for each stage of one share (in 32 bits 1.4, of 64 rows
+// 1.0), 4 for the joining pass, 0.1 a share, and its traffic in us at 3 TB/s.  These are weights
+// by which the plan that measured faster is chosen, not times: a stage takes 0.43 us in 16 bits and
+// 0.7 in 32 where a tile has its CU to itself, 1.1 and 2.0 where two of 128 rows share it, and a
+// small product 4.2 us beside its stages.  With 128 x 128 tiles: 1000 x 100 x 4096 in 32 bits 14 us
+// (64 rows 10.6), in one 45; 150 x 150 x 65536 21, 328; 512 x 512 x 2048 10.9, 13.7; 1024 x 1024 x
+// 2048 stayed in one, 14.0, in two 18.5.  Shares of 64 rows in 16 bits by the 0.42 that a stage took
+// in them were fewer and slower: 64 x 10000 x 4096 21.2, by 0.6 14.8.
 Plan plan_of(uint64_t m, uint64_t n, uint64_t kp, int type)
 {
     const uint64_t kblocks = kp / KB, cus = cu_count();
