@@ -11,7 +11,8 @@ scores queries against its table.  Thin calls of the C ABI's score operators
                      call, and the differentiable function
   entries_of_neighbors  neighbour rows (ids, distances) as a teacher's top scores
 
-Scores may have any row stride; bfloat16, float16 and float32.  A wrong argument raises
+linear_fp8 and distill_loss are differentiable, once; the passes and products return results
+without a graph.  Scores may have any row stride; bfloat16, float16 and float32.  A wrong argument raises
 ``ValueError`` or ``UngHipError``; there is no CPU fallback.
 """
 from __future__ import annotations
