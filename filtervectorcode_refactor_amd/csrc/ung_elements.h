@@ -1,10 +1,12 @@
 // ung_elements.h -- device helpers shared by the score operators' translation units
-// (ung_fp8.hip, ung_scores.hip): element types, 16-byte vectors of them, reductions over a
-// wave and a block, and the host's launch checks.  Not part of the public ABI.
+// (ung_fp8.hip, ung_scores.hip, ung_int8.hip, ung_table_loss.hip, ung_gradients.hip): element
+// types, 16-byte vectors of them, reductions over a wave and a block, loads past the registers,
+// the order of tiles, and the host's launch checks.  Not part of the public ABI.
 #pragma once
 
 #include <hip/hip_runtime.h>
 
+#include <atomic>
 #include <cstdint>
 #include <type_traits>
 
@@ -115,6 +117,120 @@ __device__ inline float block_reduce(float v, float *red, F f)
             v = f(v, red[w]);
     }
     return v;
+}
+
+using f32x4 = __attribute__((ext_vector_type(4))) float;
+using bf16x8 = __attribute__((ext_vector_type(8))) __bf16;
+using u32x4 = __attribute__((ext_vector_type(4))) uint32_t;
+
+// 16 bytes from an address that is aligned to its elements alone; global memory takes such
+// loads whole (300000 x 203 bf16 44 us, by elements 67).
+template <class T>
+__device__ inline Vec<T> load_loose(const T *p)
+{
+    Vec<T> v;
+    __builtin_memcpy(&v, p, sizeof v);
+    return v;
+}
+
+template <class T>
+__device__ inline void store_loose(T *p, const Vec<T> &v)
+{
+    __builtin_memcpy(p, &v, sizeof v);
+}
+
+// Largest magnitude as the bits of its absolute value: whole numbers order like the
+// magnitudes, and a NaN is above every one of them, so it reaches the scale.
+__device__ inline uint32_t magnitude(float x) { return __float_as_uint(x) & 0x7FFFFFFFu; }
+
+// x / s rounded as the division rounds, with r = 1 / s from one division a block: the
+// product's remainder, exact in a fused multiply-add, corrects it (Markstein's step; r is
+// itself correctly rounded, s is a normal number).  A block with an infinity has s = inf,
+// r = 0, where the step would make a NaN of every value: with s = 0 there it adds nothing.
+struct alignas(8) Divisor {
+    float s, r;
+    Divisor() = default;
+    __device__ explicit Divisor(float scale) : s(scale), r(1.0f / scale)
+    {
+        if (r == 0.0f)
+            s = 0.0f;
+    }
+};
+__device__ inline float quotient(float x, Divisor d)
+{
+    const float q = x * d.r;
+    return __builtin_fmaf(__builtin_fmaf(-d.s, q, x), d.r, q);
+}
+
+// What lanes of a wave wrote to LDS is read by others after this, and the other way round (a
+// wave's LDS operations are done in order).
+__device__ inline void wave_lds_fence()
+{
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+}
+
+// 16 (or 4) bytes a lane from global memory straight into LDS, at `lds` + 16 (4) * lane.
+using lds_ptr = __attribute__((address_space(3))) void *;
+__device__ inline void to_lds16(__amdgpu_buffer_rsrc_t from, uint32_t offset, uint32_t advance, void *lds)
+{
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(from, (lds_ptr)lds, 16, offset, advance, 0, 0);
+}
+__device__ inline void to_lds4(__amdgpu_buffer_rsrc_t from, uint32_t offset, uint32_t advance, void *lds)
+{
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(from, (lds_ptr)lds, 4, offset, advance, 0, 0);
+}
+
+__device__ inline __amdgpu_buffer_rsrc_t buffer_of(const void *p, uint32_t bytes = 0xFFFFFFFFu)
+{
+    return __builtin_amdgcn_make_buffer_rsrc(const_cast<void *>(p), 0, bytes, 0x00020000);
+}
+
+template <int N>
+__device__ inline void await_loads()
+{
+    // at most N of the wave's memory operations are still under way; loads into LDS count
+    asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
+}
+
+// Blocks go to the eight XCDs in turn; with this each XCD takes a contiguous run of `total`.
+__device__ inline uint32_t xcd_run(uint32_t id, uint32_t total)
+{
+    const uint32_t xcd = id & 7, each = total >> 3, extra = total & 7;
+    return xcd * each + (xcd < extra ? xcd : extra) + (id >> 3);
+}
+
+// Tile t of m_tiles x n_tiles, in bands of `band` tiles of m.
+__device__ inline void tile_of(uint32_t t, uint32_t band, uint32_t m_tiles, uint32_t n_tiles, uint32_t &tm,
+                               uint32_t &tn)
+{
+    const uint32_t b = t / (band * n_tiles), in = t - b * band * n_tiles;
+    const uint32_t high = m_tiles - b * band < band ? m_tiles - b * band : band;
+    tm = b * band + in % high;
+    tn = in / high;
+}
+
+// Divisions leave a block's numbers in vector registers.
+__device__ inline uint32_t uniform(uint32_t v) { return __builtin_amdgcn_readfirstlane(v); }
+
+// CUs of the current device, asked for once.
+inline uint32_t cu_count()
+{
+    static std::atomic<uint32_t> known[64];
+    int device = 0, n = 0;
+    if (hipGetDevice(&device) != hipSuccess || device < 0 || device >= 64) {
+        (void)hipGetLastError();
+        return 256;
+    }
+    uint32_t got = known[device].load(std::memory_order_relaxed);
+    if (!got) {
+        if (hipDeviceGetAttribute(&n, hipDeviceAttributeMultiprocessorCount, device) != hipSuccess || n < 8) {
+            (void)hipGetLastError();
+            n = 256;
+        }
+        known[device].store(got = (uint32_t)n, std::memory_order_relaxed);
+    }
+    return got;
 }
 
 inline bool known_type(int t) { return t == UNG_HIP_F32 || t == UNG_HIP_F16 || t == UNG_HIP_BF16; }

@@ -7,7 +7,6 @@
 // block's scale, s = max(largest magnitude, 2^-64) * (1 / 448), rounded to 32 bits.
 #include <hip/hip_runtime.h>
 
-#include <atomic>
 #include <cstdint>
 
 #include "ung_elements.h"
@@ -22,54 +21,12 @@ constexpr int KB = UNG_HIP_FP8_BLOCK; // inner length of a block: 128
 constexpr float LARGEST = 448.0f;     // largest finite e4m3 value
 constexpr float SMALLEST = 0x1p-64f;  // a block's largest magnitude counts as this at least
 
-// ---- order of the tiles ----------------------------------------------------------------
-
-// Blocks go to the eight XCDs in turn; with this each XCD takes a contiguous run of `total`.
-__device__ inline uint32_t xcd_run(uint32_t id, uint32_t total)
-{
-    const uint32_t xcd = id & 7, each = total >> 3, extra = total & 7;
-    return xcd * each + (xcd < extra ? xcd : extra) + (id >> 3);
-}
-
-// Tile t of m_tiles x n_tiles, in bands of `band` tiles of m.
-__device__ inline void tile_of(uint32_t t, uint32_t band, uint32_t m_tiles, uint32_t n_tiles, uint32_t &tm,
-                               uint32_t &tn)
-{
-    const uint32_t b = t / (band * n_tiles), in = t - b * band * n_tiles;
-    const uint32_t high = m_tiles - b * band < band ? m_tiles - b * band : band;
-    tm = b * band + in % high;
-    tn = in / high;
-}
-
 // ---- quantisation --------------------------------------------------------------------
-
-// Largest magnitude as the bits of its absolute value: whole numbers order like the
-// magnitudes, and a NaN is above every one of them, so it reaches the scale.
-__device__ inline uint32_t magnitude(float x) { return __float_as_uint(x) & 0x7FFFFFFFu; }
 
 __device__ inline float scale_of(uint32_t most)
 {
     const uint32_t least = __float_as_uint(SMALLEST);
     return __uint_as_float(most > least ? most : least) * (1.0f / LARGEST);
-}
-
-// x / s rounded as the division rounds, with r = 1 / s from one division a block: the
-// product's remainder, exact in a fused multiply-add, corrects it (Markstein's step; r is
-// itself correctly rounded, s is a normal number).  A block with an infinity has s = inf,
-// r = 0, where the step would make a NaN of every value: with s = 0 there it adds nothing.
-struct alignas(8) Divisor {
-    float s, r;
-    Divisor() = default;
-    __device__ explicit Divisor(float scale) : s(scale), r(1.0f / scale)
-    {
-        if (r == 0.0f)
-            s = 0.0f;
-    }
-};
-__device__ inline float quotient(float x, Divisor d)
-{
-    const float q = x * d.r;
-    return __builtin_fmaf(__builtin_fmaf(-d.s, q, x), d.r, q);
 }
 
 __device__ inline uint32_t pack4(const float *y)
@@ -78,22 +35,6 @@ __device__ inline uint32_t pack4(const float *y)
     return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(y[2], y[3], w, true);
 }
 __device__ inline uint2 pack8(const float *y) { return make_uint2(pack4(y), pack4(y + 4)); }
-
-// 16 bytes from an address that is aligned to its elements alone; global memory takes such
-// loads whole (300000 x 203 bf16 44 us, by elements 67).
-template <class T>
-__device__ inline Vec<T> load_loose(const T *p)
-{
-    Vec<T> v;
-    __builtin_memcpy(&v, p, sizeof v);
-    return v;
-}
-
-template <class T>
-__device__ inline void store_loose(T *p, const Vec<T> &v)
-{
-    __builtin_memcpy(p, &v, sizeof v);
-}
 
 // Eight consecutive elements of a row from column c; those at or past `cols` are 0.
 template <class T>
@@ -364,9 +305,7 @@ __global__ __launch_bounds__(TILE_NT) void ung_fp8_tile_kernel(const T *x, uint6
 // ---- product -------------------------------------------------------------------------
 
 using i32x8 = __attribute__((ext_vector_type(8))) int;
-using f32x4 = __attribute__((ext_vector_type(4))) float;
 using bf16x2 = __attribute__((ext_vector_type(2))) __bf16;
-using bf16x8 = __attribute__((ext_vector_type(8))) __bf16;
 
 // A lane's part of 16 rows of one block: row lane % 16, 32 of its 128 bytes by lane / 16.
 union Frag {
@@ -414,30 +353,6 @@ __device__ inline f32x4 block_product(const Wide &x, const Wide &y)
     for (int i = 0; i < 4; ++i)
         p = __builtin_amdgcn_mfma_f32_16x16x32_bf16(x.q[i], y.q[i], p, 0, 0, 0);
     return p;
-}
-
-// What lanes of a wave wrote to LDS is read by others after this, and the other way round (a
-// wave's LDS operations are done in order).
-__device__ inline void wave_lds_fence()
-{
-    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-    __builtin_amdgcn_wave_barrier();
-}
-
-// 16 (or 4) bytes a lane from global memory straight into LDS, at `lds` + 16 (4) * lane.
-using lds_ptr = __attribute__((address_space(3))) void *;
-__device__ inline void to_lds16(__amdgpu_buffer_rsrc_t from, uint32_t offset, uint32_t advance, void *lds)
-{
-    __builtin_amdgcn_raw_ptr_buffer_load_lds(from, (lds_ptr)lds, 16, offset, advance, 0, 0);
-}
-__device__ inline void to_lds4(__amdgpu_buffer_rsrc_t from, uint32_t offset, uint32_t advance, void *lds)
-{
-    __builtin_amdgcn_raw_ptr_buffer_load_lds(from, (lds_ptr)lds, 4, offset, advance, 0, 0);
-}
-
-__device__ inline __amdgpu_buffer_rsrc_t buffer_of(const void *p, uint32_t bytes = 0xFFFFFFFFu)
-{
-    return __builtin_amdgcn_make_buffer_rsrc(const_cast<void *>(p), 0, bytes, 0x00020000);
 }
 
 // What block `id` makes: a tile of the product, and which share of the inner length's blocks it
@@ -654,14 +569,6 @@ __global__ __launch_bounds__(WM * WN * 64, 2) void ung_fp8_product_kernel(const 
 // ---- large 16-bit products -------------------------------------------------------------
 
 using f32x16 = __attribute__((ext_vector_type(16))) float;
-using u32x4 = __attribute__((ext_vector_type(4))) uint32_t;
-
-template <int N>
-__device__ inline void await_loads()
-{
-    // at most N of the wave's memory operations are still under way; loads into LDS count
-    asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
-}
 
 constexpr int BIG = 256; // a tile is BIG x BIG
 // Tiles of m that follow each other before the next one of n.  The tiles that an XCD works on
@@ -670,9 +577,6 @@ constexpr int BIG = 256; // a tile is BIG x BIG
 // 32768 x 768: 16: 209, 8: 218, 4: 150, 2: 144, 1: 152 us; 8192 x 8192 x 8192: 520, 502, 497,
 // 515, 553 us.
 constexpr uint32_t BAND = 4;
-
-// Divisions leave a block's numbers in vector registers.
-__device__ inline uint32_t uniform(uint32_t v) { return __builtin_amdgcn_readfirstlane(v); }
 
 // Work of one block: one (tile, share of the inner length) item in each round of its XCD's
 // run of items.  XCDs begin in different rounds: in the same one they would write columns a
@@ -1081,26 +985,6 @@ __global__ __launch_bounds__(256) void ung_fp8_join_kernel(const float *part, ui
 }
 
 // ---- choice of the kernel ----------------------------------------------------------------
-
-// CUs of the current device, asked for once.
-uint32_t cu_count()
-{
-    static std::atomic<uint32_t> known[64];
-    int device = 0, n = 0;
-    if (hipGetDevice(&device) != hipSuccess || device < 0 || device >= 64) {
-        (void)hipGetLastError();
-        return 256;
-    }
-    uint32_t got = known[device].load(std::memory_order_relaxed);
-    if (!got) {
-        if (hipDeviceGetAttribute(&n, hipDeviceAttributeMultiprocessorCount, device) != hipSuccess || n < 8) {
-            (void)hipGetLastError();
-            n = 256;
-        }
-        known[device].store(got = (uint32_t)n, std::memory_order_relaxed);
-    }
-    return got;
-}
 
 // How a product is made: by tiles of BIG x BIG, or of `high` x 128, and from how many shares of
 // the inner length.
