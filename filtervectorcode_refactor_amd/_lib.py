@@ -101,6 +101,17 @@ SIGNATURES = {
                                         _vp]),
     "ung_hip_distill_step": (_int, [_vp, _int, _u64, _u64, _u64, _vp, _vp, _u32, _vp, _vp, C.c_float, _vp, _vp, _u64,
                                     _vp, _u64, _vp]),
+    "ung_hip_int8_quantize": (_int, [_vp, _int, _u64, _u64, _u64, _vp, _vp, _vp]),
+    "ung_hip_int8_matmul_workspace": (_int, [_u64, _u64, _u64, _int, C.POINTER(_u64)]),
+    "ung_hip_int8_matmul": (_int, [_vp, _vp, _vp, _vp, _u64, _u64, _u64, _vp, _int, _u64, _vp, _u64, _vp]),
+    "ung_hip_table_loss_workspace": (_int, [_vp, _u64, _vp, _u64, _int, _u64, _u64, _u64, _int, C.POINTER(_u64)]),
+    "ung_hip_table_loss_forward": (_int, [_vp, _u64, _vp, _u64, _int, _u64, _u64, _u64, _vp, _vp, C.c_float, _vp, _vp,
+                                          _vp, _u64, _vp]),
+    "ung_hip_table_loss_backward": (_int, [_vp, _u64, _vp, _u64, _int, _u64, _u64, _u64, _vp, _vp, _vp, _vp, C.c_float,
+                                           _vp, _u64, _vp, _u64, _vp, _u64, _vp]),
+    "ung_hip_gradient_workspace": (_int, [_vp, _u32, C.POINTER(_u64)]),
+    "ung_hip_gradient_norm": (_int, [_vp, _vp, _vp, _u32, _vp, _vp, _u64, _vp]),
+    "ung_hip_clip_gradients": (_int, [_vp, _vp, _vp, _vp, _u32, C.c_float, _vp, _vp, _u64, _vp]),
     "ung_divide_groups": (_int, [_u64, _vp, _vp, _vp, _vp, _vp, C.POINTER(_u32)]),
     "ung_group_label_sets": (_int, [_u64, _vp, _vp, _vp, _vp, _u32, _vp, _vp, _u64]),
     "ung_lng_build": (_int, [_u32, _vp, _vp, _vp, _vp, _u64, C.POINTER(_u64), _int]),

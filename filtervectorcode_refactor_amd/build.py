@@ -5,7 +5,8 @@ travels with the repository snapshot to the GPU box:
   * ung_host.cpp    -> g++ (host C++: synthetic inputs, groups, LNG, reorder)
   * ung_runtime.hip -> hipcc --offload-arch=gfx950 (context, planning, launches, C ABI;
                        includes ung_kernels.hip, the device code: one translation unit)
-  * ung_fp8.hip, ung_scores.hip -> hipcc (score operators: kernels and C ABI)
+  * ung_fp8.hip, ung_scores.hip, ung_int8.hip, ung_table_loss.hip, ung_gradients.hip
+    -> hipcc (score operators: kernels and C ABI)
 Packed-FP32 instruction selection is disabled for all device code.
 """
 from __future__ import annotations
@@ -19,7 +20,7 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 ROOT = os.path.dirname(HERE)
 CSRC = os.path.join(HERE, "csrc")
 INCLUDE = os.path.join(ROOT, "include")
-HIP_UNITS = ("ung_runtime", "ung_fp8", "ung_scores")  # translation units with device code
+HIP_UNITS = ("ung_runtime", "ung_fp8", "ung_scores", "ung_int8", "ung_table_loss", "ung_gradients")  # translation units with device code
 LIB_NAME = "libung_hip.so"
 LIB_PATH = os.path.join(HERE, LIB_NAME)
 ARCH = os.environ.get("UNG_HIP_ARCH", "gfx950")

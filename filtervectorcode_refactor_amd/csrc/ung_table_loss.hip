@@ -1,0 +1,637 @@
+// ung_table_loss.hip -- cross entropy of hidden states against every row of a table, and its
+// gradients, without the scores in memory, on gfx950: the kernels and the entry points
+// ung_hip_table_loss_* of include/ung_hip.h.
+//
+//   z_ij = x_i . t_j / T   (j not left out by row i)        lse_i = log sum_j exp z_ij
+//   loss_i = lse_i - z_i,id                                  0 for rows without a target
+//   g_ij = w_i / T (exp(z_ij - lse_i) - [j = id_i])          dX = G T,  dT = G^T X
+//
+// The forward pass makes tiles of scores and keeps of each only its rows' largest score and sum
+// of exponentials.  The backward pass makes the scores anew, a piece of the table's rows at a
+// time: G of the piece goes to memory in the inputs' type, where two products read it.
+#include <hip/hip_runtime.h>
+
+#include <cmath>
+#include <cstdint>
+
+#include "ung_elements.h"
+#include "ung_hip.h"
+#include "ung_internal.h"
+#include "ung_tiles.h"
+
+using namespace ung;
+
+namespace {
+
+constexpr float LOG2E = 1.44269504088896340736f;
+constexpr float INF = __builtin_huge_valf();
+constexpr int BN = 128; // columns of a tile
+
+// ---- forward -------------------------------------------------------------------------
+
+// A row's part of a tile of scores: the largest score s and sum exp((s - largest) / T).
+struct Part {
+    float top, sum;
+};
+
+__device__ inline Part joined(Part a, Part b, float c)
+{
+    const float top = fmaxf(a.top, b.top), from = top == -INF ? 0.0f : top;
+    return {top, a.sum * weight_of(a.top, from, c) + b.sum * weight_of(b.top, from, c)};
+}
+
+// Of a tile of scores (rows of x, columns: rows of the table): every row's part, and the
+// target's score where the tile holds it.
+struct LogSum {
+    const int32_t *ids, *without;
+    float *target; // [n]
+    Part *parts;   // [tiles of the table][n]
+    uint64_t n, v;
+    float c; // log2(e) / T
+
+    template <int TM>
+    __device__ inline void operator()(const Tile &t, f32x4 (&acc)[TM][4], uint8_t *lds) const
+    {
+        Part *red = reinterpret_cast<Part *>(lds); // [2][rows of the tile]
+        const uint32_t r = t.lane & 15, g = t.lane >> 4, high = t.high;
+        const uint64_t col0 = t.n0 + t.wn + g * 16;
+#pragma unroll
+        for (int i = 0; i < TM; ++i) {
+            const uint64_t row = t.m0 + t.wm + i * 16 + r, at = min(row, n - 1);
+            const uint32_t id = (uint32_t)ids[at] - (uint32_t)col0;
+            const uint32_t out = (without ? (uint32_t)without[at] : ~0u) - (uint32_t)col0;
+            if (__any(id < 16 || out < 16 || col0 + 16 > v)) {
+#pragma unroll
+                for (int e = 0; e < 16; ++e) {
+                    if (id == e && row < n)
+                        target[row] = acc[i][e / 4][e % 4];
+                    if (out == e || col0 + e >= v)
+                        acc[i][e / 4][e % 4] = -INF;
+                }
+            }
+            float top = -INF;
+#pragma unroll
+            for (int e = 0; e < 16; ++e)
+                top = fmaxf(top, acc[i][e / 4][e % 4]);
+            top = fmaxf(top, __shfl_xor(top, 16));
+            top = fmaxf(top, __shfl_xor(top, 32));
+            const float from = top == -INF ? 0.0f : top;
+            float sum = 0.0f;
+#pragma unroll
+            for (int e = 0; e < 16; ++e)
+                sum += weight_of(acc[i][e / 4][e % 4], from, c);
+            sum += __shfl_xor(sum, 16);
+            sum += __shfl_xor(sum, 32);
+            if (g == 0)
+                red[t.wn / 64 * high + t.wm + i * 16 + r] = {top, sum};
+        }
+        __syncthreads();
+        const uint64_t row = t.m0 + threadIdx.x;
+        if (threadIdx.x < high && row < n)
+            parts[t.n0 / BN * n + row] = joined(red[threadIdx.x], red[high + threadIdx.x], c);
+    }
+};
+
+// R rows a block, 256 / R threads each: a row's parts to its log-sum-exp and loss.
+template <int R>
+__global__ __launch_bounds__(256) void ung_table_join_kernel(const Part *parts, uint64_t tiles, uint64_t n, uint64_t v,
+                                                             const float *target, const int32_t *ids,
+                                                             const int32_t *without, float c, float by, float *loss,
+                                                             float *lse)
+{
+    __shared__ Part red[256];
+    constexpr uint32_t EACH = 256 / R;
+    const uint32_t in = threadIdx.x % R, which = threadIdx.x / R;
+    const uint64_t row = (uint64_t)blockIdx.x * R + in;
+    Part p = {-INF, 0.0f};
+    if (row < n) {
+#pragma unroll 4
+        for (uint64_t t = which; t < tiles; t += EACH)
+            p = joined(p, parts[t * n + row], c);
+    }
+    red[threadIdx.x] = p;
+    __syncthreads();
+#pragma unroll
+    for (uint32_t half = EACH / 2; half; half /= 2) {
+        if (which < half)
+            red[threadIdx.x] = joined(red[threadIdx.x], red[threadIdx.x + half * R], c);
+        __syncthreads();
+    }
+    if (which || row >= n)
+        return;
+    p = red[in];
+    const float log_sum = logf(p.sum);
+    const int32_t id = ids[row];
+    const bool there = (uint64_t)(uint32_t)id < v && !(without && without[row] == id);
+    // the difference first: it is exact where the target is near the largest score
+    loss[row] = there ? (p.top - target[row]) * by + log_sum : 0.0f;
+    lse[row] = p.sum == 0.0f ? -INF : p.top * by + log_sum;
+}
+
+// ---- backward ------------------------------------------------------------------------
+
+// What the gradient needs of a row: log-sum-exp in bits, weight / T, the target and the column
+// left out.  A row without a target: weight 0, log-sum-exp +inf and zeros in the place of x, so
+// that no number of a row of padding reaches the table's gradient.
+struct alignas(16) Row {
+    float lse2, weight;
+    int32_t id, out;
+};
+
+// fp16 holds no numbers below 2^-24: weights are brought to the top of its range by a power of
+// two (G is at most 2 |w| / T), which the gradients are divided by at the end.  scale: {by, 1 / by}.
+__global__ __launch_bounds__(1024) void ung_table_range_kernel(const float *weight, uint64_t n, float by, float *scale)
+{
+    __shared__ float red[16];
+    float most = weight || !n ? 0.0f : 1.0f;
+    if (weight)
+        for (uint64_t i = threadIdx.x; i < n; i += 1024) {
+            const float w = fabsf(weight[i]);
+            if (w < INF)
+                most = fmaxf(most, w);
+        }
+    most = block_reduce<1024>(most, red, [](float a, float b) { return fmaxf(a, b); }) * by;
+    if (threadIdx.x == 0) {
+        int e = 0;
+        if (most > 0.0f && most < INF)
+            (void)frexpf(most, &e); // most < 2^e
+        e = 14 - e;
+        e = e > 100 ? 100 : e < -100 ? -100 : e;
+        scale[0] = ldexpf(1.0f, e);
+        scale[1] = ldexpf(1.0f, -e);
+    }
+}
+
+// A wave a row: its numbers, and its elements as rows of whole vectors.
+template <class E>
+__global__ __launch_bounds__(256) void ung_table_rows_kernel(const E *x, uint64_t stride, uint64_t n, uint64_t v,
+                                                             uint64_t d, const int32_t *ids, const int32_t *without,
+                                                             const float *lse, const float *weight, float by,
+                                                             const float *scale, Row *rows, E *to, uint64_t pitch)
+{
+    const uint32_t lane = threadIdx.x & 63;
+    for (uint64_t row = blockIdx.x * 4ull + (threadIdx.x >> 6); row < n; row += gridDim.x * 4ull) {
+        const int32_t id = ids[row], out = without ? without[row] : -1;
+        const bool there = (uint64_t)(uint32_t)id < v && id != out;
+        if (lane == 0)
+            rows[row] = there ? Row{lse[row] * LOG2E, (weight ? weight[row] : 1.0f) * by * (scale ? scale[0] : 1.0f), id, out}
+                              : Row{INF, 0.0f, -1, -1};
+        for (uint64_t c = lane; c < pitch; c += 64)
+            to[row * pitch + c] = there && c < d ? x[row * stride + c] : (E)0.0f;
+    }
+}
+
+// Rows of any stride and length as rows of whole vectors.
+template <class E>
+__global__ __launch_bounds__(256) void ung_table_pack_kernel(const E *x, uint64_t stride, uint64_t rows, uint64_t d,
+                                                             E *to, uint64_t pitch)
+{
+    const uint32_t lane = threadIdx.x & 63;
+    for (uint64_t row = blockIdx.x * 4ull + (threadIdx.x >> 6); row < rows; row += gridDim.x * 4ull)
+        for (uint64_t c = lane; c < pitch; c += 64)
+            to[row * pitch + c] = c < d ? x[row * stride + c] : (E)0.0f;
+}
+
+// A tile of scores to G, in the inputs' type: half a step of it, 2^-9 of an element in bf16 and 2^-12 in
+// fp16, as far as the gradients' own rounding; the products that read it sum in 32 bits.
+template <class E>
+struct Weights {
+    const Row *rows;
+    E *g; // [n][pitch], pitch whole tiles: columns past the piece's end are zero
+    uint64_t pitch, n, v0, v;
+    float c;
+
+    template <int TM>
+    __device__ inline void operator()(const Tile &t, f32x4 (&acc)[TM][4], uint8_t *) const
+    {
+        const uint32_t r = t.lane & 15, gr = t.lane >> 4;
+        const uint64_t col0 = t.n0 + t.wn + gr * 16;
+#pragma unroll
+        for (int i = 0; i < TM; ++i) {
+            const uint64_t row = t.m0 + t.wm + i * 16 + r;
+            const Row p = rows[min(row, n - 1)];
+#pragma unroll
+            for (int e = 0; e < 16; ++e)
+                acc[i][e / 4][e % 4] = __builtin_amdgcn_exp2f(__builtin_fmaf(acc[i][e / 4][e % 4], c, -p.lse2));
+            const uint32_t id = (uint32_t)p.id - (uint32_t)(v0 + col0), out = (uint32_t)p.out - (uint32_t)(v0 + col0);
+            if (__any(id < 16 || out < 16 || col0 + 16 > v)) {
+#pragma unroll
+                for (int e = 0; e < 16; ++e) {
+                    if (id == e)
+                        acc[i][e / 4][e % 4] -= 1.0f;
+                    if (out == e || col0 + e >= v)
+                        acc[i][e / 4][e % 4] = 0.0f;
+                }
+            }
+            if (row >= n)
+                continue;
+            Vec<E> o[16 / Vec<E>::N];
+#pragma unroll
+            for (int e = 0; e < 16; e += 2)
+                o[e / Vec<E>::N].put2(e % Vec<E>::N, acc[i][e / 4][e % 4] * p.weight, acc[i][e / 4][e % 4 + 1] * p.weight);
+#pragma unroll
+            for (int x = 0; x < 16 / Vec<E>::N; ++x)
+                *reinterpret_cast<Vec<E> *>(g + row * pitch + col0 + x * Vec<E>::N) = o[x];
+        }
+    }
+};
+
+// A gradient's tile in its own type.
+template <class E>
+struct Whole {
+    E *c;
+    uint64_t stride, m, n;
+    const float *by;
+    int vectors;
+
+    template <int TM>
+    __device__ inline void operator()(const Tile &t, f32x4 (&acc)[TM][4], uint8_t *lds) const
+    {
+        const uint64_t col0 = t.n0 + t.wn;
+        if (col0 >= n)
+            return;
+        const float s = by ? by[0] : 1.0f;
+#pragma unroll
+        for (int i = 0; i < TM; ++i) {
+            const uint64_t row0 = t.m0 + t.wm + i * 16;
+            if (row0 >= m)
+                return;
+            Vec<E> o[16 / Vec<E>::N];
+#pragma unroll
+            for (int e = 0; e < 16; e += 2)
+                o[e / Vec<E>::N].put2(e % Vec<E>::N, acc[i][e / 4][e % 4] * s, acc[i][e / 4][e % 4 + 1] * s);
+            store_rows(c + row0 * stride + col0, stride, (uint32_t)min(m - row0, (uint64_t)16), n - col0, vectors, o,
+                       lds + t.wave * TURN, t.lane);
+        }
+    }
+};
+
+// Sums of a share of the inner length in 32 bits, alone or on top of an earlier piece's.
+struct Sums {
+    float *part;
+    uint64_t stride, m; // stride: whole tiles
+    int add;
+
+    template <int TM>
+    __device__ inline void operator()(const Tile &t, f32x4 (&acc)[TM][4], uint8_t *) const
+    {
+        const uint32_t r = t.lane & 15, g = t.lane >> 4;
+#pragma unroll
+        for (int i = 0; i < TM; ++i) {
+            const uint64_t row = t.m0 + t.wm + i * 16 + r;
+            if (row >= m)
+                continue;
+            f32x4 *to = reinterpret_cast<f32x4 *>(part + (t.split * m + row) * stride + t.n0 + t.wn + g * 16);
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                to[j] = add ? to[j] + acc[i][j] : acc[i][j];
+        }
+    }
+};
+
+template <class E>
+__global__ __launch_bounds__(256) void ung_table_sum_kernel(const float *part, uint32_t splits, uint64_t rows,
+                                                            uint64_t cols, uint64_t part_stride, const float *by, E *c,
+                                                            uint64_t c_stride)
+{
+    const uint64_t quads = (cols + 3) / 4;
+    const float scale = by ? by[0] : 1.0f;
+    for (uint64_t at = blockIdx.x * 256ull + threadIdx.x; at < rows * quads; at += gridDim.x * 256ull) {
+        const uint64_t row = at / quads, col = (at - row * quads) * 4;
+        f32x4 sum = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll 8
+        for (uint32_t s = 0; s < splits; ++s)
+            sum += *reinterpret_cast<const f32x4 *>(part + (s * rows + row) * part_stride + col);
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+            if (col + e < cols)
+                c[row * c_stride + col + e] = from_float<E>(sum[e] * scale);
+    }
+}
+
+// ---- plan and workspace ------------------------------------------------------------------
+
+uint32_t height_of(uint64_t m, uint64_t n)
+{
+    return m <= 32 ? 32 : m <= 64 || ceil_div(m, 64) * ceil_div(n, BN) <= 3 * (uint64_t)cu_count() ? 64 : 128;
+}
+
+// Shares of the inner length that fill the chip twice, of at least 4 chunks.
+uint32_t shares_of(uint64_t m, uint64_t n, uint64_t chunks)
+{
+    const uint64_t tiles = ceil_div(m, height_of(m, n)) * ceil_div(n, BN), most = 2 * (uint64_t)cu_count();
+    const uint64_t by_cu = most / (tiles ? tiles : 1), by_k = chunks / 4, s = by_cu < by_k ? by_cu : by_k;
+    return s > 1 ? (uint32_t)s : 1;
+}
+
+struct Inputs {
+    const void *x, *table;
+    uint64_t x_stride, table_stride;
+    int type;
+    uint64_t n, v, d;
+};
+
+// Where the parts of a workspace lie, all at 256-byte boundaries.
+struct Layout {
+    uint64_t bytes = 0;
+    uint64_t take(uint64_t size)
+    {
+        const uint64_t at = bytes;
+        bytes += ceil_div(size, 256) * 256;
+        return at;
+    }
+};
+
+struct Packed { // a side of the products, copied to rows of whole vectors where it does not lie so
+    bool copy;
+    uint64_t at, pitch; // bytes
+};
+
+Packed packed(Layout &l, const void *p, uint64_t stride, uint64_t rows, uint64_t d, uint64_t size, bool always)
+{
+    Packed o = {always, 0, ceil_div(d * size, 16) * 16};
+    if ((uintptr_t)p % 16 || d * size % 16 || (rows > 1 && (stride * size % 16 || stride * size >= MOST_STRIDE)))
+        o.copy = true;
+    if (o.copy)
+        o.at = l.take(rows * o.pitch);
+    return o;
+}
+
+struct Forward {
+    Layout l;
+    Packed x, table;
+    uint64_t tiles, parts, target;
+    explicit Forward(const Inputs &in)
+    {
+        const uint64_t size = type_size(in.type);
+        x = packed(l, in.x, in.x_stride, in.n, in.d, size, false);
+        table = packed(l, in.table, in.table_stride, in.v, in.d, size, false);
+        tiles = ceil_div(in.v, BN);
+        parts = l.take(tiles * in.n * sizeof(Part));
+        target = l.take(in.n * 4);
+    }
+};
+
+// G of a piece takes about this much (it is read while it lies in the last-level cache), of at
+// least 1024 rows of the table.
+constexpr uint64_t PIECE_BYTES = 128ull << 20;
+
+struct Backward {
+    Layout l;
+    Packed x, table;
+    uint64_t rows, scale, piece, pieces, g, x_sums, t_sums, sum_stride;
+    uint32_t x_splits, t_splits;
+    explicit Backward(const Inputs &in)
+    {
+        const uint64_t size = type_size(in.type);
+        x = packed(l, in.x, in.x_stride, in.n, in.d, size, true);
+        table = packed(l, in.table, in.table_stride, in.v, in.d, size, false);
+        rows = l.take(in.n * sizeof(Row));
+        scale = l.take(8);
+        const uint64_t all = ceil_div(in.v, BN) * BN;
+        uint64_t fits = PIECE_BYTES / ((in.n ? in.n : 1) * size) / BN * BN;
+        fits = fits < 1024 ? 1024 : fits;
+        pieces = in.v ? ceil_div(all, fits) : 1;
+        piece = ceil_div(ceil_div(all, pieces), BN) * BN;
+        pieces = in.v ? ceil_div(all, piece) : 1;
+        g = l.take(in.n * piece * size);
+        sum_stride = ceil_div(in.d, BN) * BN;
+        x_splits = shares_of(in.n, in.d, piece * size / CHUNK);
+        t_splits = shares_of(piece, in.d, ceil_div(in.n * size, CHUNK));
+        x_sums = t_sums = 0;
+        if (x_splits > 1 || pieces > 1)
+            x_sums = l.take(x_splits * in.n * sum_stride * 4);
+        if (t_splits > 1)
+            t_sums = l.take(t_splits * piece * sum_stride * 4);
+    }
+};
+
+int check_inputs(const char *what, const Inputs &in)
+{
+    if (!known_type(in.type)) {
+        set_error("%s: unknown element type %d", what, in.type);
+        return UNG_HIP_EINVAL;
+    }
+    if (in.n > INT32_MAX - 256 || in.v > INT32_MAX - 256 || in.d > (1u << 24) ||
+        ceil_div(in.n, 32) * ceil_div(in.v, BN) > most_blocks(256) / 2 ||
+        (in.n > in.v ? in.n : in.v) / 32 * ceil_div(in.d, BN) > most_blocks(256) / 2) {
+        set_error("%s: %llu rows of %llu elements against a table of %llu are too many", what, (unsigned long long)in.n,
+                  (unsigned long long)in.d, (unsigned long long)in.v);
+        return UNG_HIP_EINVAL;
+    }
+    if ((in.n > 1 && in.x_stride < in.d) || (in.v > 1 && in.table_stride < in.d)) {
+        set_error("%s: strides %llu and %llu are less than %llu columns", what, (unsigned long long)in.x_stride,
+                  (unsigned long long)in.table_stride, (unsigned long long)in.d);
+        return UNG_HIP_EINVAL;
+    }
+    if ((uintptr_t)in.x % type_size(in.type) || (uintptr_t)in.table % type_size(in.type)) {
+        set_error("%s: x and table need to be aligned to their elements", what);
+        return UNG_HIP_EINVAL;
+    }
+    return UNG_HIP_OK;
+}
+
+int check_call(const char *what, const Inputs &in, const int32_t *ids, const int32_t *without, float temperature,
+               uint64_t needed, const void *workspace, uint64_t bytes)
+{
+    if (!(temperature > 0.0f) || !(1.0f / temperature > 0.0f) || !(LOG2E / temperature < INF)) {
+        set_error("%s: temperature %g is not a positive number with a reciprocal", what, (double)temperature);
+        return UNG_HIP_EINVAL;
+    }
+    if ((in.n && !ids) || (in.n && in.d && !in.x) || (in.v && in.d && !in.table)) {
+        set_error("%s: null argument", what);
+        return UNG_HIP_EINVAL;
+    }
+    if ((uintptr_t)ids % 4 || (uintptr_t)without % 4) {
+        set_error("%s: ids and without need to be aligned to their elements", what);
+        return UNG_HIP_EINVAL;
+    }
+    if (needed && (!workspace || bytes < needed || (uintptr_t)workspace % 16)) {
+        set_error("%s: needs %llu bytes of workspace at a 16-byte boundary (got %llu)", what, (unsigned long long)needed,
+                  (unsigned long long)(workspace ? bytes : 0));
+        return UNG_HIP_EINVAL;
+    }
+    return UNG_HIP_OK;
+}
+
+uint32_t some_blocks(uint64_t n) { return (uint32_t)(n < 1 ? 1 : n < 8192 ? n : 8192); }
+
+// The product of two sides, its tiles finished by `finish`.
+template <class E, bool A_ACROSS, bool B_ACROSS, class Finish>
+void product(const Operand &a, const Operand &b, uint32_t splits, const Finish &finish, hipStream_t st)
+{
+    auto tiles = [&](auto high, auto wm) {
+        constexpr int BM = decltype(high)::value, WM = decltype(wm)::value;
+        const Grid grid = {(uint32_t)ceil_div(a.rows, BM), (uint32_t)ceil_div(b.rows, BN), splits,
+                           ceil_div(a.k * sizeof(E), CHUNK)};
+        if (const uint32_t blocks = grid.m_tiles * grid.n_tiles * grid.splits)
+            ung_tile_kernel<E, BM, WM, 2, A_ACROSS, B_ACROSS><<<blocks, WM * 128, 0, st>>>(a, b, grid, finish);
+    };
+    constexpr std::integral_constant<int, 1> one;
+    constexpr std::integral_constant<int, 2> two;
+    const uint32_t high = height_of(a.rows, b.rows);
+    if (high == 32)
+        tiles(std::integral_constant<int, 32>{}, one);
+    else if (high == 64)
+        tiles(std::integral_constant<int, 64>{}, two);
+    else
+        tiles(std::integral_constant<int, 128>{}, two);
+}
+
+template <class E>
+Operand side(const Packed &p, const void *x, uint64_t stride, uint64_t rows, uint64_t d, uint8_t *ws, hipStream_t st,
+             bool fill)
+{
+    if (!p.copy)
+        return {x, rows > 1 ? stride * sizeof(E) : p.pitch, rows, d};
+    if (fill && rows && p.pitch)
+        ung_table_pack_kernel<E><<<some_blocks(ceil_div(rows, 4)), 256, 0, st>>>((const E *)x, stride, rows, d,
+                                                                              (E *)(ws + p.at), p.pitch / sizeof(E));
+    return {ws + p.at, p.pitch, rows, d};
+}
+
+// The same rows with lines across the inner length: element k of `cols` columns, side by side.
+Operand across(const Operand &o) { return {o.p, o.stride, o.k, o.rows}; }
+
+} // namespace
+
+extern "C" {
+
+int ung_hip_table_loss_workspace(const void *x, uint64_t x_stride, const void *table, uint64_t table_stride, int type,
+                                 uint64_t rows, uint64_t table_rows, uint64_t cols, int backward, uint64_t *bytes)
+{
+    static const char what[] = "ung_hip_table_loss_workspace";
+    clear_error();
+    if (!bytes) {
+        set_error("%s: null bytes", what);
+        return UNG_HIP_EINVAL;
+    }
+    const Inputs in = {x, table, x_stride, table_stride, type, rows, table_rows, cols};
+    if (const int rc = check_inputs(what, in))
+        return rc;
+    *bytes = backward ? Backward(in).l.bytes : Forward(in).l.bytes;
+    return UNG_HIP_OK;
+}
+
+int ung_hip_table_loss_forward(const void *x, uint64_t x_stride, const void *table, uint64_t table_stride, int type,
+                               uint64_t rows, uint64_t table_rows, uint64_t cols, const int32_t *ids,
+                               const int32_t *without, float temperature, float *loss, float *lse, void *workspace,
+                               uint64_t workspace_bytes, void *stream)
+{
+    static const char what[] = "ung_hip_table_loss_forward";
+    clear_error();
+    const Inputs in = {x, table, x_stride, table_stride, type, rows, table_rows, cols};
+    if (const int rc = check_inputs(what, in))
+        return rc;
+    const Forward f(in);
+    if (const int rc = check_call(what, in, ids, without, temperature, f.l.bytes, workspace, workspace_bytes))
+        return rc;
+    if (rows == 0)
+        return UNG_HIP_OK;
+    if (!loss || !lse || (uintptr_t)loss % 4 || (uintptr_t)lse % 4) {
+        set_error("%s: null or unaligned loss or lse", what);
+        return UNG_HIP_EINVAL;
+    }
+    const hipStream_t st = (hipStream_t)stream;
+    uint8_t *ws = (uint8_t *)workspace;
+    return with_type(type, [&](auto zero) {
+        using E = decltype(zero);
+        const float c = LOG2E / temperature, by = 1.0f / temperature;
+        const Operand a = side<E>(f.x, x, x_stride, rows, cols, ws, st, true);
+        const Operand b = side<E>(f.table, table, table_stride, table_rows, cols, ws, st, true);
+        Part *parts = (Part *)(ws + f.parts);
+        float *target = (float *)(ws + f.target);
+        product<E, false, false>(a, b, 1, LogSum{ids, without, target, parts, rows, table_rows, c}, st);
+        auto join = [&](auto each) {
+            constexpr int R = decltype(each)::value;
+            ung_table_join_kernel<R><<<(uint32_t)ceil_div(rows, R), 256, 0, st>>>(parts, f.tiles, rows, table_rows, target,
+                                                                              ids, without, c, by, loss, lse);
+        };
+        if (rows < 16)
+            join(std::integral_constant<int, 1>{});
+        else
+            join(std::integral_constant<int, 16>{});
+        return launched(what);
+    });
+}
+
+int ung_hip_table_loss_backward(const void *x, uint64_t x_stride, const void *table, uint64_t table_stride, int type,
+                                uint64_t rows, uint64_t table_rows, uint64_t cols, const int32_t *ids,
+                                const int32_t *without, const float *lse, const float *weight, float temperature,
+                                void *dx, uint64_t dx_stride, void *dtable, uint64_t dtable_stride, void *workspace,
+                                uint64_t workspace_bytes, void *stream)
+{
+    static const char what[] = "ung_hip_table_loss_backward";
+    clear_error();
+    const Inputs in = {x, table, x_stride, table_stride, type, rows, table_rows, cols};
+    if (const int rc = check_inputs(what, in))
+        return rc;
+    const Backward f(in);
+    if (const int rc = check_call(what, in, ids, without, temperature, f.l.bytes, workspace, workspace_bytes))
+        return rc;
+    if ((dx && rows > 1 && dx_stride < cols) || (dtable && table_rows > 1 && dtable_stride < cols)) {
+        set_error("%s: strides %llu and %llu of the gradients are less than %llu columns", what,
+                  (unsigned long long)dx_stride, (unsigned long long)dtable_stride, (unsigned long long)cols);
+        return UNG_HIP_EINVAL;
+    }
+    if ((rows && !lse) || (uintptr_t)lse % 4 || (uintptr_t)weight % 4 || (uintptr_t)dx % type_size(type) ||
+        (uintptr_t)dtable % type_size(type)) {
+        set_error("%s: null lse, or lse, weight, dx or dtable not aligned to their elements", what);
+        return UNG_HIP_EINVAL;
+    }
+    if (cols == 0 || (!dx && !dtable))
+        return UNG_HIP_OK;
+    const hipStream_t st = (hipStream_t)stream;
+    uint8_t *ws = (uint8_t *)workspace;
+    return with_type(type, [&](auto zero) {
+        using E = decltype(zero);
+        const float c = LOG2E / temperature, by = 1.0f / temperature;
+        Row *row = (Row *)(ws + f.rows);
+        float *scale = sizeof(E) == 2 && std::is_same_v<E, fp16_t> ? (float *)(ws + f.scale) : nullptr;
+        const float *back = scale ? scale + 1 : nullptr;
+        if (scale)
+            ung_table_range_kernel<<<1, 1024, 0, st>>>(weight, rows, by, scale);
+        const Operand a = side<E>(f.x, x, x_stride, rows, cols, ws, st, false);
+        if (rows)
+            ung_table_rows_kernel<E><<<some_blocks(ceil_div(rows, 4)), 256, 0, st>>>(
+                (const E *)x, x_stride, rows, table_rows, cols, ids, without, lse, weight, by, scale, row,
+                (E *)(ws + f.x.at), f.x.pitch / sizeof(E));
+        const Operand t = side<E>(f.table, table, table_stride, table_rows, cols, ws, st, true);
+        auto vectors = [](const void *p, uint64_t stride, uint64_t rows) {
+            return (uintptr_t)p % 4 == 0 && (rows == 1 || stride * sizeof(E) % 4 == 0);
+        };
+        for (uint64_t p = 0; p < f.pieces; ++p) {
+            const uint64_t v0 = p * f.piece, v = table_rows - v0 < f.piece ? table_rows - v0 : f.piece;
+            const Operand part = {(const uint8_t *)t.p + v0 * t.stride, t.stride, v, cols};
+            const Operand g = {ws + f.g, f.piece * sizeof(E), rows, v}, x_side = {a.p, a.stride, rows, cols};
+            product<E, false, false>(x_side, part, 1,
+                                     Weights<E>{row, (E *)(ws + f.g), f.piece, rows, v0, v, c}, st);
+            if (dx && rows) {
+                if (f.x_splits == 1 && f.pieces == 1)
+                    product<E, false, true>(g, across(part), 1,
+                                            Whole<E>{(E *)dx, dx_stride, rows, cols, back, vectors(dx, dx_stride, rows)}, st);
+                else
+                    product<E, false, true>(g, across(part), f.x_splits,
+                                            Sums{(float *)(ws + f.x_sums), f.sum_stride, rows, p > 0}, st);
+            }
+            if (dtable && v) {
+                E *to = (E *)dtable + v0 * dtable_stride;
+                if (f.t_splits == 1)
+                    product<E, true, true>(across(g), across(x_side), 1,
+                                           Whole<E>{to, dtable_stride, v, cols, back, vectors(to, dtable_stride, v)}, st);
+                else {
+                    product<E, true, true>(across(g), across(x_side), f.t_splits,
+                                           Sums{(float *)(ws + f.t_sums), f.sum_stride, v, 0}, st);
+                    ung_table_sum_kernel<E><<<some_blocks(ceil_div(v * ceil_div(cols, 4), 256)), 256, 0, st>>>(
+                        (const float *)(ws + f.t_sums), f.t_splits, v, cols, f.sum_stride, back, to, dtable_stride);
+                }
+            }
+        }
+        if (dx && rows && !(f.x_splits == 1 && f.pieces == 1))
+            ung_table_sum_kernel<E><<<some_blocks(ceil_div(rows * ceil_div(cols, 4), 256)), 256, 0, st>>>(
+                (const float *)(ws + f.x_sums), f.x_splits, rows, cols, f.sum_stride, back, (E *)dx, dx_stride);
+        return launched(what);
+    });
+}
+
+} // extern "C"

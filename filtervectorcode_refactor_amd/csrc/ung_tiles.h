@@ -1,0 +1,303 @@
+// ung_tiles.h -- tiles of a matrix product C[m][n] = sum_k A[m][k] B[n][k] on gfx950's matrix
+// instructions, shared by the operators that make one (ung_int8.hip, ung_table_loss.hip); what
+// becomes of a tile's sums is the operator's own (its `Finish`).  Not part of the public ABI.
+//
+// The inner length is taken in chunks of 128 bytes of a row: 128 8-bit whole numbers, 64 16-bit
+// or 32 32-bit numbers.  A matrix instruction takes 16 bytes a lane in each of these types, so
+// panels, fragments and loads are the same for all of them.
+#pragma once
+
+#include "ung_elements.h"
+
+namespace ung {
+
+using i32x4 = __attribute__((ext_vector_type(4))) int;
+using fp16x8 = __attribute__((ext_vector_type(8))) _Float16;
+
+constexpr uint32_t CHUNK = 128; // bytes of the inner length in a panel
+
+// 16 rows of x times 16 rows of y over 64 bytes of the inner length, added to c.  A lane brings
+// 16 bytes of row lane % 16 (bytes lane / 16 * 16) of each; of the result it holds row lane % 16 of y
+// and rows lane / 16 * 4 + 0..3 of x.
+template <class E>
+struct Matrix;
+template <>
+struct Matrix<int8_t> {
+    using Acc = i32x4;
+    static __device__ inline Acc mul(u32x4 x, u32x4 y, Acc c)
+    {
+        return __builtin_amdgcn_mfma_i32_16x16x64_i8(__builtin_bit_cast(i32x4, x), __builtin_bit_cast(i32x4, y), c, 0, 0,
+                                                     0);
+    }
+};
+template <>
+struct Matrix<bf16_t> {
+    using Acc = f32x4;
+    static __device__ inline Acc mul(u32x4 x, u32x4 y, Acc c)
+    {
+        return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, x), __builtin_bit_cast(bf16x8, y), c,
+                                                       0, 0, 0);
+    }
+};
+template <>
+struct Matrix<fp16_t> {
+    using Acc = f32x4;
+    static __device__ inline Acc mul(u32x4 x, u32x4 y, Acc c)
+    {
+        return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(fp16x8, x), __builtin_bit_cast(fp16x8, y), c, 0,
+                                                      0, 0);
+    }
+};
+template <>
+struct Matrix<float> {
+    using Acc = f32x4;
+    static __device__ inline Acc mul(u32x4 x, u32x4 y, Acc c)
+    {
+        const f32x4 a = __builtin_bit_cast(f32x4, x), b = __builtin_bit_cast(f32x4, y);
+#pragma unroll
+        for (int t = 0; t < 4; ++t)
+            c = __builtin_amdgcn_mfma_f32_16x16x4f32(a[t], b[t], c, 0, 0, 0);
+        return c;
+    }
+};
+
+// One side of a product: `rows` rows of `k` elements.  Along the inner length: elements of a row
+// lie side by side, rows `stride` bytes apart.  Across it: element k of all rows lies side by
+// side, `stride` bytes after element k - 1 of them.  Either way these lines begin at 16-byte
+// boundaries and are whole vectors of 16 bytes long, or zero up to one; stride < 2^23.
+struct Operand {
+    const void *p;
+    uint64_t stride;
+    uint64_t rows, k;
+};
+constexpr uint64_t MOST_STRIDE = 1ull << 23;
+
+constexpr uint32_t OUTSIDE = 0x80000000u; // a range-checked load from here gives zeros
+
+// Loads and reads R rows of one side.  As m side (LANES) its rows are the lanes' own, as n side they
+// are spread over four instructions so that a lane ends with 16 neighbouring ones.
+template <class E, int R, bool ACROSS, bool LANES, int WAVES>
+struct Side {
+    static_assert(R / 8 % WAVES == 0 && (!ACROSS || sizeof(E) > 1), "");
+    static constexpr uint32_t KE = CHUNK / sizeof(E);        // elements of a chunk
+    static constexpr uint32_t LINE = R * sizeof(E) / 16;     // vectors of a line across
+    static constexpr uint32_t BYTES = R * CHUNK;
+
+    // Position of a vector is turned by exclusive-or with a number of its line, so that lanes
+    // that read different lines meet different banks.  The turn is made on the global side, as
+    // loads past the registers land in lane order.
+    static __device__ inline uint32_t turn(uint32_t line)
+    {
+        if constexpr (!ACROSS)
+            return LANES ? line & 7 : (line & 3) | (line >> 2 & 4);
+        else if constexpr (sizeof(E) == 4)
+            return (LANES ? (line >> 2 & 3) << 2 : line >> 2 & 3) & (LINE - 1);
+        else
+            return (LANES ? (line & 3) << 1 | (line >> 3 & 1) << 3 : (line & 1) | (line >> 1 & 1) << 3) & (LINE - 1);
+    }
+
+    // Chunk kb of rows row0... to `to`; every wave of the block takes part.
+    static __device__ inline void load(const Operand &of, uint64_t row0, uint32_t kb, uint8_t *to, uint32_t wave,
+                                       uint32_t lane)
+    {
+        const uint32_t stride = (uint32_t)of.stride;
+        if constexpr (!ACROSS) {
+            const __amdgpu_buffer_rsrc_t from =
+                buffer_of((const uint8_t *)of.p + row0 * of.stride + (uint64_t)kb * CHUNK, 0x7FFFFFFFu);
+            const uint64_t there = of.k * sizeof(E) - (uint64_t)kb * CHUNK; // bytes of a row from here
+            const uint32_t bytes = there < CHUNK ? (uint32_t)there : CHUNK;
+            const uint32_t last = (uint32_t)min(of.rows - row0, (uint64_t)R) - 1; // rows past the end repeat it
+#pragma unroll
+            for (int i = 0; i < R / 8 / WAVES; ++i) {
+                const uint32_t row = i * WAVES * 8 + wave * 8 + (lane >> 3), at = ((lane & 7) ^ turn(row)) * 16;
+                to_lds16(from, at < bytes ? min(row, last) * stride + at : OUTSIDE, 0, to + (i * WAVES + wave) * 1024);
+            }
+        } else {
+            const uint64_t k0 = (uint64_t)kb * KE;
+            const __amdgpu_buffer_rsrc_t from =
+                buffer_of((const uint8_t *)of.p + k0 * of.stride + row0 * sizeof(E), 0x7FFFFFFFu);
+            const uint32_t lines = (uint32_t)min(of.k - k0, (uint64_t)KE);
+            const uint32_t bytes = (uint32_t)min(of.rows - row0, (uint64_t)R) * (uint32_t)sizeof(E);
+#pragma unroll
+            for (int i = 0; i < R / 8 / WAVES; ++i) {
+                const uint32_t v = (i * WAVES + wave) * 64 + lane, line = v / LINE, at = (v % LINE ^ turn(line)) * 16;
+                to_lds16(from, line < lines && at < bytes ? line * stride + at : OUTSIDE, 0,
+                         to + (i * WAVES + wave) * 1024);
+            }
+        }
+    }
+
+    // A lane's 16 bytes of 16 rows for half `half` of the chunk: rows first + t * 16 + 0..15 as m
+    // side; as n side row first + 16 q + 4 t + i for instruction row 4 q + i.
+    static __device__ inline u32x4 fragment(const uint8_t *panel, uint32_t first, int t, int half, uint32_t lane)
+    {
+        const uint32_t r = lane & 15, g = lane >> 4;
+        if constexpr (!ACROSS) {
+            const uint32_t row = LANES ? first + t * 16 + r : first + (r >> 2) * 16 + t * 4 + (r & 3);
+            return *reinterpret_cast<const u32x4 *>(panel + row * CHUNK + ((half * 4 + g) ^ (r & 7)) * 16);
+        } else if constexpr (sizeof(E) == 4) {
+            const uint32_t row = LANES ? first + t * 16 + r : first + (r >> 2) * 16 + t * 4 + (r & 3);
+            u32x4 f;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const uint32_t line = half * 16 + g * 4 + i;
+                f[i] = *reinterpret_cast<const uint32_t *>(panel + line * (R * 4) + (((row >> 2) ^ turn(line)) * 4 + (row & 3)) * 4);
+            }
+            return f;
+        } else {
+            // The transposing read: of 16 lanes, lane l brings the place of four neighbouring rows of
+            // line l / 4, and gets the four lines of row l % 4 of place l / 4.
+            using s16x4 = __attribute__((ext_vector_type(4))) short;
+            using lds_s16x4 = __attribute__((address_space(3))) s16x4;
+            const uint32_t place = r & 3;
+            const uint32_t row = LANES ? first + t * 16 + place * 4 : first + place * 16 + t * 4;
+            union {
+                s16x4 h[2];
+                u32x4 v;
+            } f;
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const uint32_t line = half * 32 + g * 8 + h * 4 + (r >> 2);
+                const uint8_t *at = panel + line * (R * 2) + ((row >> 3) ^ turn(line)) * 16 + (row & 4) * 2;
+                f.h[h] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4 *)at);
+            }
+            return f.v;
+        }
+    }
+};
+
+// The grid of a product: tiles along both sides, and shares of the inner length, whose sums are
+// joined afterwards.
+struct Grid {
+    uint32_t m_tiles, n_tiles, splits;
+    uint64_t chunks;
+};
+
+// What a block makes: where its tile lies and which chunks it sums.  An XCD takes a contiguous
+// run, in bands of 8 tiles of m, so that the tiles it works on at a time share panels in its L2.
+struct Tile {
+    uint64_t m0, n0;
+    uint32_t high; // rows of a tile
+    uint32_t split, kb, kb_end;
+    uint32_t wm, wn; // the wave's part begins at row m0 + wm and column n0 + wn
+    uint32_t lane, wave;
+};
+
+// A block of WM x WN waves makes a BM x (64 WN) tile, each wave BM / WM x 64 of it in 16 x 16
+// matrix instructions.  Both panels of a chunk are staged in LDS by loads that bypass the
+// registers, one chunk ahead.  A lane ends with results [i][j][e]: row wm + 16 i + lane % 16,
+// column wn + lane / 16 * 16 + 4 j + e.
+template <class E, int BM, int WM, int WN, bool A_ACROSS, bool B_ACROSS, class Finish>
+__global__ __launch_bounds__(WM * WN * 64, 2) void ung_tile_kernel(Operand a, Operand b, Grid grid, Finish finish)
+{
+    constexpr int WAVES = WM * WN, BN = WN * 64, TM = BM / WM / 16;
+    using A = Side<E, BM, A_ACROSS, true, WAVES>;
+    using B = Side<E, BN, B_ACROSS, false, WAVES>;
+    struct Panels {
+        alignas(16) uint8_t a[A::BYTES], b[B::BYTES];
+    };
+    __shared__ Panels even, odd;
+    Tile at;
+    at.high = BM;
+    at.lane = threadIdx.x & 63;
+    at.wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    at.wm = (at.wave % WM) * (BM / WM);
+    at.wn = (at.wave / WM) * 64;
+    {
+        const uint32_t tiles = grid.m_tiles * grid.n_tiles, item = xcd_run(blockIdx.x, tiles * grid.splits);
+        uint32_t tm, tn;
+        at.split = uniform(item / tiles);
+        tile_of(item - at.split * tiles, 8, grid.m_tiles, grid.n_tiles, tm, tn);
+        at.m0 = (uint64_t)uniform(tm) * BM;
+        at.n0 = (uint64_t)uniform(tn) * BN;
+        const uint32_t share = (uint32_t)(grid.chunks / grid.splits), longer = (uint32_t)(grid.chunks % grid.splits);
+        at.kb = at.split * share + min(at.split, longer);
+        at.kb_end = at.kb + share + (at.split < longer ? 1 : 0);
+    }
+    typename Matrix<E>::Acc acc[TM][4];
+#pragma unroll
+    for (int i = 0; i < TM; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+            acc[i][j] = typename Matrix<E>::Acc{0, 0, 0, 0};
+
+    auto load = [&](Panels &to, uint32_t kb) {
+        A::load(a, at.m0, kb, to.a, at.wave, at.lane);
+        B::load(b, at.n0, kb, to.b, at.wave, at.lane);
+    };
+    auto multiply = [&](const Panels &p) {
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+            u32x4 y[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                y[j] = B::fragment(p.b, at.wn, j, half, at.lane);
+#pragma unroll
+            for (int i = 0; i < TM; ++i) {
+                const u32x4 x = A::fragment(p.a, at.wm, i, half, at.lane);
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                    acc[i][j] = Matrix<E>::mul(y[j], x, acc[i][j]);
+            }
+        }
+    };
+    auto step = [&](const Panels &now, Panels &next, uint32_t kb) {
+        await_loads<0>(); // loads into LDS are counted as memory loads, which a barrier alone does not await
+        __syncthreads();  // `now` has landed; every wave is done with `next`
+        if (kb + 1 < at.kb_end)
+            load(next, kb + 1);
+        multiply(now);
+    };
+    if (at.kb < at.kb_end)
+        load(even, at.kb);
+    for (uint32_t kb = at.kb; kb < at.kb_end; kb += 2) {
+        step(even, odd, kb);
+        if (kb + 1 < at.kb_end)
+            step(odd, even, kb + 1);
+    }
+    __syncthreads(); // the panels are free for the finish
+    finish(at, acc, reinterpret_cast<uint8_t *>(&even));
+}
+
+// ---- storing a tile's results ------------------------------------------------------------
+
+// A wave's 16 x 64 results (row r, columns g * 16 + 0..15 of each lane 16 g + r) to `to`, rows
+// `stride` elements apart, of which `rows` and `cols` are there.  16-bit vectors go out as they lie where
+// `vectors`; the others are turned in LDS first, so that a store's lanes write neighbouring elements.
+// `own`: TURN bytes of LDS of the wave's own.
+constexpr uint32_t TURN = 16 * (64 * 4 + 16);
+template <class T>
+__device__ inline void store_rows(T *to, uint64_t stride, uint32_t rows, uint64_t cols, bool vectors,
+                                  const Vec<T> (&o)[16 / Vec<T>::N], uint8_t *own, uint32_t lane)
+{
+    constexpr int N = Vec<T>::N;
+    constexpr uint32_t PITCH = 64 * sizeof(T) + 16;
+    const uint32_t r = lane & 15, g = lane >> 4;
+    if (sizeof(T) == 2 && vectors && cols >= 64) {
+        if (r < rows)
+#pragma unroll
+            for (int x = 0; x < 16 / N; ++x)
+                store_loose(to + r * stride + g * 16 + x * N, o[x]);
+        return;
+    }
+#pragma unroll
+    for (int x = 0; x < 16 / N; ++x)
+        *reinterpret_cast<Vec<T> *>(own + r * PITCH + (g * 16 + x * N) * sizeof(T)) = o[x];
+    wave_lds_fence();
+    if (vectors && cols >= 64) {
+        constexpr int LANES = 64 / N; // that hold a row
+        const uint32_t y0 = lane / LANES, x = lane % LANES * N;
+#pragma unroll
+        for (uint32_t y = 0; y < 16; y += N)
+            if (y + y0 < rows)
+                store_loose(to + (y + y0) * stride + x,
+                            *reinterpret_cast<const Vec<T> *>(own + (y + y0) * PITCH + x * sizeof(T)));
+    } else if (lane < cols) {
+#pragma unroll 4
+        for (uint32_t y = 0; y < rows; ++y)
+            to[y * stride + lane] = *reinterpret_cast<const T *>(own + y * PITCH + lane * sizeof(T));
+    }
+    wave_lds_fence();
+}
+
+} // namespace ung

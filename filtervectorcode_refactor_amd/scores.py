@@ -5,14 +5,21 @@ scores queries against its table.  Thin calls of the C ABI's score operators
   quantize_fp8       rows to 8 bits with a scale for each block of 128, transposed too
   matmul_fp8         product of such operands; matmul_fp8_grad: its gradients
   linear_fp8         the differentiable layer made of them
+  quantize_int8      rows to 8-bit whole numbers with a scale a row; matmul_int8: their product
+  linear_int8        rows times a table kept in 8-bit whole numbers
   top_scores         first k scores of each row in (score, id) order, and log-sum-exp
   distill_forward, distill_backward, distill_step, distill_loss
                      the loss against a teacher's top scores: its passes, both passes in one
                      call, and the differentiable function
   entries_of_neighbors  neighbour rows (ids, distances) as a teacher's top scores
+  table_loss_forward, table_loss_backward, table_loss
+                     cross entropy against every row of a table, without the scores in memory: its
+                     passes and the differentiable function
+  gradient_norm, clip_gradients
+                     the norm of many gradients together; the gradients scaled to a largest norm
 
-linear_fp8 and distill_loss are differentiable, once; the passes and products return results
-without a graph.  Scores may have any row stride; bfloat16, float16 and float32.  A wrong argument raises
+linear_fp8, distill_loss and table_loss are differentiable, once; the passes and products return
+results without a graph.  Scores may have any row stride; bfloat16, float16 and float32.  A wrong argument raises
 ``ValueError`` or ``UngHipError``; there is no CPU fallback.
 """
 from __future__ import annotations
@@ -293,6 +300,79 @@ def linear_fp8(x, w, dtype=torch.bfloat16):
     return _LinearFp8.apply(x, w, dtype)
 
 
+# ---- 8-bit whole numbers ------------------------------------------------------------------
+def quantize_int8(x):
+    """Rows in 8-bit whole numbers: (q int8 [n, columns rounded up to whole chunks of 128], padded
+    with zeros; scale float32 [n]).  A row's scale is its largest magnitude / 127, an element's
+    number the quotient by it to the nearest, ties to even.  A row with an infinity or NaN gets
+    the scale NaN and zeros."""
+    kind, stride = _matrix("x", x)
+    with _On(x) as stream:
+        return _integers(x, kind, stride, _library(), stream)
+
+
+def _integers(x, kind, row_stride, lib, stream):
+    n, d = x.shape
+    q = torch.empty(n, _blocks(d) * BLOCK, dtype=torch.int8, device=x.device)
+    scale = torch.empty(n, device=x.device)
+    check(lib.ung_hip_int8_quantize(x.data_ptr(), kind, n, d, row_stride, q.data_ptr(), scale.data_ptr(), stream))
+    return q, scale
+
+
+def _numbers(name, q, scale, like=None):
+    """Checks rows of whole numbers; returns how many there are and their length."""
+    _on_gpu(name, q, like)
+    if q.dim() != 2 or q.dtype != torch.int8 or q.shape[1] % BLOCK or not q.is_contiguous():
+        raise ValueError(f"{name}: contiguous int8 rows of a multiple of {BLOCK} are needed, got {tuple(q.shape)} of "
+                         f"{q.dtype}")
+    _on_gpu(f"{name}_scale", scale, q)
+    if scale.dtype != torch.float32 or tuple(scale.shape) != (q.shape[0],) or not scale.is_contiguous():
+        raise ValueError(f"{name}_scale: contiguous float32 ({q.shape[0]},) is needed, got {tuple(scale.shape)} of "
+                         f"{scale.dtype}")
+    return q.shape
+
+
+def matmul_int8(a, a_scale, b, b_scale, dtype=torch.bfloat16):
+    """a b^T of rows in 8-bit whole numbers (quantize_int8) in ``dtype``: the sums are exact whole
+    numbers, times both rows' scales in float32, rounded once to ``dtype``."""
+    m, kp = _numbers("a", a, a_scale)
+    n, b_kp = _numbers("b", b, b_scale, a)
+    if dtype not in _TYPES:
+        raise ValueError(f"dtype: float32, float16 or bfloat16 is needed, got {dtype}")
+    if b_kp != kp:
+        raise ValueError(f"a and b: rows of {kp} and {b_kp} bytes do not go together")
+    with _On(a) as stream:
+        return _integer_product(a, a_scale, b, b_scale, m, n, kp, dtype, _library(), stream)
+
+
+def _integer_product(a, a_scale, b, b_scale, m, n, kp, dtype, lib, stream):
+    kind, device = _TYPES[dtype], a.device
+    c = torch.empty(m, n, dtype=dtype, device=device)
+    keep, at, size = _workspace(lib.ung_hip_int8_matmul_workspace, m, n, kp, kind, device=device)
+    check(lib.ung_hip_int8_matmul(a.data_ptr(), a_scale.data_ptr(), b.data_ptr(), b_scale.data_ptr(), m, n, kp,
+                                  c.data_ptr(), kind, n, at, size, stream))
+    return c
+
+
+def linear_int8(x, q, scale, dtype=torch.bfloat16):
+    """x w^T with x brought to 8-bit whole numbers on the way and w kept in them (q, scale =
+    quantize_int8(w), made once).  For answering: it has no gradient, and of an x that requires
+    one, differentiating the result raises."""
+    kind, stride = _matrix("x", x)
+    n, kp = _numbers("q", q, scale, x)
+    if dtype not in _TYPES:
+        raise ValueError(f"dtype: float32, float16 or bfloat16 is needed, got {dtype}")
+    m, d = x.shape
+    if _blocks(d) * BLOCK != kp:
+        raise ValueError(f"x and q: rows of {d} and {kp} do not go together")
+    lib = _library()
+    with _On(x) as stream:
+        c = _integer_product(*_integers(x, kind, stride, lib, stream), q, scale, m, n, kp, dtype, lib, stream)
+    if x.requires_grad and torch.is_grad_enabled():
+        c, = _Underivable.apply("linear_int8 has no gradient: detach its result", x, c)
+    return c
+
+
 # ---- the first scores of a row ------------------------------------------------------------
 def top_scores(scores, k, temperature=1.0):
     """(values [n, k] float32, ids [n, k] int32, lse [n] float32): the first k scores of each
@@ -456,3 +536,163 @@ def distill_loss(scores, ids, values, teacher_lse=None, temperature=1.0):
     """The loss of each row (distill_forward), differentiable in the scores, once; the teacher's
     side is taken as given."""
     return _DistillLoss.apply(scores, ids, values, teacher_lse, temperature)
+
+
+# ---- cross entropy against a table -----------------------------------------------------------
+def _against(x, table, ids, without):
+    kind, stride = _matrix("x", x)
+    table_kind, table_stride = _matrix("table", table, x)
+    n, d = x.shape
+    if table_kind != kind or table.shape[1] != d:
+        raise ValueError(f"table: rows of {d} elements of {x.dtype} are needed, got {table.shape[1]} of {table.dtype}")
+    out = []
+    for name, t in (("ids", ids), ("without", without)):
+        if t is not None:
+            _on_gpu(name, t, x)
+            if t.dtype != torch.int32 or tuple(t.shape) != (n,):
+                raise ValueError(f"{name}: int32 ({n},) is needed, got {tuple(t.shape)} of {t.dtype}")
+            t = t if t.is_contiguous() else t.contiguous()
+        out.append(t)
+    if out[0] is None:
+        raise ValueError("ids: a tensor on the GPU is needed")
+    return (x.data_ptr(), stride, table.data_ptr(), table_stride, kind, n, table.shape[0], d), *out
+
+
+def table_loss_forward(x, table, ids, without=None, temperature=1.0):
+    """(loss [n], lse [n]) float32: cross entropy of each row of ``x`` with row ``ids`` of the table
+    as its target, scores being x table^T / temperature, and the log-sum-exp of all its scores,
+    which table_loss_backward needs.  The scores themselves are never in memory.
+
+    ``without`` names one row of the table that each row of x leaves out (its own entry; -1: none).
+    A row whose id is outside the table, or the one left out, has no target: its loss is 0."""
+    sizes, ids, without = _against(x, table, ids, without)
+    n, device = x.shape[0], x.device
+    loss, lse = torch.empty(n, device=device), torch.empty(n, device=device)
+    lib = _library()
+    with _On(x) as stream:
+        keep, at, size = _workspace(lib.ung_hip_table_loss_workspace, *sizes, False, device=device)
+        check(lib.ung_hip_table_loss_forward(*sizes, ids.data_ptr(), _address(without), temperature, loss.data_ptr(),
+                                             lse.data_ptr(), at, size, stream))
+    return loss, lse
+
+
+def table_loss_backward(weight, x, table, ids, lse, without=None, temperature=1.0, need=(True, True)):
+    """Gradients of sum(weight * loss) by x and by the table, in their type; the arguments are those
+    of the forward call and its log-sum-exp.  ``need``: which of the two to make (the other is
+    None).  Rows without a target are not read: padding of any value, NaN too, may stand there."""
+    sizes, ids, without = _against(x, table, ids, without)
+    n, device = x.shape[0], x.device
+    lse = _vector("lse", lse, n, x)
+    weight = None if weight is None else _vector("weight", weight, n, x)
+    dx = torch.empty(x.shape, dtype=x.dtype, device=device) if need[0] else None
+    dtable = torch.empty(table.shape, dtype=x.dtype, device=device) if need[1] else None
+    lib = _library()
+    with _On(x) as stream:
+        keep, at, size = _workspace(lib.ung_hip_table_loss_workspace, *sizes, True, device=device)
+        check(lib.ung_hip_table_loss_backward(*sizes, ids.data_ptr(), _address(without), lse.data_ptr(),
+                                              _address(weight), temperature, _address(dx), x.shape[1],
+                                              _address(dtable), x.shape[1], at, size, stream))
+    return dx, dtable
+
+
+class _TableLoss(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, table, ids, without, temperature):
+        loss, lse = table_loss_forward(x, table, ids, without, temperature)
+        ctx.save_for_backward(x, table, ids, without, lse)
+        ctx.temperature = temperature
+        return loss
+
+    @staticmethod
+    def backward(ctx, g):
+        x, table, ids, without, lse = ctx.saved_tensors
+        grads = table_loss_backward(g, x, table, ids, lse, without, ctx.temperature, ctx.needs_input_grad[:2])
+        return *_once("table_loss", *grads), None, None, None
+
+
+def table_loss(x, table, ids, without=None, temperature=1.0):
+    """The loss of each row (table_loss_forward), differentiable in x and the table, once."""
+    return _TableLoss.apply(x, table, ids, without, temperature)
+
+
+# ---- gradients of a step -----------------------------------------------------------------------
+def _side_by_side(t):
+    """Whether a tensor's elements fill a stretch of memory, in any order of its dimensions."""
+    if t.is_contiguous():
+        return True
+    room = 1
+    for stride, size in sorted((st, n) for st, n in zip(t.stride(), t.shape) if n != 1):
+        if stride != room:
+            return False
+        room *= size
+    return True
+
+
+def _tensors(name, tensors):
+    tensors = list(tensors)
+    for t in tensors:
+        _on_gpu(name, t, tensors[0])
+        if t.dtype not in _TYPES:
+            raise ValueError(f"{name}: float32, float16 or bfloat16 is needed, got {t.dtype}")
+        if not _side_by_side(t):
+            raise ValueError(f"{name}: elements have to lie side by side, got strides {t.stride()} of {tuple(t.shape)}")
+    return tensors
+
+
+def _addresses(tensors):
+    return (C.c_void_p * len(tensors))(*[t.data_ptr() for t in tensors])
+
+
+def _gradient_list(grads):
+    grads = _tensors("grads", [g for g in grads if g is not None])
+    if not grads:
+        raise ValueError("grads: at least one tensor is needed")
+    count = len(grads)
+    return (grads, _addresses(grads), (C.c_int * count)(*[_TYPES[g.dtype] for g in grads]),
+            (C.c_uint64 * count)(*[g.numel() for g in grads]))
+
+
+def gradient_norm(grads):
+    """The norm of all gradients together, a float32 tensor of no dimensions: the root of the sum
+    of every element's square, made in 64 bits.  ``grads``: tensors on one GPU (None is skipped)
+    of any types and shapes."""
+    grads, at, types, sizes = _gradient_list(grads)
+    norm = torch.empty((), device=grads[0].device)
+    lib = _library()
+    with _On(grads[0]) as stream:
+        keep, work, size = _workspace(lib.ung_hip_gradient_workspace, sizes, len(grads), device=norm.device)
+        check(lib.ung_hip_gradient_norm(at, types, sizes, len(grads), norm.data_ptr(), work, size, stream))
+    if torch.is_grad_enabled():
+        for g in grads:
+            if g.requires_grad:
+                return _Underivable.apply("gradient_norm has no gradient: detach it", g, norm)[0]
+    return norm
+
+
+def clip_gradients(grads, max_norm, out=None):
+    """Scales the gradients by min(1, max_norm / norm) of their norm together, which it returns
+    (gradient_norm).  In place, or to ``out``: as many tensors of the same types and shapes, laid out
+    the same way.  Nothing waits for the norm.  Where it is infinite or NaN the gradients stay as
+    they are, so that a program that asks later can leave the step out."""
+    given = list(grads)
+    grads, at, types, sizes = _gradient_list(given)
+    written, to = grads, None
+    if out is not None:
+        out = list(out)
+        if len(out) != len(given):
+            raise ValueError(f"out: {len(given)} tensors are needed, got {len(out)}")
+        written = _tensors("out", [o for o, g in zip(out, given) if g is not None])
+        for o, g in zip(written, grads):
+            if o.dtype != g.dtype or o.shape != g.shape or o.stride() != g.stride() or o.device != g.device:
+                raise ValueError("out: the gradients' shapes, types and strides are needed")
+        to = _addresses(written)
+    if torch.is_grad_enabled() and any(t.requires_grad and not t.is_leaf for t in grads + written):
+        raise ValueError("grads: gradients that require a gradient themselves are clipped under torch.no_grad()")
+    norm = torch.empty((), device=grads[0].device)
+    lib = _library()
+    with _On(grads[0]) as stream:
+        keep, work, size = _workspace(lib.ung_hip_gradient_workspace, sizes, len(grads), device=norm.device)
+        check(lib.ung_hip_clip_gradients(at, to, types, sizes, len(grads), max_norm, norm.data_ptr(), work, size,
+                                         stream))
+    torch.autograd.graph.increment_version([t for t in written if not t.is_inference()])
+    return norm

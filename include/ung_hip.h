@@ -356,6 +356,68 @@ int ung_hip_fp8_matmul(const uint8_t *a, const float *a_scale, const uint8_t *b,
                        uint64_t m, uint64_t n, uint64_t kp, void *c, int type, uint64_t c_stride, void *workspace,
                        uint64_t workspace_bytes, void *stream);
 
+/* Rows x [rows x cols] in 8-bit whole numbers: q [rows x cp], cp = cols rounded up to a multiple of
+ * UNG_HIP_INT8_CHUNK, the padding zero, and a scale a row s = max(largest magnitude of the row,
+ * 2^-64) * (1.0f / 127) in 32 bits; an element's number, -127..127, is the 32-bit quotient x / s
+ * rounded to nearest even.  A row with an infinity or NaN has the scale NaN and zeros.  q 16-byte
+ * aligned. */
+#define UNG_HIP_INT8_CHUNK 128
+int ung_hip_int8_quantize(const void *x, int type, uint64_t rows, uint64_t cols, uint64_t row_stride, int8_t *q,
+                          float *scale, void *stream);
+
+/* c [m x n] = a b^T of such rows of length kp (a multiple of UNG_HIP_INT8_CHUNK):
+ * c[i][j] = (float)(sum_k a[i][k] * b[j][k]) * (a_scale[i] * b_scale[j]), the sum a whole number in
+ * 32 bits, exact for every number of 8 bits up to the largest kp; then rounded to `type`.  Rows of
+ * c may have any stride and alignment; at 4-byte boundaries they are written fastest. */
+#define UNG_HIP_INT8_LONGEST 130944
+int ung_hip_int8_matmul_workspace(uint64_t m, uint64_t n, uint64_t kp, int type, uint64_t *bytes);
+int ung_hip_int8_matmul(const int8_t *a, const float *a_scale, const int8_t *b, const float *b_scale, uint64_t m,
+                        uint64_t n, uint64_t kp, void *c, int type, uint64_t c_stride, void *workspace,
+                        uint64_t workspace_bytes, void *stream);
+
+/* Cross entropy of rows x [rows x cols] against every row of a table [table_rows x cols] (both of
+ * `type`), without the scores in memory.  z[i][j] = x[i] . table[j] / temperature, without[i]
+ * (nullable; -1 or any other number outside the table: none) names a row of the table that row i
+ * leaves out:
+ *   lse  [rows] = log sum_j exp z[i][j]                                    32 bits
+ *   loss [rows] = lse[i] - z[i][ids[i]]                                    32 bits
+ *   g[i][j]     = weight[i] / temperature * (exp(z[i][j] - lse[i]) - [j is ids[i]])
+ *   dx = g table, dtable = g^T x, of sum(weight[i] * loss[i]) (weight NULL: ones), in `type`
+ * Products are summed in 32 bits; the backward pass, which makes the scores anew, rounds g to `type`
+ * between its two products.  A row whose id is outside 0..table_rows-1 or the row left out has no
+ * target: its loss and gradient are 0, and its x (padding, of any value) does not reach dtable.  A
+ * row left out counts in dx with the factor 0.  The temperature is as below, at
+ * UNG_HIP_TOP_SCORES_MAX.  Rows at 16-byte boundaries of whole 16-byte vectors are read where they
+ * lie; others are copied to the workspace first.  dx or dtable may be NULL; neither may overlap an
+ * input.  `backward`: which pass the workspace is for. */
+int ung_hip_table_loss_workspace(const void *x, uint64_t x_stride, const void *table, uint64_t table_stride, int type,
+                                 uint64_t rows, uint64_t table_rows, uint64_t cols, int backward, uint64_t *bytes);
+int ung_hip_table_loss_forward(const void *x, uint64_t x_stride, const void *table, uint64_t table_stride, int type,
+                               uint64_t rows, uint64_t table_rows, uint64_t cols, const int32_t *ids,
+                               const int32_t *without, float temperature, float *loss, float *lse, void *workspace,
+                               uint64_t workspace_bytes, void *stream);
+int ung_hip_table_loss_backward(const void *x, uint64_t x_stride, const void *table, uint64_t table_stride, int type,
+                                uint64_t rows, uint64_t table_rows, uint64_t cols, const int32_t *ids,
+                                const int32_t *without, const float *lse, const float *weight, float temperature,
+                                void *dx, uint64_t dx_stride, void *dtable, uint64_t dtable_stride, void *workspace,
+                                uint64_t workspace_bytes, void *stream);
+
+/* The norm of `count` gradients together, and the gradients scaled to a largest norm.  grads, out,
+ * types, sizes: arrays on the host, read before the call returns; a gradient is sizes[i] elements of
+ * types[i], side by side.
+ *   norm = sqrt(sum over all elements of g^2), squares and sums in 64 bits, in a fixed order
+ *   out  = g * (norm > max_norm ? max_norm / norm : 1), rounded once to its type
+ * norm (device, 32 bits) may be NULL in the second call.  out NULL, or out[i] == grads[i]: in place;
+ * gradients whose norm is no larger are then not written.  Where the norm is infinite or NaN they
+ * stay as they are.  Gradients and outputs that overlap in another way are refused.  max_norm >= 0, +inf
+ * included.  The workspace is the same for both calls. */
+int ung_hip_gradient_workspace(const uint64_t *sizes, uint32_t count, uint64_t *bytes);
+int ung_hip_gradient_norm(const void *const *grads, const int *types, const uint64_t *sizes, uint32_t count,
+                          float *norm, void *workspace, uint64_t workspace_bytes, void *stream);
+int ung_hip_clip_gradients(const void *const *grads, void *const *out, const int *types, const uint64_t *sizes,
+                           uint32_t count, float max_norm, float *norm, void *workspace, uint64_t workspace_bytes,
+                           void *stream);
+
 /* Largest k of the two operators below.  Their temperature T is a positive number with 1 / T and
  * log2(e) / T in the range of 32 bits. */
 #define UNG_HIP_TOP_SCORES_MAX 128
