@@ -119,8 +119,15 @@ __global__ __launch_bounds__(256) void ung_int8_rows_kernel(const T *x, uint64_t
 
 // ---- product -------------------------------------------------------------------------
 
-// Results in the output's type: the sum, exact in 32 bits, times the rows' scales.
-__device__ inline float scaled(int sum, float by) { return (float)sum * by; }
+// The sum, exact in 32 bits, times the rows' scales: a 32-bit number, whatever follows (the
+// compiler would make one instruction of the product and its rounding to fp16, which rounds once
+// less than where it does not).
+__device__ inline float scaled(int sum, float by)
+{
+    float y = (float)sum * by;
+    asm("" : "+v"(y));
+    return y;
+}
 
 template <class T>
 struct Scaled {

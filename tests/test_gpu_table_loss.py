@@ -1,0 +1,487 @@
+"""GPU tests of the cross entropy against a table (scores.table_loss_*): against the formula in 64
+bits with derived bounds, against differences, where masks, lengths, strides and types can go
+wrong, in graphs, on streams and in autograd."""
+import math
+
+import pytest
+import torch
+
+import filtervectorcode_refactor_amd as F
+from filtervectorcode_refactor_amd import scores as S
+
+pytestmark = pytest.mark.gpu
+
+TYPES = {"fp32": torch.float32, "fp16": torch.float16, "bf16": torch.bfloat16}
+HALF_ULP = {"fp32": 2.0 ** -24, "fp16": 2.0 ** -11, "bf16": 2.0 ** -8}
+TINY = {"fp32": 2.0 ** -126, "fp16": 2.0 ** -25, "bf16": 2.0 ** -126}  # half a step next to 0
+EPS = 2.0 ** -24
+
+
+def _inputs(n, v, d, kind, seed=0, size=1.0):
+    g = torch.Generator(device="cuda").manual_seed(seed * 7919 + n * 31 + v * 7 + d)
+    x = (torch.randn(n, d, device="cuda", generator=g) * size / d ** 0.25).to(TYPES[kind])
+    t = (torch.randn(v, d, device="cuda", generator=g) / d ** 0.25).to(TYPES[kind])
+    ids = torch.randint(0, v, (n,), device="cuda", generator=g).int()
+    out = torch.randint(-1, v, (n,), device="cuda", generator=g).int()
+    w = torch.randn(n, device="cuda", generator=g)
+    return x, t, ids, out, w
+
+
+def _exact(x, t, ids, out, w, temperature, kind):
+    """(loss, lse, dx, dtable) in 64 bits and a bound of each one's error.
+
+    A score passes d products and sums of 32 bits (the matrix instruction may drop what lies below
+    the last bit instead of rounding it: 2 EPS each), then a scaling by the temperature and the
+    difference from the largest or the log-sum-exp, each rounded once.  An exponential is off by that
+    and 2^-22 of itself; a sum of v of them by v EPS.  g = w / T (p - [target]) is rounded to the
+    type once, summed over n or v terms in 32 bits, and the gradient rounded to the type; in dx the
+    target's weight is not rounded, but the bound counts it."""
+    n, d = x.shape
+    v = t.shape[0]
+    x, t, w = x.double(), t.double(), w.double()
+    z = x @ t.t().contiguous() / temperature
+    dz = (2 * (d + 2) * EPS * (x.abs() @ t.abs().t().contiguous()) / temperature).amax(dim=1) if v else x.new_zeros(n)
+    there = (ids >= 0) & (ids < v)
+    if out is not None:
+        there &= ids != out
+        hit = (out >= 0) & (out < v)
+        z[hit.nonzero()[:, 0], out[hit].long()] = -math.inf
+    rows = there.nonzero()[:, 0]
+    lse = torch.logsumexp(z, dim=1) if v else x.new_full((n,), -math.inf)
+    loss = torch.zeros_like(lse)
+    loss[rows] = lse[rows] - z[rows, ids[rows].long()]
+    span = z.masked_fill(z == -math.inf, 0.0).abs().amax(dim=1) if v else x.new_zeros(n)
+    dlse = 2 * dz + (v + 8) * EPS + 2.0 ** -22 + 8 * EPS * (span + 1 + math.log(v + 1))
+    p = torch.zeros_like(z)
+    p[rows] = (z[rows] - lse[rows, None]).exp()
+    g, size = p.clone(), p.clone()
+    g[rows, ids[rows].long()] -= 1
+    size[rows, ids[rows].long()] += 1
+    by = (w / temperature)[:, None]
+    g, size = g * by, (size * by.abs())
+    off = (dz + dlse + 2.0 ** -21)[:, None] + HALF_ULP[kind]
+    xz = torch.where(there[:, None], x, torch.zeros_like(x))
+    dx, dt = g @ t, g.t().contiguous() @ xz
+    inner = (2 * (max(n, v) + 4)) * EPS
+    # a type's smallest numbers: 2^x gives 0 below 2^-126 (of an exponential, so 2^-126 |w| / T of g), and a
+    # product may take an element of g below 2^-126 as 0.  G is scaled to the top of fp16's range,
+    # so what is lost there is 2^-24 / 2^13 of the largest weight.
+    most = float(by.abs().max()) if n else 0.0
+    low = (most + 1) * 2.0 ** -126 + (most * 2.0 ** -37 if kind == "fp16" else 0.0)
+    bound_x = (size * (off + inner) + low) @ t.abs() + HALF_ULP[kind] * 1.01 * dx.abs() + TINY[kind]
+    bound_t = (size * (off + inner) + low).t().contiguous() @ xz.abs() + HALF_ULP[kind] * 1.01 * dt.abs() + TINY[kind]
+    return (loss, lse, dx, dt), (torch.where(there, dlse, torch.zeros_like(dlse)), dlse, bound_x, bound_t)
+
+
+def _run(x, t, ids, out, w, temperature):
+    loss, lse = S.table_loss_forward(x, t, ids, without=out, temperature=temperature)
+    dx, dt = S.table_loss_backward(w, x, t, ids, lse, without=out, temperature=temperature)
+    assert loss.dtype == lse.dtype == torch.float32 and dx.dtype == dt.dtype == x.dtype
+    assert dx.shape == x.shape and dt.shape == t.shape
+    return loss, lse, dx, dt
+
+
+def _check(x, t, ids, out, w, temperature, kind):
+    got = _run(x, t, ids, out, w, temperature)
+    want, bound = _exact(x, t, ids, out, w, temperature, kind)
+    for name, a, b, most in zip(("loss", "lse", "dx", "dtable"), got, want, bound):
+        same = a.double() == b  # infinities
+        err = torch.where(same, torch.zeros_like(b), (a.double() - b).abs())
+        assert (err <= most).all(), (name, float((err / most).max()))
+    return got
+
+
+SIZES = [(1, 1, 1), (1, 5, 3), (2, 2, 8), (3, 129, 64), (17, 1000, 100), (32, 127, 16), (33, 128, 8), (64, 257, 130),
+         (65, 640, 72), (130, 300, 384), (257, 77, 24), (300, 2000, 129), (2, 40_000, 16), (700, 1300, 256), (5, 130, 1)]
+
+
+@pytest.mark.parametrize("kind", list(TYPES))
+@pytest.mark.parametrize("n,v,d", SIZES)
+def test_against_64_bits(n, v, d, kind):
+    x, t, ids, out, w = _inputs(n, v, d, kind)
+    _check(x, t, ids, None, w, 1.0, kind)
+    _check(x, t, ids, out, w, 0.2, kind)
+
+
+@pytest.mark.parametrize("kind", list(TYPES))
+@pytest.mark.parametrize("n,v,d", [(513, 5000, 128), (1100, 3001, 200), (3000, 1500, 64), (40, 20_000, 700),
+                                   (2100, 2600, 1000), (260, 9000, 512), (1024, 20_000, 96)])
+def test_larger_against_64_bits(n, v, d, kind):
+    """Every tile height, shares of the inner length, ragged last tiles."""
+    x, t, ids, out, w = _inputs(n, v, d, kind)
+    _check(x, t, ids, out, w, 0.5, kind)
+
+
+@pytest.mark.parametrize("kind,n,v,d", [("bf16", 70_000, 2500, 16), ("fp32", 40_000, 1700, 8), ("bf16", 9000, 20_000, 72)])
+def test_table_in_pieces(kind, n, v, d):
+    """More scores than a piece of G holds: dx is summed over pieces of the table."""
+    x, t, ids, out, w = _inputs(n, v, d, kind)
+    _check(x, t, ids, out, w / n, 0.5, kind)
+
+
+@pytest.mark.parametrize("kind", list(TYPES))
+@pytest.mark.parametrize("pad_x,pad_t,first", [(0, 0, 1), (8, 8, 0), (3, 0, 0), (0, 5, 0), (1, 1, 3), (24, 16, 8)])
+def test_strides_and_alignment(pad_x, pad_t, first, kind):
+    """Rows of wider buffers, off every boundary: what lies around them does not count."""
+    n, v, d = 70, 300, 40
+    x, t, ids, out, w = _inputs(n, v, d, kind)
+    want = _check(x, t, ids, out, w, 0.3, kind)
+    views = []
+    for a, pad in ((x, pad_x), (t, pad_t)):
+        whole = torch.full((a.shape[0], d + pad + first), math.nan, dtype=a.dtype, device="cuda")
+        whole[:, first:first + d] = a
+        views.append(whole[:, first:first + d])
+    got = _run(*views, ids, out, w, 0.3)
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+def test_columns_of_a_transposed_input_are_refused():
+    x, t, ids, _, _ = _inputs(8, 9, 8, "fp32")
+    with pytest.raises(ValueError, match="side by side"):
+        S.table_loss_forward(x.t(), t, ids)
+    with pytest.raises(ValueError, match="side by side"):
+        S.table_loss_forward(x, torch.randn(8, 9, device="cuda").t(), ids)
+
+
+@pytest.mark.parametrize("kind", list(TYPES))
+def test_rows_without_a_target(kind):
+    """Ids outside the table, or the row left out: loss and gradient 0, and whatever stands in such
+    a row (padding) reaches nothing else."""
+    n, v, d = 90, 200, 48
+    x, t, ids, out, w = _inputs(n, v, d, kind)
+    ids[3], ids[20], ids[40], ids[41] = -1, v, -2 ** 31, 2 ** 31 - 1
+    out[7] = ids[7]
+    gone = torch.tensor([3, 7, 20, 40, 41], device="cuda")
+    want = _check(x, t, ids, out, w, 0.5, kind)
+    assert (want[0][gone] == 0).all() and (want[2][gone] == 0).all()
+    x[3], x[20, 5], x[40], x[41, 0] = math.nan, math.inf, -math.inf, math.nan
+    w[3], w[41] = math.nan, math.inf
+    got = _run(x, t, ids, out, w, 0.5)
+    keep = torch.ones(n, dtype=torch.bool, device="cuda")
+    keep[gone] = False
+    assert (got[0][gone] == 0).all() and (got[2][gone] == 0).all()
+    assert torch.equal(got[0][keep], want[0][keep])
+    if kind != "fp16":  # (there the largest weight, maybe of a row without a target, scales all of G)
+        assert torch.equal(got[2][keep], want[2][keep]) and torch.equal(got[3], want[3])
+    assert torch.isfinite(got[3]).all()
+    none = torch.full_like(ids, -1)
+    loss, lse, dx, dt = _run(torch.full_like(x, math.nan), t, none, None, w, 0.5)
+    assert not loss.any() and not dx.any() and not dt.any()
+
+
+def test_nothing_left_of_a_row():
+    """A table of one row, left out: log-sum-exp -inf, loss and gradients 0."""
+    x, t, ids, _, w = _inputs(5, 1, 8, "bf16")
+    out = torch.tensor([0, -1, 0, 7, 0], device="cuda", dtype=torch.int32)
+    loss, lse, dx, dt = _check(x, t, ids, out, w, 1.0, "bf16")
+    assert (lse[[0, 2, 4]] == -math.inf).all() and not loss.any() and not dx.any() and not dt.any()
+
+
+@pytest.mark.parametrize("kind", list(TYPES))
+def test_empty(kind):
+    x, t, ids, _, w = _inputs(6, 10, 8, kind)
+    loss, lse, dx, dt = _run(x[:0], t, ids[:0], None, w[:0], 1.0)
+    assert loss.shape == lse.shape == (0,) and dx.shape == (0, 8) and dt.shape == t.shape and not dt.any()
+    loss, lse, dx, dt = _run(x, t[:0], ids, None, w, 1.0)
+    assert not loss.any() and (lse == -math.inf).all() and not dx.any() and dt.shape == (0, 8)
+    loss, lse, dx, dt = _run(x[:, :0], t[:, :0], ids, None, w, 1.0)
+    assert torch.allclose(lse, torch.full_like(lse, math.log(10)), rtol=1e-6) and dx.shape == (6, 0)
+    assert torch.equal(loss, lse)
+
+
+def test_spoilt_rows_stay_apart():
+    """A NaN or infinity of one row spoils that row's loss and dx, and no other row's; one of the
+    table spoils every row that does not leave it out."""
+    x, t, ids, _, w = _inputs(40, 300, 64, "fp32")
+    clean = _run(x, t, ids, None, w, 1.0)
+    x[7, 3] = math.nan
+    loss, lse, dx, _ = _run(x, t, ids, None, w, 1.0)
+    keep = torch.arange(40, device="cuda") != 7
+    assert loss[7].isnan() and lse[7].isnan() and dx[7].isnan().all()
+    assert torch.equal(loss[keep], clean[0][keep]) and torch.equal(dx[keep], clean[2][keep])
+    x[7, 3] = 0.0
+    t[11, 5] = math.nan
+    ids[ids == 11] = 12
+    out = torch.full_like(ids, 11)
+    out[20:] = -1
+    loss, lse = S.table_loss_forward(x, t, ids, without=out)
+    assert torch.isfinite(loss[:20]).all() and torch.isfinite(lse[:20]).all() and loss[20:].isnan().all()
+
+
+@pytest.mark.parametrize("kind", list(TYPES))
+def test_scores_of_any_size(kind):
+    """Scores far from 0 (and rows of one dominant score): differences are taken before exponentials."""
+    n, v, d = 33, 500, 32
+    x, t, ids, out, w = _inputs(n, v, d, kind, size=30.0)
+    _check(x, t, ids, out, w, 0.05, kind)
+    x = torch.full((4, 8), 100.0, device="cuda").to(TYPES[kind])
+    t = torch.full((6, 8), 100.0, device="cuda").to(TYPES[kind])
+    loss, _ = S.table_loss_forward(x, t, torch.arange(4, device="cuda").int())
+    assert (loss - math.log(6)).abs().max() < 1e-6  # scores of 80000, all equal: exact differences
+
+
+@pytest.mark.parametrize("scale", [1e-6, 1.0, 3e4])
+def test_small_and_large_weights_in_fp16(scale):
+    """G is brought to the top of fp16's range: the gradients' own rounding is what is left."""
+    n, v, d = 200, 3000, 64
+    x, t, ids, out, w = _inputs(n, v, d, "fp16")
+    w = w * scale / 20
+    w[5] = 0.0
+    _check(x, t, ids, out, w, 1.0, "fp16")
+    _check(x, t, ids, out, torch.zeros_like(w), 1.0, "fp16")
+
+
+def test_weights_none_and_one_gradient_alone():
+    for kind in TYPES:
+        x, t, ids, out, w = _inputs(70, 900, 40, kind)
+        _, lse = S.table_loss_forward(x, t, ids, without=out)
+        dx, dt = S.table_loss_backward(None, x, t, ids, lse, without=out)
+        dx1, dt1 = S.table_loss_backward(torch.ones_like(w), x, t, ids, lse, without=out)
+        assert torch.equal(dx, dx1) and torch.equal(dt, dt1)
+        only_x = S.table_loss_backward(None, x, t, ids, lse, without=out, need=(True, False))
+        only_t = S.table_loss_backward(None, x, t, ids, lse, without=out, need=(False, True))
+        assert only_x[1] is None and torch.equal(only_x[0], dx)
+        assert only_t[0] is None and torch.equal(only_t[1], dt)
+        assert S.table_loss_backward(None, x, t, ids, lse, need=(False, False)) == (None, None)
+
+
+@pytest.mark.parametrize("of", ["x", "table"])
+def test_against_differences(of):
+    """Along a random direction u of length 1: (f(+h) - f(-h)) / 2h of f = sum(w loss) in 32 bits.  The
+    third derivative along u is at most sum |w| s^3 with s the largest change of a score, so the
+    difference is off by h^2 / 6 of that, and by the losses' own errors over h."""
+    n, v, d, h = 24, 700, 56, 2.0 ** -5
+    x, t, ids, out, w = _inputs(n, v, d, "fp32")
+    (_, _, dx, dt), _ = _exact(x, t, ids, out, w, 1.0, "fp32")
+    _, lse = S.table_loss_forward(x, t, ids, without=out)
+    gx, gt = S.table_loss_backward(w, x, t, ids, lse, without=out)
+    g = torch.Generator(device="cuda").manual_seed(3)
+    for _ in range(4):
+        u = torch.randn(x.shape if of == "x" else t.shape, device="cuda", generator=g)
+        u = u / u.norm()
+        f = []
+        for step in (h, -h):
+            a, b = (x + step * u, t) if of == "x" else (x, t + step * u)
+            loss, _ = S.table_loss_forward(a, b, ids, without=out)
+            f.append((loss.double() * w.double()).sum())
+        slope = float(((gx if of == "x" else gt).double() * u.double()).sum())
+        s = 2 * float((u.double() @ t.double().t()).abs().max() if of == "x" else (x.double() @ u.double().t()).abs().max())
+        _, (dloss, _, _, _) = _exact(x, t, ids, out, w, 1.0, "fp32")
+        bound = h * h / 6 * float(w.abs().sum()) * s ** 3 + float((dloss * w.double().abs()).sum()) / h
+        bound += 2.0 ** -23 / h * float(w.abs().sum()) * 10  # the shifted inputs' rounding
+        assert abs(float(f[0] - f[1]) / (2 * h) - slope) <= bound
+        assert bound < 0.2 * float((dx if of == "x" else dt).norm())  # the bound says something
+
+
+def test_the_same_every_time():
+    for kind, sizes in (("bf16", (500, 3000, 128)), ("fp32", (40, 9000, 33)), ("fp16", (1, 30_000, 256))):
+        x, t, ids, out, w = _inputs(*sizes, kind)
+        first = _run(x, t, ids, out, w, 0.1)
+        for _ in range(3):
+            assert all(torch.equal(a, b) for a, b in zip(first, _run(x, t, ids, out, w, 0.1)))
+
+
+def test_autograd():
+    for kind in TYPES:
+        x, t, ids, out, w = _inputs(50, 400, 24, kind)
+        _, _, dx, dt = _run(x, t, ids, out, w, 0.5)
+        a, b = x.clone().requires_grad_(), t.clone().requires_grad_()
+        S.table_loss(a, b, ids, out, 0.5).backward(w)
+        assert torch.equal(a.grad, dx) and torch.equal(b.grad, dt)
+        b.grad = None
+        S.table_loss(x, b, ids, without=out, temperature=0.5).backward(w)
+        assert torch.equal(b.grad, dt)
+        a.grad = None
+        S.table_loss(a, t, ids, without=out, temperature=0.5).backward(w)
+        assert torch.equal(a.grad, dx)
+        assert not S.table_loss(x, t, ids).requires_grad
+
+
+def test_autograd_of_shared_and_broadcast_inputs():
+    """The same leaf as states and table; an upstream gradient that is one value for all rows."""
+    x, _, _, _, _ = _inputs(60, 60, 32, "fp32")
+    ids = torch.arange(60, device="cuda").roll(1).int()
+    own = torch.arange(60, device="cuda").int()
+    leaf = x.clone().requires_grad_()
+    S.table_loss(leaf, leaf, ids, own, 0.5).mean().backward()
+    _, lse = S.table_loss_forward(x, x, ids, own, 0.5)
+    dx, dt = S.table_loss_backward(torch.full((60,), 1 / 60, device="cuda"), x, x, ids, lse, own, 0.5)
+    # mean's backward divides by 60, which may round apart from 1 / 60
+    assert torch.allclose(leaf.grad, dx + dt, rtol=1e-5, atol=1e-8)
+    want = x.double().clone().requires_grad_()
+    z = (want @ want.t() / 0.5).masked_fill(torch.eye(60, dtype=torch.bool, device="cuda"), -math.inf)
+    torch.nn.functional.cross_entropy(z, ids.long()).backward()
+    assert (leaf.grad - want.grad).abs().max() < 1e-5 * want.grad.abs().max() + 1e-7
+
+
+def test_no_second_derivative():
+    x, t, ids, _, _ = _inputs(5, 30, 8, "fp32")
+    x.requires_grad_()
+    (dx,) = torch.autograd.grad(S.table_loss(x, t, ids).sum(), x, create_graph=True)
+    with pytest.raises(RuntimeError, match="no second derivative"):
+        dx.square().sum().backward()
+
+
+def test_inputs_are_not_written_and_saved_ones_are_watched():
+    x, t, ids, out, w = _inputs(50, 400, 24, "bf16")
+    before = [a.clone() for a in (x, t, ids, out, w)]
+    _run(x, t, ids, out, w, 1.0)
+    assert all(torch.equal(a, b) for a, b in zip(before, (x, t, ids, out, w)))
+    x.requires_grad_()
+    loss = S.table_loss(x, t, ids)
+    t.mul_(2)
+    with pytest.raises(RuntimeError, match="modified by an inplace"):
+        loss.sum().backward()
+
+
+def test_strided_outputs_of_the_c_entry():
+    """Gradients into wider rows: what lies between them is left alone."""
+    lib = F.load()
+    for kind, code in (("fp32", 0), ("fp16", 1), ("bf16", 2)):
+        for n, v, d, pad in ((40, 300, 33, 3), (300, 700, 64, 8), (2000, 1500, 24, 2)):
+            x, t, ids, _, w = _inputs(n, v, d, kind)
+            _, lse, dx, dt = _run(x, t, ids, None, w, 1.0)
+            ox = torch.full((n, d + pad), -5.0, device="cuda", dtype=TYPES[kind])
+            ot = torch.full((v, d + pad), -5.0, device="cuda", dtype=TYPES[kind])
+            sizes = (x.data_ptr(), d, t.data_ptr(), d, code, n, v, d)
+            keep, at, size = S._workspace(lib.ung_hip_table_loss_workspace, *sizes, 1, device="cuda")
+            rc = lib.ung_hip_table_loss_backward(*sizes, ids.data_ptr(), None, lse.data_ptr(), w.data_ptr(), 1.0,
+                                                 ox.data_ptr(), d + pad, ot.data_ptr(), d + pad, at, size,
+                                                 torch.cuda.current_stream().cuda_stream)
+            assert rc == 0
+            assert torch.equal(ox[:, :d], dx) and torch.equal(ot[:, :d], dt)
+            assert (ox[:, d:] == -5.0).all() and (ot[:, d:] == -5.0).all()
+
+
+def test_workspace_past_its_size_is_left_alone():
+    lib = F.load()
+    for n, v, d, kind, code in ((40, 300, 33, "fp32", 0), (700, 1300, 72, "bf16", 2), (3, 5000, 9, "fp16", 1)):
+        x, t, ids, out, w = _inputs(n, v, d, kind)
+        loss, lse, dx, dt = _run(x, t, ids, out, w, 1.0)
+        sizes = (x.data_ptr(), d, t.data_ptr(), d, code, n, v, d)
+        st = torch.cuda.current_stream().cuda_stream
+        for backward in (0, 1):
+            _, _, size = S._workspace(lib.ung_hip_table_loss_workspace, *sizes, backward, device="cuda")
+            room = torch.full((size + 4096,), 0xA5, dtype=torch.uint8, device="cuda")
+            if backward:
+                a, b = torch.empty_like(dx), torch.empty_like(dt)
+                rc = lib.ung_hip_table_loss_backward(*sizes, ids.data_ptr(), out.data_ptr(), lse.data_ptr(), w.data_ptr(),
+                                                     1.0, a.data_ptr(), d, b.data_ptr(), d, room.data_ptr(), size, st)
+                assert rc == 0 and torch.equal(a, dx) and torch.equal(b, dt)
+            else:
+                a, b = torch.empty_like(loss), torch.empty_like(lse)
+                rc = lib.ung_hip_table_loss_forward(*sizes, ids.data_ptr(), out.data_ptr(), 1.0, a.data_ptr(),
+                                                    b.data_ptr(), room.data_ptr(), size, st)
+                assert rc == 0 and torch.equal(a, loss) and torch.equal(b, lse)
+            assert (room[size:] == 0xA5).all()
+
+
+def test_a_graph_replays_with_new_inputs():
+    n, v, d = 300, 5000, 96
+    x, t, ids, out, w = _inputs(n, v, d, "bf16")
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        _run(x, t, ids, out, w, 0.5)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = _run(x, t, ids, out, w, 0.5)
+    for seed in range(4):
+        for a, b in zip((x, t, ids, out, w), _inputs(n, v, d, "bf16", seed)):
+            a.copy_(b)
+        want = _run(x, t, ids, out, w, 0.5)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+def test_threads_and_streams_at_once():
+    from concurrent.futures import ThreadPoolExecutor
+
+    def work(seed):
+        x, t, ids, out, w = _inputs(50 + 100 * seed, 2000 + 500 * seed, 60 + 8 * seed, ("bf16", "fp32", "fp16")[seed], seed)
+        got = [_run(x, t, ids, out, w, 0.3) for _ in range(4)]
+        torch.cuda.current_stream().synchronize()
+        return [a.cpu() for row in got for a in row]
+
+    alone = [work(i) for i in range(3)]
+
+    def on_a_stream(seed):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            return work(seed)
+
+    with ThreadPoolExecutor(3) as pool:
+        together = list(pool.map(on_a_stream, range(3)))
+    for a, b in zip(alone, together):
+        assert all(torch.equal(s, u) for s, u in zip(a, b))
+
+
+def test_table_past_32_bit_offsets():
+    """A table of 4.6 GB: rows at either end of it."""
+    v, d = 3_000_000, 768
+    g = torch.Generator(device="cuda").manual_seed(1)
+    t = torch.empty(v, d, dtype=torch.bfloat16, device="cuda")
+    for i in range(0, v, 1 << 18):
+        t[i:i + (1 << 18)] = torch.randn(min(1 << 18, v - i), d, device="cuda", generator=g) / d ** 0.5
+    ids = torch.tensor([0, v - 1, 2_796_203, -1], dtype=torch.int32, device="cuda")
+    out = torch.tensor([v - 1, 0, 2_796_202, 5], dtype=torch.int32, device="cuda")
+    x = torch.randn(4, d, device="cuda", generator=g).bfloat16()
+    w = torch.randn(4, device="cuda", generator=g)
+    loss, lse, dx, dt = _run(x, t, ids, out, w, 1.0)
+    parts, target = [], torch.zeros(4, dtype=torch.float64, device="cuda")
+    for i in range(0, v, 1 << 18):
+        z = x.double() @ t[i:i + (1 << 18)].double().t().contiguous()
+        for r in range(4):
+            if 0 <= int(out[r]) - i < z.shape[1]:
+                z[r, int(out[r]) - i] = -math.inf
+            if 0 <= int(ids[r]) - i < z.shape[1]:
+                target[r] = z[r, int(ids[r]) - i]
+        parts.append(torch.logsumexp(z, dim=1))
+    want = torch.logsumexp(torch.stack(parts), dim=0)
+    span = 2 * (d + 2) * EPS * (x.double().abs() @ t[:1000].double().abs().t().contiguous()).amax(dim=1) * 4
+    # sums of 128 exponentials, joined in 24 thousand parts by 256 threads: under 500 roundings a term
+    most = span + 500 * EPS + 2.0 ** -20
+    assert ((lse.double() - want).abs() <= most).all()
+    there = torch.tensor([True, True, True, False], device="cuda")
+    assert ((loss.double() - (want - target))[there].abs() <= 2 * most[there]).all() and loss[3] == 0
+    for first in (0, 2_796_000, v - 300):
+        rows = slice(first, first + 300)
+        p = (x.double() @ t[rows].double().t().contiguous() - want[:, None]).exp()
+        p[3] = 0
+        for r in range(3):
+            if first <= int(out[r]) < first + 300:
+                p[r, int(out[r]) - first] = 0
+            if first <= int(ids[r]) < first + 300:
+                p[r, int(ids[r]) - first] -= 1
+        want_t = (p * w.double()[:, None]).t().contiguous() @ x.double()
+        size = (p.abs() * w.double().abs()[:, None]).t().contiguous() @ x.double().abs()
+        bound = size * (HALF_ULP["bf16"] + 2 * most.max()) + HALF_ULP["bf16"] * 1.01 * want_t.abs() + 2.0 ** -126
+        assert ((dt[rows].double() - want_t).abs() <= bound).all()
+
+
+def test_refusals():
+    x, t, ids, out, w = _inputs(10, 20, 8, "fp32")
+    _, lse = S.table_loss_forward(x, t, ids)
+    bad = [
+        (lambda: S.table_loss_forward(x.cpu(), t, ids), "x: a tensor on the GPU"),
+        (lambda: S.table_loss_forward(x, t.cpu(), ids), "table: a tensor on the GPU"),
+        (lambda: S.table_loss_forward(x, t.half(), ids), "table: rows of 8 elements of torch.float32"),
+        (lambda: S.table_loss_forward(x, t[:, :7], ids), "table: rows of 8"),
+        (lambda: S.table_loss_forward(x.double(), t.double(), ids), "x: float32, float16 or bfloat16"),
+        (lambda: S.table_loss_forward(x[0], t, ids), "x: a matrix"),
+        (lambda: S.table_loss_forward(x, t, ids.long()), "ids: int32"),
+        (lambda: S.table_loss_forward(x, t, ids[:9]), "ids: int32"),
+        (lambda: S.table_loss_forward(x, t, None), "ids"),
+        (lambda: S.table_loss_forward(x, t, ids, without=out[:, None]), "without: int32"),
+        (lambda: S.table_loss_backward(w.double(), x, t, ids, lse), "weight: 10 float32"),
+        (lambda: S.table_loss_backward(w, x, t, ids, lse[:9]), "lse: 10 float32"),
+    ]
+    for call, words in bad:
+        with pytest.raises(ValueError, match=words):
+            call()
+    for temperature in (0.0, -1.0, math.nan, math.inf, 1e-45):
+        with pytest.raises(F.UngHipError, match="temperature"):
+            S.table_loss_forward(x, t, ids, temperature=temperature)
+        with pytest.raises(F.UngHipError, match="temperature"):
+            S.table_loss_backward(w, x, t, ids, lse, temperature=temperature)
