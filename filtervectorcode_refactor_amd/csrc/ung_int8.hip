@@ -130,14 +130,14 @@ __device__ inline float scaled(int sum, float by)
 }
 
 template <class T>
-struct Scaled {
+struct Scaled : Plainly {
     const float *a_scale, *b_scale;
     T *c;
     uint64_t c_stride, m, n;
     int vectors;
 
     template <int TM>
-    __device__ inline void operator()(const Tile &t, i32x4 (&acc)[TM][4], uint8_t *lds) const
+    __device__ inline void operator()(const Tile &t, const uint8_t *, i32x4 (&acc)[TM][4], uint8_t *lds) const
     {
         const uint32_t r = t.lane & 15, g = t.lane >> 4;
         const uint64_t col0 = t.n0 + t.wn;
@@ -161,18 +161,19 @@ struct Scaled {
             for (int e = 0; e < 16; e += 2)
                 o[e / Vec<T>::N].put2(e % Vec<T>::N, scaled(acc[i][e / 4][e % 4], sa * sb[e / 4][e % 4]),
                                       scaled(acc[i][e / 4][e % 4 + 1], sa * sb[e / 4][e % 4 + 1]));
-            store_rows(c + row0 * c_stride + col0, c_stride, rows, n - col0, vectors, o, lds + t.wave * TURN, t.lane);
+            store_rows(c + row0 * c_stride + col0, c_stride, rows, n - col0, vectors, o, lds + t.wave * turn_bytes(sizeof(T)), t.lane);
+            __builtin_amdgcn_sched_barrier(0); // 16 rows at a time: all of them need more registers than there are
         }
     }
 };
 
 // The sums of a share of the inner length, as they are.
-struct Shares {
+struct Shares : Plainly {
     float *part; // whole numbers, moved as 32-bit elements
     uint64_t stride, m, n;
 
     template <int TM>
-    __device__ inline void operator()(const Tile &t, i32x4 (&acc)[TM][4], uint8_t *lds) const
+    __device__ inline void operator()(const Tile &t, const uint8_t *, i32x4 (&acc)[TM][4], uint8_t *lds) const
     {
         const uint64_t col0 = t.n0 + t.wn;
         if (col0 >= n)
@@ -187,7 +188,7 @@ struct Shares {
             for (int e = 0; e < 16; ++e)
                 o[e / 4].w[e % 4] = (uint32_t)acc[i][e / 4][e % 4];
             store_rows(part + (t.split * m + row0) * stride + col0, stride, (uint32_t)min(m - row0, (uint64_t)16),
-                       stride - col0, true, o, lds + t.wave * TURN, t.lane);
+                       stride - col0, true, o, lds + t.wave * turn_bytes(4), t.lane);
         }
     }
 };
@@ -215,15 +216,20 @@ __global__ __launch_bounds__(256) void ung_int8_join_kernel(const int *part, uin
 // ---- choice of the kernel ----------------------------------------------------------------
 
 struct Plan {
-    uint32_t high, splits;
+    uint32_t high, wide, splits;
 };
 
 Plan plan_of(uint64_t m, uint64_t n, uint64_t kp)
 {
     const uint64_t chunks = kp / CHUNK, cus = cu_count();
-    Plan p = {128, 1};
+    Plan p = {128, 128, 1};
     if (m == 0 || n == 0 || chunks == 0)
         return p;
+    if (m > 128 && n > 128) {
+        const uint64_t tiles = ceil_div(m, BIG) * ceil_div(n, BIG);
+        if (tiles * 8 > ceil_div(tiles, cus) * cus * 5)
+            return {BIG, BIG, 1};
+    }
     const bool few_tiles = ceil_div(m, 64) * ceil_div(n, 128) <= 3 * cus;
     p.high = m <= 32 ? 32 : m <= 64 || few_tiles ? 64 : 128;
     const uint64_t tiles = ceil_div(m, p.high) * ceil_div(n, 128);
@@ -367,29 +373,32 @@ int ung_hip_int8_matmul(const int8_t *a, const float *a_scale, const int8_t *b, 
     const hipStream_t st = (hipStream_t)stream;
     const Operand oa = {a, kp, m, kp}, ob = {b, kp, n, kp};
     auto run = [&](auto finish) {
-        auto tiles = [&](auto high, auto wm) {
-            constexpr int BM = decltype(high)::value, WM = decltype(wm)::value;
-            const Grid grid = {(uint32_t)ceil_div(m, BM), (uint32_t)ceil_div(n, 128), plan.splits, kp / CHUNK};
-            ung_tile_kernel<int8_t, BM, WM, 2, false, false>
-                <<<grid.m_tiles * grid.n_tiles * grid.splits, WM * 128, 0, st>>>(oa, ob, grid, finish);
+        auto tiles = [&](auto high, auto wm, auto wn) {
+            constexpr int BM = decltype(high)::value, WM = decltype(wm)::value, WN = decltype(wn)::value;
+            const Grid grid = {(uint32_t)ceil_div(m, BM), (uint32_t)ceil_div(n, WN * 64), plan.splits, kp / CHUNK,
+                               plan.high == BIG ? 16u : 8u};
+            ung_tile_kernel<int8_t, BM, WM, WN, false, false>
+                <<<grid.m_tiles * grid.n_tiles * grid.splits, WM * WN * 64, 0, st>>>(oa, ob, grid, finish);
         };
         constexpr std::integral_constant<int, 1> one;
         constexpr std::integral_constant<int, 2> two;
         if (plan.high == 32)
-            tiles(std::integral_constant<int, 32>{}, one);
+            tiles(std::integral_constant<int, 32>{}, one, two);
         else if (plan.high == 64)
-            tiles(std::integral_constant<int, 64>{}, two);
+            tiles(std::integral_constant<int, 64>{}, two, two);
+        else if (plan.high == 128)
+            tiles(std::integral_constant<int, 128>{}, two, two);
         else
-            tiles(std::integral_constant<int, 128>{}, two);
+            tiles(std::integral_constant<int, BIG>{}, two, std::integral_constant<int, 4>{});
     };
     return with_type(type, [&](auto zero) {
         using T = decltype(zero);
         if (plan.splits == 1) {
             const bool vectors = (uintptr_t)c % 4 == 0 && (m == 1 || c_stride * sizeof(T) % 4 == 0);
-            run(Scaled<T>{a_scale, b_scale, (T *)c, c_stride, m, n, vectors});
+            run(Scaled<T>{{}, a_scale, b_scale, (T *)c, c_stride, m, n, vectors});
         } else {
             const uint64_t stride = share_stride(n), blocks = ceil_div(m * (stride / 4), 256);
-            run(Shares{(float *)workspace, stride, m, n});
+            run(Shares{{}, (float *)workspace, stride, m, n});
             ung_int8_join_kernel<T><<<(uint32_t)(blocks < 4096 ? blocks : 4096), 256, 0, st>>>(
                 (const int *)workspace, plan.splits, m, n, stride, a_scale, b_scale, (T *)c, c_stride);
         }

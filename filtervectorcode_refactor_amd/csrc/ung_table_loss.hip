@@ -25,7 +25,7 @@ namespace {
 
 constexpr float LOG2E = 1.44269504088896340736f;
 constexpr float INF = __builtin_huge_valf();
-constexpr int BN = 128; // columns of a tile
+constexpr int WHOLE = 256; // columns that every tile's width divides
 
 // ---- forward -------------------------------------------------------------------------
 
@@ -42,24 +42,36 @@ __device__ inline Part joined(Part a, Part b, float c)
 
 // Of a tile of scores (rows of x, columns: rows of the table): every row's part, and the
 // target's score where the tile holds it.
-struct LogSum {
+struct LogSum : Plainly {
     const int32_t *ids, *without;
     float *target; // [n]
     Part *parts;   // [tiles of the table][n]
     uint64_t n, v;
     float c; // log2(e) / T
 
-    template <int TM>
-    __device__ inline void operator()(const Tile &t, f32x4 (&acc)[TM][4], uint8_t *lds) const
+    struct Columns { // of a row: the target's and the one left out
+        int32_t id, out;
+    };
+    static constexpr uint32_t AHEAD = sizeof(Columns);
+    __device__ inline void ahead(const Tile &t, uint8_t *side) const
     {
-        Part *red = reinterpret_cast<Part *>(lds); // [2][rows of the tile]
+        if (threadIdx.x >= t.high)
+            return;
+        const uint64_t at = min(t.m0 + threadIdx.x, n - 1);
+        reinterpret_cast<Columns *>(side)[threadIdx.x] = {ids[at], without ? without[at] : -1};
+    }
+
+    template <int TM>
+    __device__ inline void operator()(const Tile &t, const uint8_t *side, f32x4 (&acc)[TM][4], uint8_t *lds) const
+    {
+        Part *red = reinterpret_cast<Part *>(lds); // [strips][rows of the tile]
         const uint32_t r = t.lane & 15, g = t.lane >> 4, high = t.high;
         const uint64_t col0 = t.n0 + t.wn + g * 16;
 #pragma unroll
         for (int i = 0; i < TM; ++i) {
-            const uint64_t row = t.m0 + t.wm + i * 16 + r, at = min(row, n - 1);
-            const uint32_t id = (uint32_t)ids[at] - (uint32_t)col0;
-            const uint32_t out = (without ? (uint32_t)without[at] : ~0u) - (uint32_t)col0;
+            const uint64_t row = t.m0 + t.wm + i * 16 + r;
+            const Columns of = reinterpret_cast<const Columns *>(side)[t.wm + i * 16 + r];
+            const uint32_t id = (uint32_t)of.id - (uint32_t)col0, out = (uint32_t)of.out - (uint32_t)col0;
             if (__any(id < 16 || out < 16 || col0 + 16 > v)) {
 #pragma unroll
                 for (int e = 0; e < 16; ++e) {
@@ -84,11 +96,16 @@ struct LogSum {
             sum += __shfl_xor(sum, 32);
             if (g == 0)
                 red[t.wn / 64 * high + t.wm + i * 16 + r] = {top, sum};
+            __builtin_amdgcn_sched_barrier(0); // 16 rows at a time: all of them need more registers than there are
         }
         __syncthreads();
         const uint64_t row = t.m0 + threadIdx.x;
-        if (threadIdx.x < high && row < n)
-            parts[t.n0 / BN * n + row] = joined(red[threadIdx.x], red[high + threadIdx.x], c);
+        if (threadIdx.x < high && row < n) {
+            Part p = red[threadIdx.x];
+            for (uint32_t w = 1; w < t.strips; ++w)
+                p = joined(p, red[w * high + threadIdx.x], c);
+            parts[t.n0 / (t.strips * 64) * n + row] = p;
+        }
     }
 };
 
@@ -198,22 +215,29 @@ __global__ __launch_bounds__(256) void ung_table_pack_kernel(const E *x, uint64_
 // weight, which is the largest, is kept in 32 bits and joins dX with the table's row at the end (4096 x
 // 100000 x 384 at T = 0.05: 0.0017 of the norm from dX, 0.0038 without).
 template <class E>
-struct Weights {
+struct Weights : Plainly {
     const Row *rows;
     float *rest; // [n]
     E *g; // [n][pitch], pitch whole tiles: columns past the piece's end are zero
     uint64_t pitch, n, v0, v;
     float c;
 
+    static constexpr uint32_t AHEAD = sizeof(Row);
+    __device__ inline void ahead(const Tile &t, uint8_t *side) const
+    {
+        if (threadIdx.x < t.high)
+            reinterpret_cast<Row *>(side)[threadIdx.x] = rows[min(t.m0 + threadIdx.x, n - 1)];
+    }
+
     template <int TM>
-    __device__ inline void operator()(const Tile &t, f32x4 (&acc)[TM][4], uint8_t *) const
+    __device__ inline void operator()(const Tile &t, const uint8_t *side, f32x4 (&acc)[TM][4], uint8_t *) const
     {
         const uint32_t r = t.lane & 15, gr = t.lane >> 4;
         const uint64_t col0 = t.n0 + t.wn + gr * 16;
 #pragma unroll
         for (int i = 0; i < TM; ++i) {
             const uint64_t row = t.m0 + t.wm + i * 16 + r;
-            const Row p = rows[min(row, n - 1)];
+            const Row p = reinterpret_cast<const Row *>(side)[t.wm + i * 16 + r];
 #pragma unroll
             for (int e = 0; e < 16; ++e)
                 acc[i][e / 4][e % 4] = __builtin_amdgcn_exp2f(__builtin_fmaf(acc[i][e / 4][e % 4], c, -p.lse2));
@@ -232,15 +256,15 @@ struct Weights {
                         acc[i][e / 4][e % 4] = 0.0f;
                 }
             }
-            if (row >= n)
-                continue;
             Vec<E> o[16 / Vec<E>::N];
 #pragma unroll
             for (int e = 0; e < 16; e += 2)
                 o[e / Vec<E>::N].put2(e % Vec<E>::N, acc[i][e / 4][e % 4] * p.weight, acc[i][e / 4][e % 4 + 1] * p.weight);
+            if (row < n)
 #pragma unroll
-            for (int x = 0; x < 16 / Vec<E>::N; ++x)
-                *reinterpret_cast<Vec<E> *>(g + row * pitch + col0 + x * Vec<E>::N) = o[x];
+                for (int x = 0; x < 16 / Vec<E>::N; ++x)
+                    *reinterpret_cast<Vec<E> *>(g + row * pitch + col0 + x * Vec<E>::N) = o[x];
+            __builtin_amdgcn_sched_barrier(0);
         }
     }
 };
@@ -273,7 +297,7 @@ struct Rest {
 
 // A gradient's tile in its own type.
 template <class E>
-struct Whole {
+struct Whole : Plainly {
     E *c;
     uint64_t stride, m, n;
     const float *by;
@@ -281,7 +305,7 @@ struct Whole {
     Rest<E> rest;
 
     template <int TM>
-    __device__ inline void operator()(const Tile &t, f32x4 (&acc)[TM][4], uint8_t *lds) const
+    __device__ inline void operator()(const Tile &t, const uint8_t *, f32x4 (&acc)[TM][4], uint8_t *lds) const
     {
         const uint64_t col0 = t.n0 + t.wn;
         if (col0 >= n)
@@ -303,31 +327,43 @@ struct Whole {
             for (int e = 0; e < 16; e += 2)
                 o[e / Vec<E>::N].put2(e % Vec<E>::N, all[e] * s, all[e + 1] * s);
             store_rows(c + row0 * stride + col0, stride, (uint32_t)min(m - row0, (uint64_t)16), n - col0, vectors, o,
-                       lds + t.wave * TURN, t.lane);
+                       lds + t.wave * turn_bytes(sizeof(E)), t.lane);
+            __builtin_amdgcn_sched_barrier(0);
         }
     }
 };
 
-// Sums of a share of the inner length in 32 bits, alone or on top of an earlier piece's.
+// Sums of a share of the inner length in 32 bits, from 0 or (ADD) from an earlier piece's.
+template <bool ADD>
 struct Sums {
     float *part;
     uint64_t stride, m; // stride: whole tiles
-    int add;
 
-    template <int TM>
-    __device__ inline void operator()(const Tile &t, f32x4 (&acc)[TM][4], uint8_t *) const
+    static constexpr uint32_t AHEAD = 0;
+    __device__ inline void ahead(const Tile &, uint8_t *) const {}
+    __device__ inline f32x4 *at(const Tile &t, int i) const
     {
-        const uint32_t r = t.lane & 15, g = t.lane >> 4;
+        const uint64_t row = min(t.m0 + t.wm + i * 16 + (t.lane & 15), m - 1);
+        return reinterpret_cast<f32x4 *>(part + (t.split * m + row) * stride + t.n0 + t.wn + (t.lane >> 4) * 16);
+    }
+    template <int TM>
+    __device__ inline void start(const Tile &t, f32x4 (&acc)[TM][4]) const
+    {
 #pragma unroll
-        for (int i = 0; i < TM; ++i) {
-            const uint64_t row = t.m0 + t.wm + i * 16 + r;
-            if (row >= m)
-                continue;
-            f32x4 *to = reinterpret_cast<f32x4 *>(part + (t.split * m + row) * stride + t.n0 + t.wn + g * 16);
+        for (int i = 0; i < TM; ++i)
 #pragma unroll
             for (int j = 0; j < 4; ++j)
-                to[j] = add ? to[j] + acc[i][j] : acc[i][j];
-        }
+                acc[i][j] = ADD ? at(t, i)[j] : f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    }
+    template <int TM>
+    __device__ inline void operator()(const Tile &t, const uint8_t *, f32x4 (&acc)[TM][4], uint8_t *) const
+    {
+#pragma unroll
+        for (int i = 0; i < TM; ++i)
+            if (t.m0 + t.wm + i * 16 + (t.lane & 15) < m)
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                    at(t, i)[j] = acc[i][j];
     }
 };
 
@@ -355,17 +391,36 @@ __global__ __launch_bounds__(256) void ung_table_sum_kernel(const float *part, u
 
 // ---- plan and workspace ------------------------------------------------------------------
 
-uint32_t height_of(uint64_t m, uint64_t n)
-{
-    return m <= 32 ? 32 : m <= 64 || ceil_div(m, 64) * ceil_div(n, BN) <= 3 * (uint64_t)cu_count() ? 64 : 128;
-}
+// How a product of m x n results is made: by tiles of `high` x `wide` in so many shares of the inner
+// length.
+struct Shape {
+    uint32_t high, wide, splits;
+};
 
-// Shares of the inner length that fill the chip twice, of at least 4 chunks.
-uint32_t shares_of(uint64_t m, uint64_t n, uint64_t chunks)
+Shape shape_of(uint64_t m, uint64_t n, uint64_t k, int type, bool shares)
 {
-    const uint64_t tiles = ceil_div(m, height_of(m, n)) * ceil_div(n, BN), most = 2 * (uint64_t)cu_count();
-    const uint64_t by_cu = most / (tiles ? tiles : 1), by_k = chunks / 4, s = by_cu < by_k ? by_cu : by_k;
-    return s > 1 ? (uint32_t)s : 1;
+    const uint64_t cus = cu_count(), chunks = ceil_div(k * type_size(type), CHUNK);
+    auto with = [&](uint32_t high, uint32_t wide, uint32_t at_once, uint64_t fewest) {
+        Shape s = {high, wide, 1};
+        const uint64_t tiles = ceil_div(m, high) * ceil_div(n, wide);
+        if (shares && tiles) {
+            const uint64_t by_cu = at_once * cus / tiles, by_k = chunks / fewest, most = by_cu < by_k ? by_cu : by_k;
+            s.splits = most > 1 ? (uint32_t)most : 1;
+        }
+        return s;
+    };
+    if (type != UNG_HIP_F32 && m > 128 && n > 128 && ceil_div(n, 128) % 2 == 0 && chunks) {
+        const Shape s = with(BIG, BIG, 1, 8);
+        const uint64_t items = ceil_div(m, BIG) * ceil_div(n, BIG) * s.splits;
+        if (items * 8 > ceil_div(items, cus) * cus * 5)
+            return s;
+    }
+    if (m > 64 && n > 64) {
+        const Shape s = with(128, 128, 2, 8);
+        if (ceil_div(m, 128) * ceil_div(n, 128) * s.splits * 4 > 3 * cus)
+            return s;
+    }
+    return with(m <= 32 ? 32 : 64, 128, 3, 4);
 }
 
 struct Inputs {
@@ -404,13 +459,15 @@ Packed packed(Layout &l, const void *p, uint64_t stride, uint64_t rows, uint64_t
 struct Forward {
     Layout l;
     Packed x, table;
+    Shape shape;
     uint64_t tiles, parts, target;
     explicit Forward(const Inputs &in)
     {
         const uint64_t size = type_size(in.type);
         x = packed(l, in.x, in.x_stride, in.n, in.d, size, false);
         table = packed(l, in.table, in.table_stride, in.v, in.d, size, false);
-        tiles = ceil_div(in.v, BN);
+        shape = shape_of(in.n, in.v, in.d, in.type, false);
+        tiles = ceil_div(in.v, shape.wide);
         parts = l.take(tiles * in.n * sizeof(Part));
         target = l.take(in.n * 4);
     }
@@ -424,7 +481,7 @@ struct Backward {
     Layout l;
     Packed x, table;
     uint64_t rows, scale, rest, piece, pieces, g, x_sums, t_sums, sum_stride;
-    uint32_t x_splits, t_splits;
+    Shape g_shape, x_shape, t_shape;
     explicit Backward(const Inputs &in)
     {
         const uint64_t size = type_size(in.type);
@@ -433,21 +490,23 @@ struct Backward {
         rows = l.take(in.n * sizeof(Row));
         scale = l.take(8);
         rest = l.take(in.n * 4);
-        const uint64_t all = ceil_div(in.v, BN) * BN;
-        uint64_t fits = PIECE_BYTES / ((in.n ? in.n : 1) * size) / BN * BN;
+        const uint64_t all = ceil_div(in.v, WHOLE) * WHOLE;
+        uint64_t fits = PIECE_BYTES / ((in.n ? in.n : 1) * size) / WHOLE * WHOLE;
         fits = fits < 1024 ? 1024 : fits;
         pieces = in.v ? ceil_div(all, fits) : 1;
-        piece = ceil_div(ceil_div(all, pieces), BN) * BN;
+        piece = ceil_div(ceil_div(all, pieces), WHOLE) * WHOLE;
         pieces = in.v ? ceil_div(all, piece) : 1;
         g = l.take(in.n * piece * size);
-        sum_stride = ceil_div(in.d, BN) * BN;
-        x_splits = shares_of(in.n, in.d, piece * size / CHUNK);
-        t_splits = shares_of(piece, in.d, ceil_div(in.n * size, CHUNK));
+        sum_stride = ceil_div(in.d, WHOLE) * WHOLE;
+        const uint64_t v = in.v < piece ? in.v : piece;
+        g_shape = shape_of(in.n, v, in.d, in.type, false);
+        x_shape = shape_of(in.n, in.d, v, in.type, true);
+        t_shape = shape_of(v, in.d, in.n, in.type, true);
         x_sums = t_sums = 0;
-        if (x_splits > 1 || pieces > 1)
-            x_sums = l.take(x_splits * in.n * sum_stride * 4);
-        if (t_splits > 1)
-            t_sums = l.take(t_splits * piece * sum_stride * 4);
+        if (x_shape.splits > 1 || pieces > 1)
+            x_sums = l.take(x_shape.splits * in.n * sum_stride * 4);
+        if (t_shape.splits > 1)
+            t_sums = l.take(t_shape.splits * piece * sum_stride * 4);
     }
 };
 
@@ -458,8 +517,8 @@ int check_inputs(const char *what, const Inputs &in)
         return UNG_HIP_EINVAL;
     }
     if (in.n > INT32_MAX - 256 || in.v > INT32_MAX - 256 || in.d > (1u << 24) ||
-        ceil_div(in.n, 32) * ceil_div(in.v, BN) > most_blocks(256) / 2 ||
-        (in.n > in.v ? in.n : in.v) / 32 * ceil_div(in.d, BN) > most_blocks(256) / 2) {
+        ceil_div(in.n, 32) * ceil_div(in.v, 128) > most_blocks(256) / 2 ||
+        (in.n > in.v ? in.n : in.v) / 32 * ceil_div(in.d, 128) > most_blocks(256) / 2) {
         set_error("%s: %llu rows of %llu elements against a table of %llu are too many", what, (unsigned long long)in.n,
                   (unsigned long long)in.d, (unsigned long long)in.v);
         return UNG_HIP_EINVAL;
@@ -503,24 +562,27 @@ uint32_t some_blocks(uint64_t n) { return (uint32_t)(n < 1 ? 1 : n < 8192 ? n : 
 
 // The product of two sides, its tiles finished by `finish`.
 template <class E, bool A_ACROSS, bool B_ACROSS, class Finish>
-void product(const Operand &a, const Operand &b, uint32_t splits, const Finish &finish, hipStream_t st)
+void product(const Operand &a, const Operand &b, Shape shape, const Finish &finish, hipStream_t st)
 {
-    auto tiles = [&](auto high, auto wm) {
-        constexpr int BM = decltype(high)::value, WM = decltype(wm)::value;
-        const Grid grid = {(uint32_t)ceil_div(a.rows, BM), (uint32_t)ceil_div(b.rows, BN), splits,
-                           ceil_div(a.k * sizeof(E), CHUNK)};
-        if (const uint32_t blocks = grid.m_tiles * grid.n_tiles * grid.splits)
-            ung_tile_kernel<E, BM, WM, 2, A_ACROSS, B_ACROSS><<<blocks, WM * 128, 0, st>>>(a, b, grid, finish);
-    };
+    const Grid grid = {(uint32_t)ceil_div(a.rows, shape.high), (uint32_t)ceil_div(b.rows, shape.wide), shape.splits,
+                       ceil_div(a.k * sizeof(E), CHUNK), shape.high == BIG ? 16u : 8u};
+    const uint32_t items = grid.m_tiles * grid.n_tiles * grid.splits;
+    if (!items)
+        return;
     constexpr std::integral_constant<int, 1> one;
     constexpr std::integral_constant<int, 2> two;
-    const uint32_t high = height_of(a.rows, b.rows);
-    if (high == 32)
-        tiles(std::integral_constant<int, 32>{}, one);
-    else if (high == 64)
-        tiles(std::integral_constant<int, 64>{}, two);
-    else
-        tiles(std::integral_constant<int, 128>{}, two);
+    auto tiles = [&](auto high, auto wm, auto wn) {
+        constexpr int BM = decltype(high)::value, WM = decltype(wm)::value, WN = decltype(wn)::value;
+        ung_tile_kernel<E, BM, WM, WN, A_ACROSS, B_ACROSS><<<items, WM * WN * 64, 0, st>>>(a, b, grid, finish);
+    };
+    if (shape.high == 32)
+        tiles(std::integral_constant<int, 32>{}, one, two);
+    else if (shape.high == 64)
+        tiles(std::integral_constant<int, 64>{}, two, two);
+    else if (shape.high == 128)
+        tiles(std::integral_constant<int, 128>{}, two, two);
+    else if constexpr (sizeof(E) == 2)
+        tiles(std::integral_constant<int, BIG>{}, two, std::integral_constant<int, 4>{});
 }
 
 template <class E>
@@ -586,7 +648,7 @@ int ung_hip_table_loss_forward(const void *x, uint64_t x_stride, const void *tab
         const Operand b = side<E>(f.table, table, table_stride, table_rows, cols, ws, st, true);
         Part *parts = (Part *)(ws + f.parts);
         float *target = (float *)(ws + f.target);
-        product<E, false, false>(a, b, 1, LogSum{ids, without, target, parts, rows, table_rows, c}, st);
+        product<E, false, false>(a, b, f.shape, LogSum{{}, ids, without, target, parts, rows, table_rows, c}, st);
         auto join = [&](auto each) {
             constexpr int R = decltype(each)::value;
             ung_table_join_kernel<R><<<(uint32_t)ceil_div(rows, R), 256, 0, st>>>(parts, f.tiles, rows, table_rows, target,
@@ -650,32 +712,35 @@ int ung_hip_table_loss_backward(const void *x, uint64_t x_stride, const void *ta
             const uint64_t v0 = p * f.piece, v = table_rows - v0 < f.piece ? table_rows - v0 : f.piece;
             const Operand part = {(const uint8_t *)t.p + v0 * t.stride, t.stride, v, cols};
             const Operand g = {ws + f.g, f.piece * sizeof(E), rows, v}, x_side = {a.p, a.stride, rows, cols};
-            product<E, false, false>(x_side, part, 1,
-                                     Weights<E>{row, (float *)(ws + f.rest), (E *)(ws + f.g), f.piece, rows, v0, v, c}, st);
+            product<E, false, false>(x_side, part, f.g_shape,
+                                     Weights<E>{{}, row, (float *)(ws + f.rest), (E *)(ws + f.g), f.piece, rows, v0, v, c}, st);
             if (dx && rows) {
-                if (f.x_splits == 1 && f.pieces == 1)
-                    product<E, false, true>(g, across(part), 1,
-                                            Whole<E>{(E *)dx, dx_stride, rows, cols, back, vectors(dx, dx_stride, rows), rest}, st);
+                if (f.x_shape.splits == 1 && f.pieces == 1)
+                    product<E, false, true>(g, across(part), f.x_shape,
+                                            Whole<E>{{}, (E *)dx, dx_stride, rows, cols, back, vectors(dx, dx_stride, rows), rest}, st);
+                else if (p == 0)
+                    product<E, false, true>(g, across(part), f.x_shape,
+                                            Sums<false>{(float *)(ws + f.x_sums), f.sum_stride, rows}, st);
                 else
-                    product<E, false, true>(g, across(part), f.x_splits,
-                                            Sums{(float *)(ws + f.x_sums), f.sum_stride, rows, p > 0}, st);
+                    product<E, false, true>(g, across(part), f.x_shape,
+                                            Sums<true>{(float *)(ws + f.x_sums), f.sum_stride, rows}, st);
             }
             if (dtable && v) {
                 E *to = (E *)dtable + v0 * dtable_stride;
-                if (f.t_splits == 1)
-                    product<E, true, true>(across(g), across(x_side), 1,
-                                           Whole<E>{to, dtable_stride, v, cols, back, vectors(to, dtable_stride, v), none}, st);
+                if (f.t_shape.splits == 1)
+                    product<E, true, true>(across(g), across(x_side), f.t_shape,
+                                           Whole<E>{{}, to, dtable_stride, v, cols, back, vectors(to, dtable_stride, v), none}, st);
                 else {
-                    product<E, true, true>(across(g), across(x_side), f.t_splits,
-                                           Sums{(float *)(ws + f.t_sums), f.sum_stride, v, 0}, st);
+                    product<E, true, true>(across(g), across(x_side), f.t_shape,
+                                           Sums<false>{(float *)(ws + f.t_sums), f.sum_stride, v}, st);
                     ung_table_sum_kernel<E><<<some_blocks(ceil_div(v * ceil_div(cols, 4), 256)), 256, 0, st>>>(
-                        (const float *)(ws + f.t_sums), f.t_splits, v, cols, f.sum_stride, back, to, dtable_stride, none);
+                        (const float *)(ws + f.t_sums), f.t_shape.splits, v, cols, f.sum_stride, back, to, dtable_stride, none);
                 }
             }
         }
-        if (dx && rows && !(f.x_splits == 1 && f.pieces == 1))
+        if (dx && rows && !(f.x_shape.splits == 1 && f.pieces == 1))
             ung_table_sum_kernel<E><<<some_blocks(ceil_div(rows * ceil_div(cols, 4), 256)), 256, 0, st>>>(
-                (const float *)(ws + f.x_sums), f.x_splits, rows, cols, f.sum_stride, back, (E *)dx, dx_stride, rest);
+                (const float *)(ws + f.x_sums), f.x_shape.splits, rows, cols, f.sum_stride, back, (E *)dx, dx_stride, rest);
         return launched(what);
     });
 }

@@ -64,24 +64,25 @@ struct Matrix<float> {
 // One side of a product: `rows` rows of `k` elements.  Along the inner length: elements of a row
 // lie side by side, rows `stride` bytes apart.  Across it: element k of all rows lies side by
 // side, `stride` bytes after element k - 1 of them.  Either way these lines begin at 16-byte
-// boundaries and are whole vectors of 16 bytes long, or zero up to one; stride < 2^23.
+// boundaries and are whole vectors of 16 bytes long, or zero up to one; stride < 2^22.
 struct Operand {
     const void *p;
     uint64_t stride;
     uint64_t rows, k;
 };
-constexpr uint64_t MOST_STRIDE = 1ull << 23;
+constexpr uint64_t MOST_STRIDE = 1ull << 22;
 
 constexpr uint32_t OUTSIDE = 0x80000000u; // a range-checked load from here gives zeros
 
-// Loads and reads R rows of one side.  As m side (LANES) its rows are the lanes' own, as n side they
-// are spread over four instructions so that a lane ends with 16 neighbouring ones.
+// A block's loads and a wave's reads of R rows of one side.  As m side (LANES) its rows are the lanes'
+// own, as n side they are spread over four instructions so that a lane ends with 16 neighbouring ones.
 template <class E, int R, bool ACROSS, bool LANES, int WAVES>
 struct Side {
     static_assert(R / 8 % WAVES == 0 && (!ACROSS || sizeof(E) > 1), "");
-    static constexpr uint32_t KE = CHUNK / sizeof(E);        // elements of a chunk
-    static constexpr uint32_t LINE = R * sizeof(E) / 16;     // vectors of a line across
+    static constexpr uint32_t KE = CHUNK / sizeof(E);                         // elements of a chunk
+    static constexpr uint32_t LINE = ACROSS ? R * sizeof(E) / 16 : CHUNK / 16; // vectors of a line
     static constexpr uint32_t BYTES = R * CHUNK;
+    static constexpr int LOADS = R / 8 / WAVES; // of a wave, 64 vectors each
 
     // Position of a vector is turned by exclusive-or with a number of its line, so that lanes
     // that read different lines meet different banks.  The turn is made on the global side, as
@@ -96,35 +97,44 @@ struct Side {
             return (LANES ? (line & 3) << 1 | (line >> 3 & 1) << 3 : (line & 1) | (line >> 1 & 1) << 3) & (LINE - 1);
     }
 
-    // Chunk kb of rows row0... to `to`; every wave of the block takes part.
-    static __device__ inline void load(const Operand &of, uint64_t row0, uint32_t kb, uint8_t *to, uint32_t wave,
-                                       uint32_t lane)
+    // Where the next chunk is loaded from.  A lane's offsets are made once a tile: made for every
+    // chunk they cost a tenth (8192 x 8192 x 8192 bf16 1166 us, 1053; 4096 x 16384 x 768 137, 121).
+    const uint8_t *from;
+    uint64_t step;
+    int64_t left;           // elements of the inner length from here on
+    uint32_t offset[LOADS]; // rows past the end repeat the last one, vectors past it are outside
+    uint32_t key[LOADS];    // the element (along) or line (across) of the chunk that a load begins with
+
+    __device__ inline void begin(const Operand &of, uint64_t row0, uint32_t kb, uint32_t wave, uint32_t lane)
     {
-        const uint32_t stride = (uint32_t)of.stride;
-        if constexpr (!ACROSS) {
-            const __amdgpu_buffer_rsrc_t from =
-                buffer_of((const uint8_t *)of.p + row0 * of.stride + (uint64_t)kb * CHUNK, 0x7FFFFFFFu);
-            const uint64_t there = of.k * sizeof(E) - (uint64_t)kb * CHUNK; // bytes of a row from here
-            const uint32_t bytes = there < CHUNK ? (uint32_t)there : CHUNK;
-            const uint32_t last = (uint32_t)min(of.rows - row0, (uint64_t)R) - 1; // rows past the end repeat it
+        const uint32_t stride = (uint32_t)of.stride, last = (uint32_t)min(of.rows - row0, (uint64_t)R) - 1;
+        from = (const uint8_t *)of.p + (ACROSS ? (uint64_t)kb * KE * of.stride + row0 * sizeof(E)
+                                               : row0 * of.stride + (uint64_t)kb * CHUNK);
+        step = ACROSS ? KE * of.stride : CHUNK;
+        left = (int64_t)of.k - (int64_t)kb * KE;
 #pragma unroll
-            for (int i = 0; i < R / 8 / WAVES; ++i) {
-                const uint32_t row = i * WAVES * 8 + wave * 8 + (lane >> 3), at = ((lane & 7) ^ turn(row)) * 16;
-                to_lds16(from, at < bytes ? min(row, last) * stride + at : OUTSIDE, 0, to + (i * WAVES + wave) * 1024);
-            }
-        } else {
-            const uint64_t k0 = (uint64_t)kb * KE;
-            const __amdgpu_buffer_rsrc_t from =
-                buffer_of((const uint8_t *)of.p + k0 * of.stride + row0 * sizeof(E), 0x7FFFFFFFu);
-            const uint32_t lines = (uint32_t)min(of.k - k0, (uint64_t)KE);
-            const uint32_t bytes = (uint32_t)min(of.rows - row0, (uint64_t)R) * (uint32_t)sizeof(E);
-#pragma unroll
-            for (int i = 0; i < R / 8 / WAVES; ++i) {
-                const uint32_t v = (i * WAVES + wave) * 64 + lane, line = v / LINE, at = (v % LINE ^ turn(line)) * 16;
-                to_lds16(from, line < lines && at < bytes ? line * stride + at : OUTSIDE, 0,
-                         to + (i * WAVES + wave) * 1024);
+        for (int i = 0; i < LOADS; ++i) {
+            const uint32_t v = (i * WAVES + wave) * 64 + lane, line = v / LINE, at = (v % LINE ^ turn(line)) * 16;
+            if constexpr (!ACROSS) {
+                offset[i] = min(line, last) * stride + at;
+                key[i] = at / sizeof(E);
+            } else {
+                offset[i] = at < (last + 1) * sizeof(E) ? line * stride + at : OUTSIDE;
+                key[i] = line;
             }
         }
+    }
+
+    // The next chunk to `to`, zeros past the end; every wave of the block takes part.
+    __device__ inline void load(uint8_t *to, uint32_t wave)
+    {
+        const __amdgpu_buffer_rsrc_t at = buffer_of(from, 0x7FFFFFFFu);
+        const uint32_t there = uniform(left >= (int64_t)KE ? KE : left > 0 ? (uint32_t)left : 0u);
+#pragma unroll
+        for (int i = 0; i < LOADS; ++i)
+            to_lds16(at, key[i] < there ? offset[i] : OUTSIDE, 0, to + (i * WAVES + wave) * 1024);
+        from += step;
+        left -= KE;
     }
 
     // A lane's 16 bytes of 16 rows for half `half` of the chunk: rows first + t * 16 + 0..15 as m
@@ -171,107 +181,147 @@ struct Side {
 struct Grid {
     uint32_t m_tiles, n_tiles, splits;
     uint64_t chunks;
+    uint32_t band; // tiles of m that follow each other before the next one of n
 };
 
-// What a block makes: where its tile lies and which chunks it sums.  An XCD takes a contiguous
-// run, in bands of 8 tiles of m, so that the tiles it works on at a time share panels in its L2.
+// Where a block's tile lies.  An XCD takes a contiguous run of them, in bands of tiles of m, so that the
+// tiles it works on at a time share panels in its L2.
 struct Tile {
     uint64_t m0, n0;
-    uint32_t high; // rows of a tile
-    uint32_t split, kb, kb_end;
-    uint32_t wm, wn; // the wave's part begins at row m0 + wm and column n0 + wn
+    uint32_t split;
+    uint32_t high, strips; // rows of a tile; waves side by side along n, 64 columns each
+    uint32_t wm, wn;       // the wave's part begins at row m0 + wm and column n0 + wn
     uint32_t lane, wave;
 };
+
+constexpr int BIG = 256; // rows and columns of the largest tile
 
 // A block of WM x WN waves makes a BM x (64 WN) tile, each wave BM / WM x 64 of it in 16 x 16
 // matrix instructions.  Both panels of a chunk are staged in LDS by loads that bypass the
 // registers, one chunk ahead.  A lane ends with results [i][j][e]: row wm + 16 i + lane % 16,
-// column wn + lane / 16 * 16 + 4 j + e.
+// column wn + lane / 16 * 16 + 4 j + e.  `finish` brings what it needs of the tile's rows to LDS before
+// the sums (ahead), the values they begin with (start), and takes the results.
+//   256 x 256 tiles of eight waves: a wave reads 24 KB of LDS for a chunk's 4 M products where 64 x 64
+// parts read 32; 8192 x 8192 x 8192 bf16 1249 TFLOP/s in bands of 16 (4: 1168), 128 x 128 tiles, two
+// blocks to a CU, 1097 (the library's product 1377); without the results' stores 4096 x 16384 x 384 1065
+// and 950.  Chunks of 64 bytes in three or four stages were slower (1106 and 864): a row's loads
+// are then half a line of memory each.
+//   The panels lie in LDS variables of their own, and the loads are without branches: so the compiler
+// knows which loads a read of LDS depends on, and adds no wait of its own.
 template <class E, int BM, int WM, int WN, bool A_ACROSS, bool B_ACROSS, class Finish>
 __global__ __launch_bounds__(WM * WN * 64, 2) void ung_tile_kernel(Operand a, Operand b, Grid grid, Finish finish)
 {
+    // The largest tile takes chunks in pairs (a last odd one with zeros): a loop that can end between the
+    // two moves the sums from registers to others, and there are none left.
+    constexpr bool PAIRS = BM == BIG;
     constexpr int WAVES = WM * WN, BN = WN * 64, TM = BM / WM / 16;
     using A = Side<E, BM, A_ACROSS, true, WAVES>;
     using B = Side<E, BN, B_ACROSS, false, WAVES>;
-    struct Panels {
-        alignas(16) uint8_t a[A::BYTES], b[B::BYTES];
-    };
-    __shared__ Panels even, odd;
+    __shared__ alignas(16) uint8_t a_even[A::BYTES], a_odd[A::BYTES], b_even[B::BYTES], b_odd[B::BYTES];
+    __shared__ alignas(16) uint8_t side[BM * Finish::AHEAD + 16];
     Tile at;
     at.high = BM;
+    at.strips = WN;
     at.lane = threadIdx.x & 63;
     at.wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    at.wm = (at.wave % WM) * (BM / WM);
-    at.wn = (at.wave / WM) * 64;
+    at.wm = at.wave % WM * (BM / WM);
+    at.wn = at.wave / WM * 64;
+    uint32_t kb, kb_end;
     {
         const uint32_t tiles = grid.m_tiles * grid.n_tiles, item = xcd_run(blockIdx.x, tiles * grid.splits);
         uint32_t tm, tn;
         at.split = uniform(item / tiles);
-        tile_of(item - at.split * tiles, 8, grid.m_tiles, grid.n_tiles, tm, tn);
+        tile_of(item - at.split * tiles, grid.band, grid.m_tiles, grid.n_tiles, tm, tn);
         at.m0 = (uint64_t)uniform(tm) * BM;
         at.n0 = (uint64_t)uniform(tn) * BN;
-        const uint32_t share = (uint32_t)(grid.chunks / grid.splits), longer = (uint32_t)(grid.chunks % grid.splits);
-        at.kb = at.split * share + min(at.split, longer);
-        at.kb_end = at.kb + share + (at.split < longer ? 1 : 0);
+        constexpr uint32_t UNIT = PAIRS ? 2 : 1;
+        const uint32_t units = (uint32_t)((grid.chunks + UNIT - 1) / UNIT);
+        const uint32_t share = units / grid.splits, longer = units % grid.splits;
+        kb = UNIT * (at.split * share + min(at.split, longer));
+        kb_end = kb + UNIT * (share + (at.split < longer ? 1 : 0));
     }
-    typename Matrix<E>::Acc acc[TM][4];
-#pragma unroll
-    for (int i = 0; i < TM; ++i)
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-            acc[i][j] = typename Matrix<E>::Acc{0, 0, 0, 0};
-
-    auto load = [&](Panels &to, uint32_t kb) {
-        A::load(a, at.m0, kb, to.a, at.wave, at.lane);
-        B::load(b, at.n0, kb, to.b, at.wave, at.lane);
+    A left;
+    B right;
+    left.begin(a, at.m0, kb, at.wave, at.lane);
+    right.begin(b, at.n0, kb, at.wave, at.lane);
+    auto load = [&](uint8_t *to_a, uint8_t *to_b) {
+        left.load(to_a, at.wave);
+        right.load(to_b, at.wave);
+        __builtin_amdgcn_sched_barrier(0);
     };
-    auto multiply = [&](const Panels &p) {
+    load(a_even, b_even);
+    typename Matrix<E>::Acc acc[TM][4];
+    finish.ahead(at, side);
+    finish.start(at, acc);
+
+    auto step = [&](const uint8_t *pa, const uint8_t *pb, uint8_t *next_a, uint8_t *next_b) {
+        await_loads<0>(); // loads into LDS are counted as memory loads, which a barrier alone does not await
+        __builtin_amdgcn_s_barrier(); // the panels have landed; every wave is done with the others
+        __builtin_amdgcn_sched_barrier(0);
+        load(next_a, next_b);
 #pragma unroll
         for (int half = 0; half < 2; ++half) {
             u32x4 y[4];
 #pragma unroll
             for (int j = 0; j < 4; ++j)
-                y[j] = B::fragment(p.b, at.wn, j, half, at.lane);
+                y[j] = B::fragment(pb, at.wn, j, half, at.lane);
 #pragma unroll
             for (int i = 0; i < TM; ++i) {
-                const u32x4 x = A::fragment(p.a, at.wm, i, half, at.lane);
+                const u32x4 x = A::fragment(pa, at.wm, i, half, at.lane);
 #pragma unroll
                 for (int j = 0; j < 4; ++j)
                     acc[i][j] = Matrix<E>::mul(y[j], x, acc[i][j]);
             }
         }
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); // the panels are read
     };
-    auto step = [&](const Panels &now, Panels &next, uint32_t kb) {
-        await_loads<0>(); // loads into LDS are counted as memory loads, which a barrier alone does not await
-        __syncthreads();  // `now` has landed; every wave is done with `next`
-        if (kb + 1 < at.kb_end)
-            load(next, kb + 1);
-        multiply(now);
-    };
-    if (at.kb < at.kb_end)
-        load(even, at.kb);
-    for (uint32_t kb = at.kb; kb < at.kb_end; kb += 2) {
-        step(even, odd, kb);
-        if (kb + 1 < at.kb_end)
-            step(odd, even, kb + 1);
+    if constexpr (PAIRS) {
+        for (uint32_t pairs = (kb_end - kb) / 2; pairs; --pairs) {
+            step(a_even, b_even, a_odd, b_odd);
+            step(a_odd, b_odd, a_even, b_even);
+        }
+    } else {
+        while (kb < kb_end) {
+            step(a_even, b_even, a_odd, b_odd);
+            if (++kb == kb_end)
+                break;
+            step(a_odd, b_odd, a_even, b_even);
+            ++kb;
+        }
     }
-    __syncthreads(); // the panels are free for the finish
-    finish(at, acc, reinterpret_cast<uint8_t *>(&even));
+    await_loads<0>(); // the last step's loads, of the chunk past the end, land here
+    __syncthreads();  // the panels are free for the finish
+    finish(at, side, acc, b_even);
 }
+
+// A finish that needs nothing ahead, and sums that begin at 0.
+struct Plainly {
+    static constexpr uint32_t AHEAD = 0; // bytes of LDS for a row
+    __device__ inline void ahead(const Tile &, uint8_t *) const {}
+    template <class Acc, int TM>
+    __device__ inline void start(const Tile &, Acc (&acc)[TM][4]) const
+    {
+#pragma unroll
+        for (int i = 0; i < TM; ++i)
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                acc[i][j] = Acc{0, 0, 0, 0};
+    }
+};
 
 // ---- storing a tile's results ------------------------------------------------------------
 
 // A wave's 16 x 64 results (row r, columns g * 16 + 0..15 of each lane 16 g + r) to `to`, rows
 // `stride` elements apart, of which `rows` and `cols` are there.  16-bit vectors go out as they lie where
 // `vectors`; the others are turned in LDS first, so that a store's lanes write neighbouring elements.
-// `own`: TURN bytes of LDS of the wave's own.
-constexpr uint32_t TURN = 16 * (64 * 4 + 16);
+// `own`: turn_bytes of LDS of the wave's own; a block's are no more than its panel of the n side.
+constexpr uint32_t turn_bytes(uint32_t size) { return 16 * 64 * size; }
 template <class T>
 __device__ inline void store_rows(T *to, uint64_t stride, uint32_t rows, uint64_t cols, bool vectors,
                                   const Vec<T> (&o)[16 / Vec<T>::N], uint8_t *own, uint32_t lane)
 {
     constexpr int N = Vec<T>::N;
-    constexpr uint32_t PITCH = 64 * sizeof(T) + 16;
+    constexpr uint32_t V = 64 / N; // vectors of a row; their positions are turned by its number
     const uint32_t r = lane & 15, g = lane >> 4;
     if (sizeof(T) == 2 && vectors && cols >= 64) {
         if (r < rows)
@@ -280,22 +330,21 @@ __device__ inline void store_rows(T *to, uint64_t stride, uint32_t rows, uint64_
                 store_loose(to + r * stride + g * 16 + x * N, o[x]);
         return;
     }
+    auto place = [&](uint32_t row, uint32_t v) { return own + (row * V + (v ^ (row & (V - 1)))) * 16; };
 #pragma unroll
-    for (int x = 0; x < 16 / N; ++x)
-        *reinterpret_cast<Vec<T> *>(own + r * PITCH + (g * 16 + x * N) * sizeof(T)) = o[x];
+    for (uint32_t x = 0; x < 16 / N; ++x)
+        *reinterpret_cast<Vec<T> *>(place(r, g * (16 / N) + x)) = o[x];
     wave_lds_fence();
     if (vectors && cols >= 64) {
-        constexpr int LANES = 64 / N; // that hold a row
-        const uint32_t y0 = lane / LANES, x = lane % LANES * N;
+        const uint32_t y0 = lane / V, x = lane % V; // V lanes hold a row
 #pragma unroll
         for (uint32_t y = 0; y < 16; y += N)
             if (y + y0 < rows)
-                store_loose(to + (y + y0) * stride + x,
-                            *reinterpret_cast<const Vec<T> *>(own + (y + y0) * PITCH + x * sizeof(T)));
+                store_loose(to + (y + y0) * stride + x * N, *reinterpret_cast<const Vec<T> *>(place(y + y0, x)));
     } else if (lane < cols) {
 #pragma unroll 4
         for (uint32_t y = 0; y < rows; ++y)
-            to[y * stride + lane] = *reinterpret_cast<const T *>(own + y * PITCH + lane * sizeof(T));
+            to[y * stride + lane] = *reinterpret_cast<const T *>(place(y, lane / N) + lane % N * sizeof(T));
     }
     wave_lds_fence();
 }
