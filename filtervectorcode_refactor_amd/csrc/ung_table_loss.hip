@@ -11,6 +11,7 @@
 // time: G of the piece goes to memory in the inputs' type, where two products read it.
 #include <hip/hip_runtime.h>
 
+#include <algorithm>
 #include <cmath>
 #include <cstdint>
 
@@ -29,19 +30,22 @@ constexpr int WHOLE = 256; // columns that every tile's width divides
 
 // ---- forward -------------------------------------------------------------------------
 
-// A row's part of a tile of scores: the largest score s and sum exp((s - largest) / T).
+// A row's part of a tile of scores: sum 2^(c s - top) with c = log2(e) / T and `top` the whole number
+// nearest to the largest c s.  So a term's exponent is rounded once, near 0 where it counts, and parts
+// are joined with factors that are powers of two.
 struct Part {
     float top, sum;
 };
+constexpr float NO_TOP = -INF; // of a part without a score
 
-__device__ inline Part joined(Part a, Part b, float c)
+__device__ inline Part joined(Part a, Part b)
 {
-    const float top = fmaxf(a.top, b.top), from = top == -INF ? 0.0f : top;
-    return {top, a.sum * weight_of(a.top, from, c) + b.sum * weight_of(b.top, from, c)};
+    const float top = fmaxf(a.top, b.top), from = top == NO_TOP ? 0.0f : top;
+    return {top, a.sum * __builtin_amdgcn_exp2f(a.top - from) + b.sum * __builtin_amdgcn_exp2f(b.top - from)};
 }
 
 // Of a tile of scores (rows of x, columns: rows of the table): every row's part, and the
-// target's score where the tile holds it.
+// target's score where the tile holds it.  A lane makes a part of its 16 columns; the block joins them.
 struct LogSum : Plainly {
     const int32_t *ids, *without;
     float *target; // [n]
@@ -64,7 +68,7 @@ struct LogSum : Plainly {
     template <int TM>
     __device__ inline void operator()(const Tile &t, const uint8_t *side, f32x4 (&acc)[TM][4], uint8_t *lds) const
     {
-        Part *red = reinterpret_cast<Part *>(lds); // [strips][rows of the tile]
+        Part *red = reinterpret_cast<Part *>(lds); // [4 strips][rows of the tile]
         const uint32_t r = t.lane & 15, g = t.lane >> 4, high = t.high;
         const uint64_t col0 = t.n0 + t.wn + g * 16;
 #pragma unroll
@@ -81,29 +85,25 @@ struct LogSum : Plainly {
                         acc[i][e / 4][e % 4] = -INF;
                 }
             }
-            float top = -INF;
+            float top = acc[i][0][0];
 #pragma unroll
-            for (int e = 0; e < 16; ++e)
+            for (int e = 1; e < 16; ++e)
                 top = fmaxf(top, acc[i][e / 4][e % 4]);
-            top = fmaxf(top, __shfl_xor(top, 16));
-            top = fmaxf(top, __shfl_xor(top, 32));
-            const float from = top == -INF ? 0.0f : top;
+            top = __builtin_rintf(top * c);
+            const float from = top == NO_TOP ? 0.0f : -top;
             float sum = 0.0f;
 #pragma unroll
             for (int e = 0; e < 16; ++e)
-                sum += weight_of(acc[i][e / 4][e % 4], from, c);
-            sum += __shfl_xor(sum, 16);
-            sum += __shfl_xor(sum, 32);
-            if (g == 0)
-                red[t.wn / 64 * high + t.wm + i * 16 + r] = {top, sum};
+                sum += __builtin_amdgcn_exp2f(__builtin_fmaf(acc[i][e / 4][e % 4], c, from));
+            red[(t.wn / 16 + g) * high + t.wm + i * 16 + r] = {top, sum};
             __builtin_amdgcn_sched_barrier(0); // 16 rows at a time: all of them need more registers than there are
         }
         __syncthreads();
         const uint64_t row = t.m0 + threadIdx.x;
         if (threadIdx.x < high && row < n) {
             Part p = red[threadIdx.x];
-            for (uint32_t w = 1; w < t.strips; ++w)
-                p = joined(p, red[w * high + threadIdx.x], c);
+            for (uint32_t w = 1; w < t.strips * 4; ++w)
+                p = joined(p, red[w * high + threadIdx.x]);
             parts[t.n0 / (t.strips * 64) * n + row] = p;
         }
     }
@@ -113,36 +113,39 @@ struct LogSum : Plainly {
 template <int R>
 __global__ __launch_bounds__(256) void ung_table_join_kernel(const Part *parts, uint64_t tiles, uint64_t n, uint64_t v,
                                                              const float *target, const int32_t *ids,
-                                                             const int32_t *without, float c, float by, float *loss,
-                                                             float *lse)
+                                                             const int32_t *without, float c, float *loss, float *lse)
 {
     __shared__ Part red[256];
     constexpr uint32_t EACH = 256 / R;
+    constexpr float LN2 = 0.693147180559945309417f;
     const uint32_t in = threadIdx.x % R, which = threadIdx.x / R;
     const uint64_t row = (uint64_t)blockIdx.x * R + in;
-    Part p = {-INF, 0.0f};
+    Part p = {NO_TOP, 0.0f};
     if (row < n) {
 #pragma unroll 4
         for (uint64_t t = which; t < tiles; t += EACH)
-            p = joined(p, parts[t * n + row], c);
+            p = joined(p, parts[t * n + row]);
     }
     red[threadIdx.x] = p;
     __syncthreads();
 #pragma unroll
     for (uint32_t half = EACH / 2; half; half /= 2) {
         if (which < half)
-            red[threadIdx.x] = joined(red[threadIdx.x], red[threadIdx.x + half * R], c);
+            red[threadIdx.x] = joined(red[threadIdx.x], red[threadIdx.x + half * R]);
         __syncthreads();
     }
     if (which || row >= n)
         return;
     p = red[in];
-    const float log_sum = logf(p.sum);
+    const float log_sum = log2f(p.sum);
     const int32_t id = ids[row];
     const bool there = (uint64_t)(uint32_t)id < v && !(without && without[row] == id);
-    // the difference first: it is exact where the target is near the largest score
-    loss[row] = there ? (p.top - target[row]) * by + log_sum : 0.0f;
-    lse[row] = p.sum == 0.0f ? -INF : p.top * by + log_sum;
+    // as the logarithm of a quotient, which is 1 or more as the sum holds the target's term; as a
+    // difference where that term is nothing beside the sum
+    const float u = __builtin_fmaf(there ? target[row] : 0.0f, c, -p.top);
+    const float nll = u > -100.0f ? log2f(p.sum / __builtin_amdgcn_exp2f(u)) : log_sum - u;
+    loss[row] = there ? nll * LN2 : 0.0f;
+    lse[row] = p.sum == 0.0f ? -INF : (p.top + log_sum) * LN2;
 }
 
 // ---- backward ------------------------------------------------------------------------
@@ -395,32 +398,39 @@ __global__ __launch_bounds__(256) void ung_table_sum_kernel(const float *part, u
 // length.
 struct Shape {
     uint32_t high, wide, splits;
+    double score; // share of the chip's rate that the tiles' results are made at
 };
 
+// The tile with the best of three factors: its rate on a full chip (256 x 256 1.08, 128 x 128 1, of 64 and 32
+// rows 0.75 and 0.5), the share of it that lies in the product, and the share of the places that the items of
+// all rounds fill.  Measured both ways, us, bf16: 2048 x 32768 of 768 125 by 256, 137 by 128; 32768 x 768 of
+// 2048 141 and 131 (1.5 rounds, 3 whole ones); 14336 x 384 of 4096 64 by 128 rows, 67 by 64.
+// `shares`: sums may be made in shares of the inner length of at least `fewest` chunks.
 Shape shape_of(uint64_t m, uint64_t n, uint64_t k, int type, bool shares)
 {
     const uint64_t cus = cu_count(), chunks = ceil_div(k * type_size(type), CHUNK);
-    auto with = [&](uint32_t high, uint32_t wide, uint32_t at_once, uint64_t fewest) {
-        Shape s = {high, wide, 1};
-        const uint64_t tiles = ceil_div(m, high) * ceil_div(n, wide);
-        if (shares && tiles) {
-            const uint64_t by_cu = at_once * cus / tiles, by_k = chunks / fewest, most = by_cu < by_k ? by_cu : by_k;
+    Shape best = {32, 128, 1, -1.0};
+    auto with = [&](uint32_t high, uint32_t wide, uint32_t at_once, uint64_t fewest, double rate) {
+        Shape s = {high, wide, 1, 0.0};
+        const uint64_t tiles = ceil_div(m, high) * ceil_div(n, wide), places = at_once * cus;
+        if (!tiles)
+            return;
+        if (shares) {
+            const uint64_t by_cu = places / tiles, by_k = chunks / fewest, most = by_cu < by_k ? by_cu : by_k;
             s.splits = most > 1 ? (uint32_t)most : 1;
         }
-        return s;
+        const uint64_t items = tiles * s.splits;
+        s.score = rate * (double)m * (double)n / ((double)(tiles * high) * wide) * (double)items /
+                  (double)(ceil_div(items, places) * places);
+        if (s.score > best.score)
+            best = s;
     };
-    if (type != UNG_HIP_F32 && m > 128 && n > 128 && ceil_div(n, 128) % 2 == 0 && chunks) {
-        const Shape s = with(BIG, BIG, 1, 8);
-        const uint64_t items = ceil_div(m, BIG) * ceil_div(n, BIG) * s.splits;
-        if (items * 8 > ceil_div(items, cus) * cus * 5)
-            return s;
-    }
-    if (m > 64 && n > 64) {
-        const Shape s = with(128, 128, 2, 8);
-        if (ceil_div(m, 128) * ceil_div(n, 128) * s.splits * 4 > 3 * cus)
-            return s;
-    }
-    return with(m <= 32 ? 32 : 64, 128, 3, 4);
+    if (type != UNG_HIP_F32)
+        with(BIG, BIG, 1, 8, 1.08);
+    with(128, 128, 2, 8, 1.0);
+    with(64, 128, 3, 4, 0.75);
+    with(32, 128, 3, 4, 0.5);
+    return best;
 }
 
 struct Inputs {
@@ -473,9 +483,9 @@ struct Forward {
     }
 };
 
-// G of a piece takes about this much (it is read while it lies in the last-level cache), of at
+// G of a piece takes this much at most (it is read while it lies in the last-level cache), but for at
 // least 1024 rows of the table.
-constexpr uint64_t PIECE_BYTES = 128ull << 20;
+constexpr uint64_t PIECE_BYTES = 168ull << 20;
 
 struct Backward {
     Layout l;
@@ -493,15 +503,24 @@ struct Backward {
         const uint64_t all = ceil_div(in.v, WHOLE) * WHOLE;
         uint64_t fits = PIECE_BYTES / ((in.n ? in.n : 1) * size) / WHOLE * WHOLE;
         fits = fits < 1024 ? 1024 : fits;
-        pieces = in.v ? ceil_div(all, fits) : 1;
-        piece = ceil_div(ceil_div(all, pieces), WHOLE) * WHOLE;
-        pieces = in.v ? ceil_div(all, piece) : 1;
-        g = l.take(in.n * piece * size);
+        // of the least number of pieces and half as many again, the one whose dT fills its rounds best
+        // (4096 x 100000 x 384: 5 of 20224 rows 1596 us, 7 of 14336 1702, 4 of 25088 1686)
+        const uint64_t least = all ? ceil_div(all, fits) : 1;
+        pieces = least, piece = all;
+        double most = -1.0;
+        for (uint64_t p = least; p <= least + least / 2; ++p) {
+            const uint64_t rows_of_it = ceil_div(ceil_div(all, p), WHOLE) * WHOLE;
+            const double score = shape_of(rows_of_it, in.d, in.n, in.type, true).score;
+            if (score > most * 1.02)
+                most = score, piece = rows_of_it, pieces = p;
+        }
+        pieces = all ? ceil_div(all, piece) : 1;
         sum_stride = ceil_div(in.d, WHOLE) * WHOLE;
         const uint64_t v = in.v < piece ? in.v : piece;
         g_shape = shape_of(in.n, v, in.d, in.type, false);
         x_shape = shape_of(in.n, in.d, v, in.type, true);
         t_shape = shape_of(v, in.d, in.n, in.type, true);
+        g = l.take(in.n * piece * size);
         x_sums = t_sums = 0;
         if (x_shape.splits > 1 || pieces > 1)
             x_sums = l.take(x_shape.splits * in.n * sum_stride * 4);
@@ -643,7 +662,7 @@ int ung_hip_table_loss_forward(const void *x, uint64_t x_stride, const void *tab
     uint8_t *ws = (uint8_t *)workspace;
     return with_type(type, [&](auto zero) {
         using E = decltype(zero);
-        const float c = LOG2E / temperature, by = 1.0f / temperature;
+        const float c = LOG2E / temperature;
         const Operand a = side<E>(f.x, x, x_stride, rows, cols, ws, st, true);
         const Operand b = side<E>(f.table, table, table_stride, table_rows, cols, ws, st, true);
         Part *parts = (Part *)(ws + f.parts);
@@ -652,7 +671,7 @@ int ung_hip_table_loss_forward(const void *x, uint64_t x_stride, const void *tab
         auto join = [&](auto each) {
             constexpr int R = decltype(each)::value;
             ung_table_join_kernel<R><<<(uint32_t)ceil_div(rows, R), 256, 0, st>>>(parts, f.tiles, rows, table_rows, target,
-                                                                              ids, without, c, by, loss, lse);
+                                                                              ids, without, c, loss, lse);
         };
         if (rows < 16)
             join(std::integral_constant<int, 1>{});
@@ -708,29 +727,42 @@ int ung_hip_table_loss_backward(const void *x, uint64_t x_stride, const void *ta
             return (uintptr_t)p % 4 == 0 && (rows == 1 || stride * sizeof(E) % 4 == 0);
         };
         const Rest<E> none = {}, rest = sizeof(E) == 4 ? none : Rest<E>{row, (float *)(ws + f.rest), (const E *)t.p, t.stride / sizeof(E)};
+        const Operand x_side = {a.p, a.stride, rows, cols};
+        float *const x_sums = (float *)(ws + f.x_sums);
+        // Of piece p: its rows of the table, and its G
+        auto length = [&](uint64_t p) { return std::min(table_rows - p * f.piece, f.piece); };
+        auto table_of = [&](uint64_t p) {
+            return Operand{(const uint8_t *)t.p + p * f.piece * t.stride, t.stride, length(p), cols};
+        };
+        E *const g_at = (E *)(ws + f.g);
+        auto g_of = [&](uint64_t p) { return Operand{g_at, f.piece * sizeof(E), rows, length(p)}; };
+        auto weights = [&](uint64_t p) {
+            return Weights<E>{{}, row, (float *)(ws + f.rest), g_at, f.piece, rows, p * f.piece, length(p), c};
+        };
+        auto whole = [&](uint64_t p) {
+            E *to = (E *)dtable + p * f.piece * dtable_stride;
+            return Whole<E>{{}, to, dtable_stride, length(p), cols, back, vectors(to, dtable_stride, length(p)), none};
+        };
         for (uint64_t p = 0; p < f.pieces; ++p) {
-            const uint64_t v0 = p * f.piece, v = table_rows - v0 < f.piece ? table_rows - v0 : f.piece;
-            const Operand part = {(const uint8_t *)t.p + v0 * t.stride, t.stride, v, cols};
-            const Operand g = {ws + f.g, f.piece * sizeof(E), rows, v}, x_side = {a.p, a.stride, rows, cols};
-            product<E, false, false>(x_side, part, f.g_shape,
-                                     Weights<E>{{}, row, (float *)(ws + f.rest), (E *)(ws + f.g), f.piece, rows, v0, v, c}, st);
+            const uint64_t v = length(p);
+            const Operand part = table_of(p), g = g_of(p);
+            product<E, false, false>(x_side, part, f.g_shape, weights(p), st);
             if (dx && rows) {
                 if (f.x_shape.splits == 1 && f.pieces == 1)
                     product<E, false, true>(g, across(part), f.x_shape,
                                             Whole<E>{{}, (E *)dx, dx_stride, rows, cols, back, vectors(dx, dx_stride, rows), rest}, st);
                 else if (p == 0)
                     product<E, false, true>(g, across(part), f.x_shape,
-                                            Sums<false>{(float *)(ws + f.x_sums), f.sum_stride, rows}, st);
+                                            Sums<false>{x_sums, f.sum_stride, rows}, st);
                 else
                     product<E, false, true>(g, across(part), f.x_shape,
-                                            Sums<true>{(float *)(ws + f.x_sums), f.sum_stride, rows}, st);
+                                            Sums<true>{x_sums, f.sum_stride, rows}, st);
             }
             if (dtable && v) {
-                E *to = (E *)dtable + v0 * dtable_stride;
                 if (f.t_shape.splits == 1)
-                    product<E, true, true>(across(g), across(x_side), f.t_shape,
-                                           Whole<E>{{}, to, dtable_stride, v, cols, back, vectors(to, dtable_stride, v), none}, st);
+                    product<E, true, true>(across(g), across(x_side), f.t_shape, whole(p), st);
                 else {
+                    E *to = (E *)dtable + p * f.piece * dtable_stride;
                     product<E, true, true>(across(g), across(x_side), f.t_shape,
                                            Sums<false>{(float *)(ws + f.t_sums), f.sum_stride, v}, st);
                     ung_table_sum_kernel<E><<<some_blocks(ceil_div(v * ceil_div(cols, 4), 256)), 256, 0, st>>>(
@@ -738,9 +770,9 @@ int ung_hip_table_loss_backward(const void *x, uint64_t x_stride, const void *ta
                 }
             }
         }
-        if (dx && rows && !(f.x_shape.splits == 1 && f.pieces == 1))
+        if (dx && rows && (f.x_shape.splits > 1 || f.pieces > 1))
             ung_table_sum_kernel<E><<<some_blocks(ceil_div(rows * ceil_div(cols, 4), 256)), 256, 0, st>>>(
-                (const float *)(ws + f.x_sums), f.x_shape.splits, rows, cols, f.sum_stride, back, (E *)dx, dx_stride, rest);
+                x_sums, f.x_shape.splits, rows, cols, f.sum_stride, back, (E *)dx, dx_stride, rest);
         return launched(what);
     });
 }

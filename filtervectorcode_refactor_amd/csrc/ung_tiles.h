@@ -209,7 +209,9 @@ constexpr int BIG = 256; // rows and columns of the largest tile
 //   The panels lie in LDS variables of their own, and the loads are without branches: so the compiler
 // knows which loads a read of LDS depends on, and adds no wait of its own.
 template <class E, int BM, int WM, int WN, bool A_ACROSS, bool B_ACROSS, class Finish>
-__global__ __launch_bounds__(WM * WN * 64, 2) void ung_tile_kernel(Operand a, Operand b, Grid grid, Finish finish)
+__device__ inline void make_tile(const Operand &a, const Operand &b, const Grid &grid, uint32_t block,
+                                 const Finish &finish, uint8_t *a_even, uint8_t *a_odd, uint8_t *b_even, uint8_t *b_odd,
+                                 uint8_t *side)
 {
     // The largest tile takes chunks in pairs (a last odd one with zeros): a loop that can end between the
     // two moves the sums from registers to others, and there are none left.
@@ -217,8 +219,6 @@ __global__ __launch_bounds__(WM * WN * 64, 2) void ung_tile_kernel(Operand a, Op
     constexpr int WAVES = WM * WN, BN = WN * 64, TM = BM / WM / 16;
     using A = Side<E, BM, A_ACROSS, true, WAVES>;
     using B = Side<E, BN, B_ACROSS, false, WAVES>;
-    __shared__ alignas(16) uint8_t a_even[A::BYTES], a_odd[A::BYTES], b_even[B::BYTES], b_odd[B::BYTES];
-    __shared__ alignas(16) uint8_t side[BM * Finish::AHEAD + 16];
     Tile at;
     at.high = BM;
     at.strips = WN;
@@ -228,7 +228,7 @@ __global__ __launch_bounds__(WM * WN * 64, 2) void ung_tile_kernel(Operand a, Op
     at.wn = at.wave / WM * 64;
     uint32_t kb, kb_end;
     {
-        const uint32_t tiles = grid.m_tiles * grid.n_tiles, item = xcd_run(blockIdx.x, tiles * grid.splits);
+        const uint32_t tiles = grid.m_tiles * grid.n_tiles, item = xcd_run(block, tiles * grid.splits);
         uint32_t tm, tn;
         at.split = uniform(item / tiles);
         tile_of(item - at.split * tiles, grid.band, grid.m_tiles, grid.n_tiles, tm, tn);
@@ -292,6 +292,15 @@ __global__ __launch_bounds__(WM * WN * 64, 2) void ung_tile_kernel(Operand a, Op
     await_loads<0>(); // the last step's loads, of the chunk past the end, land here
     __syncthreads();  // the panels are free for the finish
     finish(at, side, acc, b_even);
+}
+
+template <class E, int BM, int WM, int WN, bool A_ACROSS, bool B_ACROSS, class Finish>
+__global__ __launch_bounds__(WM * WN * 64, 2) void ung_tile_kernel(Operand a, Operand b, Grid grid, Finish finish)
+{
+    constexpr uint32_t HIGH = BM * CHUNK, WIDE = WN * 64 * CHUNK;
+    __shared__ alignas(16) uint8_t a_even[HIGH], a_odd[HIGH], b_even[WIDE], b_odd[WIDE];
+    __shared__ alignas(16) uint8_t side[BM * Finish::AHEAD + 16];
+    make_tile<E, BM, WM, WN, A_ACROSS, B_ACROSS>(a, b, grid, blockIdx.x, finish, a_even, a_odd, b_even, b_odd, side);
 }
 
 // A finish that needs nothing ahead, and sums that begin at 0.
