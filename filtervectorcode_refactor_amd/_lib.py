@@ -104,6 +104,8 @@ SIGNATURES = {
     "ung_hip_int8_quantize": (_int, [_vp, _int, _u64, _u64, _u64, _vp, _vp, _vp]),
     "ung_hip_int8_matmul_workspace": (_int, [_u64, _u64, _u64, _int, C.POINTER(_u64)]),
     "ung_hip_int8_matmul": (_int, [_vp, _vp, _vp, _vp, _u64, _u64, _u64, _vp, _int, _u64, _vp, _u64, _vp]),
+    "ung_hip_int8_linear_workspace": (_int, [_u64, _u64, _u64, _int, C.POINTER(_u64)]),
+    "ung_hip_int8_linear": (_int, [_vp, _int, _u64, _u64, _u64, _vp, _vp, _u64, _vp, _int, _u64, _vp, _u64, _vp]),
     "ung_hip_table_loss_workspace": (_int, [_vp, _u64, _vp, _u64, _int, _u64, _u64, _u64, _int, C.POINTER(_u64)]),
     "ung_hip_table_loss_forward": (_int, [_vp, _u64, _vp, _u64, _int, _u64, _u64, _u64, _vp, _vp, C.c_float, _vp, _vp,
                                           _vp, _u64, _vp]),

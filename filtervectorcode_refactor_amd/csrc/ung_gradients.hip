@@ -115,24 +115,37 @@ __global__ __launch_bounds__(NT) void ung_gradient_squares_kernel(List list, dou
         part[blockIdx.x] = sum;
 }
 
+// The sum of all partial sums, in an order that their number decides.
+__device__ inline double sum_of(const double *part, uint32_t count, double *red)
+{
+    double sum = 0.0;
+    for (uint32_t i = threadIdx.x; i < count; i += NT)
+        sum += part[i];
+    return block_sum(sum, red);
+}
+
 __global__ __launch_bounds__(NT) void ung_gradient_join_kernel(const double *part, uint32_t count, double *whole,
                                                                float *norm)
 {
     __shared__ double red[NT / 64];
-    double sum = 0.0;
-    for (uint32_t i = threadIdx.x; i < count; i += NT)
-        sum += part[i];
-    sum = block_sum(sum, red);
+    const double sum = sum_of(part, count, red);
     if (threadIdx.x == 0) {
-        whole[0] = sqrt(sum);
+        whole[0] = sum;
         if (norm)
-            norm[0] = (float)whole[0];
+            norm[0] = (float)sqrt(sum);
     }
 }
 
-__global__ __launch_bounds__(NT) void ung_gradient_scale_kernel(List list, const double *whole, double most)
+// Every block adds up the partial sums for itself: up to SUMS of them cost it less than a launch
+// between the two passes would.
+constexpr uint32_t SUMS = 2048;
+__global__ __launch_bounds__(NT) void ung_gradient_scale_kernel(List list, const double *part, uint32_t count, double most,
+                                                                float *to_norm)
 {
-    const double norm = whole[0];
+    __shared__ double red[NT / 64];
+    const double norm = sqrt(sum_of(part, count, red));
+    if (to_norm && blockIdx.x == 0 && threadIdx.x == 0)
+        to_norm[0] = (float)norm;
     const bool less = norm > most && norm < (double)__builtin_huge_val();
     const float by = less ? (float)(most / norm) : 1.0f;
     const uint32_t chunks = list.first[list.count];
@@ -307,11 +320,17 @@ int run(const char *what, const void *const *grads, void *const *out, const int 
         ung_gradient_squares_kernel<<<blocks, NT, 0, st>>>(list, part + parts);
         parts += blocks;
     });
-    ung_gradient_join_kernel<<<1, NT, 0, st>>>(part, parts, whole, norm);
-    if (scale)
+    const bool joined = !scale || parts > SUMS || parts == 0;
+    if (joined)
+        ung_gradient_join_kernel<<<1, NT, 0, st>>>(part, parts, whole, norm);
+    if (scale) {
+        float *to_norm = joined ? nullptr : norm;
         rc = lists(grads, out, types, sizes, count, [&](const List &list, uint32_t blocks) {
-            ung_gradient_scale_kernel<<<blocks, NT, 0, st>>>(list, whole, (double)most);
+            ung_gradient_scale_kernel<<<blocks, NT, 0, st>>>(list, joined ? whole : part, joined ? 1 : parts, (double)most,
+                                                             to_norm);
+            to_norm = nullptr;
         });
+    }
     return launched(what);
 }
 

@@ -40,6 +40,11 @@ __device__ inline Vec<T> load_row(const T *row, uint64_t c, uint64_t cols)
     return v;
 }
 
+__device__ inline float scale_of(uint32_t most)
+{
+    return __uint_as_float(max(most, __float_as_uint(SMALLEST))) * (1.0f / LARGEST);
+}
+
 template <class T>
 __device__ inline uint32_t most_of(const Vec<T> &v, uint32_t most)
 {
@@ -94,7 +99,7 @@ __global__ __launch_bounds__(256) void ung_int8_rows_kernel(const T *x, uint64_t
         for (int o = 32; o > 0; o >>= 1)
             most = max(most, (uint32_t)__shfl_xor((int)most, o));
         const bool finite = most < 0x7F800000u;
-        const float s = __uint_as_float(max(most, __float_as_uint(SMALLEST))) * (1.0f / LARGEST);
+        const float s = scale_of(most);
         if (lane == 0)
             scale[row] = finite ? s : __uint_as_float(0x7FC00000u);
         const Divisor by(finite ? s : 1.0f);
@@ -193,6 +198,124 @@ struct Shares : Plainly {
     }
 };
 
+// COUNT rows from `first` to whole numbers in LDS, `pitch` bytes apart, and their scales; by one wave.
+template <int COUNT, class X>
+__device__ inline void rows_to_lds(const X *x, uint64_t stride, uint64_t cols, uint32_t kp, uint32_t first, uint32_t m,
+                                   uint8_t *to, uint32_t pitch, float *scales, uint32_t lane)
+{
+    constexpr uint64_t N = Vec<X>::N;
+    const X *from[COUNT];
+    uint32_t most[COUNT];
+    Vec<X> kept[COUNT]; // a row's first vector in each lane, which is all of a short one
+#pragma unroll
+    for (int e = 0; e < COUNT; ++e) {
+        from[e] = x + min(first + e, m - 1) * stride; // rows past the end repeat the last one
+        kept[e] = load_row(from[e], lane * N, cols);
+    }
+#pragma unroll
+    for (int e = 0; e < COUNT; ++e)
+        most[e] = most_of(kept[e], 0);
+    for (uint64_t c = (64 + lane) * N; c < cols; c += 64 * N)
+#pragma unroll
+        for (int e = 0; e < COUNT; ++e)
+            most[e] = most_of(load_row(from[e], c, cols), most[e]);
+    Divisor by[COUNT];
+    bool finite[COUNT];
+#pragma unroll
+    for (int e = 0; e < COUNT; ++e) {
+#pragma unroll
+        for (int o = 32; o > 0; o >>= 1)
+            most[e] = max(most[e], (uint32_t)__shfl_xor((int)most[e], o));
+        finite[e] = most[e] < 0x7F800000u;
+        const float s = scale_of(most[e]);
+        by[e] = Divisor(finite[e] ? s : 1.0f);
+        if (lane == 0)
+            scales[first + e] = finite[e] ? s : __uint_as_float(0x7FC00000u);
+    }
+    auto put = [&](int e, Vec<X> v, uint64_t c) {
+        if (!finite[e])
+            v.w[0] = v.w[1] = v.w[2] = v.w[3] = 0;
+        store_numbers(v, by[e], to + (first + e) * pitch + c);
+    };
+    if (lane * N < kp)
+#pragma unroll
+        for (int e = 0; e < COUNT; ++e)
+            put(e, kept[e], lane * N);
+    for (uint64_t c = (64 + lane) * N; c < kp; c += 64 * N)
+#pragma unroll
+        for (int e = 0; e < COUNT; ++e)
+            put(e, load_row(from[e], c, cols), c);
+}
+
+// Up to 16 TM rows x against many rows of b in whole numbers, in one launch.  The blocks stay: their four waves
+// bring x to whole numbers in LDS once, while their first chunks of b are under way, and then take 64
+// rows of b at a time, past LDS and without barriers.
+template <class X, int TM, class T>
+__global__ __launch_bounds__(256) void ung_int8_few_rows_kernel(const X *x, uint64_t cols, uint64_t stride, uint32_t m,
+                                                                Operand b, uint32_t strips, Scaled<T> finish)
+{
+    extern __shared__ uint8_t numbers[]; // [16 TM][kp + 16], and room to read three chunks past the end
+    __shared__ alignas(16) uint8_t turned[4 * turn_bytes(sizeof(T))];
+    __shared__ float scales[16 * TM];
+    Tile at = {};
+    at.high = 16 * TM;
+    at.strips = 1;
+    at.lane = threadIdx.x & 63;
+    at.wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const uint32_t kp = (uint32_t)b.k, pitch = kp + 16, chunks = kp / CHUNK;
+    uint32_t strip = blockIdx.x * 4 + at.wave;
+    Stream<int8_t> right;
+    u32x4 y[2][2][2][4]; // two chunks and the two after them
+    auto load = [&](int set) {
+        right.load(y[set][0]);
+        right.load(y[set][1]);
+        __builtin_amdgcn_sched_barrier(0); // not where their registers are needed next
+    };
+    auto begin = [&]() {
+        right.begin(b, (uint64_t)strip * 64, at.lane);
+        load(0);
+    };
+    if (strip < strips)
+        begin();
+    if (m <= 4) {
+        if (at.wave < m)
+            rows_to_lds<1>(x, stride, cols, kp, at.wave, m, numbers, pitch, scales, at.lane);
+    } else if (at.wave * 4 * TM < m)
+        rows_to_lds<4 * TM>(x, stride, cols, kp, at.wave * 4 * TM, m, numbers, pitch, scales, at.lane);
+    __syncthreads();
+    finish.a_scale = scales;
+    const uint8_t *rows = numbers + (at.lane & 15) * pitch + (at.lane >> 4) * 16;
+    for (; strip < strips; strip += gridDim.x * 4) {
+        i32x4 acc[TM][4];
+        finish.start(at, acc);
+        auto multiply = [&](int set, uint32_t kb) {
+#pragma unroll
+            for (int h = 0; h < 4; ++h)
+#pragma unroll
+                for (int i = 0; i < TM; ++i) {
+                    const u32x4 f = *reinterpret_cast<const u32x4 *>(rows + i * 16 * pitch + kb * CHUNK + h * 64);
+#pragma unroll
+                    for (int j = 0; j < 4; ++j)
+                        acc[i][j] = Matrix<int8_t>::mul(y[set][h / 2][h % 2][j], f, acc[i][j]);
+                }
+        };
+        // four chunks at a time, with one way out: chunks past the end are zeros of b, times whatever
+        // numbers lie after x's rows
+        for (uint32_t kb = 0; kb < chunks; kb += 4) {
+            load(1);
+            multiply(0, kb);
+            load(0);
+            multiply(1, kb + 2);
+        }
+        at.n0 = (uint64_t)strip * 64;
+        strip += gridDim.x * 4;
+        if (strip < strips)
+            begin();
+        strip -= gridDim.x * 4;
+        finish(at, nullptr, acc, turned);
+    }
+}
+
 template <class T>
 __global__ __launch_bounds__(256) void ung_int8_join_kernel(const int *part, uint32_t splits, uint64_t m, uint64_t n,
                                                             uint64_t stride, const float *a_scale, const float *b_scale,
@@ -270,22 +393,16 @@ int check_product(const char *what, uint64_t m, uint64_t n, uint64_t kp, int typ
     return UNG_HIP_OK;
 }
 
-} // namespace
 
-extern "C" {
+// ---- the calls' checks and launches ----------------------------------------------------------
 
-int ung_hip_int8_quantize(const void *x, int type, uint64_t rows, uint64_t cols, uint64_t row_stride, int8_t *q,
-                          float *scale, void *stream)
+int check_rows(const char *what, const void *x, int type, uint64_t rows, uint64_t cols, uint64_t row_stride)
 {
-    static const char what[] = "ung_hip_int8_quantize";
-    clear_error();
     if (!known_type(type)) {
         set_error("%s: unknown element type %d", what, type);
         return UNG_HIP_EINVAL;
     }
-    if (rows == 0)
-        return UNG_HIP_OK;
-    if ((cols && (!x || !q)) || !scale) {
+    if (rows && cols && !x) {
         set_error("%s: null argument", what);
         return UNG_HIP_EINVAL;
     }
@@ -298,17 +415,48 @@ int ung_hip_int8_quantize(const void *x, int type, uint64_t rows, uint64_t cols,
         set_error("%s: %llu x %llu elements are too many", what, (unsigned long long)rows, (unsigned long long)cols);
         return UNG_HIP_EINVAL;
     }
-    if ((uintptr_t)q % 16 || (uintptr_t)x % type_size(type) || (uintptr_t)scale % 4) {
-        set_error("%s: q needs 16-byte alignment, x and scale that of their elements", what);
+    return UNG_HIP_OK;
+}
+
+// The other side of a product and its results.
+int check_results(const char *what, const int8_t *b, const float *b_scale, uint64_t m, uint64_t n, uint64_t kp,
+                  const void *c, int type, uint64_t c_stride)
+{
+    if (!c || !b_scale || (kp && !b)) {
+        set_error("%s: null argument", what);
         return UNG_HIP_EINVAL;
     }
-    return with_type(type, [&](auto zero) {
+    if (m > 1 && c_stride < n) {
+        set_error("%s: c_stride %llu is less than %llu columns", what, (unsigned long long)c_stride,
+                  (unsigned long long)n);
+        return UNG_HIP_EINVAL;
+    }
+    if ((uintptr_t)b % 16 || (uintptr_t)b_scale % 4 || (uintptr_t)c % type_size(type)) {
+        set_error("%s: whole numbers need 16-byte alignment, the rest that of its elements", what);
+        return UNG_HIP_EINVAL;
+    }
+    return UNG_HIP_OK;
+}
+
+int check_workspace(const char *what, uint64_t needed, const void *workspace, uint64_t bytes)
+{
+    if (needed && (!workspace || bytes < needed || (uintptr_t)workspace % 16)) {
+        set_error("%s: needs %llu bytes of workspace at a 16-byte boundary (got %llu)", what, (unsigned long long)needed,
+                  (unsigned long long)(workspace ? bytes : 0));
+        return UNG_HIP_EINVAL;
+    }
+    return UNG_HIP_OK;
+}
+
+void quantize(const void *x, int type, uint64_t rows, uint64_t cols, uint64_t row_stride, int8_t *q, float *scale,
+              hipStream_t st)
+{
+    with_type(type, [&](auto zero) {
         using T = decltype(zero);
         const uint64_t chunks = ceil_div(cols, CHUNK), blocks = ceil_div(rows, 4), cp = chunks * CHUNK;
         const uint32_t grid = (uint32_t)(blocks < 8192 ? blocks : 8192);
         auto go = [&](auto kernel) {
-            kernel<<<grid, 256, 0, (hipStream_t)stream>>>((const T *)x, rows, cols, row_stride, chunks, (uint8_t *)q,
-                                                          scale);
+            kernel<<<grid, 256, 0, st>>>((const T *)x, rows, cols, row_stride, chunks, (uint8_t *)q, scale);
         };
         constexpr uint64_t once = 64 * Vec<T>::N; // elements of a vector for each lane
         if (cp <= once)
@@ -321,8 +469,93 @@ int ung_hip_int8_quantize(const void *x, int type, uint64_t rows, uint64_t cols,
             go(ung_int8_rows_kernel<T, 8>);
         else
             go(ung_int8_rows_kernel<T, 0>);
-        return launched(what);
+        return 0;
     });
+}
+
+bool vectors_at(const void *c, uint64_t c_stride, uint64_t m, uint64_t size)
+{
+    return (uintptr_t)c % 4 == 0 && (m == 1 || c_stride * size % 4 == 0);
+}
+
+void product(const int8_t *a, const float *a_scale, const int8_t *b, const float *b_scale, uint64_t m, uint64_t n,
+             uint64_t kp, void *c, int type, uint64_t c_stride, const Plan &plan, void *workspace, hipStream_t st)
+{
+    const Operand oa = {a, kp, m, kp}, ob = {b, kp, n, kp};
+    auto run = [&](auto finish) {
+        auto tiles = [&](auto high, auto wm, auto wn) {
+            constexpr int BM = decltype(high)::value, WM = decltype(wm)::value, WN = decltype(wn)::value;
+            const Grid grid = {(uint32_t)ceil_div(m, BM), (uint32_t)ceil_div(n, WN * 64), plan.splits, kp / CHUNK,
+                               plan.high == BIG ? 16u : 8u};
+            ung_tile_kernel<int8_t, BM, WM, WN, false, false>
+                <<<grid.m_tiles * grid.n_tiles * grid.splits, WM * WN * 64, 0, st>>>(oa, ob, grid, finish);
+        };
+        constexpr std::integral_constant<int, 1> one;
+        constexpr std::integral_constant<int, 2> two;
+        if (plan.high == 32)
+            tiles(std::integral_constant<int, 32>{}, one, two);
+        else if (plan.high == 64)
+            tiles(std::integral_constant<int, 64>{}, two, two);
+        else if (plan.high == 128)
+            tiles(std::integral_constant<int, 128>{}, two, two);
+        else
+            tiles(std::integral_constant<int, BIG>{}, two, std::integral_constant<int, 4>{});
+    };
+    with_type(type, [&](auto zero) {
+        using T = decltype(zero);
+        if (plan.splits == 1) {
+            run(Scaled<T>{{}, a_scale, b_scale, (T *)c, c_stride, m, n, vectors_at(c, c_stride, m, sizeof(T))});
+        } else {
+            const uint64_t stride = share_stride(n), blocks = ceil_div(m * (stride / 4), 256);
+            run(Shares{{}, (float *)workspace, stride, m, n});
+            ung_int8_join_kernel<T><<<(uint32_t)(blocks < 4096 ? blocks : 4096), 256, 0, st>>>(
+                (const int *)workspace, plan.splits, m, n, stride, a_scale, b_scale, (T *)c, c_stride);
+        }
+        return 0;
+    });
+}
+
+// How linear is made: few rows in one launch, or brought to whole numbers in the workspace first.
+struct Linear {
+    uint64_t kp, at_scale = 0, at_shares = 0, bytes = 0;
+    bool few;
+    Plan plan;
+    Linear(uint64_t m, uint64_t n, uint64_t cols) : kp(ceil_div(cols, CHUNK) * CHUNK)
+    {
+        // whole numbers of 16 or 32 rows, beside the waves' turned results, in 64 KB of LDS
+        few = m <= 32 && kp && (m <= 16 ? 16 : 32) * (kp + 16) + 3 * CHUNK <= 65536 - 16384 - 256;
+        plan = plan_of(m, n, kp);
+        if (few || !m || !n)
+            return;
+        at_scale = ceil_div(m * kp, 16) * 16;
+        at_shares = at_scale + ceil_div(m * 4, 16) * 16;
+        bytes = at_shares + share_bytes(m, n, plan.splits);
+    }
+};
+
+} // namespace
+
+extern "C" {
+
+int ung_hip_int8_quantize(const void *x, int type, uint64_t rows, uint64_t cols, uint64_t row_stride, int8_t *q,
+                          float *scale, void *stream)
+{
+    static const char what[] = "ung_hip_int8_quantize";
+    clear_error();
+    if (const int rc = check_rows(what, x, type, rows, cols, row_stride))
+        return rc;
+    if (rows == 0)
+        return UNG_HIP_OK;
+    if ((cols && !q) || !scale) {
+        set_error("%s: null argument", what);
+        return UNG_HIP_EINVAL;
+    }
+    if ((uintptr_t)q % 16 || (uintptr_t)x % type_size(type) || (uintptr_t)scale % 4) {
+        set_error("%s: q needs 16-byte alignment, x and scale that of their elements", what);
+        return UNG_HIP_EINVAL;
+    }
+    quantize(x, type, rows, cols, row_stride, q, scale, (hipStream_t)stream);
+    return launched(what);
 }
 
 int ung_hip_int8_matmul_workspace(uint64_t m, uint64_t n, uint64_t kp, int type, uint64_t *bytes)
@@ -349,60 +582,85 @@ int ung_hip_int8_matmul(const int8_t *a, const float *a_scale, const int8_t *b, 
         return rc;
     if (m == 0 || n == 0)
         return UNG_HIP_OK;
-    if (!c || !a_scale || !b_scale || (kp && (!a || !b))) {
+    if (!a_scale || (kp && !a)) {
         set_error("%s: null argument", what);
         return UNG_HIP_EINVAL;
     }
-    if (m > 1 && c_stride < n) {
-        set_error("%s: c_stride %llu is less than %llu columns", what, (unsigned long long)c_stride,
-                  (unsigned long long)n);
+    if ((uintptr_t)a % 16 || (uintptr_t)a_scale % 4) {
+        set_error("%s: whole numbers need 16-byte alignment, the rest that of its elements", what);
         return UNG_HIP_EINVAL;
     }
-    if ((uintptr_t)a % 16 || (uintptr_t)b % 16 || (uintptr_t)a_scale % 4 || (uintptr_t)b_scale % 4 ||
-        (uintptr_t)c % type_size(type)) {
-        set_error("%s: a and b need 16-byte alignment, the rest that of its elements", what);
-        return UNG_HIP_EINVAL;
-    }
+    if (const int rc = check_results(what, b, b_scale, m, n, kp, c, type, c_stride))
+        return rc;
     const Plan plan = plan_of(m, n, kp);
-    const uint64_t needed = share_bytes(m, n, plan.splits);
-    if (needed && (!workspace || workspace_bytes < needed || (uintptr_t)workspace % 16)) {
-        set_error("%s: needs %llu bytes of workspace at a 16-byte boundary (got %llu)", what, (unsigned long long)needed,
-                  (unsigned long long)(workspace ? workspace_bytes : 0));
+    if (const int rc = check_workspace(what, share_bytes(m, n, plan.splits), workspace, workspace_bytes))
+        return rc;
+    product(a, a_scale, b, b_scale, m, n, kp, c, type, c_stride, plan, workspace, (hipStream_t)stream);
+    return launched(what);
+}
+
+int ung_hip_int8_linear_workspace(uint64_t rows, uint64_t cols, uint64_t n, int type, uint64_t *bytes)
+{
+    static const char what[] = "ung_hip_int8_linear_workspace";
+    clear_error();
+    if (!bytes) {
+        set_error("%s: null bytes", what);
         return UNG_HIP_EINVAL;
     }
+    if (const int rc = check_product(what, rows, n, ceil_div(cols, CHUNK) * CHUNK, type))
+        return rc;
+    *bytes = Linear(rows, n, cols).bytes;
+    return UNG_HIP_OK;
+}
+
+int ung_hip_int8_linear(const void *x, int type, uint64_t rows, uint64_t cols, uint64_t row_stride, const int8_t *b,
+                        const float *b_scale, uint64_t n, void *c, int c_type, uint64_t c_stride, void *workspace,
+                        uint64_t workspace_bytes, void *stream)
+{
+    static const char what[] = "ung_hip_int8_linear";
+    clear_error();
+    const uint64_t kp = ceil_div(cols, CHUNK) * CHUNK;
+    if (const int rc = check_product(what, rows, n, kp, c_type))
+        return rc;
+    if (const int rc = check_rows(what, x, type, rows, cols, row_stride))
+        return rc;
+    if (rows == 0 || n == 0)
+        return UNG_HIP_OK;
+    if ((uintptr_t)x % type_size(type)) {
+        set_error("%s: x needs to be aligned to its elements", what);
+        return UNG_HIP_EINVAL;
+    }
+    if (const int rc = check_results(what, b, b_scale, rows, n, kp, c, c_type, c_stride))
+        return rc;
+    const Linear how(rows, n, cols);
+    if (const int rc = check_workspace(what, how.bytes, workspace, workspace_bytes))
+        return rc;
     const hipStream_t st = (hipStream_t)stream;
-    const Operand oa = {a, kp, m, kp}, ob = {b, kp, n, kp};
-    auto run = [&](auto finish) {
-        auto tiles = [&](auto high, auto wm, auto wn) {
-            constexpr int BM = decltype(high)::value, WM = decltype(wm)::value, WN = decltype(wn)::value;
-            const Grid grid = {(uint32_t)ceil_div(m, BM), (uint32_t)ceil_div(n, WN * 64), plan.splits, kp / CHUNK,
-                               plan.high == BIG ? 16u : 8u};
-            ung_tile_kernel<int8_t, BM, WM, WN, false, false>
-                <<<grid.m_tiles * grid.n_tiles * grid.splits, WM * WN * 64, 0, st>>>(oa, ob, grid, finish);
-        };
-        constexpr std::integral_constant<int, 1> one;
-        constexpr std::integral_constant<int, 2> two;
-        if (plan.high == 32)
-            tiles(std::integral_constant<int, 32>{}, one, two);
-        else if (plan.high == 64)
-            tiles(std::integral_constant<int, 64>{}, two, two);
-        else if (plan.high == 128)
-            tiles(std::integral_constant<int, 128>{}, two, two);
-        else
-            tiles(std::integral_constant<int, BIG>{}, two, std::integral_constant<int, 4>{});
-    };
-    return with_type(type, [&](auto zero) {
-        using T = decltype(zero);
-        if (plan.splits == 1) {
-            const bool vectors = (uintptr_t)c % 4 == 0 && (m == 1 || c_stride * sizeof(T) % 4 == 0);
-            run(Scaled<T>{{}, a_scale, b_scale, (T *)c, c_stride, m, n, vectors});
-        } else {
-            const uint64_t stride = share_stride(n), blocks = ceil_div(m * (stride / 4), 256);
-            run(Shares{{}, (float *)workspace, stride, m, n});
-            ung_int8_join_kernel<T><<<(uint32_t)(blocks < 4096 ? blocks : 4096), 256, 0, st>>>(
-                (const int *)workspace, plan.splits, m, n, stride, a_scale, b_scale, (T *)c, c_stride);
-        }
+    if (!how.few) {
+        uint8_t *ws = (uint8_t *)workspace;
+        float *scale = (float *)(ws + how.at_scale);
+        quantize(x, type, rows, cols, row_stride, (int8_t *)ws, scale, st);
+        product((int8_t *)ws, scale, b, b_scale, rows, n, kp, c, c_type, c_stride, how.plan, ws + how.at_shares, st);
         return launched(what);
+    }
+    return with_type(type, [&](auto x_zero) {
+        using X = decltype(x_zero);
+        return with_type(c_type, [&](auto c_zero) {
+            using T = decltype(c_zero);
+            const Operand ob = {b, kp, n, kp};
+            const Scaled<T> finish = {{}, nullptr, b_scale, (T *)c, c_stride, rows, n,
+                                      vectors_at(c, c_stride, rows, sizeof(T))};
+            const uint32_t strips = (uint32_t)ceil_div(n, 64), blocks = (uint32_t)ceil_div(strips, 4), most = 2 * cu_count();
+            auto go = [&](auto kernel, uint32_t high) {
+                kernel<<<blocks < most ? blocks : most, 256, high * ((uint32_t)kp + 16) + 3 * CHUNK, st>>>(
+                    (const X *)x, cols, row_stride, (uint32_t)rows, ob, strips, finish);
+            };
+            if (rows <= 16)
+                go(ung_int8_few_rows_kernel<X, 1, T>, 16);
+            else
+                go(ung_int8_few_rows_kernel<X, 2, T>, 32);
+            return launched(what);
+        });
     });
 }
 

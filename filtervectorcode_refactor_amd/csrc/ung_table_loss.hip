@@ -370,67 +370,114 @@ struct Sums {
     }
 };
 
-template <class E>
+// The shares' sums in the gradient's type.  P threads add up every P-th share of four results, and are
+// joined in order (1 x 384 results of 256 shares by one thread each 18.6 us).
+template <class E, uint32_t P>
 __global__ __launch_bounds__(256) void ung_table_sum_kernel(const float *part, uint32_t splits, uint64_t rows,
                                                             uint64_t cols, uint64_t part_stride, const float *by, E *c,
                                                             uint64_t c_stride, Rest<E> rest)
 {
-    const uint64_t quads = (cols + 3) / 4;
+    constexpr uint32_t EACH = 256 / P; // quads of a block
+    __shared__ f32x4 red[P > 1 ? 256 : 1];
+    const uint64_t quads = (cols + 3) / 4, all = rows * quads;
+    const uint32_t in = threadIdx.x % EACH, which = threadIdx.x / EACH;
     const float scale = by ? by[0] : 1.0f;
-    for (uint64_t at = blockIdx.x * 256ull + threadIdx.x; at < rows * quads; at += gridDim.x * 256ull) {
-        const uint64_t row = at / quads, col = (at - row * quads) * 4;
+    for (uint64_t first = (uint64_t)blockIdx.x * EACH; first < all; first += (uint64_t)gridDim.x * EACH) {
+        const uint64_t at = min(first + in, all - 1), row = at / quads, col = (at - row * quads) * 4;
         f32x4 sum = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll 8
-        for (uint32_t s = 0; s < splits; ++s)
+        for (uint32_t s = which; s < splits; s += P)
             sum += *reinterpret_cast<const f32x4 *>(part + (s * rows + row) * part_stride + col);
-        float all[4] = {sum[0], sum[1], sum[2], sum[3]};
-        rest.add(row, col, cols, all);
+        if constexpr (P > 1) {
+            __syncthreads(); // the last round's sums are read
+            red[threadIdx.x] = sum;
+            __syncthreads();
+            if (which)
+                continue;
+#pragma unroll
+            for (uint32_t p = 1; p < P; ++p)
+                sum += red[p * EACH + in];
+        }
+        if (first + in >= all)
+            continue;
+        float out[4] = {sum[0], sum[1], sum[2], sum[3]};
+        rest.add(row, col, cols, out);
 #pragma unroll
         for (int e = 0; e < 4; ++e)
             if (col + e < cols)
-                c[row * c_stride + col + e] = from_float<E>(all[e] * scale);
+                c[row * c_stride + col + e] = from_float<E>(out[e] * scale);
     }
 }
 
 // ---- plan and workspace ------------------------------------------------------------------
 
 // How a product of m x n results is made: by tiles of `high` x `wide` in so many shares of the inner
-// length.
+// length, and about how long it takes.
 struct Shape {
     uint32_t high, wide, splits;
-    double score; // share of the chip's rate that the tiles' results are made at
+    double us;
 };
 
-// The tile with the best of three factors: its rate on a full chip (256 x 256 1.08, 128 x 128 1, of 64 and 32
-// rows 0.75 and 0.5), the share of it that lies in the product, and the share of the places that the items of
-// all rounds fill.  Measured both ways, us, bf16: 2048 x 32768 of 768 125 by 256, 137 by 128; 32768 x 768 of
-// 2048 141 and 131 (1.5 rounds, 3 whole ones); 14336 x 384 of 4096 64 by 128 rows, 67 by 64.
-// `shares`: sums may be made in shares of the inner length of at least `fewest` chunks.
+// The time of a chunk of a tile alone on its CU, or of each of the tiles there where they share its matrix
+// instructions, and of a tile's begin and end: weights by which the faster plan is chosen, not times to
+// be had.  Measured, us, bf16: 2048 x 32768 of 768 125 by 256 x 256, 137 by 128 x 128; 32768 x 768 of 2048
+// 141 and 131 (1.5 rounds, 3 whole ones); 14336 x 384 of 4096 64 by 128 rows, 67 by 64; float32: 500 x
+// 10001 of 100 24.4 by 128 rows, 19.6 by 64.
+struct Weight {
+    uint32_t high, wide, at_once; // tiles that fit a CU
+    double alone, shared, ends;
+};
+constexpr Weight WEIGHTS_16[] = {{BIG, BIG, 1, 1.75, 1.75, 5.0}, {128, 128, 2, 0.6, 0.52, 3.5}, {64, 128, 3, 0.55, 0.33, 3.0},
+                                 {32, 128, 3, 0.5, 0.25, 2.5}};
+constexpr Weight WEIGHTS_32[] = {{128, 128, 2, 2.0, 1.95, 4.0}, {64, 128, 3, 1.1, 0.98, 3.0}, {32, 128, 3, 2.2, 0.8, 2.5}};
+
+// `shares`: sums may be made in shares of the inner length, joined by a pass of their own.
 Shape shape_of(uint64_t m, uint64_t n, uint64_t k, int type, bool shares)
 {
     const uint64_t cus = cu_count(), chunks = ceil_div(k * type_size(type), CHUNK);
-    Shape best = {32, 128, 1, -1.0};
-    auto with = [&](uint32_t high, uint32_t wide, uint32_t at_once, uint64_t fewest, double rate) {
-        Shape s = {high, wide, 1, 0.0};
-        const uint64_t tiles = ceil_div(m, high) * ceil_div(n, wide), places = at_once * cus;
+    Shape best = {32, 128, 1, 1e30};
+    auto consider = [&](const Weight &w) {
+        const uint64_t tiles = ceil_div(m, w.high) * ceil_div(n, w.wide);
+        auto time = [&](uint64_t each, uint64_t steps) { // of a round with `each` tiles on a CU
+            const double step = w.alone > w.shared * (double)each ? w.alone : w.shared * (double)each;
+            return step * (double)steps + w.ends;
+        };
+        auto with = [&](uint64_t splits) {
+            const uint64_t items = tiles * splits, places = w.at_once * cus, rounds = items / places, rest = items % places;
+            const uint64_t steps = ceil_div(chunks, splits);
+            Shape s = {w.high, w.wide, (uint32_t)splits, (double)rounds * time(w.at_once, steps)};
+            if (rest)
+                s.us += time(ceil_div(rest, cus), steps);
+            if (splits > 1)
+                s.us += 3.0 + (double)splits * (double)m * (double)n * 8 / 4e6;
+            if (s.us < best.us)
+                best = s;
+        };
         if (!tiles)
             return;
-        if (shares) {
-            const uint64_t by_cu = places / tiles, by_k = chunks / fewest, most = by_cu < by_k ? by_cu : by_k;
-            s.splits = most > 1 ? (uint32_t)most : 1;
-        }
-        const uint64_t items = tiles * s.splits;
-        s.score = rate * (double)m * (double)n / ((double)(tiles * high) * wide) * (double)items /
-                  (double)(ceil_div(items, places) * places);
-        if (s.score > best.score)
-            best = s;
+        with(1);
+        if (shares)
+            for (uint64_t each = 1; each <= w.at_once; ++each) {
+                const uint64_t by_cu = each * cus / tiles, by_k = chunks / (w.high == BIG ? 8 : 2), most = by_cu < by_k ? by_cu : by_k;
+                if (most > 1)
+                    with(most);
+            }
     };
-    if (type != UNG_HIP_F32)
-        with(BIG, BIG, 1, 8, 1.08);
-    with(128, 128, 2, 8, 1.0);
-    with(64, 128, 3, 4, 0.75);
-    with(32, 128, 3, 4, 0.5);
+    if (type == UNG_HIP_F32)
+        for (const Weight &w : WEIGHTS_32)
+            consider(w);
+    else
+        for (const Weight &w : WEIGHTS_16)
+            consider(w);
     return best;
+}
+
+constexpr uint32_t FEW = 32; // rows that the table is streamed for
+
+// How scores are made.
+Shape scores_shape(uint64_t n, uint64_t v, uint64_t d, int type)
+{
+    return n <= FEW ? Shape{n <= 16 ? 16u : 32u, 64, 1, 0.0} : shape_of(n, v, d, type, false);
 }
 
 struct Inputs {
@@ -476,7 +523,7 @@ struct Forward {
         const uint64_t size = type_size(in.type);
         x = packed(l, in.x, in.x_stride, in.n, in.d, size, false);
         table = packed(l, in.table, in.table_stride, in.v, in.d, size, false);
-        shape = shape_of(in.n, in.v, in.d, in.type, false);
+        shape = scores_shape(in.n, in.v, in.d, in.type);
         tiles = ceil_div(in.v, shape.wide);
         parts = l.take(tiles * in.n * sizeof(Part));
         target = l.take(in.n * 4);
@@ -506,18 +553,18 @@ struct Backward {
         // of the least number of pieces and half as many again, the one whose dT fills its rounds best
         // (4096 x 100000 x 384: 5 of 20224 rows 1596 us, 7 of 14336 1702, 4 of 25088 1686)
         const uint64_t least = all ? ceil_div(all, fits) : 1;
-        pieces = least, piece = all;
-        double most = -1.0;
-        for (uint64_t p = least; p <= least + least / 2; ++p) {
-            const uint64_t rows_of_it = ceil_div(ceil_div(all, p), WHOLE) * WHOLE;
-            const double score = shape_of(rows_of_it, in.d, in.n, in.type, true).score;
-            if (score > most * 1.02)
-                most = score, piece = rows_of_it, pieces = p;
+        piece = all;
+        double best = 1e30;
+        for (uint64_t p = least; p <= least + least / 2 && least > 1; ++p) {
+            const uint64_t of_it = ceil_div(ceil_div(all, p), WHOLE) * WHOLE;
+            const double us = (double)p * shape_of(of_it, in.d, in.n, in.type, true).us;
+            if (us < best * 0.98)
+                best = us, piece = of_it;
         }
         pieces = all ? ceil_div(all, piece) : 1;
         sum_stride = ceil_div(in.d, WHOLE) * WHOLE;
         const uint64_t v = in.v < piece ? in.v : piece;
-        g_shape = shape_of(in.n, v, in.d, in.type, false);
+        g_shape = scores_shape(in.n, v, in.d, in.type);
         x_shape = shape_of(in.n, in.d, v, in.type, true);
         t_shape = shape_of(v, in.d, in.n, in.type, true);
         g = l.take(in.n * piece * size);
@@ -583,11 +630,29 @@ uint32_t some_blocks(uint64_t n) { return (uint32_t)(n < 1 ? 1 : n < 8192 ? n : 
 template <class E, bool A_ACROSS, bool B_ACROSS, class Finish>
 void product(const Operand &a, const Operand &b, Shape shape, const Finish &finish, hipStream_t st)
 {
+    if constexpr (!A_ACROSS && !B_ACROSS) {
+        if (shape.high <= FEW && shape.wide == 64) {
+            const uint32_t blocks = (uint32_t)ceil_div(b.rows, 64);
+            if (!blocks)
+                return;
+            if (shape.high == 16)
+                ung_few_rows_kernel<E, 1><<<blocks, 64, 0, st>>>(a, b, finish);
+            else
+                ung_few_rows_kernel<E, 2><<<blocks, 64, 0, st>>>(a, b, finish);
+            return;
+        }
+    }
     const Grid grid = {(uint32_t)ceil_div(a.rows, shape.high), (uint32_t)ceil_div(b.rows, shape.wide), shape.splits,
                        ceil_div(a.k * sizeof(E), CHUNK), shape.high == BIG ? 16u : 8u};
     const uint32_t items = grid.m_tiles * grid.n_tiles * grid.splits;
     if (!items)
         return;
+    if constexpr (A_ACROSS) {
+        if (shape.high == 128 && grid.chunks == 1) {
+            ung_one_chunk_kernel<E, A_ACROSS, B_ACROSS><<<items, 256, 0, st>>>(a, b, grid, finish);
+            return;
+        }
+    }
     constexpr std::integral_constant<int, 1> one;
     constexpr std::integral_constant<int, 2> two;
     auto tiles = [&](auto high, auto wm, auto wn) {
@@ -673,8 +738,11 @@ int ung_hip_table_loss_forward(const void *x, uint64_t x_stride, const void *tab
             ung_table_join_kernel<R><<<(uint32_t)ceil_div(rows, R), 256, 0, st>>>(parts, f.tiles, rows, table_rows, target,
                                                                               ids, without, c, loss, lse);
         };
-        if (rows < 16)
+        // threads enough for a row where there are few of them (16 rows of 1563 parts by one block 10 us more)
+        if (rows < 128)
             join(std::integral_constant<int, 1>{});
+        else if (rows < 2048)
+            join(std::integral_constant<int, 4>{});
         else
             join(std::integral_constant<int, 16>{});
         return launched(what);
@@ -729,6 +797,15 @@ int ung_hip_table_loss_backward(const void *x, uint64_t x_stride, const void *ta
         const Rest<E> none = {}, rest = sizeof(E) == 4 ? none : Rest<E>{row, (float *)(ws + f.rest), (const E *)t.p, t.stride / sizeof(E)};
         const Operand x_side = {a.p, a.stride, rows, cols};
         float *const x_sums = (float *)(ws + f.x_sums);
+        auto sum = [&](const float *sums, uint32_t splits, uint64_t n, E *to, uint64_t stride, const Rest<E> &more) {
+            const uint64_t quads = n * ceil_div(cols, 4);
+            if (splits >= 16 && quads < 65536)
+                ung_table_sum_kernel<E, 16><<<some_blocks(ceil_div(quads, 16)), 256, 0, st>>>(
+                    sums, splits, n, cols, f.sum_stride, back, to, stride, more);
+            else
+                ung_table_sum_kernel<E, 1><<<some_blocks(ceil_div(quads, 256)), 256, 0, st>>>(
+                    sums, splits, n, cols, f.sum_stride, back, to, stride, more);
+        };
         // Of piece p: its rows of the table, and its G
         auto length = [&](uint64_t p) { return std::min(table_rows - p * f.piece, f.piece); };
         auto table_of = [&](uint64_t p) {
@@ -765,14 +842,12 @@ int ung_hip_table_loss_backward(const void *x, uint64_t x_stride, const void *ta
                     E *to = (E *)dtable + p * f.piece * dtable_stride;
                     product<E, true, true>(across(g), across(x_side), f.t_shape,
                                            Sums<false>{(float *)(ws + f.t_sums), f.sum_stride, v}, st);
-                    ung_table_sum_kernel<E><<<some_blocks(ceil_div(v * ceil_div(cols, 4), 256)), 256, 0, st>>>(
-                        (const float *)(ws + f.t_sums), f.t_shape.splits, v, cols, f.sum_stride, back, to, dtable_stride, none);
+                    sum((const float *)(ws + f.t_sums), f.t_shape.splits, v, to, dtable_stride, none);
                 }
             }
         }
         if (dx && rows && (f.x_shape.splits > 1 || f.pieces > 1))
-            ung_table_sum_kernel<E><<<some_blocks(ceil_div(rows * ceil_div(cols, 4), 256)), 256, 0, st>>>(
-                x_sums, f.x_shape.splits, rows, cols, f.sum_stride, back, (E *)dx, dx_stride, rest);
+            sum(x_sums, f.x_shape.splits, rows, (E *)dx, dx_stride, rest);
         return launched(what);
     });
 }

@@ -195,6 +195,8 @@ struct Tile {
 };
 
 constexpr int BIG = 256; // rows and columns of the largest tile
+// LDS that a wave needs to turn 16 x 64 results of a size
+constexpr uint32_t turn_bytes(uint32_t size) { return 16 * 64 * size; }
 
 // A block of WM x WN waves makes a BM x (64 WN) tile, each wave BM / WM x 64 of it in 16 x 16
 // matrix instructions.  Both panels of a chunk are staged in LDS by loads that bypass the
@@ -208,7 +210,7 @@ constexpr int BIG = 256; // rows and columns of the largest tile
 // are then half a line of memory each.
 //   The panels lie in LDS variables of their own, and the loads are without branches: so the compiler
 // knows which loads a read of LDS depends on, and adds no wait of its own.
-template <class E, int BM, int WM, int WN, bool A_ACROSS, bool B_ACROSS, class Finish>
+template <class E, int BM, int WM, int WN, bool A_ACROSS, bool B_ACROSS, bool ONE, class Finish>
 __device__ inline void make_tile(const Operand &a, const Operand &b, const Grid &grid, uint32_t block,
                                  const Finish &finish, uint8_t *a_even, uint8_t *a_odd, uint8_t *b_even, uint8_t *b_odd,
                                  uint8_t *side)
@@ -258,7 +260,8 @@ __device__ inline void make_tile(const Operand &a, const Operand &b, const Grid 
         await_loads<0>(); // loads into LDS are counted as memory loads, which a barrier alone does not await
         __builtin_amdgcn_s_barrier(); // the panels have landed; every wave is done with the others
         __builtin_amdgcn_sched_barrier(0);
-        load(next_a, next_b);
+        if constexpr (!ONE)
+            load(next_a, next_b);
 #pragma unroll
         for (int half = 0; half < 2; ++half) {
             u32x4 y[4];
@@ -275,7 +278,9 @@ __device__ inline void make_tile(const Operand &a, const Operand &b, const Grid 
         }
         asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); // the panels are read
     };
-    if constexpr (PAIRS) {
+    if constexpr (ONE) {
+        step(a_even, b_even, nullptr, nullptr);
+    } else if constexpr (PAIRS) {
         for (uint32_t pairs = (kb_end - kb) / 2; pairs; --pairs) {
             step(a_even, b_even, a_odd, b_odd);
             step(a_odd, b_odd, a_even, b_even);
@@ -300,7 +305,125 @@ __global__ __launch_bounds__(WM * WN * 64, 2) void ung_tile_kernel(Operand a, Op
     constexpr uint32_t HIGH = BM * CHUNK, WIDE = WN * 64 * CHUNK;
     __shared__ alignas(16) uint8_t a_even[HIGH], a_odd[HIGH], b_even[WIDE], b_odd[WIDE];
     __shared__ alignas(16) uint8_t side[BM * Finish::AHEAD + 16];
-    make_tile<E, BM, WM, WN, A_ACROSS, B_ACROSS>(a, b, grid, blockIdx.x, finish, a_even, a_odd, b_even, b_odd, side);
+    make_tile<E, BM, WM, WN, A_ACROSS, B_ACROSS, false>(a, b, grid, blockIdx.x, finish, a_even, a_odd, b_even, b_odd, side);
+}
+
+// Products of one chunk, where the results' stores are what takes the time: half the LDS, so that four blocks
+// are on a CU at different places of a tile.  100000 x 384 results of 1 to 64 16-bit numbers 20 us, two
+// blocks to a CU 26.
+template <class E, bool A_ACROSS, bool B_ACROSS, class Finish>
+__global__ __launch_bounds__(256, 4) void ung_one_chunk_kernel(Operand a, Operand b, Grid grid, Finish finish)
+{
+    __shared__ alignas(16) uint8_t a_panel[128 * CHUNK], b_panel[128 * CHUNK];
+    __shared__ alignas(16) uint8_t side[128 * Finish::AHEAD + 16];
+    make_tile<E, 128, 2, 2, A_ACROSS, B_ACROSS, true>(a, b, grid, blockIdx.x, finish, a_panel, nullptr, b_panel, nullptr, side);
+}
+
+// ---- few rows against many ------------------------------------------------------------------
+
+// 64 rows of the n side, a wave's, straight to registers: nothing else reads them.
+template <class E>
+struct Stream {
+    const uint8_t *from;
+    int32_t left; // bytes of a row from here on
+    uint32_t offset[4], at;
+
+    __device__ inline void begin(const Operand &of, uint64_t row0, uint32_t lane)
+    {
+        const uint32_t r = lane & 15, last = (uint32_t)min(of.rows - row0, (uint64_t)64) - 1;
+        at = (lane >> 4) * 16;
+        from = (const uint8_t *)of.p + row0 * of.stride;
+        left = (int32_t)(of.k * sizeof(E));
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+            offset[j] = min((r >> 2) * 16 + j * 4 + (r & 3), last) * (uint32_t)of.stride + at;
+    }
+    // The next chunk, zeros past the end.
+    __device__ inline void load(u32x4 (&y)[2][4])
+    {
+        const __amdgpu_buffer_rsrc_t p = buffer_of(from, 0x7FFFFFFFu);
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                y[h][j] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(
+                                                        p, (int32_t)(at + h * 64) < left ? offset[j] + h * 64 : OUTSIDE, 0, 0));
+        from += CHUNK;
+        left -= CHUNK;
+    }
+};
+
+// A wave's own rows of the m side, up to 16 TM of them, read by every wave from memory (its caches).
+template <class E, int TM>
+struct Rows {
+    const uint8_t *from;
+    int32_t left;
+    uint32_t offset[TM], at;
+
+    __device__ inline void begin(const Operand &of, uint32_t lane)
+    {
+        at = (lane >> 4) * 16;
+        from = (const uint8_t *)of.p;
+        left = (int32_t)(of.k * sizeof(E));
+#pragma unroll
+        for (int i = 0; i < TM; ++i)
+            offset[i] = min(i * 16 + (lane & 15), (uint32_t)of.rows - 1) * (uint32_t)of.stride + at;
+    }
+    __device__ inline void load(u32x4 (&x)[2][TM])
+    {
+        const __amdgpu_buffer_rsrc_t p = buffer_of(from, 0x7FFFFFFFu);
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int i = 0; i < TM; ++i)
+                x[h][i] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(
+                                                        p, (int32_t)(at + h * 64) < left ? offset[i] + h * 64 : OUTSIDE, 0, 0));
+        from += CHUNK;
+        left -= CHUNK;
+    }
+};
+
+// Up to 16 TM rows of a against all of b, where reading b is what takes the time: a wave takes 64 rows of
+// b and no more, past LDS and without barriers, the next two chunks' loads under way while two are
+// multiplied.  Results as ung_tile_kernel's.
+template <class E, int TM, class Finish>
+__global__ __launch_bounds__(64) void ung_few_rows_kernel(Operand a, Operand b, Finish finish)
+{
+    __shared__ alignas(16) uint8_t own[turn_bytes(4)];
+    __shared__ alignas(16) uint8_t side[16 * TM * Finish::AHEAD + 16];
+    Tile at = {};
+    at.high = 16 * TM;
+    at.strips = 1;
+    at.lane = threadIdx.x;
+    at.n0 = (uint64_t)xcd_run(blockIdx.x, gridDim.x) * 64;
+    Stream<E> right;
+    Rows<E, TM> left;
+    right.begin(b, at.n0, at.lane);
+    left.begin(a, at.lane);
+    u32x4 y[2][2][4], x[2][2][TM];
+    right.load(y[0]);
+    left.load(x[0]);
+    finish.ahead(at, side);
+    typename Matrix<E>::Acc acc[TM][4];
+    finish.start(at, acc);
+    const uint32_t chunks = ((uint32_t)(b.k * sizeof(E)) + CHUNK - 1) / CHUNK;
+    auto step = [&](int now) {
+        right.load(y[now ^ 1]);
+        left.load(x[now ^ 1]);
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int i = 0; i < TM; ++i)
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                    acc[i][j] = Matrix<E>::mul(y[now][h][j], x[now][h][i], acc[i][j]);
+    };
+    for (uint32_t pairs = (chunks + 1) / 2; pairs; --pairs) { // (a last odd one with zeros)
+        step(0);
+        step(1);
+    }
+    __syncthreads();
+    finish(at, side, acc, own);
 }
 
 // A finish that needs nothing ahead, and sums that begin at 0.
@@ -324,7 +447,6 @@ struct Plainly {
 // `stride` elements apart, of which `rows` and `cols` are there.  16-bit vectors go out as they lie where
 // `vectors`; the others are turned in LDS first, so that a store's lanes write neighbouring elements.
 // `own`: turn_bytes of LDS of the wave's own; a block's are no more than its panel of the n side.
-constexpr uint32_t turn_bytes(uint32_t size) { return 16 * 64 * size; }
 template <class T>
 __device__ inline void store_rows(T *to, uint64_t stride, uint32_t rows, uint64_t cols, bool vectors,
                                   const Vec<T> (&o)[16 / Vec<T>::N], uint8_t *own, uint32_t lane)

@@ -25,6 +25,7 @@ results without a graph.  Scores may have any row stride; bfloat16, float16 and 
 from __future__ import annotations
 
 import ctypes as C
+from array import array
 
 import torch  # before libung_hip.so is loaded: one HIP runtime for both
 
@@ -307,15 +308,11 @@ def quantize_int8(x):
     number the quotient by it to the nearest, ties to even.  A row with an infinity or NaN gets
     the scale NaN and zeros."""
     kind, stride = _matrix("x", x)
-    with _On(x) as stream:
-        return _integers(x, kind, stride, _library(), stream)
-
-
-def _integers(x, kind, row_stride, lib, stream):
     n, d = x.shape
     q = torch.empty(n, _blocks(d) * BLOCK, dtype=torch.int8, device=x.device)
     scale = torch.empty(n, device=x.device)
-    check(lib.ung_hip_int8_quantize(x.data_ptr(), kind, n, d, row_stride, q.data_ptr(), scale.data_ptr(), stream))
+    with _On(x) as stream:
+        check(_library().ung_hip_int8_quantize(x.data_ptr(), kind, n, d, stride, q.data_ptr(), scale.data_ptr(), stream))
     return q, scale
 
 
@@ -341,17 +338,16 @@ def matmul_int8(a, a_scale, b, b_scale, dtype=torch.bfloat16):
         raise ValueError(f"dtype: float32, float16 or bfloat16 is needed, got {dtype}")
     if b_kp != kp:
         raise ValueError(f"a and b: rows of {kp} and {b_kp} bytes do not go together")
+    kind, lib = _TYPES[dtype], _library()
+    c = torch.empty(m, n, dtype=dtype, device=a.device)
     with _On(a) as stream:
-        return _integer_product(a, a_scale, b, b_scale, m, n, kp, dtype, _library(), stream)
-
-
-def _integer_product(a, a_scale, b, b_scale, m, n, kp, dtype, lib, stream):
-    kind, device = _TYPES[dtype], a.device
-    c = torch.empty(m, n, dtype=dtype, device=device)
-    keep, at, size = _workspace(lib.ung_hip_int8_matmul_workspace, m, n, kp, kind, device=device)
-    check(lib.ung_hip_int8_matmul(a.data_ptr(), a_scale.data_ptr(), b.data_ptr(), b_scale.data_ptr(), m, n, kp,
-                                  c.data_ptr(), kind, n, at, size, stream))
+        keep, at, size = _workspace(lib.ung_hip_int8_matmul_workspace, m, n, kp, kind, device=a.device)
+        check(lib.ung_hip_int8_matmul(a.data_ptr(), a_scale.data_ptr(), b.data_ptr(), b_scale.data_ptr(), m, n, kp,
+                                      c.data_ptr(), kind, n, at, size, stream))
     return c
+
+
+FEW_ROWS, FEW_LONG = 32, 1408  # rows that linear_int8 takes in one launch without a workspace
 
 
 def linear_int8(x, q, scale, dtype=torch.bfloat16):
@@ -366,8 +362,12 @@ def linear_int8(x, q, scale, dtype=torch.bfloat16):
     if _blocks(d) * BLOCK != kp:
         raise ValueError(f"x and q: rows of {d} and {kp} do not go together")
     lib = _library()
+    c = torch.empty(m, n, dtype=dtype, device=x.device)
     with _On(x) as stream:
-        c = _integer_product(*_integers(x, kind, stride, lib, stream), q, scale, m, n, kp, dtype, lib, stream)
+        keep, at, size = (None, None, 0) if m <= FEW_ROWS and d <= FEW_LONG else \
+            _workspace(lib.ung_hip_int8_linear_workspace, m, d, n, _TYPES[dtype], device=x.device)
+        check(lib.ung_hip_int8_linear(x.data_ptr(), kind, m, d, stride, q.data_ptr(), scale.data_ptr(), n, c.data_ptr(),
+                                      _TYPES[dtype], n, at, size, stream))
     if x.requires_grad and torch.is_grad_enabled():
         c, = _Underivable.apply("linear_int8 has no gradient: detach its result", x, c)
     return c
@@ -628,40 +628,53 @@ def _side_by_side(t):
     return True
 
 
-def _tensors(name, tensors):
-    tensors = list(tensors)
+def _checked(name, tensors):
+    """Why a list of tensors is refused."""
     for t in tensors:
         _on_gpu(name, t, tensors[0])
         if t.dtype not in _TYPES:
             raise ValueError(f"{name}: float32, float16 or bfloat16 is needed, got {t.dtype}")
         if not _side_by_side(t):
             raise ValueError(f"{name}: elements have to lie side by side, got strides {t.stride()} of {tuple(t.shape)}")
-    return tensors
 
 
-def _addresses(tensors):
-    return (C.c_void_p * len(tensors))(*[t.data_ptr() for t in tensors])
+def _addresses(name, tensors):
+    """(type codes, addresses) of tensors on one GPU whose elements lie side by side.  Many at a time:
+    a call for each tensor and property costs more than the kernels of small ones."""
+    try:
+        kinds = [_TYPES[t.dtype] for t in tensors]
+        fine = min(devices := set(map(torch.Tensor.get_device, tensors))) >= 0 and len(devices) == 1 and \
+            all(map(torch.Tensor.is_contiguous, tensors))
+    except (KeyError, TypeError, AttributeError):
+        fine = False
+    if not fine:
+        _checked(name, tensors)
+    return kinds, array("Q", map(torch.Tensor.data_ptr, tensors))
 
 
 def _gradient_list(grads):
-    grads = _tensors("grads", [g for g in grads if g is not None])
+    grads = [g for g in grads if g is not None]
     if not grads:
         raise ValueError("grads: at least one tensor is needed")
-    count = len(grads)
-    return (grads, _addresses(grads), (C.c_int * count)(*[_TYPES[g.dtype] for g in grads]),
-            (C.c_uint64 * count)(*[g.numel() for g in grads]))
+    kinds, at = _addresses("grads", grads)
+    return grads, kinds, at, array("i", kinds), array("Q", map(torch.Tensor.numel, grads))
+
+
+def _address_of(a):
+    return a.buffer_info()[0]
 
 
 def gradient_norm(grads):
     """The norm of all gradients together, a float32 tensor of no dimensions: the root of the sum
     of every element's square, made in 64 bits.  ``grads``: tensors on one GPU (None is skipped)
     of any types and shapes."""
-    grads, at, types, sizes = _gradient_list(grads)
-    norm = torch.empty((), device=grads[0].device)
+    grads, _, at, types, sizes = _gradient_list(grads)
+    norm, count, sizes_at = torch.empty((), device=grads[0].device), len(grads), _address_of(sizes)
     lib = _library()
     with _On(grads[0]) as stream:
-        keep, work, size = _workspace(lib.ung_hip_gradient_workspace, sizes, len(grads), device=norm.device)
-        check(lib.ung_hip_gradient_norm(at, types, sizes, len(grads), norm.data_ptr(), work, size, stream))
+        keep, work, size = _workspace(lib.ung_hip_gradient_workspace, sizes_at, count, device=norm.device)
+        check(lib.ung_hip_gradient_norm(_address_of(at), _address_of(types), sizes_at, count, norm.data_ptr(), work, size,
+                                        stream))
     if torch.is_grad_enabled():
         for g in grads:
             if g.requires_grad:
@@ -675,24 +688,28 @@ def clip_gradients(grads, max_norm, out=None):
     the same way.  Nothing waits for the norm.  Where it is infinite or NaN the gradients stay as
     they are, so that a program that asks later can leave the step out."""
     given = list(grads)
-    grads, at, types, sizes = _gradient_list(given)
-    written, to = grads, None
+    grads, kinds, at, types, sizes = _gradient_list(given)
+    written, to, to_at = grads, None, None
     if out is not None:
         out = list(out)
         if len(out) != len(given):
             raise ValueError(f"out: {len(given)} tensors are needed, got {len(out)}")
-        written = _tensors("out", [o for o, g in zip(out, given) if g is not None])
-        for o, g in zip(written, grads):
-            if o.dtype != g.dtype or o.shape != g.shape or o.stride() != g.stride() or o.device != g.device:
-                raise ValueError("out: the gradients' shapes, types and strides are needed")
-        to = _addresses(written)
-    if torch.is_grad_enabled() and any(t.requires_grad and not t.is_leaf for t in grads + written):
-        raise ValueError("grads: gradients that require a gradient themselves are clipped under torch.no_grad()")
-    norm = torch.empty((), device=grads[0].device)
+        written = [o for o, g in zip(out, given) if g is not None]
+        to_kinds, to = _addresses("out", written)
+        to_at = _address_of(to)
+        if kinds != to_kinds or list(map(torch.Tensor.size, written)) != list(map(torch.Tensor.size, grads)) or \
+                written[0].get_device() != grads[0].get_device() or \
+                not all(o.is_contiguous() and g.is_contiguous() or o.stride() == g.stride() for o, g in zip(written, grads)):
+            raise ValueError("out: the gradients' shapes, types and strides are needed")
+    if torch.is_grad_enabled():
+        for t in (*grads, *written):
+            if t.requires_grad and not t.is_leaf:
+                raise ValueError("grads: gradients that require a gradient themselves are clipped under torch.no_grad()")
+    norm, count, sizes_at = torch.empty((), device=grads[0].device), len(grads), _address_of(sizes)
     lib = _library()
     with _On(grads[0]) as stream:
-        keep, work, size = _workspace(lib.ung_hip_gradient_workspace, sizes, len(grads), device=norm.device)
-        check(lib.ung_hip_clip_gradients(at, to, types, sizes, len(grads), max_norm, norm.data_ptr(), work, size,
-                                         stream))
-    torch.autograd.graph.increment_version([t for t in written if not t.is_inference()])
+        keep, work, size = _workspace(lib.ung_hip_gradient_workspace, sizes_at, count, device=norm.device)
+        check(lib.ung_hip_clip_gradients(_address_of(at), to_at, _address_of(types), sizes_at, count, max_norm,
+                                         norm.data_ptr(), work, size, stream))
+    torch.autograd.graph.increment_version(written)
     return norm

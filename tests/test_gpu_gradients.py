@@ -212,3 +212,22 @@ def test_refusals():
     for call, words in bad:
         with pytest.raises(ValueError, match=words):
             call()
+
+
+def test_inference_tensors():
+    """Tensors of inference mode have no versions that autograd counts."""
+    with torch.inference_mode():
+        grads = _grads([100, 9000], "mixed")
+        before = [g.clone() for g in grads]
+        S.clip_gradients(grads, 0.5)
+        _check(grads, before, _norm(before), 0.5)
+
+
+def test_more_partial_sums_than_a_block_adds_up():
+    """Three lists of 64 tensors each: the partial sums are joined by a launch of their own."""
+    grads = _grads([9000 * 16] * 150, "bf16")
+    norm = S.gradient_norm(grads)
+    assert abs(float(norm) - _norm(grads)) <= _norm(grads) * (2.0 ** -24 + 2.0 ** -40)
+    out = [torch.empty_like(g) for g in grads]
+    assert torch.equal(S.clip_gradients(grads, 10.0, out=out), norm)
+    _check(out, grads, _norm(grads), 10.0)
