@@ -198,71 +198,27 @@ struct Shares : Plainly {
     }
 };
 
-// COUNT rows from `first` to whole numbers in LDS, `pitch` bytes apart, and their scales; by one wave.
-template <int COUNT, class X>
-__device__ inline void rows_to_lds(const X *x, uint64_t stride, uint64_t cols, uint32_t kp, uint32_t first, uint32_t m,
-                                   uint8_t *to, uint32_t pitch, float *scales, uint32_t lane)
-{
-    constexpr uint64_t N = Vec<X>::N;
-    const X *from[COUNT];
-    uint32_t most[COUNT];
-    Vec<X> kept[COUNT]; // a row's first vector in each lane, which is all of a short one
-#pragma unroll
-    for (int e = 0; e < COUNT; ++e) {
-        from[e] = x + min(first + e, m - 1) * stride; // rows past the end repeat the last one
-        kept[e] = load_row(from[e], lane * N, cols);
-    }
-#pragma unroll
-    for (int e = 0; e < COUNT; ++e)
-        most[e] = most_of(kept[e], 0);
-    for (uint64_t c = (64 + lane) * N; c < cols; c += 64 * N)
-#pragma unroll
-        for (int e = 0; e < COUNT; ++e)
-            most[e] = most_of(load_row(from[e], c, cols), most[e]);
-    Divisor by[COUNT];
-    bool finite[COUNT];
-#pragma unroll
-    for (int e = 0; e < COUNT; ++e) {
-#pragma unroll
-        for (int o = 32; o > 0; o >>= 1)
-            most[e] = max(most[e], (uint32_t)__shfl_xor((int)most[e], o));
-        finite[e] = most[e] < 0x7F800000u;
-        const float s = scale_of(most[e]);
-        by[e] = Divisor(finite[e] ? s : 1.0f);
-        if (lane == 0)
-            scales[first + e] = finite[e] ? s : __uint_as_float(0x7FC00000u);
-    }
-    auto put = [&](int e, Vec<X> v, uint64_t c) {
-        if (!finite[e])
-            v.w[0] = v.w[1] = v.w[2] = v.w[3] = 0;
-        store_numbers(v, by[e], to + (first + e) * pitch + c);
-    };
-    if (lane * N < kp)
-#pragma unroll
-        for (int e = 0; e < COUNT; ++e)
-            put(e, kept[e], lane * N);
-    for (uint64_t c = (64 + lane) * N; c < kp; c += 64 * N)
-#pragma unroll
-        for (int e = 0; e < COUNT; ++e)
-            put(e, load_row(from[e], c, cols), c);
-}
+// Up to FEW short rows x against many rows of b in whole numbers, in one launch.  The blocks stay: a wave
+// brings a row of x to whole numbers in LDS, while its first chunks of b are under way, and then
+// takes 64 rows of b at a time, past LDS and without barriers.  4 x 384 against 1000 rows 6.4 us, in two
+// launches 7.1; 100000 rows 10.6 and 11.9; 1000000 rows 94 and 87.  With longer rows the first step costs
+// more than the launch: 1 x 1536 against 1000 rows 14.7 and 9.8.
+constexpr uint32_t FEW = 4, FEW_LONG = 512, FEW_TABLE = 200000;
 
-// Up to 16 TM rows x against many rows of b in whole numbers, in one launch.  The blocks stay: their four waves
-// bring x to whole numbers in LDS once, while their first chunks of b are under way, and then take 64
-// rows of b at a time, past LDS and without barriers.
-template <class X, int TM, class T>
+template <class X, class T>
 __global__ __launch_bounds__(256) void ung_int8_few_rows_kernel(const X *x, uint64_t cols, uint64_t stride, uint32_t m,
                                                                 Operand b, uint32_t strips, Scaled<T> finish)
 {
-    extern __shared__ uint8_t numbers[]; // [16 TM][kp + 16], and room to read three chunks past the end
+    constexpr uint32_t PITCH = FEW_LONG + 16;
+    __shared__ alignas(16) uint8_t numbers[FEW * PITCH + 3 * CHUNK]; // (three chunks past the end are read)
     __shared__ alignas(16) uint8_t turned[4 * turn_bytes(sizeof(T))];
-    __shared__ float scales[16 * TM];
+    __shared__ float scales[FEW];
     Tile at = {};
-    at.high = 16 * TM;
+    at.high = 16;
     at.strips = 1;
     at.lane = threadIdx.x & 63;
     at.wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const uint32_t kp = (uint32_t)b.k, pitch = kp + 16, chunks = kp / CHUNK;
+    const uint32_t kp = (uint32_t)b.k, chunks = kp / CHUNK;
     uint32_t strip = blockIdx.x * 4 + at.wave;
     Stream<int8_t> right;
     u32x4 y[2][2][2][4]; // two chunks and the two after them
@@ -277,27 +233,47 @@ __global__ __launch_bounds__(256) void ung_int8_few_rows_kernel(const X *x, uint
     };
     if (strip < strips)
         begin();
-    if (m <= 4) {
-        if (at.wave < m)
-            rows_to_lds<1>(x, stride, cols, kp, at.wave, m, numbers, pitch, scales, at.lane);
-    } else if (at.wave * 4 * TM < m)
-        rows_to_lds<4 * TM>(x, stride, cols, kp, at.wave * 4 * TM, m, numbers, pitch, scales, at.lane);
+    if (at.wave < m) {
+        constexpr uint32_t N = Vec<X>::N, NV = FEW_LONG / (64 * N);
+        const X *from = x + at.wave * stride;
+        Vec<X> v[NV];
+        uint32_t most = 0;
+#pragma unroll
+        for (uint32_t i = 0; i < NV; ++i)
+            v[i] = load_row(from, (i * 64 + at.lane) * N, cols);
+#pragma unroll
+        for (uint32_t i = 0; i < NV; ++i)
+            most = most_of(v[i], most);
+#pragma unroll
+        for (int o = 32; o > 0; o >>= 1)
+            most = max(most, (uint32_t)__shfl_xor((int)most, o));
+        const bool finite = most < 0x7F800000u;
+        const float s = scale_of(most);
+        const Divisor by(finite ? s : 1.0f);
+        if (at.lane == 0)
+            scales[at.wave] = finite ? s : __uint_as_float(0x7FC00000u);
+#pragma unroll
+        for (uint32_t i = 0; i < NV; ++i) {
+            if (!finite)
+                v[i].w[0] = v[i].w[1] = v[i].w[2] = v[i].w[3] = 0;
+            store_numbers(v[i], by, numbers + at.wave * PITCH + (i * 64 + at.lane) * N);
+        }
+    }
     __syncthreads();
     finish.a_scale = scales;
-    const uint8_t *rows = numbers + (at.lane & 15) * pitch + (at.lane >> 4) * 16;
+    // lanes of rows past the last one take another's; their results are not stored
+    const uint8_t *row = numbers + (at.lane & (FEW - 1)) * PITCH + (at.lane >> 4) * 16;
     for (; strip < strips; strip += gridDim.x * 4) {
-        i32x4 acc[TM][4];
+        i32x4 acc[1][4];
         finish.start(at, acc);
         auto multiply = [&](int set, uint32_t kb) {
 #pragma unroll
-            for (int h = 0; h < 4; ++h)
+            for (int h = 0; h < 4; ++h) {
+                const u32x4 f = *reinterpret_cast<const u32x4 *>(row + kb * CHUNK + h * 64);
 #pragma unroll
-                for (int i = 0; i < TM; ++i) {
-                    const u32x4 f = *reinterpret_cast<const u32x4 *>(rows + i * 16 * pitch + kb * CHUNK + h * 64);
-#pragma unroll
-                    for (int j = 0; j < 4; ++j)
-                        acc[i][j] = Matrix<int8_t>::mul(y[set][h / 2][h % 2][j], f, acc[i][j]);
-                }
+                for (int j = 0; j < 4; ++j)
+                    acc[0][j] = Matrix<int8_t>::mul(y[set][h / 2][h % 2][j], f, acc[0][j]);
+            }
         };
         // four chunks at a time, with one way out: chunks past the end are zeros of b, times whatever
         // numbers lie after x's rows
@@ -308,10 +284,11 @@ __global__ __launch_bounds__(256) void ung_int8_few_rows_kernel(const X *x, uint
             multiply(1, kb + 2);
         }
         at.n0 = (uint64_t)strip * 64;
-        strip += gridDim.x * 4;
-        if (strip < strips)
+        if (strip + gridDim.x * 4 < strips) {
+            strip += gridDim.x * 4;
             begin();
-        strip -= gridDim.x * 4;
+            strip -= gridDim.x * 4;
+        }
         finish(at, nullptr, acc, turned);
     }
 }
@@ -515,15 +492,14 @@ void product(const int8_t *a, const float *a_scale, const int8_t *b, const float
     });
 }
 
-// How linear is made: few rows in one launch, or brought to whole numbers in the workspace first.
+// How linear is made: few short rows in one launch, or brought to whole numbers in the workspace first.
 struct Linear {
     uint64_t kp, at_scale = 0, at_shares = 0, bytes = 0;
     bool few;
     Plan plan;
     Linear(uint64_t m, uint64_t n, uint64_t cols) : kp(ceil_div(cols, CHUNK) * CHUNK)
     {
-        // whole numbers of 16 or 32 rows, beside the waves' turned results, in 64 KB of LDS
-        few = m <= 32 && kp && (m <= 16 ? 16 : 32) * (kp + 16) + 3 * CHUNK <= 65536 - 16384 - 256;
+        few = m <= FEW && kp && kp <= FEW_LONG && n <= FEW_TABLE;
         plan = plan_of(m, n, kp);
         if (few || !m || !n)
             return;
@@ -651,14 +627,8 @@ int ung_hip_int8_linear(const void *x, int type, uint64_t rows, uint64_t cols, u
             const Scaled<T> finish = {{}, nullptr, b_scale, (T *)c, c_stride, rows, n,
                                       vectors_at(c, c_stride, rows, sizeof(T))};
             const uint32_t strips = (uint32_t)ceil_div(n, 64), blocks = (uint32_t)ceil_div(strips, 4), most = 2 * cu_count();
-            auto go = [&](auto kernel, uint32_t high) {
-                kernel<<<blocks < most ? blocks : most, 256, high * ((uint32_t)kp + 16) + 3 * CHUNK, st>>>(
-                    (const X *)x, cols, row_stride, (uint32_t)rows, ob, strips, finish);
-            };
-            if (rows <= 16)
-                go(ung_int8_few_rows_kernel<X, 1, T>, 16);
-            else
-                go(ung_int8_few_rows_kernel<X, 2, T>, 32);
+            ung_int8_few_rows_kernel<X, T><<<blocks < most ? blocks : most, 256, 0, st>>>(
+                (const X *)x, cols, row_stride, (uint32_t)rows, ob, strips, finish);
             return launched(what);
         });
     });

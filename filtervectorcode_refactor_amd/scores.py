@@ -347,7 +347,7 @@ def matmul_int8(a, a_scale, b, b_scale, dtype=torch.bfloat16):
     return c
 
 
-FEW_ROWS, FEW_LONG = 32, 1408  # rows that linear_int8 takes in one launch without a workspace
+FEW_ROWS, FEW_LONG, FEW_TABLE = 4, 512, 200_000  # what linear_int8 takes in one launch, without a workspace
 
 
 def linear_int8(x, q, scale, dtype=torch.bfloat16):
@@ -364,7 +364,7 @@ def linear_int8(x, q, scale, dtype=torch.bfloat16):
     lib = _library()
     c = torch.empty(m, n, dtype=dtype, device=x.device)
     with _On(x) as stream:
-        keep, at, size = (None, None, 0) if m <= FEW_ROWS and d <= FEW_LONG else \
+        keep, at, size = (None, None, 0) if m <= FEW_ROWS and d <= FEW_LONG and n <= FEW_TABLE else \
             _workspace(lib.ung_hip_int8_linear_workspace, m, d, n, _TYPES[dtype], device=x.device)
         check(lib.ung_hip_int8_linear(x.data_ptr(), kind, m, d, stride, q.data_ptr(), scale.data_ptr(), n, c.data_ptr(),
                                       _TYPES[dtype], n, at, size, stream))

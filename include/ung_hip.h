@@ -376,8 +376,8 @@ int ung_hip_int8_matmul(const int8_t *a, const float *a_scale, const int8_t *b, 
                         uint64_t workspace_bytes, void *stream);
 
 /* The product with rows x brought to whole numbers on the way, as the two calls above do one after the
- * other; up to 32 rows in one launch where their numbers fit in LDS (16 rows of up to 2944 columns, 32
- * of up to 1408).  b [n x kp], kp = cols rounded up to a multiple of UNG_HIP_INT8_CHUNK. */
+ * other; up to 4 rows of up to 512 columns against up to 200000 in one launch.  b [n x kp], kp = cols
+ * rounded up to a multiple of UNG_HIP_INT8_CHUNK. */
 int ung_hip_int8_linear_workspace(uint64_t rows, uint64_t cols, uint64_t n, int type, uint64_t *bytes);
 int ung_hip_int8_linear(const void *x, int type, uint64_t rows, uint64_t cols, uint64_t row_stride, const int8_t *b,
                         const float *b_scale, uint64_t n, void *c, int c_type, uint64_t c_stride, void *workspace,

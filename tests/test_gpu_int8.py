@@ -251,3 +251,26 @@ def test_refusals():
     for call, words in bad:
         with pytest.raises(ValueError, match=words):
             call()
+
+
+@pytest.mark.parametrize("kind", list(TYPES))
+def test_few_rows_in_one_launch(kind):
+    """Up to 4 rows of up to 512 columns against up to 200000, and the first sizes past each bound, with
+    a spoilt row among them."""
+    g = torch.Generator(device="cuda").manual_seed(7)
+    q, scale = _operand(200_001, 512, 9)
+    for m, n, d in ((1, 1, 1), (4, 63, 130), (3, 65, 512), (2, 129, 127), (5, 300, 512), (4, 300, 513), (4, 200_000, 100),
+                    (4, 200_001, 100), (3, 130_000, 512), (4, 64, 129)):
+        kp = -(-d // 128) * 128
+        b = torch.zeros(n, kp, dtype=torch.int8, device="cuda")
+        b[:, :min(d, 512)] = q[:n, :min(d, 512)]
+        x = torch.randn(m, d + 1, device="cuda", generator=g).to(TYPES[kind])[:, 1:]
+        if m > 2:
+            x[1, d - 1] = math.nan
+        xq, xs = S.quantize_int8(x)
+        for dtype in TYPES.values():
+            got = S.linear_int8(x, b, scale[:n] * 2.0 ** -8, dtype=dtype)
+            want = _product(xq, xs, b, scale[:n] * 2.0 ** -8, dtype)
+            assert torch.equal(got.isnan(), want.isnan()) and torch.equal(got.nan_to_num(), want.nan_to_num()), (m, n, d)
+            if m > 2:
+                assert got[1].isnan().all() and not got[0].isnan().any()

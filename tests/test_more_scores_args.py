@@ -51,6 +51,34 @@ def test_int8_matmul():
     _refused(F.load().ung_hip_int8_matmul_workspace(4, 4, 128, 0, None), "null")
 
 
+def test_int8_linear():
+    lib = F.load()
+    f = lib.ung_hip_int8_linear
+    _refused(f(P, 9, 4, 4, 4, P, P, 4, P, 0, 4, None, 0, None), "type 9")
+    _refused(f(P, 0, 4, 4, 4, P, P, 4, P, 9, 4, None, 0, None), "type 9")
+    _refused(f(None, 0, 4, 4, 4, P, P, 4, P, 0, 4, None, 0, None), "null")
+    _refused(f(P, 0, 4, 4, 4, None, P, 4, P, 0, 4, None, 0, None), "null")
+    _refused(f(P, 0, 4, 4, 4, P, None, 4, P, 0, 4, None, 0, None), "null")
+    _refused(f(P, 0, 4, 4, 4, P, P, 4, None, 0, 4, None, 0, None), "null")
+    _refused(f(P, 0, 4, 4, 3, P, P, 4, P, 0, 4, None, 0, None), "row_stride 3")
+    _refused(f(P, 0, 4, 4, 4, P, P, 4, P, 0, 3, None, 0, None), "c_stride 3")
+    _refused(f(P + 2, 0, 4, 4, 4, P, P, 4, P, 0, 4, None, 0, None), "aligned")
+    _refused(f(P, 0, 4, 4, 4, P + 8, P, 4, P, 0, 4, None, 0, None), "alignment")
+    _refused(f(P, 0, 4, 130945, 130945, P, P, 4, P, 0, 4, None, 0, None), "131072")
+    _refused(f(P, 0, 1 << 33, 4, 4, P, P, 4, P, 0, 4, None, 0, None), "too large")
+    need = C.c_uint64()
+    # what scores.linear_int8 counts on: no workspace for few short rows, one past each bound
+    for rows, cols, n, none in ((S.FEW_ROWS, S.FEW_LONG, S.FEW_TABLE, True), (S.FEW_ROWS + 1, 4, 4, False),
+                                (1, S.FEW_LONG + 1, 4, False), (1, 4, S.FEW_TABLE + 1, False)):
+        assert lib.ung_hip_int8_linear_workspace(rows, cols, n, 0, C.byref(need)) == 0 and (need.value == 0) == none
+    assert lib.ung_hip_int8_linear_workspace(5, 4, 4, 0, C.byref(need)) == 0
+    _refused(f(P, 0, 5, 4, 4, P, P, 4, P, 0, 4, P, need.value - 1, None), "workspace")
+    _refused(f(P, 0, 5, 4, 4, P, P, 4, P, 0, 4, None, need.value, None), "workspace")
+    _refused(lib.ung_hip_int8_linear_workspace(5, 4, 4, 0, None), "null")
+    _refused(lib.ung_hip_int8_linear_workspace(5, 4, 4, 7, C.byref(need)), "type 7")
+    assert f(None, 0, 0, 4, 4, None, None, 4, None, 0, 4, None, 0, None) == 0
+
+
 def _sizes(type=0, n=4, v=8, d=4, xs=4, ts=4, x=P, t=P):
     return x, xs, t, ts, type, n, v, d
 
