@@ -582,7 +582,8 @@ int check_inputs(const char *what, const Inputs &in)
         set_error("%s: unknown element type %d", what, in.type);
         return UNG_HIP_EINVAL;
     }
-    if (in.n > INT32_MAX - 256 || in.v > INT32_MAX - 256 || in.d > (1u << 24) ||
+    // (rows of a packed copy have to stay below 2^23 bytes, and a launch's threads below 2^32)
+    if (in.n > (1u << 27) || in.v > INT32_MAX - 256 || in.d > (1u << 20) ||
         ceil_div(in.n, 32) * ceil_div(in.v, 128) > most_blocks(256) / 2 ||
         (in.n > in.v ? in.n : in.v) / 32 * ceil_div(in.d, 128) > most_blocks(256) / 2) {
         set_error("%s: %llu rows of %llu elements against a table of %llu are too many", what, (unsigned long long)in.n,

@@ -112,6 +112,13 @@ def test_larger_against_64_bits(n, v, d, kind):
     _check(x, t, ids, out, w, 0.5, kind)
 
 
+@pytest.mark.parametrize("kind", list(TYPES))
+@pytest.mark.parametrize("n,v,d", [(3, 5, 100_000), (300, 270, 40_001)])
+def test_long_rows(n, v, d, kind):
+    x, t, ids, out, w = _inputs(n, v, d, kind, seed=5)
+    _check(x, t, ids, out, w, 0.7, kind)
+
+
 @pytest.mark.parametrize("kind,n,v,d", [("bf16", 70_000, 2500, 16), ("fp32", 40_000, 1700, 8), ("bf16", 9000, 20_000, 72)])
 def test_table_in_pieces(kind, n, v, d):
     """More scores than a piece of G holds: dx is summed over pieces of the table."""

@@ -99,7 +99,8 @@ def test_table_loss():
         _refused(f(_sizes(type=3)), "type 3")
         _refused(f(_sizes(n=1 << 40)), "too many")
         _refused(f(_sizes(v=1 << 31)), "too many")
-        _refused(f(_sizes(d=1 << 25, xs=1 << 25, ts=1 << 25)), "too many")
+        _refused(f(_sizes(d=(1 << 20) + 1, xs=1 << 21, ts=1 << 21)), "too many")
+        _refused(f(_sizes(n=(1 << 27) + 1, v=0)), "too many")
         _refused(f(_sizes(n=1 << 24, v=1 << 24)), "too many")
         _refused(f(_sizes(xs=3)), "strides 3")
         _refused(f(_sizes(ts=3)), "and 3")
