@@ -472,6 +472,55 @@ Shape shape_of(uint64_t m, uint64_t n, uint64_t k, int type, bool shares)
     return best;
 }
 
+// dT and dX in one launch: the shape of dX, of whose height dT's tiles are too; us is 0 where two launches
+// are faster.  Each alone leaves a part of the chip idle in its last or only round, and the second waits
+// for the first's last tile.  The backward pass, us, by one launch and by two: 16 x 1000 of 64 bf16 12.5
+// and 15.6, 500 x 10001 of 100 float32 65 and 74, 2000 x 2000 of 768 bf16 55 and 72, 300 x 20000 of 512 bf16
+// 55 and 62.
+Shape together_of(uint64_t n, uint64_t v, uint64_t d, int type, double two_us)
+{
+    const uint64_t cus = cu_count();
+    const uint64_t x_chunks = ceil_div(v * type_size(type), CHUNK), t_chunks = ceil_div(n * type_size(type), CHUNK);
+    Shape best = {0, 128, 1, two_us + 2.0};
+    auto consider = [&](const Weight &w) {
+        const uint64_t x_tiles = ceil_div(n, w.high) * ceil_div(d, w.wide), t_tiles = ceil_div(v, w.high) * ceil_div(d, w.wide);
+        if (w.high == BIG || !x_tiles || !t_tiles)
+            return;
+        const double even = w.shared * (double)(x_tiles * x_chunks + t_tiles * t_chunks) / (double)cus;
+        // dX in shares that leave every CU with the same number of tiles; the first CUs have the more of dT's
+        const uint64_t of_t = ceil_div(t_tiles, cus);
+        for (uint64_t each = of_t; each <= of_t + w.at_once; ++each) {
+            const uint64_t splits = (each * cus - t_tiles) / x_tiles;
+            if (splits < 2 || splits * 2 > x_chunks || splits > 256)
+                continue;
+            const uint64_t steps = ceil_div(x_chunks, splits);
+            const double first = (double)(of_t * t_chunks + (each - of_t) * steps), longest = (double)std::max(steps, t_chunks);
+            const double busy = each <= w.at_once ? w.shared * first : even + w.shared * (double)steps;
+            const double us = std::max({even, busy, w.alone * longest}) + w.ends * (double)ceil_div(each, (uint64_t)w.at_once) +
+                              3.0 + (double)splits * (double)n * (double)d * 8 / 4e6;
+            if (us < best.us)
+                best = {w.high, w.wide, (uint32_t)splits, us};
+        }
+        // few tiles in all: dX in shares as long as one of dT's
+        const uint64_t splits = ceil_div(x_chunks, std::max<uint64_t>(t_chunks, 2));
+        if (splits >= 2 && splits <= 256 && t_tiles + x_tiles * splits <= cus) {
+            const double us = w.alone * (double)std::max<uint64_t>(t_chunks, 2) + w.ends + 3.0 +
+                              (double)splits * (double)n * (double)d * 8 / 4e6;
+            if (us < best.us)
+                best = {w.high, w.wide, (uint32_t)splits, us};
+        }
+    };
+    if (type == UNG_HIP_F32)
+        for (const Weight &w : WEIGHTS_32)
+            consider(w);
+    else
+        for (const Weight &w : WEIGHTS_16)
+            consider(w);
+    if (!best.high)
+        best.us = 0.0;
+    return best;
+}
+
 constexpr uint32_t FEW = 32; // rows that the table is streamed for
 
 // How scores are made.
@@ -539,6 +588,7 @@ struct Backward {
     Packed x, table;
     uint64_t rows, scale, rest, piece, pieces, g, x_sums, t_sums, sum_stride;
     Shape g_shape, x_shape, t_shape;
+    bool together = false; // dX and dT in one launch (where both are asked for)
     explicit Backward(const Inputs &in)
     {
         const uint64_t size = type_size(in.type);
@@ -567,6 +617,12 @@ struct Backward {
         g_shape = scores_shape(in.n, v, in.d, in.type);
         x_shape = shape_of(in.n, in.d, v, in.type, true);
         t_shape = shape_of(v, in.d, in.n, in.type, true);
+        if (pieces == 1) {
+            const Shape both = together_of(in.n, v, in.d, in.type, x_shape.us + t_shape.us);
+            together = both.us > 0.0;
+            if (together)
+                x_shape = both, t_shape = {both.high, both.wide, 1, 0.0};
+        }
         g = l.take(in.n * piece * size);
         x_sums = t_sums = 0;
         if (x_shape.splits > 1 || pieces > 1)
@@ -627,6 +683,14 @@ int check_call(const char *what, const Inputs &in, const int32_t *ids, const int
 
 uint32_t some_blocks(uint64_t n) { return (uint32_t)(n < 1 ? 1 : n < 8192 ? n : 8192); }
 
+Grid grid_of(const Operand &a, const Operand &b, Shape shape, uint64_t size)
+{
+    return {(uint32_t)ceil_div(a.rows, shape.high), (uint32_t)ceil_div(b.rows, shape.wide), shape.splits,
+            ceil_div(a.k * size, CHUNK), shape.high == BIG ? 16u : 8u};
+}
+
+uint32_t items_of(const Grid &g) { return g.m_tiles * g.n_tiles * g.splits; }
+
 // The product of two sides, its tiles finished by `finish`.
 template <class E, bool A_ACROSS, bool B_ACROSS, class Finish>
 void product(const Operand &a, const Operand &b, Shape shape, const Finish &finish, hipStream_t st)
@@ -643,9 +707,8 @@ void product(const Operand &a, const Operand &b, Shape shape, const Finish &fini
             return;
         }
     }
-    const Grid grid = {(uint32_t)ceil_div(a.rows, shape.high), (uint32_t)ceil_div(b.rows, shape.wide), shape.splits,
-                       ceil_div(a.k * sizeof(E), CHUNK), shape.high == BIG ? 16u : 8u};
-    const uint32_t items = grid.m_tiles * grid.n_tiles * grid.splits;
+    const Grid grid = grid_of(a, b, shape, sizeof(E));
+    const uint32_t items = items_of(grid);
     if (!items)
         return;
     if constexpr (A_ACROSS) {
@@ -668,6 +731,24 @@ void product(const Operand &a, const Operand &b, Shape shape, const Finish &fini
         tiles(std::integral_constant<int, 128>{}, two, two);
     else if constexpr (sizeof(E) == 2)
         tiles(std::integral_constant<int, BIG>{}, two, std::integral_constant<int, 4>{});
+}
+
+// dT of G and X, and dX of G and the table, by one launch.
+template <class E>
+void both_products(const Operand &gt, const Operand &x, Shape t_shape, const Whole<E> &whole, const Operand &g,
+                   const Operand &table, Shape x_shape, const Sums<false> &sums, hipStream_t st)
+{
+    const Grid t_grid = grid_of(gt, x, t_shape, sizeof(E)), x_grid = grid_of(g, table, x_shape, sizeof(E));
+    const uint32_t items = items_of(t_grid) + items_of(x_grid);
+    if (x_shape.high == 32)
+        ung_two_products_kernel<E, 32, 1, 2, true, true, false, true>
+            <<<items, 128, 0, st>>>(gt, x, t_grid, whole, g, table, x_grid, sums);
+    else if (x_shape.high == 64)
+        ung_two_products_kernel<E, 64, 2, 2, true, true, false, true>
+            <<<items, 256, 0, st>>>(gt, x, t_grid, whole, g, table, x_grid, sums);
+    else
+        ung_two_products_kernel<E, 128, 2, 2, true, true, false, true>
+            <<<items, 256, 0, st>>>(gt, x, t_grid, whole, g, table, x_grid, sums);
 }
 
 template <class E>
@@ -825,6 +906,11 @@ int ung_hip_table_loss_backward(const void *x, uint64_t x_stride, const void *ta
             const uint64_t v = length(p);
             const Operand part = table_of(p), g = g_of(p);
             product<E, false, false>(x_side, part, f.g_shape, weights(p), st);
+            if (f.together && dx && dtable) {
+                both_products<E>(across(g), across(x_side), f.t_shape, whole(p), g, across(part), f.x_shape,
+                                 Sums<false>{x_sums, f.sum_stride, rows}, st);
+                break;
+            }
             if (dx && rows) {
                 if (f.x_shape.splits == 1 && f.pieces == 1)
                     product<E, false, true>(g, across(part), f.x_shape,

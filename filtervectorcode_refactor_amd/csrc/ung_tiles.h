@@ -308,6 +308,26 @@ __global__ __launch_bounds__(WM * WN * 64, 2) void ung_tile_kernel(Operand a, Op
     make_tile<E, BM, WM, WN, A_ACROSS, B_ACROSS, false>(a, b, grid, blockIdx.x, finish, a_even, a_odd, b_even, b_odd, side);
 }
 
+// Two products in one launch, the first's tiles before the second's, for two that do not need each other
+// and do not fill the chip's rounds by themselves.
+template <class E, int BM, int WM, int WN, bool A_ACROSS, bool B_ACROSS, bool A2_ACROSS, bool B2_ACROSS, class Finish,
+          class Finish2>
+__global__ __launch_bounds__(WM * WN * 64, 2) void ung_two_products_kernel(Operand a, Operand b, Grid grid, Finish finish,
+                                                                         Operand a2, Operand b2, Grid grid2,
+                                                                         Finish2 finish2)
+{
+    constexpr uint32_t HIGH = BM * CHUNK, WIDE = WN * 64 * CHUNK;
+    constexpr uint32_t AHEAD = Finish::AHEAD > Finish2::AHEAD ? Finish::AHEAD : Finish2::AHEAD;
+    __shared__ alignas(16) uint8_t a_even[HIGH], a_odd[HIGH], b_even[WIDE], b_odd[WIDE];
+    __shared__ alignas(16) uint8_t side[BM * AHEAD + 16];
+    const uint32_t first = grid.m_tiles * grid.n_tiles * grid.splits;
+    if (blockIdx.x < first)
+        make_tile<E, BM, WM, WN, A_ACROSS, B_ACROSS, false>(a, b, grid, blockIdx.x, finish, a_even, a_odd, b_even, b_odd, side);
+    else
+        make_tile<E, BM, WM, WN, A2_ACROSS, B2_ACROSS, false>(a2, b2, grid2, blockIdx.x - first, finish2, a_even, a_odd,
+                                                              b_even, b_odd, side);
+}
+
 // Products of one chunk, where the results' stores are what takes the time: half the LDS, so that four blocks
 // are on a CU at different places of a tile.  100000 x 384 results of 1 to 64 16-bit numbers 20 us, two
 // blocks to a CU 26.

@@ -252,6 +252,19 @@ def test_weights_none_and_one_gradient_alone():
         assert S.table_loss_backward(None, x, t, ids, lse, need=(False, False)) == (None, None)
 
 
+@pytest.mark.parametrize("kind", list(TYPES))
+@pytest.mark.parametrize("n,v,d", [(16, 1000, 64), (100, 3000, 256), (300, 20_000, 130), (500, 10_001, 100), (2000, 2000, 600),
+                                   (2000, 40, 24), (40, 2001, 1000), (1000, 5000, 384)])
+def test_both_gradients_are_each_ones(n, v, d, kind):
+    """By one launch or by two, sums are made in the same order."""
+    x, t, ids, out, w = _inputs(n, v, d, kind)
+    dx, dt = _check(x, t, ids, out, w, 0.5, kind)[2:]
+    _, lse = S.table_loss_forward(x, t, ids, without=out, temperature=0.5)
+    need = dict(without=out, temperature=0.5)
+    assert torch.equal(S.table_loss_backward(w, x, t, ids, lse, need=(True, False), **need)[0], dx)
+    assert torch.equal(S.table_loss_backward(w, x, t, ids, lse, need=(False, True), **need)[1], dt)
+
+
 @pytest.mark.parametrize("of", ["x", "table"])
 def test_against_differences(of):
     """Along a random direction u of length 1: (f(+h) - f(-h)) / 2h of f = sum(w loss) in 32 bits.  The
