@@ -139,6 +139,21 @@ __device__ inline void store_loose(T *p, const Vec<T> &v)
     __builtin_memcpy(p, &v, sizeof v);
 }
 
+// N consecutive elements of a row from column c; those at or past `cols` are 0.
+template <class T>
+__device__ inline Vec<T> load_row(const T *row, uint64_t c, uint64_t cols)
+{
+    Vec<T> v;
+    if (c + Vec<T>::N <= cols)
+        return load_loose(row + c);
+    v.w[0] = v.w[1] = v.w[2] = v.w[3] = 0;
+#pragma unroll
+    for (int e = 0; e < Vec<T>::N; ++e)
+        if (c + e < cols)
+            v.set(e, row[c + e]);
+    return v;
+}
+
 // Largest magnitude as the bits of its absolute value: whole numbers order like the
 // magnitudes, and a NaN is above every one of them, so it reaches the scale.
 __device__ inline uint32_t magnitude(float x) { return __float_as_uint(x) & 0x7FFFFFFFu; }

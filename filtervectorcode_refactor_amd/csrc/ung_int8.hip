@@ -25,21 +25,6 @@ static_assert((uint64_t)UNG_HIP_INT8_LONGEST * 128 * 128 < 1ull << 31 && UNG_HIP
 
 // ---- quantisation --------------------------------------------------------------------
 
-// N consecutive elements of a row from column c; those at or past `cols` are 0.
-template <class T>
-__device__ inline Vec<T> load_row(const T *row, uint64_t c, uint64_t cols)
-{
-    Vec<T> v;
-    if (c + Vec<T>::N <= cols)
-        return load_loose(row + c);
-    v.w[0] = v.w[1] = v.w[2] = v.w[3] = 0;
-#pragma unroll
-    for (int e = 0; e < Vec<T>::N; ++e)
-        if (c + e < cols)
-            v.set(e, row[c + e]);
-    return v;
-}
-
 __device__ inline float scale_of(uint32_t most)
 {
     return __uint_as_float(max(most, __float_as_uint(SMALLEST))) * (1.0f / LARGEST);

@@ -403,10 +403,78 @@ struct Rows {
     }
 };
 
+// The same of rows that are aligned to their elements alone, and end anywhere: the chunk that a row's end
+// is in comes first (zeros past the end), then the whole ones, by loads that are in range without a check.
+// Loads off 4-byte boundaries are slow (100000 x 384 bf16 at an odd stride 47 us): 16-bit rows are loaded
+// from the boundary before, a word more of them, and shifted when they are used.
+template <class E, int ROWS>
+struct Loose {
+    static constexpr bool HALVES = sizeof(E) == 2;
+    struct Words {
+        u32x4 w;
+        uint32_t next; // (16-bit rows alone)
+    };
+    using Chunk = Words[2][ROWS];
+    const uint8_t *from;
+    uint32_t left; // whole chunks
+    uint32_t offset[ROWS], shift[ROWS];
+
+    // place(i): the lane's i-th row.  `end`: the chunk of the row's end.
+    template <class Place>
+    __device__ inline void begin(const Operand &of, uint64_t row0, uint32_t lane, u32x4 (&end)[2][ROWS], const Place &place)
+    {
+        const uint32_t last = (uint32_t)min(of.rows - row0, (uint64_t)64) - 1, at = (lane >> 4) * 16;
+        from = (const uint8_t *)of.p + row0 * of.stride;
+        const uint32_t off = (uint32_t)(uintptr_t)from & 3;
+        left = (uint32_t)(of.k * sizeof(E)) / CHUNK;
+#pragma unroll
+        for (int i = 0; i < ROWS; ++i) {
+            const uint32_t row = min(place(i), last) * (uint32_t)of.stride;
+            offset[i] = row + at + off;
+            shift[i] = offset[i] & 3;
+            offset[i] -= shift[i];
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+                end[h][i] = __builtin_bit_cast(u32x4, load_row((const E *)(from + row), (left * CHUNK + h * 64 + at) / sizeof(E), of.k));
+        }
+        from -= off;
+    }
+    // The next whole chunk, or the last again.
+    __device__ inline void load(Chunk &y)
+    {
+        if (!left)
+            return;
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int i = 0; i < ROWS; ++i) {
+                const uint32_t *p = reinterpret_cast<const uint32_t *>(from + offset[i] + h * 64);
+                __builtin_memcpy(&y[h][i].w, p, 16);
+                if constexpr (HALVES) // (the word that holds the last element)
+                    y[h][i].next = p[shift[i] ? 4 : 3];
+            }
+        if (--left)
+            from += CHUNK;
+        else
+            left = 1;
+    }
+    __device__ inline u32x4 of(const Words &y, int i) const
+    {
+        if constexpr (!HALVES)
+            return y.w;
+        else
+            return u32x4{__builtin_amdgcn_alignbyte(y.w[1], y.w[0], shift[i]), __builtin_amdgcn_alignbyte(y.w[2], y.w[1], shift[i]),
+                         __builtin_amdgcn_alignbyte(y.w[3], y.w[2], shift[i]),
+                         __builtin_amdgcn_alignbyte(y.next, y.w[3], shift[i])};
+    }
+};
+
 // Up to 16 TM rows of a against all of b, where reading b is what takes the time: a wave takes 64 rows of
 // b and no more, past LDS and without barriers, the next two chunks' loads under way while two are
-// multiplied.  Results as ung_tile_kernel's.
-template <class E, int TM, class Finish>
+// multiplied.  Results as ung_tile_kernel's.  LOOSE: rows need no alignment (100000 x 384 bf16 at an odd
+// stride 25.6 us, copied to rows of whole vectors first 51.5; at whole vectors 19.7 as they are.  float32
+// 36, 95 and 32; 100000 x 100 bf16 13, 26, and 9 where they are 104).
+template <class E, int TM, bool LOOSE, class Finish>
 __global__ __launch_bounds__(64) void ung_few_rows_kernel(Operand a, Operand b, Finish finish)
 {
     __shared__ alignas(16) uint8_t own[turn_bytes(4)];
@@ -416,31 +484,60 @@ __global__ __launch_bounds__(64) void ung_few_rows_kernel(Operand a, Operand b, 
     at.strips = 1;
     at.lane = threadIdx.x;
     at.n0 = (uint64_t)xcd_run(blockIdx.x, gridDim.x) * 64;
-    Stream<E> right;
-    Rows<E, TM> left;
-    right.begin(b, at.n0, at.lane);
-    left.begin(a, at.lane);
-    u32x4 y[2][2][4], x[2][2][TM];
-    right.load(y[0]);
-    left.load(x[0]);
-    finish.ahead(at, side);
     typename Matrix<E>::Acc acc[TM][4];
-    finish.start(at, acc);
-    const uint32_t chunks = ((uint32_t)(b.k * sizeof(E)) + CHUNK - 1) / CHUNK;
-    auto step = [&](int now) {
-        right.load(y[now ^ 1]);
-        left.load(x[now ^ 1]);
+    auto multiply = [&](const auto &y, const auto &x) {
 #pragma unroll
         for (int h = 0; h < 2; ++h)
 #pragma unroll
             for (int i = 0; i < TM; ++i)
 #pragma unroll
                 for (int j = 0; j < 4; ++j)
-                    acc[i][j] = Matrix<E>::mul(y[now][h][j], x[now][h][i], acc[i][j]);
+                    acc[i][j] = Matrix<E>::mul(y(h, j), x(h, i), acc[i][j]);
     };
-    for (uint32_t pairs = (chunks + 1) / 2; pairs; --pairs) { // (a last odd one with zeros)
-        step(0);
-        step(1);
+    const uint32_t bytes = (uint32_t)(b.k * sizeof(E)), r = at.lane & 15;
+    if constexpr (LOOSE) {
+        Loose<E, 4> right;
+        Loose<E, TM> left;
+        typename Loose<E, 4>::Chunk y[2];
+        typename Loose<E, TM>::Chunk x[2];
+        u32x4 y_end[2][4], x_end[2][TM];
+        right.begin(b, at.n0, at.lane, y_end, [&](int j) { return (r >> 2) * 16 + j * 4 + (r & 3); });
+        left.begin(a, 0, at.lane, x_end, [&](int i) { return i * 16 + r; });
+        right.load(y[0]);
+        left.load(x[0]);
+        finish.ahead(at, side);
+        finish.start(at, acc);
+        multiply([&](int h, int j) { return y_end[h][j]; }, [&](int h, int i) { return x_end[h][i]; });
+        auto step = [&](int now) {
+            right.load(y[now ^ 1]);
+            left.load(x[now ^ 1]);
+            multiply([&](int h, int j) { return right.of(y[now][h][j], j); }, [&](int h, int i) { return left.of(x[now][h][i], i); });
+        };
+        for (uint32_t chunks = bytes / CHUNK; chunks; --chunks) {
+            step(0);
+            if (!--chunks)
+                break;
+            step(1);
+        }
+    } else {
+        u32x4 y[2][2][4], x[2][2][TM];
+        Stream<E> right;
+        Rows<E, TM> left;
+        right.begin(b, at.n0, at.lane);
+        left.begin(a, at.lane);
+        right.load(y[0]);
+        left.load(x[0]);
+        finish.ahead(at, side);
+        finish.start(at, acc);
+        auto step = [&](int now) {
+            right.load(y[now ^ 1]);
+            left.load(x[now ^ 1]);
+            multiply([&](int h, int j) { return y[now][h][j]; }, [&](int h, int i) { return x[now][h][i]; });
+        };
+        for (uint32_t pairs = ((bytes + CHUNK - 1) / CHUNK + 1) / 2; pairs; --pairs) { // (a last odd one with zeros)
+            step(0);
+            step(1);
+        }
     }
     __syncthreads();
     finish(at, side, acc, own);

@@ -142,6 +142,20 @@ def test_strides_and_alignment(pad_x, pad_t, first, kind):
     assert all(torch.equal(a, b) for a, b in zip(got, want))
 
 
+@pytest.mark.parametrize("kind", list(TYPES))
+@pytest.mark.parametrize("pad_x,pad_t,first", [(1, 1, 1), (0, 3, 0), (5, 0, 0), (0, 0, 3), (8, 9, 0)])
+def test_few_rows_off_boundaries(pad_x, pad_t, first, kind):
+    for n, v, d in [(1, 1, 1), (1, 65, 7), (2, 64, 31), (16, 130, 32), (17, 200, 33), (32, 63, 64), (5, 300, 65),
+                    (31, 1000, 128), (1, 700, 200), (16, 129, 385), (32, 500, 1023)]:
+        x, t, ids, out, w = _inputs(n, v, d, kind)
+        views = []
+        for a, pad in ((x, pad_x), (t, pad_t)):
+            whole = torch.full((a.shape[0], d + pad + first), math.nan, dtype=a.dtype, device="cuda")
+            whole[:, first:first + d] = a
+            views.append(whole[:, first:first + d])
+        _check(*views, ids, out, w, 0.3, kind)
+
+
 def test_columns_of_a_transposed_input_are_refused():
     x, t, ids, _, _ = _inputs(8, 9, 8, "fp32")
     with pytest.raises(ValueError, match="side by side"):
