@@ -285,6 +285,77 @@ struct Weights : Plainly {
     }
 };
 
+// ---- scores in shares of the inner length ------------------------------------------------------
+
+// Where the rows are long and tiles of scores too few for the chip, the tiles' sums are made in shares
+// (Sums), and these kernels take LogSum's and Weights' place: a wave four columns a lane of a row's 256,
+// the shares added in order.  They cost a pass over the sums.  Both passes, us, with shares and
+// without: 613 x 3520 of 4096 float32 691 and 855, 983 x 859 298 and 439; 3 x 145 of 1984 36 and 115;
+// bf16 225 x 1269 of 4096 62 and 104, 3 x 5269 71 and 112.
+__device__ inline f32x4 shares_sum(const float *part, uint32_t splits, uint64_t n, uint64_t stride, uint64_t row, uint64_t col)
+{
+    f32x4 s = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll 4
+    for (uint32_t k = 0; k < splits; ++k)
+        s += *reinterpret_cast<const f32x4 *>(part + (k * n + row) * stride + col);
+    return s;
+}
+
+__global__ __launch_bounds__(256) void ung_table_parts_kernel(const float *part, uint32_t splits, uint64_t stride, LogSum f)
+{
+    const uint32_t lane = threadIdx.x & 63;
+    const uint64_t strips = stride / WHOLE;
+    for (uint64_t item = blockIdx.x * 4ull + (threadIdx.x >> 6); item < f.n * strips; item += gridDim.x * 4ull) {
+        const uint64_t row = item / strips, strip = item - row * strips, col = strip * WHOLE + lane * 4;
+        f32x4 s = shares_sum(part, splits, f.n, stride, row, col);
+        const uint32_t id = (uint32_t)f.ids[row] - (uint32_t)col, out = (uint32_t)(f.without ? f.without[row] : -1) - (uint32_t)col;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            if (id == e)
+                f.target[row] = s[e];
+            if (out == e || col + e >= f.v)
+                s[e] = -INF;
+        }
+        float top = wave_reduce(fmaxf(fmaxf(s[0], s[1]), fmaxf(s[2], s[3])), [](float a, float b) { return fmaxf(a, b); });
+        top = __builtin_rintf(top * f.c);
+        const float from = top == NO_TOP ? 0.0f : -top;
+        float sum = 0.0f;
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+            sum += __builtin_amdgcn_exp2f(__builtin_fmaf(s[e], f.c, from));
+        sum = wave_reduce(sum, [](float a, float b) { return a + b; });
+        if (lane == 0)
+            f.parts[strip * f.n + row] = {top, sum};
+    }
+}
+
+template <class E>
+__global__ __launch_bounds__(256) void ung_table_weights_kernel(const float *part, uint32_t splits, uint64_t stride, Weights<E> f)
+{
+    const uint32_t lane = threadIdx.x & 63;
+    const uint64_t strips = stride / WHOLE;
+    for (uint64_t item = blockIdx.x * 4ull + (threadIdx.x >> 6); item < f.n * strips; item += gridDim.x * 4ull) {
+        const uint64_t row = item / strips, col = (item - row * strips) * WHOLE + lane * 4;
+        const f32x4 s = shares_sum(part, splits, f.n, stride, row, col);
+        const Row p = f.rows[row];
+        const uint32_t id = (uint32_t)p.id - (uint32_t)(f.v0 + col), out = (uint32_t)p.out - (uint32_t)(f.v0 + col);
+        alignas(4 * sizeof(E)) E o[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            float y = __builtin_amdgcn_exp2f(__builtin_fmaf(s[e], f.c, -p.lse2));
+            if (id == e) {
+                y -= 1.0f;
+                const float all = y * p.weight;
+                f.rest[row] = all - to_float(from_float<E>(all));
+            }
+            if (out == e || col + e >= f.v)
+                y = 0.0f;
+            o[e] = from_float<E>(y * p.weight);
+        }
+        __builtin_memcpy(__builtin_assume_aligned(f.g + row * f.pitch + col, sizeof o), o, sizeof o);
+    }
+}
+
 // The rest of the targets' weights (rows null: none), added to dX.
 template <class E>
 struct Rest {
@@ -538,10 +609,14 @@ Shape together_of(uint64_t n, uint64_t v, uint64_t d, int type, double two_us)
 
 constexpr uint32_t FEW = 32; // rows that the table is streamed for
 
-// How scores are made.
+// How scores are made.  A wave of few rows takes 0.5 to 0.7 us for a chunk, one after the other.
 Shape scores_shape(uint64_t n, uint64_t v, uint64_t d, int type)
 {
-    return n <= FEW ? Shape{n <= 16 ? 16u : 32u, 64, 1, 0.0} : shape_of(n, v, d, type, false);
+    if (n > FEW)
+        return shape_of(n, v, d, type, true);
+    const uint64_t waves = ceil_div(v, 64), chunks = ceil_div(d * type_size(type), CHUNK);
+    const uint64_t splits = chunks < 16 || !waves ? 1 : std::min<uint64_t>({4 * (uint64_t)cu_count() / waves, chunks / 4, 32});
+    return {n <= 16 ? 16u : 32u, 64, splits > 1 ? (uint32_t)ceil_div(chunks, ceil_div(chunks, splits)) : 1, 0.0};
 }
 
 struct Inputs {
@@ -584,7 +659,7 @@ struct Forward {
     Layout l;
     Packed x, table;
     Shape shape;
-    uint64_t tiles, parts, target;
+    uint64_t tiles, parts, target, sums, stride;
     bool loose;
     explicit Forward(const Inputs &in)
     {
@@ -593,7 +668,9 @@ struct Forward {
         table = packed(l, in.table, in.table_stride, in.v, in.d, size, false, in.n <= FEW);
         loose = (!x.copy && x.loose) || (!table.copy && table.loose);
         shape = scores_shape(in.n, in.v, in.d, in.type);
-        tiles = ceil_div(in.v, shape.wide);
+        stride = ceil_div(in.v, WHOLE) * WHOLE;
+        tiles = ceil_div(in.v, shape.splits > 1 ? WHOLE : shape.wide);
+        sums = shape.splits > 1 ? l.take(shape.splits * in.n * stride * 4) : 0;
         parts = l.take(tiles * in.n * sizeof(Part));
         target = l.take(in.n * 4);
     }
@@ -606,7 +683,7 @@ constexpr uint64_t PIECE_BYTES = 168ull << 20;
 struct Backward {
     Layout l;
     Packed x, table;
-    uint64_t rows, scale, rest, piece, pieces, g, x_sums, t_sums, sum_stride;
+    uint64_t rows, scale, rest, piece, pieces, g, g_sums, x_sums, t_sums, sum_stride;
     Shape g_shape, x_shape, t_shape;
     bool together = false; // dX and dT in one launch (where both are asked for)
     explicit Backward(const Inputs &in)
@@ -644,7 +721,9 @@ struct Backward {
                 x_shape = both, t_shape = {both.high, both.wide, 1, 0.0};
         }
         g = l.take(in.n * piece * size);
-        x_sums = t_sums = 0;
+        g_sums = x_sums = t_sums = 0;
+        if (g_shape.splits > 1)
+            g_sums = l.take(g_shape.splits * in.n * piece * 4);
         if (x_shape.splits > 1 || pieces > 1)
             x_sums = l.take(x_shape.splits * in.n * sum_stride * 4);
         if (t_shape.splits > 1)
@@ -715,13 +794,14 @@ uint32_t items_of(const Grid &g) { return g.m_tiles * g.n_tiles * g.splits; }
 template <class E, bool LOOSE, class Finish>
 void few_rows(const Operand &a, const Operand &b, Shape shape, const Finish &finish, hipStream_t st)
 {
-    const uint32_t blocks = (uint32_t)ceil_div(b.rows, 64);
-    if (!blocks)
+    const uint32_t each = (uint32_t)ceil_div(ceil_div(b.k * sizeof(E), CHUNK), shape.splits);
+    const dim3 blocks((uint32_t)ceil_div(b.rows, 64), shape.splits);
+    if (!blocks.x)
         return;
     if (shape.high == 16)
-        ung_few_rows_kernel<E, 1, LOOSE><<<blocks, 64, 0, st>>>(a, b, finish);
+        ung_few_rows_kernel<E, 1, LOOSE><<<blocks, 64, 0, st>>>(a, b, each, finish);
     else
-        ung_few_rows_kernel<E, 2, LOOSE><<<blocks, 64, 0, st>>>(a, b, finish);
+        ung_few_rows_kernel<E, 2, LOOSE><<<blocks, 64, 0, st>>>(a, b, each, finish);
 }
 
 // The product of two sides, its tiles finished by `finish`.
@@ -842,10 +922,18 @@ int ung_hip_table_loss_forward(const void *x, uint64_t x_stride, const void *tab
         Part *parts = (Part *)(ws + f.parts);
         float *target = (float *)(ws + f.target);
         const LogSum finish = {{}, ids, without, target, parts, rows, table_rows, c};
-        if (f.loose)
-            few_rows<E, true>(a, b, f.shape, finish, st);
-        else
-            product<E, false, false>(a, b, f.shape, finish, st);
+        auto scores = [&](const auto &finish) {
+            if (f.loose)
+                few_rows<E, true>(a, b, f.shape, finish, st);
+            else
+                product<E, false, false>(a, b, f.shape, finish, st);
+        };
+        if (f.shape.splits > 1) {
+            float *const sums = (float *)(ws + f.sums);
+            scores(Sums<false>{sums, f.stride, rows});
+            ung_table_parts_kernel<<<some_blocks(ceil_div(rows * f.tiles, 4)), 256, 0, st>>>(sums, f.shape.splits, f.stride, finish);
+        } else
+            scores(finish);
         auto join = [&](auto each) {
             constexpr int R = decltype(each)::value;
             ung_table_join_kernel<R><<<(uint32_t)ceil_div(rows, R), 256, 0, st>>>(parts, f.tiles, rows, table_rows, target,
@@ -936,7 +1024,14 @@ int ung_hip_table_loss_backward(const void *x, uint64_t x_stride, const void *ta
         for (uint64_t p = 0; p < f.pieces; ++p) {
             const uint64_t v = length(p);
             const Operand part = table_of(p), g = g_of(p);
-            product<E, false, false>(x_side, part, f.g_shape, weights(p), st);
+            if (f.g_shape.splits > 1 && rows && v) {
+                float *const sums = (float *)(ws + f.g_sums);
+                const uint64_t stride = ceil_div(v, WHOLE) * WHOLE;
+                product<E, false, false>(x_side, part, f.g_shape, Sums<false>{sums, stride, rows}, st);
+                ung_table_weights_kernel<E><<<some_blocks(ceil_div(rows * (stride / WHOLE), 4)), 256, 0, st>>>(
+                    sums, f.g_shape.splits, stride, weights(p));
+            } else
+                product<E, false, false>(x_side, part, f.g_shape, weights(p), st);
             if (f.together && dx && dtable) {
                 both_products<E>(across(g), across(x_side), f.t_shape, whole(p), g, across(part), f.x_shape,
                                  Sums<false>{x_sums, f.sum_stride, rows}, st);

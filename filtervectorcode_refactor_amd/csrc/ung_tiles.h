@@ -474,8 +474,9 @@ struct Loose {
 // multiplied.  Results as ung_tile_kernel's.  LOOSE: rows need no alignment (100000 x 384 bf16 at an odd
 // stride 25.6 us, copied to rows of whole vectors first 51.5; at whole vectors 19.7 as they are.  float32
 // 36, 95 and 32; 100000 x 100 bf16 13, 26, and 9 where they are 104).
+// Blocks y: shares of the inner length, `each` chunks long.
 template <class E, int TM, bool LOOSE, class Finish>
-__global__ __launch_bounds__(64) void ung_few_rows_kernel(Operand a, Operand b, Finish finish)
+__global__ __launch_bounds__(64) void ung_few_rows_kernel(Operand a, Operand b, uint32_t each, Finish finish)
 {
     __shared__ alignas(16) uint8_t own[turn_bytes(4)];
     __shared__ alignas(16) uint8_t side[16 * TM * Finish::AHEAD + 16];
@@ -484,6 +485,13 @@ __global__ __launch_bounds__(64) void ung_few_rows_kernel(Operand a, Operand b, 
     at.strips = 1;
     at.lane = threadIdx.x;
     at.n0 = (uint64_t)xcd_run(blockIdx.x, gridDim.x) * 64;
+    if (gridDim.y > 1) {
+        const uint64_t first = (uint64_t)blockIdx.y * each * CHUNK;
+        a.p = (const uint8_t *)a.p + first;
+        b.p = (const uint8_t *)b.p + first;
+        a.k = b.k = min(b.k - first / sizeof(E), (uint64_t)each * CHUNK / sizeof(E));
+        at.split = blockIdx.y;
+    }
     typename Matrix<E>::Acc acc[TM][4];
     auto multiply = [&](const auto &y, const auto &x) {
 #pragma unroll

@@ -119,6 +119,19 @@ def test_long_rows(n, v, d, kind):
     _check(x, t, ids, out, w, 0.7, kind)
 
 
+@pytest.mark.parametrize("kind", list(TYPES))
+@pytest.mark.parametrize("n,v,d,pad", [(1, 1, 2048, 0), (3, 145, 1984, 0), (14, 700, 4096, 3), (32, 260, 1001, 0), (31, 5000, 1024, 1),
+                                       (33, 64, 4096, 0), (225, 1269, 4096, 0), (600, 520, 2049, 0), (100, 257, 3000, 8)])
+def test_scores_in_shares(n, v, d, pad, kind):
+    """Few tiles of long rows."""
+    x, t, ids, out, w = _inputs(n, v, d + pad, kind, seed=9)
+    x, t = x[:, :d], t[:, :d]
+    ids[::5] = out[::5]
+    ids[1::7] = v + 3
+    x[1::7] = 1.0
+    _check(x, t, ids, out, w, 0.7, kind)
+
+
 @pytest.mark.parametrize("kind,n,v,d", [("bf16", 70_000, 2500, 16), ("fp32", 40_000, 1700, 8), ("bf16", 9000, 20_000, 72)])
 def test_table_in_pieces(kind, n, v, d):
     """More scores than a piece of G holds: dx is summed over pieces of the table."""
