@@ -296,7 +296,7 @@ __device__ inline void make_tile(const Operand &a, const Operand &b, const Grid 
     }
     await_loads<0>(); // the last step's loads, of the chunk past the end, land here
     __syncthreads();  // the panels are free for the finish
-    finish(at, side, acc, b_even);
+    finish(at, side, acc, WN == 1 ? a_even : b_even); // (turn_bytes of every wave)
 }
 
 template <class E, int BM, int WM, int WN, bool A_ACROSS, bool B_ACROSS, class Finish>
@@ -571,7 +571,7 @@ struct Plainly {
 // A wave's 16 x 64 results (row r, columns g * 16 + 0..15 of each lane 16 g + r) to `to`, rows
 // `stride` elements apart, of which `rows` and `cols` are there.  16-bit vectors go out as they lie where
 // `vectors`; the others are turned in LDS first, so that a store's lanes write neighbouring elements.
-// `own`: turn_bytes of LDS of the wave's own; a block's are no more than its panel of the n side.
+// `own`: turn_bytes of LDS of the wave's own; a block's are no more than its larger panel.
 template <class T>
 __device__ inline void store_rows(T *to, uint64_t stride, uint32_t rows, uint64_t cols, bool vectors,
                                   const Vec<T> (&o)[16 / Vec<T>::N], uint8_t *own, uint32_t lane)

@@ -281,7 +281,8 @@ def test_weights_none_and_one_gradient_alone():
 
 @pytest.mark.parametrize("kind", list(TYPES))
 @pytest.mark.parametrize("n,v,d", [(16, 1000, 64), (100, 3000, 256), (300, 20_000, 130), (500, 10_001, 100), (2000, 2000, 600),
-                                   (2000, 40, 24), (40, 2001, 1000), (1000, 5000, 384)])
+                                   (2000, 40, 24), (40, 2001, 1000), (1000, 5000, 384), (2000, 20_000, 64), (1500, 9000, 33),
+                                   (9000, 2500, 60)])
 def test_both_gradients_are_each_ones(n, v, d, kind):
     """By one launch or by two, sums are made in the same order."""
     x, t, ids, out, w = _inputs(n, v, d, kind)
