@@ -1,5 +1,5 @@
 // ung_table_loss.hip -- cross entropy of hidden states against every row of a table, and its
-// gradients, without the scores in memory, on gfx950: the kernels and the entry points
+// gradients, without a large batch's scores in memory, on gfx950: the kernels and the entry points
 // ung_hip_table_loss_* of include/ung_hip.h.
 //
 //   z_ij = x_i . t_j / T   (j not left out by row i)        lse_i = log sum_j exp z_ij
@@ -8,7 +8,8 @@
 //
 // The forward pass makes tiles of scores and keeps of each only its rows' largest score and sum
 // of exponentials.  The backward pass makes the scores anew, a piece of the table's rows at a
-// time: G of the piece goes to memory in the inputs' type, where two products read it.
+// time: G of the piece goes to memory in the inputs' type, where two products read it.  Few scores of
+// long rows go through memory as sums of shares of the inner length.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -573,8 +574,8 @@ Shape shape_of(uint64_t m, uint64_t n, uint64_t k, int type, bool shares, bool g
 // dT and dX in one launch: the shape of dX, of whose height dT's tiles are too; us is 0 where two launches
 // are faster.  Each alone leaves a part of the chip idle in its last or only round, and the second waits
 // for the first's last tile.  The backward pass, us, by one launch and by two: 16 x 1000 of 64 bf16 12.5
-// and 15.6, 500 x 10001 of 100 float32 65 and 74, 2000 x 2000 of 768 bf16 55 and 72, 300 x 20000 of 512 bf16
-// 55 and 62.
+// and 15.6, 500 x 10001 of 100 float32 62 and 74, 2000 x 2000 of 768 bf16 52 and 72, 300 x 20000 of 512 bf16
+// 53 and 62.
 Shape together_of(uint64_t n, uint64_t v, uint64_t d, int type, double two_us)
 {
     const uint64_t cus = cu_count();

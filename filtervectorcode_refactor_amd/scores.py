@@ -561,7 +561,7 @@ def _against(x, table, ids, without):
 def table_loss_forward(x, table, ids, without=None, temperature=1.0):
     """(loss [n], lse [n]) float32: cross entropy of each row of ``x`` with row ``ids`` of the table
     as its target, scores being x table^T / temperature, and the log-sum-exp of all its scores,
-    which table_loss_backward needs.  The scores themselves are never in memory.
+    which table_loss_backward needs.  A large batch's scores are never in memory.
 
     ``without`` names one row of the table that each row of x leaves out (its own entry; -1: none).
     A row whose id is outside the table, or the one left out, has no target: its loss is 0."""
