@@ -521,17 +521,17 @@ struct Weight {
     uint32_t high, wide, at_once; // tiles that fit a CU
     double alone, shared, ends;
 };
-// Tiles of 128 x 64 are for gradients, whose columns may be few: the backward pass of 1044 x 185304 of 64
-// float32 987 us (1300 by 128 columns), 2000 x 20000 of 64 bf16 74 (77); 3000 x 50000 of 192 bf16 355 by
+// Tiles of 128 x 64 are for few columns: the backward pass of 1044 x 185304 of 64
+// float32 987 us (1300 by 128 columns), 2000 x 20000 of 64 bf16 74 (77), the
+// forward pass of 6565 x 53 of 4096 float32 92 (180); 3000 x 50000 of 192 bf16 355 by
 // three of them, 332 by two of 128 (a line of 64 elements meets the same banks twice).
 constexpr Weight WEIGHTS_16[] = {{BIG, BIG, 1, 1.75, 1.75, 5.0}, {128, 128, 2, 0.6, 0.52, 3.5}, {64, 128, 3, 0.55, 0.33, 3.0},
                                  {32, 128, 3, 0.5, 0.25, 2.5}, {128, 64, 3, 0.6, 0.40, 3.0}};
 constexpr Weight WEIGHTS_32[] = {{128, 128, 2, 2.0, 1.95, 4.0}, {64, 128, 3, 1.1, 0.98, 3.0}, {32, 128, 3, 2.2, 0.8, 2.5},
                                  {128, 64, 3, 1.1, 0.98, 3.0}};
 
-// `shares`: sums may be made in shares of the inner length, joined by a pass of their own.  `gradient`: n is
-// a row's length.
-Shape shape_of(uint64_t m, uint64_t n, uint64_t k, int type, bool shares, bool gradient)
+// `shares`: sums may be made in shares of the inner length, joined by a pass of their own.
+Shape shape_of(uint64_t m, uint64_t n, uint64_t k, int type, bool shares)
 {
     const uint64_t cus = cu_count(), chunks = ceil_div(k * type_size(type), CHUNK);
     Shape best = {32, 128, 1, 1e30};
@@ -552,7 +552,7 @@ Shape shape_of(uint64_t m, uint64_t n, uint64_t k, int type, bool shares, bool g
             if (s.us < best.us)
                 best = s;
         };
-        if (!tiles || (w.wide == 64 && !gradient))
+        if (!tiles)
             return;
         with(1);
         if (shares)
@@ -626,7 +626,7 @@ constexpr uint32_t FEW = 32; // rows that the table is streamed for
 Shape scores_shape(uint64_t n, uint64_t v, uint64_t d, int type)
 {
     if (n > FEW)
-        return shape_of(n, v, d, type, true, false);
+        return shape_of(n, v, d, type, true);
     const uint64_t waves = ceil_div(v, 64), chunks = ceil_div(d * type_size(type), CHUNK);
     const uint64_t splits = chunks < 16 || !waves ? 1 : std::min<uint64_t>({4 * (uint64_t)cu_count() / waves, chunks / 4, 32});
     return {n <= 16 ? 16u : 32u, 64, splits > 1 ? (uint32_t)ceil_div(chunks, ceil_div(chunks, splits)) : 1, 0.0};
@@ -717,7 +717,7 @@ struct Backward {
         double best = 1e30;
         for (uint64_t p = least; p <= least + least / 2 && least > 1; ++p) {
             const uint64_t of_it = ceil_div(ceil_div(all, p), WHOLE) * WHOLE;
-            const double us = (double)p * shape_of(of_it, in.d, in.n, in.type, true, true).us;
+            const double us = (double)p * shape_of(of_it, in.d, in.n, in.type, true).us;
             if (us < best * 0.98)
                 best = us, piece = of_it;
         }
@@ -725,8 +725,8 @@ struct Backward {
         sum_stride = ceil_div(in.d, WHOLE) * WHOLE;
         const uint64_t v = in.v < piece ? in.v : piece;
         g_shape = scores_shape(in.n, v, in.d, in.type);
-        x_shape = shape_of(in.n, in.d, v, in.type, true, true);
-        t_shape = shape_of(v, in.d, in.n, in.type, true, true);
+        x_shape = shape_of(in.n, in.d, v, in.type, true);
+        t_shape = shape_of(v, in.d, in.n, in.type, true);
         if (pieces == 1) {
             const Shape both = together_of(in.n, v, in.d, in.type, x_shape.us + t_shape.us);
             together = both.us > 0.0;
@@ -822,7 +822,7 @@ template <class E, bool A_ACROSS, bool B_ACROSS, class Finish>
 void product(const Operand &a, const Operand &b, Shape shape, const Finish &finish, hipStream_t st)
 {
     if constexpr (!A_ACROSS && !B_ACROSS) {
-        if (shape.high <= FEW && shape.wide == 64) // (tiles are 128 wide or more here)
+        if (shape.high <= FEW && shape.wide == 64) // (tiles of 64 columns are 128 high)
             return few_rows<E, false>(a, b, shape, finish, st);
     }
     const Grid grid = grid_of(a, b, shape, sizeof(E));
@@ -847,10 +847,8 @@ void product(const Operand &a, const Operand &b, Shape shape, const Finish &fini
         tiles(std::integral_constant<int, 64>{}, two, two);
     else if (shape.high == 128 && shape.wide == 128)
         tiles(std::integral_constant<int, 128>{}, two, two);
-    else if (shape.high == 128) {
-        if constexpr (B_ACROSS)
-            tiles(std::integral_constant<int, 128>{}, std::integral_constant<int, 4>{}, one);
-    }
+    else if (shape.high == 128)
+        tiles(std::integral_constant<int, 128>{}, std::integral_constant<int, 4>{}, one);
     else if constexpr (sizeof(E) == 2)
         tiles(std::integral_constant<int, BIG>{}, two, std::integral_constant<int, 4>{});
 }
