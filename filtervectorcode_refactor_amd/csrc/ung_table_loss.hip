@@ -195,15 +195,18 @@ template <class E>
 __global__ __launch_bounds__(256) void ung_table_rows_kernel(const E *x, uint64_t stride, uint64_t n, uint64_t v,
                                                              uint64_t d, const int32_t *ids, const int32_t *without,
                                                              const float *lse, const float *weight, float by,
-                                                             const float *scale, Row *rows, E *to, uint64_t pitch)
+                                                             const float *scale, Row *rows, int32_t *targets, E *to,
+                                                             uint64_t pitch)
 {
     const uint32_t lane = threadIdx.x & 63;
     for (uint64_t row = blockIdx.x * 4ull + (threadIdx.x >> 6); row < n; row += gridDim.x * 4ull) {
         const int32_t id = ids[row], out = without ? without[row] : -1;
         const bool there = (uint64_t)(uint32_t)id < v && id != out;
-        if (lane == 0)
+        if (lane == 0) {
             rows[row] = there ? Row{lse[row] * LOG2E, (weight ? weight[row] : 1.0f) * by * (scale ? scale[0] : 1.0f), id, out}
                               : Row{INF, 0.0f, -1, -1};
+            targets[row] = there ? id : -1;
+        }
         for (uint64_t c = lane * Vec<E>::N; c < pitch; c += 64 * Vec<E>::N)
             *reinterpret_cast<Vec<E> *>(to + row * pitch + c) = load_row(x + row * stride, c, there ? d : 0);
     }
@@ -227,10 +230,10 @@ __global__ __launch_bounds__(256) void ung_table_pack_kernel(const E *x, uint64_
 }
 
 // A tile of scores to G, in the inputs' type: at most half a step of it, 2^-8 of an element in bf16 and
-// 2^-11 in fp16, as far as the gradients' own rounding; the products that read it sum in 32 bits.  In dX, where
-// the target's row is taken from a mean of rows near it, that would show: the rest of the target's
-// weight, which is the largest, is kept in 32 bits and joins dX with the table's row at the end (4096 x
-// 100000 x 384 at T = 0.05: 0.0017 of the norm from dX, 0.0038 without).
+// 2^-11 in fp16, as far as the gradients' own rounding; the products that read it sum in 32 bits.  Of a row's
+// weights the target's is the largest, and alone in most rows of dT: what its rounding leaves is kept in
+// 32 bits and joins dX with the table's row at the end (Rest), dT with the products (Targets).  4096 x 100000 x
+// 384 bf16 at T = 0.05: 0.0017 of the norm from dX and dT, which their own rounding makes; 0.0038 and 0.0024 without.
 template <class E>
 struct Weights : Plainly {
     const Row *rows;
@@ -390,9 +393,80 @@ struct Rest {
     }
 };
 
-// A gradient's tile in its own type.
+// The same for dT = G^T X: row i of x times its rest joins row id of dT.  So G has a second part with one
+// element a row, of 16 bits too: what is left then is 2^-17 of a weight in bf16, 2^-22 in fp16.  A wave
+// looks at 64 ids a chunk, and makes fragments of the second part for the halves of groups of 16 rows that
+// hold some.  The backward pass with it and without, us: 4096 x 100000 of 384 bf16 1196 and 1181, 2000 x 2000
+// of 768 64 and 57, 8192 x 1000 of 256 61 and 55.
 template <class E>
-struct Whole : Plainly {
+struct Targets {
+    static constexpr uint32_t MORE = 64 * 4; // of the chunk's rows: place among the wave's rows, and the rest
+    const int32_t *targets;                  // [n], -1: none; one is there where n is 0
+    const float *rest;
+    uint32_t n, v0; // v0: row of the table that the product's first is
+
+    struct Next {
+        uint32_t k; // of the whole wave
+        int32_t id;
+        float rest;
+    };
+    __device__ inline void fetch(Next &next, uint32_t lane) const
+    {
+        const uint32_t at = next.k + lane < n ? next.k + lane : 0;
+        next.id = targets[at]; // (looked at where the next chunk is: here it would be waited for)
+        next.rest = rest[at];
+    }
+    __device__ inline void first(Next &next, uint32_t k, uint32_t lane) const
+    {
+        static_assert(sizeof(E) == 2 && CHUNK == 64 * sizeof(E), "a lane for each row of a chunk");
+        next.k = k;
+        fetch(next, lane);
+    }
+    template <int TM>
+    __device__ inline uint32_t holds(Next &next, const Tile &t, uint8_t *own) const
+    {
+        const uint32_t place = next.k + t.lane < n ? (uint32_t)next.id - (v0 + (uint32_t)t.m0 + t.wm) : TM * 16;
+        const uint32_t rounded = __builtin_bit_cast(uint16_t, from_float<E>(next.rest));
+        next.k += 64;
+        fetch(next, t.lane);
+        uint32_t held = 0;
+        if (__any(place < TM * 16)) {
+            reinterpret_cast<uint32_t *>(own)[t.lane] = place < TM * 16 ? place << 16 | rounded : 0xFFFF0000u;
+#pragma unroll
+            for (int i = 0; i < TM; ++i) {
+                const uint64_t of = __ballot(place / 16 == i);
+                held |= ((uint32_t)of ? 1u << i : 0u) | ((uint32_t)(of >> 32) ? 1u << (16 + i) : 0u);
+            }
+            wave_lds_fence();
+        }
+        return held;
+    }
+    __device__ inline u32x4 more(const uint8_t *own, int i, int half, uint32_t lane) const
+    {
+        const u32x4 *const at = reinterpret_cast<const u32x4 *>(own + (half * 32 + (lane >> 4) * 8) * 4);
+        const u32x4 lo = at[0], hi = at[1];
+        const uint32_t place = i * 16 + (lane & 15);
+        u32x4 f;
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+            const uint32_t a = q < 2 ? lo[q * 2] : hi[q * 2 - 4], b = q < 2 ? lo[q * 2 + 1] : hi[q * 2 - 3];
+            f[q] = (a >> 16 == place ? a & 0xFFFFu : 0u) | (b >> 16 == place ? b << 16 : 0u);
+        }
+        return f;
+    }
+};
+struct NoTargets {
+    static constexpr uint32_t MORE = 0;
+    struct Next {};
+};
+template <class E> // of dT: float32 weights are not rounded
+using TargetsOf = std::conditional_t<sizeof(E) == 2, Targets<E>, NoTargets>;
+
+// A gradient's tile in its own type.
+template <class E, class More>
+struct Whole : Plainly, More {
+    using More::MORE;
+    using Next = typename More::Next;
     E *c;
     uint64_t stride, m, n;
     const float *by;
@@ -431,8 +505,8 @@ struct Whole : Plainly {
 // Sums of a share of the inner length in 32 bits, from 0 or (ADD) from an earlier piece's: dX, whose tiles
 // are few and whose inner length is the table's.  4096 x 384 of 20224 bf16, 5 shares, 73 us (870 TFLOP/s),
 // 77 onto an earlier piece's; 2048 x 768 of 32768 fp16 112 us (920).
-template <bool ADD>
-struct Sums {
+template <bool ADD, class More = NoTargets>
+struct Sums : More {
     float *part;
     uint64_t stride, m; // stride: whole tiles
 
@@ -531,9 +605,14 @@ constexpr Weight WEIGHTS_32[] = {{128, 128, 2, 2.0, 1.95, 4.0}, {64, 128, 3, 1.1
                                  {128, 64, 3, 1.1, 0.98, 3.0}};
 
 constexpr uint64_t MOST_SUMS = 64ull << 20;
+// dT's tiles, which take Targets' fragments too: a tile of 256 x 256 has no registers to choose among its groups
+// of rows, so every chunk with a target costs it all of them (backward pass of 8192 x 6000 of 768 bf16 365
+// us, by 128 x 128 319).
+constexpr uint32_t MOST_HIGH_T = 128;
 
-// `shares`: sums may be made in shares of the inner length, joined by a pass of their own.
-Shape shape_of(uint64_t m, uint64_t n, uint64_t k, int type, bool shares)
+// `shares`: sums may be made in shares of the inner length, joined by a pass of their own.  `most_high`: rows
+// of the highest tile.
+Shape shape_of(uint64_t m, uint64_t n, uint64_t k, int type, bool shares, uint32_t most_high = BIG)
 {
     const uint64_t cus = cu_count(), chunks = ceil_div(k * type_size(type), CHUNK);
     Shape best = {32, 128, 1, 1e30};
@@ -554,7 +633,7 @@ Shape shape_of(uint64_t m, uint64_t n, uint64_t k, int type, bool shares)
             if (s.us < best.us)
                 best = s;
         };
-        if (!tiles)
+        if (!tiles || w.high > most_high)
             return;
         with(1);
         if (!shares)
@@ -704,7 +783,7 @@ constexpr uint64_t PIECE_BYTES = 168ull << 20;
 struct Backward {
     Layout l;
     Packed x, table;
-    uint64_t rows, scale, rest, piece, pieces, g, g_sums, x_sums, t_sums, sum_stride;
+    uint64_t rows, scale, targets, rest, piece, pieces, g, g_sums, x_sums, t_sums, sum_stride;
     Shape g_shape, x_shape, t_shape;
     bool together = false; // dX and dT in one launch (where both are asked for)
     explicit Backward(const Inputs &in)
@@ -714,7 +793,8 @@ struct Backward {
         table = packed(l, in.table, in.table_stride, in.v, in.d, size, false);
         rows = l.take(in.n * sizeof(Row));
         scale = l.take(8);
-        rest = l.take(in.n * 4);
+        targets = l.take((in.n ? in.n : 1) * 4);
+        rest = l.take((in.n ? in.n : 1) * 4);
         const uint64_t all = ceil_div(in.v, WHOLE) * WHOLE;
         uint64_t fits = PIECE_BYTES / ((in.n ? in.n : 1) * size) / WHOLE * WHOLE;
         fits = fits < 1024 ? 1024 : fits;
@@ -725,7 +805,7 @@ struct Backward {
         double best = 1e30;
         for (uint64_t p = least; p <= least + least / 2 && least > 1; ++p) {
             const uint64_t of_it = ceil_div(ceil_div(all, p), WHOLE) * WHOLE;
-            const double us = (double)p * shape_of(of_it, in.d, in.n, in.type, true).us;
+            const double us = (double)p * shape_of(of_it, in.d, in.n, in.type, true, MOST_HIGH_T).us;
             if (us < best * 0.98)
                 best = us, piece = of_it;
         }
@@ -734,7 +814,7 @@ struct Backward {
         const uint64_t v = in.v < piece ? in.v : piece;
         g_shape = scores_shape(in.n, v, in.d, in.type);
         x_shape = shape_of(in.n, in.d, v, in.type, true);
-        t_shape = shape_of(v, in.d, in.n, in.type, true);
+        t_shape = shape_of(v, in.d, in.n, in.type, true, MOST_HIGH_T);
         if (pieces == 1) {
             const Shape both = together_of(in.n, v, in.d, in.type, x_shape.us + t_shape.us);
             together = both.us > 0.0;
@@ -857,13 +937,13 @@ void product(const Operand &a, const Operand &b, Shape shape, const Finish &fini
         tiles(std::integral_constant<int, 128>{}, two, two);
     else if (shape.high == 128)
         tiles(std::integral_constant<int, 128>{}, std::integral_constant<int, 4>{}, one);
-    else if constexpr (sizeof(E) == 2)
+    else if constexpr (sizeof(E) == 2 && !Finish::MORE)
         tiles(std::integral_constant<int, BIG>{}, two, std::integral_constant<int, 4>{});
 }
 
 // dT of G and X, and dX of G and the table, by one launch.
 template <class E>
-void both_products(const Operand &gt, const Operand &x, Shape t_shape, const Whole<E> &whole, const Operand &g,
+void both_products(const Operand &gt, const Operand &x, Shape t_shape, const Whole<E, TargetsOf<E>> &whole, const Operand &g,
                    const Operand &table, Shape x_shape, const Sums<false> &sums, hipStream_t st)
 {
     const Grid t_grid = grid_of(gt, x, t_shape, sizeof(E)), x_grid = grid_of(g, table, x_shape, sizeof(E));
@@ -956,7 +1036,7 @@ int ung_hip_table_loss_forward(const void *x, uint64_t x_stride, const void *tab
         };
         if (f.shape.splits > 1) {
             float *const sums = (float *)(ws + f.sums);
-            scores(Sums<false>{sums, f.stride, rows});
+            scores(Sums<false>{{}, sums, f.stride, rows});
             ung_table_parts_kernel<<<some_blocks(ceil_div(rows * f.tiles, 4)), 256, 0, st>>>(sums, f.shape.splits, f.stride, finish);
         } else
             scores(finish);
@@ -1016,7 +1096,7 @@ int ung_hip_table_loss_backward(const void *x, uint64_t x_stride, const void *ta
         if (rows)
             ung_table_rows_kernel<E><<<some_blocks(ceil_div(rows, 4)), 256, 0, st>>>(
                 (const E *)x, x_stride, rows, table_rows, cols, ids, without, lse, weight, by, scale, row,
-                (E *)(ws + f.x.at), f.x.pitch / sizeof(E));
+                (int32_t *)(ws + f.targets), (E *)(ws + f.x.at), f.x.pitch / sizeof(E));
         const Operand t = side<E>(f.table, table, table_stride, table_rows, cols, ws, st, true);
         auto vectors = [](const void *p, uint64_t stride, uint64_t rows) {
             return (uintptr_t)p % 4 == 0 && (rows == 1 || stride * sizeof(E) % 4 == 0);
@@ -1043,9 +1123,16 @@ int ung_hip_table_loss_backward(const void *x, uint64_t x_stride, const void *ta
         auto weights = [&](uint64_t p) {
             return Weights<E>{{}, row, (float *)(ws + f.rest), g_at, f.piece, rows, p * f.piece, length(p), c};
         };
+        auto targets = [&](uint64_t p) {
+            if constexpr (sizeof(E) == 2)
+                return Targets<E>{(const int32_t *)(ws + f.targets), (const float *)(ws + f.rest), (uint32_t)rows, (uint32_t)(p * f.piece)};
+            else
+                return NoTargets{};
+        };
         auto whole = [&](uint64_t p) {
             E *to = (E *)dtable + p * f.piece * dtable_stride;
-            return Whole<E>{{}, to, dtable_stride, length(p), cols, back, vectors(to, dtable_stride, length(p)), none};
+            return Whole<E, TargetsOf<E>>{{}, targets(p), to, dtable_stride, length(p), cols, back,
+                                          vectors(to, dtable_stride, length(p)), none};
         };
         for (uint64_t p = 0; p < f.pieces; ++p) {
             const uint64_t v = length(p);
@@ -1053,26 +1140,26 @@ int ung_hip_table_loss_backward(const void *x, uint64_t x_stride, const void *ta
             if (f.g_shape.splits > 1 && rows && v) {
                 float *const sums = (float *)(ws + f.g_sums);
                 const uint64_t stride = ceil_div(v, WHOLE) * WHOLE;
-                product<E, false, false>(x_side, part, f.g_shape, Sums<false>{sums, stride, rows}, st);
+                product<E, false, false>(x_side, part, f.g_shape, Sums<false>{{}, sums, stride, rows}, st);
                 ung_table_weights_kernel<E><<<some_blocks(ceil_div(rows * (stride / WHOLE), 4)), 256, 0, st>>>(
                     sums, f.g_shape.splits, stride, weights(p));
             } else
                 product<E, false, false>(x_side, part, f.g_shape, weights(p), st);
             if (f.together && dx && dtable) {
                 both_products<E>(across(g), across(x_side), f.t_shape, whole(p), g, across(part), f.x_shape,
-                                 Sums<false>{x_sums, f.sum_stride, rows}, st);
+                                 Sums<false>{{}, x_sums, f.sum_stride, rows}, st);
                 break;
             }
             if (dx && rows) {
                 if (f.x_shape.splits == 1 && f.pieces == 1)
                     product<E, false, true>(g, across(part), f.x_shape,
-                                            Whole<E>{{}, (E *)dx, dx_stride, rows, cols, back, vectors(dx, dx_stride, rows), rest}, st);
+                                            Whole<E, NoTargets>{{}, {}, (E *)dx, dx_stride, rows, cols, back, vectors(dx, dx_stride, rows), rest}, st);
                 else if (p == 0)
                     product<E, false, true>(g, across(part), f.x_shape,
-                                            Sums<false>{x_sums, f.sum_stride, rows}, st);
+                                            Sums<false>{{}, x_sums, f.sum_stride, rows}, st);
                 else
                     product<E, false, true>(g, across(part), f.x_shape,
-                                            Sums<true>{x_sums, f.sum_stride, rows}, st);
+                                            Sums<true>{{}, x_sums, f.sum_stride, rows}, st);
             }
             if (dtable && v) {
                 if (f.t_shape.splits == 1)
@@ -1080,7 +1167,7 @@ int ung_hip_table_loss_backward(const void *x, uint64_t x_stride, const void *ta
                 else {
                     E *to = (E *)dtable + p * f.piece * dtable_stride;
                     product<E, true, true>(across(g), across(x_side), f.t_shape,
-                                           Sums<false>{(float *)(ws + f.t_sums), f.sum_stride, v}, st);
+                                           Sums<false, TargetsOf<E>>{targets(p), (float *)(ws + f.t_sums), f.sum_stride, v}, st);
                     sum((const float *)(ws + f.t_sums), f.t_shape.splits, v, to, dtable_stride, none);
                 }
             }

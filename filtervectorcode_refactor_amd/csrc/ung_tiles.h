@@ -202,7 +202,9 @@ constexpr uint32_t turn_bytes(uint32_t size) { return 16 * 64 * size; }
 // matrix instructions.  Both panels of a chunk are staged in LDS by loads that bypass the
 // registers, one chunk ahead.  A lane ends with results [i][j][e]: row wm + 16 i + lane % 16,
 // column wn + lane / 16 * 16 + 4 j + e.  `finish` brings what it needs of the tile's rows to LDS before
-// the sums (ahead), the values they begin with (start), and takes the results.
+// the sums (ahead), the values they begin with (start), and takes the results.  One with MORE (bytes of LDS
+// for a wave) adds to a chunk's products what A's panel does not hold: of the chunks that have such elements
+// in the wave's rows (holds), a second fragment of A (more) beside the panel's, in the same order.
 //   256 x 256 tiles of eight waves: a wave reads 24 KB of LDS for a chunk's 4 M products where 64 x 64
 // parts read 32; 8192 x 8192 x 8192 bf16 1249 TFLOP/s in bands of 16 (4: 1168), 128 x 128 tiles, two
 // blocks to a CU, 1097 (the library's product 1377); without the results' stores 4096 x 16384 x 384 1065
@@ -255,11 +257,20 @@ __device__ inline void make_tile(const Operand &a, const Operand &b, const Grid 
     typename Matrix<E>::Acc acc[TM][4];
     finish.ahead(at, side);
     finish.start(at, acc);
+    constexpr bool MORE = Finish::MORE > 0;
+    static_assert(!MORE || BM < BIG, "the largest tile has no registers left for it");
+    typename Finish::Next next;
+    uint8_t *const own = side + BM * Finish::AHEAD + at.wave * Finish::MORE;
+    if constexpr (MORE)
+        finish.first(next, kb * (CHUNK / sizeof(E)), at.lane);
 
     auto step = [&](const uint8_t *pa, const uint8_t *pb, uint8_t *next_a, uint8_t *next_b) {
         await_loads<0>(); // loads into LDS are counted as memory loads, which a barrier alone does not await
         __builtin_amdgcn_s_barrier(); // the panels have landed; every wave is done with the others
         __builtin_amdgcn_sched_barrier(0);
+        uint32_t held = 0; // of the wave's groups of 16 rows, those with more: of either half, 16 bits each
+        if constexpr (MORE)
+            held = finish.template holds<TM>(next, at, own);
         if constexpr (!ONE)
             load(next_a, next_b);
 #pragma unroll
@@ -275,6 +286,16 @@ __device__ inline void make_tile(const Operand &a, const Operand &b, const Grid 
                 for (int j = 0; j < 4; ++j)
                     acc[i][j] = Matrix<E>::mul(y[j], x, acc[i][j]);
             }
+            if constexpr (MORE)
+                if (held >> half * 16 & 0xFFFF)
+#pragma unroll
+                    for (int i = 0; i < TM; ++i)
+                        if (held >> (half * 16 + i) & 1) {
+                            const u32x4 x = finish.more(own, i, half, at.lane);
+#pragma unroll
+                            for (int j = 0; j < 4; ++j)
+                                acc[i][j] = Matrix<E>::mul(y[j], x, acc[i][j]);
+                        }
         }
         asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); // the panels are read
     };
@@ -304,7 +325,7 @@ __global__ __launch_bounds__(WM * WN * 64, 2) void ung_tile_kernel(Operand a, Op
 {
     constexpr uint32_t HIGH = BM * CHUNK, WIDE = WN * 64 * CHUNK;
     __shared__ alignas(16) uint8_t a_even[HIGH], a_odd[HIGH], b_even[WIDE], b_odd[WIDE];
-    __shared__ alignas(16) uint8_t side[BM * Finish::AHEAD + 16];
+    __shared__ alignas(16) uint8_t side[BM * Finish::AHEAD + WM * WN * Finish::MORE + 16];
     make_tile<E, BM, WM, WN, A_ACROSS, B_ACROSS, false>(a, b, grid, blockIdx.x, finish, a_even, a_odd, b_even, b_odd, side);
 }
 
@@ -317,9 +338,9 @@ __global__ __launch_bounds__(WM * WN * 64, 2) void ung_two_products_kernel(Opera
                                                                          Finish2 finish2)
 {
     constexpr uint32_t HIGH = BM * CHUNK, WIDE = WN * 64 * CHUNK;
-    constexpr uint32_t AHEAD = Finish::AHEAD > Finish2::AHEAD ? Finish::AHEAD : Finish2::AHEAD;
+    constexpr uint32_t SIDE = BM * Finish::AHEAD + WM * WN * Finish::MORE, SIDE2 = BM * Finish2::AHEAD + WM * WN * Finish2::MORE;
     __shared__ alignas(16) uint8_t a_even[HIGH], a_odd[HIGH], b_even[WIDE], b_odd[WIDE];
-    __shared__ alignas(16) uint8_t side[BM * AHEAD + 16];
+    __shared__ alignas(16) uint8_t side[(SIDE > SIDE2 ? SIDE : SIDE2) + 16];
     const uint32_t first = grid.m_tiles * grid.n_tiles * grid.splits;
     if (blockIdx.x < first)
         make_tile<E, BM, WM, WN, A_ACROSS, B_ACROSS, false>(a, b, grid, blockIdx.x, finish, a_even, a_odd, b_even, b_odd, side);
@@ -335,7 +356,7 @@ template <class E, bool A_ACROSS, bool B_ACROSS, class Finish>
 __global__ __launch_bounds__(256, 4) void ung_one_chunk_kernel(Operand a, Operand b, Grid grid, Finish finish)
 {
     __shared__ alignas(16) uint8_t a_panel[128 * CHUNK], b_panel[128 * CHUNK];
-    __shared__ alignas(16) uint8_t side[128 * Finish::AHEAD + 16];
+    __shared__ alignas(16) uint8_t side[128 * Finish::AHEAD + 4 * Finish::MORE + 16];
     make_tile<E, 128, 2, 2, A_ACROSS, B_ACROSS, true>(a, b, grid, blockIdx.x, finish, a_panel, nullptr, b_panel, nullptr, side);
 }
 
@@ -551,9 +572,11 @@ __global__ __launch_bounds__(64) void ung_few_rows_kernel(Operand a, Operand b, 
     finish(at, side, acc, own);
 }
 
-// A finish that needs nothing ahead, and sums that begin at 0.
+// A finish that needs nothing ahead and adds nothing, and sums that begin at 0.
 struct Plainly {
     static constexpr uint32_t AHEAD = 0; // bytes of LDS for a row
+    static constexpr uint32_t MORE = 0;  // and for a wave
+    struct Next {};
     __device__ inline void ahead(const Tile &, uint8_t *) const {}
     template <class Acc, int TM>
     __device__ inline void start(const Tile &, Acc (&acc)[TM][4]) const

@@ -392,7 +392,7 @@ int ung_hip_int8_linear(const void *x, int type, uint64_t rows, uint64_t cols, u
  *   g[i][j]     = weight[i] / temperature * (exp(z[i][j] - lse[i]) - [j is ids[i]])
  *   dx = g table, dtable = g^T x, of sum(weight[i] * loss[i]) (weight NULL: ones), in `type`
  * Products are summed in 32 bits; the backward pass, which makes the scores anew, rounds g to `type`
- * between its two products.  A row whose id is outside 0..table_rows-1 or the row left out has no
+ * between its two products, but for the target's weight, of which it keeps what the rounding takes.  A row whose id is outside 0..table_rows-1 or the row left out has no
  * target: its loss and gradient are 0, and its x (padding, of any value) does not reach dtable.  A
  * row left out counts in dx with the factor 0.  The temperature is as below, at
  * UNG_HIP_TOP_SCORES_MAX.  Rows at 16-byte boundaries of whole 16-byte vectors are read where they

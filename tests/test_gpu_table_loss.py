@@ -533,3 +533,58 @@ def test_refusals():
             S.table_loss_forward(x, t, ids, temperature=temperature)
         with pytest.raises(F.UngHipError, match="temperature"):
             S.table_loss_backward(w, x, t, ids, lse, temperature=temperature)
+
+
+def _exact_targets(x, t, ids, out, w, temperature, kind):
+    """_exact with a narrower bound of dtable: the target's weight is kept in two parts of the type, so
+    HALF_ULP squared of it is lost, twice (the second part's last bit may lie below fp16's smallest
+    number, which the bound's own term for those counts)."""
+    want, bound = _exact(x, t, ids, out, w, temperature, kind)
+    there = (ids >= 0) & (ids < t.shape[0])
+    if out is not None:
+        there &= ids != out
+    only = torch.zeros(t.shape, dtype=torch.float64, device="cuda")
+    rows = there.nonzero()[:, 0]
+    only.index_add_(0, ids[rows].long(), x[rows].double().abs() * (w[rows].double().abs() / temperature)[:, None])
+    return want, (*bound[:3], bound[3] - (HALF_ULP[kind] - 2 * HALF_ULP[kind] ** 2) * only)
+
+
+@pytest.mark.parametrize("kind", ["bf16", "fp16"])
+@pytest.mark.parametrize("n,v,d", [(1, 1, 1), (5, 130, 1), (16, 1000, 64), (2, 2000, 768), (2, 2000, 1100), (1, 200, 4096), (400, 700, 4096),
+                                   (200, 2000, 4096), (50, 80_000, 256), (64, 80_000, 130), (3000, 200, 1024), (3000, 2000, 16),
+                                   (1, 6000, 2048), (130, 6000, 2048), (8192, 6000, 768), (800, 50, 16), (8192, 700, 16), (2300, 19_000, 520)])
+def test_the_targets_weights_in_both_gradients(n, v, d, kind):
+    """A row's largest weight is its target's: what the type's rounding takes from it joins dx and
+    dtable, by every kind of tile, alone and with other rows of the same target.
+
+    Against 1000 rows or more the others' weights are near 1.13 / v (root mean square, scores / 2 of
+    deviation 1 / 2).  In units of a target row's elements, |w x| of deviation 1, the n roundings move an
+    element of dtable by e = 1.13 sqrt(n) / v / sqrt(3) HALF_ULP, and an element a >= 1 / 2 of steps
+    >= HALF_ULP a is then not the exact value rounded in at most e / (HALF_ULP a) of the cases: 3.6 % for
+    3000 x 2000, less for the other sizes.  The rounding of the target's weight alone would make it a fifth
+    of them."""
+    x, t, ids, out, w = _inputs(n, v, d, kind)
+    ids[::3] = ids[0].clone()  # many rows of one target
+    ids[1::17] = -1
+    out[2::5] = ids[2::5]
+    for left_out in (None, out):
+        got = _run(x, t, ids, left_out, w, 2.0)
+        want, bound = _exact_targets(x, t, ids, left_out, w, 2.0, kind)
+        for name, a, b, most in zip(("loss", "lse", "dx", "dtable"), got, want, bound):
+            err = torch.where(a.double() == b, torch.zeros_like(b), (a.double() - b).abs())  # (infinities)
+            assert (err <= most).all(), (name, float((err / most).max()))
+        if v >= 1000:
+            there = ids >= 0 if left_out is None else (ids >= 0) & (ids != left_out)
+            rows = ids[there].long().unique()
+            a, b = got[3][rows], want[3][rows]
+            assert (a != b.to(a.dtype))[b.abs() >= b.square().mean().sqrt() / 2].double().mean() <= 0.05
+
+
+@pytest.mark.parametrize("n,v,d", [(70_000, 2500, 16), (9000, 20_000, 72)])
+def test_the_targets_weights_in_pieces(n, v, d):
+    x, t, ids, out, w = _inputs(n, v, d, "bf16")
+    w = w / n
+    got = _run(x, t, ids, out, w, 2.0)
+    want, bound = _exact_targets(x, t, ids, out, w, 2.0, "bf16")
+    for a, b, most in zip(got, want, bound):
+        assert ((a.double() - b).abs() <= most).all()
