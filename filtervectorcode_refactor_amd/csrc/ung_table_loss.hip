@@ -114,6 +114,11 @@ struct LogSum : Plainly {
     }
 };
 
+__device__ inline bool has_target(int32_t id, const int32_t *without, uint64_t row, uint64_t v)
+{
+    return (uint64_t)(uint32_t)id < v && !(without && without[row] == id);
+}
+
 // R rows a block, 256 / R threads each: a row's parts to its log-sum-exp and loss.  A launch's latency and
 // the few parts' bound it: 3.5 to 6.5 us from 1 to 4096 rows of up to 1563 parts.
 template <int R>
@@ -145,7 +150,7 @@ __global__ __launch_bounds__(256) void ung_table_join_kernel(const Part *parts, 
     p = red[in];
     const float log_sum = log2f(p.sum);
     const int32_t id = ids[row];
-    const bool there = (uint64_t)(uint32_t)id < v && !(without && without[row] == id);
+    const bool there = has_target(id, without, row, v);
     // as the logarithm of a quotient, which is 1 or more as the sum holds the target's term; as a
     // difference where that term is nothing beside the sum
     const float u = __builtin_fmaf(there ? target[row] : 0.0f, c, -p.top);
@@ -165,16 +170,18 @@ struct alignas(16) Row {
 };
 
 // fp16 holds no numbers below 2^-24: weights are brought to the top of its range by a power of
-// two (G is at most 2 |w| / T), which the gradients are divided by at the end.  scale: {by, 1 / by}.
-// One block, 3.4 us for 2048 weights: a launch's latency, for fp16 alone.
-__global__ __launch_bounds__(1024) void ung_table_range_kernel(const float *weight, uint64_t n, float by, float *scale)
+// two (G is at most 2 |w| / T), which the gradients are divided by at the end.  Weights of rows without a
+// target do not count: padding of any size would take the others' numbers out of range.  scale: {by, 1 / by}.
+// One block, 4.7 us for 2048 weights: a launch's latency, for fp16 alone.
+__global__ __launch_bounds__(1024) void ung_table_range_kernel(const float *weight, uint64_t n, uint64_t v, const int32_t *ids,
+                                                               const int32_t *without, float by, float *scale)
 {
     __shared__ float red[16];
     float most = weight || !n ? 0.0f : 1.0f;
     if (weight)
         for (uint64_t i = threadIdx.x; i < n; i += 1024) {
             const float w = fabsf(weight[i]);
-            if (w < INF)
+            if (w < INF && has_target(ids[i], without, i, v))
                 most = fmaxf(most, w);
         }
     most = block_reduce<1024>(most, red, [](float a, float b) { return fmaxf(a, b); }) * by;
@@ -201,7 +208,7 @@ __global__ __launch_bounds__(256) void ung_table_rows_kernel(const E *x, uint64_
     const uint32_t lane = threadIdx.x & 63;
     for (uint64_t row = blockIdx.x * 4ull + (threadIdx.x >> 6); row < n; row += gridDim.x * 4ull) {
         const int32_t id = ids[row], out = without ? without[row] : -1;
-        const bool there = (uint64_t)(uint32_t)id < v && id != out;
+        const bool there = has_target(id, without, row, v);
         if (lane == 0) {
             rows[row] = there ? Row{lse[row] * LOG2E, (weight ? weight[row] : 1.0f) * by * (scale ? scale[0] : 1.0f), id, out}
                               : Row{INF, 0.0f, -1, -1};
@@ -1091,7 +1098,7 @@ int ung_hip_table_loss_backward(const void *x, uint64_t x_stride, const void *ta
         float *scale = sizeof(E) == 2 && std::is_same_v<E, fp16_t> ? (float *)(ws + f.scale) : nullptr;
         const float *back = scale ? scale + 1 : nullptr;
         if (scale)
-            ung_table_range_kernel<<<1, 1024, 0, st>>>(weight, rows, by, scale);
+            ung_table_range_kernel<<<1, 1024, 0, st>>>(weight, rows, table_rows, ids, without, by, scale);
         const Operand a = side<E>(f.x, x, x_stride, rows, cols, ws, st, false);
         if (rows)
             ung_table_rows_kernel<E><<<some_blocks(ceil_div(rows, 4)), 256, 0, st>>>(

@@ -588,3 +588,19 @@ def test_the_targets_weights_in_pieces(n, v, d):
     want, bound = _exact_targets(x, t, ids, out, w, 2.0, "bf16")
     for a, b, most in zip(got, want, bound):
         assert ((a.double() - b).abs() <= most).all()
+
+
+@pytest.mark.parametrize("kind", list(TYPES))
+@pytest.mark.parametrize("spoilt", [1e30, 3e38, math.inf, math.nan])
+def test_weights_of_rows_without_a_target(kind, spoilt):
+    """Whatever weight a row of padding has, the other rows' gradients are the same to the last bit."""
+    for n, v, d in ((90, 200, 48), (700, 1300, 72)):
+        x, t, ids, out, w = _inputs(n, v, d, kind)
+        ids[3], ids[20], ids[40] = -1, v, -2 ** 31
+        out[7] = ids[7]
+        gone = torch.tensor([3, 7, 20, 40], device="cuda")
+        w[gone] = 0.0
+        want = _check(x, t, ids, out, w, 0.5, kind)
+        w[gone] = spoilt
+        got = _run(x, t, ids, out, w, 0.5)
+        assert all(torch.equal(a, b) for a, b in zip(got, want)) and want[3].any()
