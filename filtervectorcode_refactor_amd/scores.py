@@ -350,6 +350,10 @@ def matmul_int8(a, a_scale, b, b_scale, dtype=torch.bfloat16):
 FEW_ROWS, FEW_LONG, FEW_TABLE = 4, 512, 200_000  # what linear_int8 takes in one launch, without a workspace
 
 
+def _in_one_launch(m, d, n):
+    return m <= FEW_ROWS and 0 < d <= FEW_LONG and n <= FEW_TABLE
+
+
 def linear_int8(x, q, scale, dtype=torch.bfloat16):
     """x w^T with x brought to 8-bit whole numbers on the way and w kept in them (q, scale =
     quantize_int8(w), made once).  For answering: it has no gradient, and of an x that requires
@@ -364,7 +368,7 @@ def linear_int8(x, q, scale, dtype=torch.bfloat16):
     lib = _library()
     c = torch.empty(m, n, dtype=dtype, device=x.device)
     with _On(x) as stream:
-        keep, at, size = (None, None, 0) if m <= FEW_ROWS and d <= FEW_LONG and n <= FEW_TABLE else \
+        keep, at, size = (None, None, 0) if _in_one_launch(m, d, n) else \
             _workspace(lib.ung_hip_int8_linear_workspace, m, d, n, _TYPES[dtype], device=x.device)
         check(lib.ung_hip_int8_linear(x.data_ptr(), kind, m, d, stride, q.data_ptr(), scale.data_ptr(), n, c.data_ptr(),
                                       _TYPES[dtype], n, at, size, stream))

@@ -274,3 +274,13 @@ def test_few_rows_in_one_launch(kind):
             assert torch.equal(got.isnan(), want.isnan()) and torch.equal(got.nan_to_num(), want.nan_to_num()), (m, n, d)
             if m > 2:
                 assert got[1].isnan().all() and not got[0].isnan().any()
+
+
+def test_rows_without_columns():
+    """Sums over nothing are 0, for few rows as for many, as matmul_int8 has them."""
+    for kind in TYPES.values():
+        q, scale = S.quantize_int8(torch.empty(6, 0, device="cuda"))
+        for m in (1, 3, 4, 5, 40):
+            for dtype in TYPES.values():
+                y = S.linear_int8(torch.empty(m, 0, dtype=kind, device="cuda"), q, scale, dtype=dtype)
+                assert y.shape == (m, 6) and y.dtype == dtype and not y.any()

@@ -206,3 +206,15 @@ def test_table_loss_in_autograd(monkeypatch):
     (dx,) = torch.autograd.grad(S.table_loss(x, t, ids).sum(), x, create_graph=True)
     with pytest.raises(RuntimeError, match="no second derivative"):
         dx.square().sum().backward()
+
+
+def test_the_rule_for_one_launch_is_the_librarys():
+    """Where scores.linear_int8 brings no workspace the library needs none, from no columns on."""
+    need = C.c_uint64()
+    for rows in (0, 1, S.FEW_ROWS, S.FEW_ROWS + 1):
+        for cols in (0, 1, 128, S.FEW_LONG, S.FEW_LONG + 1):
+            for n in (0, 1, S.FEW_TABLE, S.FEW_TABLE + 1):
+                assert F.load().ung_hip_int8_linear_workspace(rows, cols, n, 0, C.byref(need)) == 0
+                assert not S._in_one_launch(rows, cols, n) or need.value == 0, (rows, cols, n)
+                if rows and n:
+                    assert S._in_one_launch(rows, cols, n) == (need.value == 0), (rows, cols, n)
