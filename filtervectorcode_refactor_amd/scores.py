@@ -690,7 +690,8 @@ def clip_gradients(grads, max_norm, out=None):
     """Scales the gradients by min(1, max_norm / norm) of their norm together, which it returns
     (gradient_norm).  In place, or to ``out``: as many tensors of the same types and shapes, laid out
     the same way.  Nothing waits for the norm.  Where it is infinite or NaN the gradients stay as
-    they are, so that a program that asks later can leave the step out."""
+    they are, so that a program that asks later can leave the step out.  Tensors that require a gradient
+    (parameters instead of their gradients) are refused but under torch.no_grad()."""
     given = list(grads)
     grads, kinds, at, types, sizes = _gradient_list(given)
     written, to, to_at = grads, None, None
@@ -707,8 +708,9 @@ def clip_gradients(grads, max_norm, out=None):
             raise ValueError("out: the gradients' shapes, types and strides are needed")
     if torch.is_grad_enabled():
         for t in (*grads, *written):
-            if t.requires_grad and not t.is_leaf:
-                raise ValueError("grads: gradients that require a gradient themselves are clipped under torch.no_grad()")
+            if t.requires_grad:  # (parameters in their gradients' place among them)
+                raise ValueError("grads: tensors that require a gradient themselves are clipped under torch.no_grad(); "
+                                 "a parameter's gradient is its .grad")
     norm, count, sizes_at = torch.empty((), device=grads[0].device), len(grads), _address_of(sizes)
     lib = _library()
     with _On(grads[0]) as stream:

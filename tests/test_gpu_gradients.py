@@ -231,3 +231,22 @@ def test_more_partial_sums_than_a_block_adds_up():
     out = [torch.empty_like(g) for g in grads]
     assert torch.equal(S.clip_gradients(grads, 10.0, out=out), norm)
     _check(out, grads, _norm(grads), 10.0)
+
+
+def test_parameters_in_their_gradients_place_are_refused():
+    """An in-place operation on a leaf that requires a gradient is an error, and changes nothing."""
+    layer = torch.nn.Linear(30, 20).cuda()
+    layer(torch.randn(5, 30, device="cuda")).square().sum().backward()
+    before = [p.detach().clone() for p in layer.parameters()]
+    grads = [p.grad for p in layer.parameters()]
+    mine = [torch.empty_like(g) for g in grads]
+    for call in (lambda: S.clip_gradients(layer.parameters(), 1e-3), lambda: S.clip_gradients(list(layer.parameters()), 1e-3),
+                 lambda: S.clip_gradients(layer.parameters(), 1e-3, out=mine),
+                 lambda: S.clip_gradients(grads, 1e-3, out=layer.parameters())):
+        with pytest.raises(ValueError, match="no_grad"):
+            call()
+    assert all(torch.equal(p, b) for p, b in zip(layer.parameters(), before))
+    S.clip_gradients(grads, 1e-3)
+    with torch.no_grad():  # where torch's own in-place operations work too
+        S.clip_gradients(layer.parameters(), 1e-3)
+    _check([p.detach() for p in layer.parameters()], before, _norm(before), torch.tensor(1e-3).item())
