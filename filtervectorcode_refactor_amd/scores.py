@@ -18,8 +18,9 @@ scores queries against its table.  Thin calls of the C ABI's score operators
   gradient_norm, clip_gradients
                      the norm of many gradients together; the gradients scaled to a largest norm
 
-linear_fp8, distill_loss and table_loss are differentiable, once; the passes and products return
-results without a graph.  Scores may have any row stride; bfloat16, float16 and float32.  A wrong argument raises
+linear_fp8, distill_loss and table_loss are differentiable, once; the passes and the 8-bit floating
+products return results without a graph, and the results of top_scores, of the 8-bit whole numbers'
+calls and of gradient_norm raise when they are differentiated.  Scores may have any row stride; bfloat16, float16 and float32.  A wrong argument raises
 ``ValueError`` or ``UngHipError``; there is no CPU fallback.
 """
 from __future__ import annotations
@@ -156,6 +157,15 @@ def _once(name, *grads):
     if not torch.is_grad_enabled():
         return grads
     return _Underivable.apply(f"{name} has no second derivative", torch.zeros((), requires_grad=True), *grads)
+
+
+def _marked(name, results, *of):
+    """The results, of which none has a derivative by `of`: marked where one of those requires a gradient."""
+    if torch.is_grad_enabled():
+        for t in of:
+            if t.requires_grad:
+                return _Underivable.apply(f"{name} has no gradient: detach its result", t, *results)
+    return results
 
 
 # ---- 8-bit operands and their product -----------------------------------------------------
@@ -306,14 +316,15 @@ def quantize_int8(x):
     """Rows in 8-bit whole numbers: (q int8 [n, columns rounded up to whole chunks of 128], padded
     with zeros; scale float32 [n]).  A row's scale is its largest magnitude / 127, an element's
     number the quotient by it to the nearest, ties to even.  A row with an infinity or NaN gets
-    the scale NaN and zeros."""
+    the scale NaN and zeros.  There is no gradient: of an x that requires one, differentiating the scale
+    raises."""
     kind, stride = _matrix("x", x)
     n, d = x.shape
     q = torch.empty(n, _blocks(d) * BLOCK, dtype=torch.int8, device=x.device)
     scale = torch.empty(n, device=x.device)
     with _On(x) as stream:
         check(_library().ung_hip_int8_quantize(x.data_ptr(), kind, n, d, stride, q.data_ptr(), scale.data_ptr(), stream))
-    return q, scale
+    return (q, *_marked("quantize_int8", (scale,), x))
 
 
 def _numbers(name, q, scale, like=None):
@@ -331,7 +342,8 @@ def _numbers(name, q, scale, like=None):
 
 def matmul_int8(a, a_scale, b, b_scale, dtype=torch.bfloat16):
     """a b^T of rows in 8-bit whole numbers (quantize_int8) in ``dtype``: the sums are exact whole
-    numbers, times both rows' scales in float32, rounded once to ``dtype``."""
+    numbers, times both rows' scales in float32, rounded once to ``dtype``.  There is no gradient: of scales
+    that require one, differentiating the result raises."""
     m, kp = _numbers("a", a, a_scale)
     n, b_kp = _numbers("b", b, b_scale, a)
     if dtype not in _TYPES:
@@ -344,7 +356,7 @@ def matmul_int8(a, a_scale, b, b_scale, dtype=torch.bfloat16):
         keep, at, size = _workspace(lib.ung_hip_int8_matmul_workspace, m, n, kp, kind, device=a.device)
         check(lib.ung_hip_int8_matmul(a.data_ptr(), a_scale.data_ptr(), b.data_ptr(), b_scale.data_ptr(), m, n, kp,
                                       c.data_ptr(), kind, n, at, size, stream))
-    return c
+    return _marked("matmul_int8", (c,), a_scale, b_scale)[0]
 
 
 FEW_ROWS, FEW_LONG, FEW_TABLE = 4, 512, 200_000  # what linear_int8 takes in one launch, without a workspace
@@ -356,7 +368,7 @@ def _in_one_launch(m, d, n):
 
 def linear_int8(x, q, scale, dtype=torch.bfloat16):
     """x w^T with x brought to 8-bit whole numbers on the way and w kept in them (q, scale =
-    quantize_int8(w), made once).  For answering: it has no gradient, and of an x that requires
+    quantize_int8(w), made once).  For answering: it has no gradient, and of an x or a scale that requires
     one, differentiating the result raises."""
     kind, stride = _matrix("x", x)
     n, kp = _numbers("q", q, scale, x)
@@ -372,9 +384,7 @@ def linear_int8(x, q, scale, dtype=torch.bfloat16):
             _workspace(lib.ung_hip_int8_linear_workspace, m, d, n, _TYPES[dtype], device=x.device)
         check(lib.ung_hip_int8_linear(x.data_ptr(), kind, m, d, stride, q.data_ptr(), scale.data_ptr(), n, c.data_ptr(),
                                       _TYPES[dtype], n, at, size, stream))
-    if x.requires_grad and torch.is_grad_enabled():
-        c, = _Underivable.apply("linear_int8 has no gradient: detach its result", x, c)
-    return c
+    return _marked("linear_int8", (c,), x, scale)[0]
 
 
 # ---- the first scores of a row ------------------------------------------------------------

@@ -284,3 +284,24 @@ def test_rows_without_columns():
             for dtype in TYPES.values():
                 y = S.linear_int8(torch.empty(m, 0, dtype=kind, device="cuda"), q, scale, dtype=dtype)
                 assert y.shape == (m, 6) and y.dtype == dtype and not y.any()
+
+
+def test_no_gradient_is_lost_in_silence():
+    """Results that depend on a tensor that requires a gradient raise when they are differentiated."""
+    w = torch.randn(7, 128, device="cuda", requires_grad=True)
+    x = torch.randn(5, 128, device="cuda")
+    q, scale = S.quantize_int8(w)
+    with pytest.raises(RuntimeError, match="quantize_int8 has no gradient"):
+        scale.sum().backward()
+    xq, xs = S.quantize_int8(x)
+    assert not xs.requires_grad and not q.requires_grad
+    factor = torch.full((7,), 2.0, device="cuda", requires_grad=True)
+    by = scale.detach() * factor
+    for call, name in ((lambda: S.linear_int8(x, q, by), "linear_int8"), (lambda: S.matmul_int8(xq, xs, q, by), "matmul_int8"),
+                       (lambda: S.matmul_int8(q, by, xq, xs), "matmul_int8")):
+        with pytest.raises(RuntimeError, match=f"{name} has no gradient"):
+            call().float().sum().backward()
+    want = S.linear_int8(x, q, by.detach())
+    assert not want.requires_grad and torch.equal(S.linear_int8(x, q, by), want)
+    with torch.no_grad():
+        assert not S.quantize_int8(w)[1].requires_grad and not S.matmul_int8(xq, xs, q, by).requires_grad
