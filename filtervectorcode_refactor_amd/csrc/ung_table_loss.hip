@@ -839,20 +839,22 @@ struct Backward {
     }
 };
 
+int too_many(const char *what, const Inputs &in)
+{
+    set_error("%s: %llu rows of %llu elements against a table of %llu are too many", what, (unsigned long long)in.n,
+              (unsigned long long)in.d, (unsigned long long)in.v);
+    return UNG_HIP_EINVAL;
+}
+
 int check_inputs(const char *what, const Inputs &in)
 {
     if (!known_type(in.type)) {
         set_error("%s: unknown element type %d", what, in.type);
         return UNG_HIP_EINVAL;
     }
-    // (rows of a packed copy have to stay below 2^23 bytes, and a launch's threads below 2^32)
-    if (in.n > (1u << 27) || in.v > INT32_MAX - 256 || in.d > (1u << 20) ||
-        ceil_div(in.n, 32) * ceil_div(in.v, 128) > most_blocks(256) / 2 ||
-        (in.n > in.v ? in.n : in.v) / 32 * ceil_div(in.d, 128) > most_blocks(256) / 2) {
-        set_error("%s: %llu rows of %llu elements against a table of %llu are too many", what, (unsigned long long)in.n,
-                  (unsigned long long)in.d, (unsigned long long)in.v);
-        return UNG_HIP_EINVAL;
-    }
+    // (rows of a packed copy have to stay below 2^23 bytes)
+    if (in.n > (1u << 27) || in.v > INT32_MAX - 256 || in.d > (1u << 20))
+        return too_many(what, in);
     if ((in.n > 1 && in.x_stride < in.d) || (in.v > 1 && in.table_stride < in.d)) {
         set_error("%s: strides %llu and %llu are less than %llu columns", what, (unsigned long long)in.x_stride,
                   (unsigned long long)in.table_stride, (unsigned long long)in.d);
@@ -863,6 +865,28 @@ int check_inputs(const char *what, const Inputs &in)
         return UNG_HIP_EINVAL;
     }
     return UNG_HIP_OK;
+}
+
+// Whether the launch of a product of m x n results, and of `more` blocks beside it, has its threads counted in 32 bits.
+bool fits_a_launch(Shape s, uint64_t m, uint64_t n, uint64_t more = 0)
+{
+    if (s.high <= FEW && s.wide == 64) // few rows, their shares along another axis
+        return ceil_div(n, 64) <= most_blocks(64);
+    const uint32_t threads = s.high == BIG ? 512 : s.high == 32 ? 128 : 256;
+    return ceil_div(m, s.high) * ceil_div(n, s.wide) * s.splits + more <= most_blocks(threads);
+}
+
+// The launches of the passes: of the forward pass for both, as the backward pass needs what it makes.
+int check_launches(const char *what, const Inputs &in, const Backward *b)
+{
+    bool fits = fits_a_launch(scores_shape(in.n, in.v, in.d, in.type), in.n, in.v);
+    if (b) {
+        const uint64_t v = in.v < b->piece ? in.v : b->piece;
+        const uint64_t of_t = b->together ? ceil_div(v, b->t_shape.high) * ceil_div(in.d, b->t_shape.wide) : 0;
+        fits = fits && fits_a_launch(b->g_shape, in.n, v) && fits_a_launch(b->x_shape, in.n, in.d, of_t) &&
+               fits_a_launch(b->t_shape, v, in.d);
+    }
+    return fits ? UNG_HIP_OK : too_many(what, in);
 }
 
 int check_call(const char *what, const Inputs &in, const int32_t *ids, const int32_t *without, float temperature,
@@ -1002,8 +1026,13 @@ int ung_hip_table_loss_workspace(const void *x, uint64_t x_stride, const void *t
     const Inputs in = {x, table, x_stride, table_stride, type, rows, table_rows, cols};
     if (const int rc = check_inputs(what, in))
         return rc;
-    *bytes = backward ? Backward(in).l.bytes : Forward(in).l.bytes;
-    return UNG_HIP_OK;
+    if (!backward) {
+        *bytes = Forward(in).l.bytes;
+        return check_launches(what, in, nullptr);
+    }
+    const Backward f(in);
+    *bytes = f.l.bytes;
+    return check_launches(what, in, &f);
 }
 
 int ung_hip_table_loss_forward(const void *x, uint64_t x_stride, const void *table, uint64_t table_stride, int type,
@@ -1017,6 +1046,8 @@ int ung_hip_table_loss_forward(const void *x, uint64_t x_stride, const void *tab
     if (const int rc = check_inputs(what, in))
         return rc;
     const Forward f(in);
+    if (const int rc = check_launches(what, in, nullptr))
+        return rc;
     if (const int rc = check_call(what, in, ids, without, temperature, f.l.bytes, workspace, workspace_bytes))
         return rc;
     if (rows == 0)
@@ -1075,6 +1106,8 @@ int ung_hip_table_loss_backward(const void *x, uint64_t x_stride, const void *ta
     if (const int rc = check_inputs(what, in))
         return rc;
     const Backward f(in);
+    if (const int rc = check_launches(what, in, &f))
+        return rc;
     if (const int rc = check_call(what, in, ids, without, temperature, f.l.bytes, workspace, workspace_bytes))
         return rc;
     if ((dx && rows > 1 && dx_stride < cols) || (dtable && table_rows > 1 && dtable_stride < cols)) {

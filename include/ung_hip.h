@@ -397,7 +397,8 @@ int ung_hip_int8_linear(const void *x, int type, uint64_t rows, uint64_t cols, u
  * row left out counts in dx with the factor 0.  The temperature is as below, at
  * UNG_HIP_TOP_SCORES_MAX.  Rows at 16-byte boundaries of whole 16-byte vectors are read where they
  * lie; others are copied to the workspace first, but not by the forward pass of 32 rows or fewer.
- * Up to 2^27 rows of up to 2^20 columns.  dx or dtable may be NULL; neither may overlap an input.
+ * Up to 2^27 rows of up to 2^20 columns, and as many tiles of scores as a launch takes: rows x
+ * table_rows of about 2.7e11 in float32, 5.4e11 in 16 bits.  dx or dtable may be NULL; neither may overlap an input.
  * `backward`: which pass the workspace is for. */
 int ung_hip_table_loss_workspace(const void *x, uint64_t x_stride, const void *table, uint64_t table_stride, int type,
                                  uint64_t rows, uint64_t table_rows, uint64_t cols, int backward, uint64_t *bytes);

@@ -604,3 +604,48 @@ def test_weights_of_rows_without_a_target(kind, spoilt):
         w[gone] = spoilt
         got = _run(x, t, ids, out, w, 0.5)
         assert all(torch.equal(a, b) for a, b in zip(got, want)) and want[3].any()
+
+
+def test_a_large_batch_against_a_large_table():
+    """65536 rows against 1000000: G in hundreds of pieces.  Some rows of either gradient against 64 bits.
+
+    A row's log-sum-exp is joined of sums of 16, of 16 of those a tile and of 245 tiles a thread: under 500
+    roundings a term; a gradient's sum is rounded once or twice for 32 of its terms."""
+    n, v, d, tp = 65_536, 1_000_000, 64, 0.5
+    x, t, ids, out, w = _inputs(n, v, d, "bf16")
+    ids[5], ids[n - 3] = -1, v
+    loss, lse, dx, dt = _run(x, t, ids, out, w, tp)
+    at = torch.tensor([0, 1, 5, 255, 256, 30_000, 65_000, n - 3, n - 1], device="cuda")
+    rows, table = x[at].double(), t.double()
+    z = rows @ table.t().contiguous() / tp
+    z[torch.arange(len(at), device="cuda")[out[at] >= 0], out[at][out[at] >= 0].long()] = -math.inf
+    there = (ids >= 0) & (ids < v) & (ids != out)
+    want = torch.logsumexp(z, dim=1)
+    dz = float(2 * (d + 2) * EPS * (x.double().abs().amax(0) * t.double().abs().amax(0)).sum() / tp)
+    dlse = 2 * dz + 500 * EPS + 2.0 ** -20
+    assert ((lse[at].double() - want).abs() <= dlse).all()
+    p = (z - want[:, None]).exp() * there[at][:, None]
+    size = p.clone()
+    hit = there[at].nonzero()[:, 0]
+    size[hit, ids[at][hit].long()] += 1
+    p[hit, ids[at][hit].long()] -= 1
+    by = (w[at].double() / tp)[:, None]
+    off = dz + dlse + 2.0 ** -21 + HALF_ULP["bf16"]
+    g = (p * by) @ table
+    assert ((dx[at].double() - g).abs() <= ((size * by.abs()) @ table.abs()) * (off + v / 16 * 2 * EPS)
+            + HALF_ULP["bf16"] * 1.01 * g.abs() + 1e-30).all()
+    for first in (0, 499_900, v - 200):
+        cols = slice(first, first + 200)
+        p = (x.double() @ table[cols].t().contiguous() / tp - lse.double()[:, None]).exp() * there[:, None]
+        for of, value in ((out, 0.0), (ids, None)):
+            inside = ((of >= first) & (of < first + 200) & there).nonzero()[:, 0]
+            if value is not None:
+                p[inside, of[inside].long() - first] = value
+            else:
+                size = p.clone()
+                size[inside, of[inside].long() - first] += 1
+                p[inside, of[inside].long() - first] -= 1
+        by = (w.double() / tp)[:, None]
+        g = (p * by).t().contiguous() @ x.double()
+        most = (size * by.abs()).t().contiguous() @ x.double().abs()
+        assert ((dt[cols].double() - g).abs() <= most * (off + n / 16 * 2 * EPS) + HALF_ULP["bf16"] * 1.01 * g.abs() + 1e-30).all()

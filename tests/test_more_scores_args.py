@@ -218,3 +218,20 @@ def test_the_rule_for_one_launch_is_the_librarys():
                 assert not S._in_one_launch(rows, cols, n) or need.value == 0, (rows, cols, n)
                 if rows and n:
                     assert S._in_one_launch(rows, cols, n) == (need.value == 0), (rows, cols, n)
+
+
+@pytest.mark.parametrize("type,n,v,d,fine", [
+    (2, 65_536, 1_000_000, 64, True), (2, 400_000, 1_300_000, 64, True), (2, 1 << 20, 1 << 20, 64, False),
+    (0, 100_000, 2_000_000, 64, True), (0, 1 << 19, 1 << 20, 64, False), (1, 1 << 27, 1000, 8, True),
+    (2, 1 << 27, 1 << 20, 8, False), (2, 32, (1 << 31) - 1000, 64, True), (2, 1, (1 << 31) - 1000, 64, True), (2, 20_000_000, 100, 2048, True),
+])
+def test_table_loss_takes_what_its_launches_take(type, n, v, d, fine):
+    """Threads of a launch are counted in 32 bits: 2^23 tiles of 256 x 256 scores in 16 bits, 2^24 of 128 x 128
+    in 32; the backward pass, which is launched in pieces, refuses what the forward pass does."""
+    need = C.c_uint64()
+    for backward in (0, 1):
+        rc = F.load().ung_hip_table_loss_workspace(*_sizes(type, n, v, d, d, d), backward, C.byref(need))
+        if fine:
+            assert rc == 0 and need.value > 0, _lib.last_error()
+        else:
+            _refused(rc, "too many")
