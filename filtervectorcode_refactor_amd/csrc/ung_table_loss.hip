@@ -156,18 +156,26 @@ __global__ __launch_bounds__(256) void ung_table_join_kernel(const Part *parts, 
     const float u = __builtin_fmaf(there ? target[row] : 0.0f, c, -p.top);
     const float nll = u > -100.0f ? log2f(p.sum / __builtin_amdgcn_exp2f(u)) : log_sum - u;
     loss[row] = there ? nll * LN2 : 0.0f;
-    lse[row] = p.sum == 0.0f ? -INF : (p.top + log_sum) * LN2;
+    // in 64 bits, rounded once: half a step of 32 is 3e-5 of all the row's weights at a score of 1000
+    lse[row] = (float)((double)p.top * 0.69314718055994530942 + log((double)p.sum));
 }
 
 // ---- backward ------------------------------------------------------------------------
 
-// What the gradient needs of a row: log-sum-exp in bits, weight / T, the target and the column
-// left out.  A row without a target: weight 0, log-sum-exp +inf and zeros in the place of x, so
-// that no number of a row of padding reaches the table's gradient.
+// What the gradient needs of a row: the log-sum-exp in bits, in 32 bits and so off by some r; weight / T,
+// as weight 2^-r, and `one` = 2^r in the place of the target's 1, so that r is in no share exp2(c s - lse2)
+// weight; the target and the column left out.  A row without a target: weight 0, log-sum-exp +inf and zeros
+// in the place of x, so that no number of a row of padding reaches the table's gradient.
 struct alignas(16) Row {
-    float lse2, weight;
+    float lse2, weight, one;
     int32_t id, out;
 };
+__device__ inline Row row_of(float lse, float weight, int32_t id, int32_t out)
+{
+    const double bits = (double)lse * 1.44269504088896340736;
+    const float lse2 = (float)bits, r = fabsf(lse2) < INF ? (float)(bits - (double)lse2) : 0.0f;
+    return {lse2, weight * exp2f(-r), exp2f(r), id, out};
+}
 
 // fp16 holds no numbers below 2^-24: weights are brought to the top of its range by a power of
 // two (G is at most 2 |w| / T), which the gradients are divided by at the end.  Weights of rows without a
@@ -210,8 +218,8 @@ __global__ __launch_bounds__(256) void ung_table_rows_kernel(const E *x, uint64_
         const int32_t id = ids[row], out = without ? without[row] : -1;
         const bool there = has_target(id, without, row, v);
         if (lane == 0) {
-            rows[row] = there ? Row{lse[row] * LOG2E, (weight ? weight[row] : 1.0f) * by * (scale ? scale[0] : 1.0f), id, out}
-                              : Row{INF, 0.0f, -1, -1};
+            rows[row] = there ? row_of(lse[row], (weight ? weight[row] : 1.0f) * by * (scale ? scale[0] : 1.0f), id, out)
+                              : Row{INF, 0.0f, 1.0f, -1, -1};
             targets[row] = there ? id : -1;
         }
         for (uint64_t c = lane * Vec<E>::N; c < pitch; c += 64 * Vec<E>::N)
@@ -273,7 +281,7 @@ struct Weights : Plainly {
 #pragma unroll
                 for (int e = 0; e < 16; ++e) {
                     if (id == e) {
-                        acc[i][e / 4][e % 4] -= 1.0f;
+                        acc[i][e / 4][e % 4] -= p.one;
                         if (row < n) {
                             const float all = acc[i][e / 4][e % 4] * p.weight;
                             rest[row] = all - to_float(from_float<E>(all));
@@ -355,7 +363,7 @@ __global__ __launch_bounds__(256) void ung_table_weights_kernel(const float *par
         for (int e = 0; e < 4; ++e) {
             float y = __builtin_amdgcn_exp2f(__builtin_fmaf(s[e], f.c, -p.lse2));
             if (id == e) {
-                y -= 1.0f;
+                y -= p.one;
                 const float all = y * p.weight;
                 f.rest[row] = all - to_float(from_float<E>(all));
             }

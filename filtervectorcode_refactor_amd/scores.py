@@ -593,7 +593,8 @@ def table_loss_forward(x, table, ids, without=None, temperature=1.0):
 def table_loss_backward(weight, x, table, ids, lse, without=None, temperature=1.0, need=(True, True)):
     """Gradients of sum(weight * loss) by x and by the table, in their type; the arguments are those
     of the forward call and its log-sum-exp.  ``need``: which of the two to make (the other is
-    None).  Rows without a target are not read: padding of any value, NaN too, may stand there."""
+    None).  All weights of a row are off together by lse's one rounding: half its step, 1e-6 of
+    themselves at scores of 20, 3e-5 at 1000.  Rows without a target are not read: padding of any value, NaN too, may stand there."""
     sizes, ids, without = _against(x, table, ids, without)
     n, device = x.shape[0], x.device
     lse = _vector("lse", lse, n, x)

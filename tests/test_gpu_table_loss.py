@@ -649,3 +649,43 @@ def test_a_large_batch_against_a_large_table():
         g = (p * by).t().contiguous() @ x.double()
         most = (size * by.abs()).t().contiguous() @ x.double().abs()
         assert ((dt[cols].double() - g).abs() <= most * (off + n / 16 * 2 * EPS) + HALF_ULP["bf16"] * 1.01 * g.abs() + 1e-30).all()
+
+
+@pytest.mark.parametrize("temperature", [1.0, 0.25])
+@pytest.mark.parametrize("base", [2, 8, 30, 100])
+def test_weights_are_off_by_one_rounding_of_the_log_sum_exp(base, temperature):
+    """Scores that 32 bits hold exactly (multiples of 2^-7 below 2^16, powers of two for temperatures), near each
+    other and far from 0: log-sum-exp is the nearest 32-bit number to a sum whose own error is under 40 EPS
+    (terms of one part joined by fours, 2^x off by 2^-22) of scores times a factor c = log2(e) / T that is
+    rounded itself (EPS of log-sum-exp).  Both passes have the same c, so the weights are off by the sum's error
+    and the rounding of log-sum-exp alone: c s - lse2 is a difference of numbers near each other, rounded once."""
+    g = torch.Generator(device="cuda").manual_seed(base)
+    n, v = 64, 40
+    x = torch.zeros(n, 16, device="cuda")
+    t = torch.zeros(v, 16, device="cuda")
+    x[:, 0], t[:, 0] = base, torch.randint(base * 8, base * 8 + 2, (v,), device="cuda", generator=g).float() / 2
+    x[:, 0] += torch.arange(n, device="cuda") / 64.0  # other scores in every row
+    x[:, 1:9], t[:, 1:9] = (torch.randint(0, 3, (m, 8), device="cuda", generator=g).float() / 4 for m in (n, v))
+    ids = torch.randint(0, v, (n,), device="cuda", generator=g).int()
+    loss, lse = S.table_loss_forward(x, t, ids, temperature=temperature)
+    z = x.double() @ t.double().t().contiguous() / temperature
+    assert torch.equal(z.float().double(), z)
+    want = torch.logsumexp(z, dim=1)
+    span = (z.amax(dim=1) - z.amin(dim=1)).amax() + 8
+    near = 40 * EPS + 4 * EPS * float(span)  # of the sum, and exponents near 0 rounded twice
+    half = torch.nextafter(lse, torch.full_like(lse, math.inf)).double().sub(lse.double()) / 2
+    assert ((lse.double() - want).abs() <= half + near + EPS * want.abs()).all()
+    p = (z - want[:, None]).exp()
+    gx = p.clone()
+    gx[torch.arange(n, device="cuda"), ids.long()] -= 1
+    # the gradient by a table of unit rows is that of the scores themselves
+    eye = torch.zeros(v, 16 + v, device="cuda")
+    eye[:, :16], eye[:, 16:] = t, torch.eye(v, device="cuda")
+    wide = torch.zeros(n, 16 + v, device="cuda")
+    wide[:, :16] = x
+    loss1, lse1 = S.table_loss_forward(wide, eye, ids, temperature=temperature)
+    assert torch.equal(lse1, lse) and torch.equal(loss1, loss)
+    dx, _ = S.table_loss_backward(None, wide, eye, ids, lse, temperature=temperature)
+    off = half[:, None] + near + 2.0 ** -21
+    got = dx[:, 16:].double() * temperature
+    assert ((got - gx).abs() <= p * off * 1.01 + 2 * EPS).all(), float(((got - gx).abs() / (p * off + 2 * EPS)).max())
