@@ -192,13 +192,14 @@ struct Shares : Plainly {
 // launches 7.1; 100000 rows 10.6 and 11.9; 1000000 rows 94 and 87.  With longer rows the first step costs
 // more than the launch: 1 x 1536 against 1000 rows 14.7 and 9.8.
 constexpr uint32_t FEW = 4, FEW_LONG = 512, FEW_TABLE = 200000;
+static_assert(FEW_LONG == 4 * CHUNK, "a row is two loads of two chunks");
 
 template <class X, class T>
 __global__ __launch_bounds__(256) void ung_int8_few_rows_kernel(const X *x, uint64_t cols, uint64_t stride, uint32_t m,
                                                                 Operand b, uint32_t strips, Scaled<T> finish)
 {
     constexpr uint32_t PITCH = FEW_LONG + 16;
-    __shared__ alignas(16) uint8_t numbers[FEW * PITCH + 3 * CHUNK]; // (three chunks past the end are read)
+    __shared__ alignas(16) uint8_t numbers[FEW * PITCH];
     __shared__ alignas(16) uint8_t turned[4 * turn_bytes(sizeof(T))];
     __shared__ float scales[FEW];
     Tile at = {};
@@ -206,10 +207,9 @@ __global__ __launch_bounds__(256) void ung_int8_few_rows_kernel(const X *x, uint
     at.strips = 1;
     at.lane = threadIdx.x & 63;
     at.wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const uint32_t kp = (uint32_t)b.k, chunks = kp / CHUNK;
     uint32_t strip = blockIdx.x * 4 + at.wave;
     Stream<int8_t> right;
-    u32x4 y[2][2][2][4]; // two chunks and the two after them
+    u32x4 y[2][2][2][4]; // the first two chunks of a row and the others
     auto load = [&](int set) {
         right.load(y[set][0]);
         right.load(y[set][1]);
@@ -254,23 +254,18 @@ __global__ __launch_bounds__(256) void ung_int8_few_rows_kernel(const X *x, uint
     for (; strip < strips; strip += gridDim.x * 4) {
         i32x4 acc[1][4];
         finish.start(at, acc);
-        auto multiply = [&](int set, uint32_t kb) {
+        auto multiply = [&](int set, uint32_t first) {
 #pragma unroll
             for (int h = 0; h < 4; ++h) {
-                const u32x4 f = *reinterpret_cast<const u32x4 *>(row + kb * CHUNK + h * 64);
+                const u32x4 f = *reinterpret_cast<const u32x4 *>(row + first * CHUNK + h * 64);
 #pragma unroll
                 for (int j = 0; j < 4; ++j)
                     acc[0][j] = Matrix<int8_t>::mul(y[set][h / 2][h % 2][j], f, acc[0][j]);
             }
         };
-        // four chunks at a time, with one way out: chunks past the end are zeros of b, times whatever
-        // numbers lie after x's rows
-        for (uint32_t kb = 0; kb < chunks; kb += 4) {
-            load(1);
-            multiply(0, kb);
-            load(0);
-            multiply(1, kb + 2);
-        }
+        load(1); // chunks past the end are zeros of b, and of x's numbers
+        multiply(0, 0);
+        multiply(1, 2);
         at.n0 = (uint64_t)strip * 64;
         if (strip + gridDim.x * 4 < strips) {
             strip += gridDim.x * 4;
