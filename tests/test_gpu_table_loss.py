@@ -689,3 +689,27 @@ def test_weights_are_off_by_one_rounding_of_the_log_sum_exp(base, temperature):
     off = half[:, None] + near + 2.0 ** -21
     got = dx[:, 16:].double() * temperature
     assert ((got - gx).abs() <= p * off * 1.01 + 2 * EPS).all(), float(((got - gx).abs() / (p * off + 2 * EPS)).max())
+
+
+@pytest.mark.parametrize("n,v,d", [(1, 2000, 4096), (100, 20_000, 1100), (1500, 12_000, 768), (1500, 40_000, 300), (200, 200, 1100),
+                                   (20_000, 50, 16), (20_000, 9000, 520), (20_000, 9000, 768), (33, 40_000, 16),
+                                   (4096, 12_000, 256), (4096, 50, 2048), (800, 80_000, 16), (8192, 20_000, 1100)])
+def test_tiles_of_float32(n, v, d):
+    """The kernels of the plan that the sizes above leave out, at 256 CUs: scores by 128 x 128 tiles in shares,
+    by 128 x 64 and 32 x 128; dX and dT by 128 x 128, 128 x 64 and 64 x 128, each alone, in shares and over
+    pieces of the table; dT of one chunk; both by 32 x 128 in one launch."""
+    x, t, ids, out, w = _inputs(n, v, d, "fp32", seed=3)
+    _check(x, t, ids, out, w, 2.0, "fp32")
+
+
+@pytest.mark.parametrize("kind", ["bf16", "fp16"])
+@pytest.mark.parametrize("n,v,d", [(1, 80_000, 130), (1500, 12_000, 2048), (1500, 80_000, 16), (20_000, 50, 130), (20_000, 50, 256),
+                                   (20_000, 9000, 2048), (20_000, 9000, 256), (3000, 200, 4096), (3000, 40_000, 768),
+                                   (3000, 50, 4096), (33, 80_000, 300), (6000, 20_000, 520)])
+def test_tiles_of_16_bits(n, v, d, kind):
+    """The same for 16 bits: dX by 256 x 256 tiles alone, in shares and over pieces, by 64 x 128, 128 x 64 and
+    128 x 128; dT of one chunk, by 128 x 64 and over pieces; scores by 128 x 64, and by both in shares."""
+    x, t, ids, out, w = _inputs(n, v, d, kind, seed=3)
+    got = _run(x, t, ids, out, w, 2.0)
+    for name, a, b, most in zip(("loss", "lse", "dx", "dtable"), got, *_exact_targets(x, t, ids, out, w, 2.0, kind)):
+        assert ((a.double() - b).abs() <= most).all(), (name, float(((a.double() - b).abs() / most).max()))
