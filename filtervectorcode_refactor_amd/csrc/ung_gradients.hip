@@ -115,12 +115,13 @@ __device__ inline double squares(const List &list, uint32_t first, uint32_t by)
     return sum;
 }
 
-// What a norm and the largest one make of the gradients.
+// What a norm and the largest one make of the gradients.  A norm past 32 bits, in which the caller gets it, is
+// an infinite one.
 struct Factor {
     bool less;
     float by;
     __device__ Factor(double norm, double most)
-        : less(norm > most && norm < (double)__builtin_huge_val()), by(less ? (float)(most / norm) : 1.0f)
+        : less(norm > most && (float)norm < __builtin_huge_valf()), by(less ? (float)(most / norm) : 1.0f)
     {
     }
 };

@@ -419,8 +419,8 @@ int ung_hip_table_loss_backward(const void *x, uint64_t x_stride, const void *ta
  *   norm = sqrt(sum over all elements of g^2), squares and sums in 64 bits, in a fixed order
  *   out  = g * (norm > max_norm ? max_norm / norm : 1), rounded once to its type
  * norm (device, 32 bits) may be NULL in the second call.  out NULL, or out[i] == grads[i]: in place;
- * gradients whose norm is no larger are then not written.  Where the norm is infinite or NaN they
- * stay as they are.  Gradients and outputs that overlap in another way are refused.  max_norm >= 0, +inf
+ * gradients whose norm is no larger are then not written.  Where the norm, in 32 bits, is infinite or NaN
+ * they stay as they are.  Gradients and outputs that overlap in another way are refused.  max_norm >= 0, +inf
  * included.  The workspace is the same for both calls. */
 int ung_hip_gradient_workspace(const uint64_t *sizes, uint32_t count, uint64_t *bytes);
 int ung_hip_gradient_norm(const void *const *grads, const int *types, const uint64_t *sizes, uint32_t count,

@@ -250,3 +250,16 @@ def test_parameters_in_their_gradients_place_are_refused():
     with torch.no_grad():  # where torch's own in-place operations work too
         S.clip_gradients(layer.parameters(), 1e-3)
     _check([p.detach() for p in layer.parameters()], before, _norm(before), torch.tensor(1e-3).item())
+
+
+@pytest.mark.parametrize("lengths", [[100, 9000], [30_000, 70_000], [500_000] * 3])
+def test_a_norm_past_32_bits_leaves_the_gradients(lengths):
+    """Finite gradients whose norm no 32-bit number holds: the norm that the caller sees is infinite, and the
+    gradients stay as they are, as with any infinite norm."""
+    grads = [torch.full((n,), 3e38, device="cuda") for n in lengths]
+    before = [g.clone() for g in grads]
+    out = [torch.empty_like(g) for g in grads]
+    assert float(S.gradient_norm(grads)) == math.inf
+    assert float(S.clip_gradients(grads, 1.0, out=out)) == math.inf
+    assert float(S.clip_gradients(grads, 1.0)) == math.inf
+    assert all(torch.equal(a, b) and torch.equal(c, b) for a, b, c in zip(grads, before, out))
