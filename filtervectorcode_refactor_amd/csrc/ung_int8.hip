@@ -120,8 +120,8 @@ __device__ inline float scaled(int sum, float by)
     return y;
 }
 
-// Sums to results.  With it the product 4096 x 4096 of 4096 takes 67 us, 2050 TOPS (the library's large
-// products 2087), matrix instructions bounding it; 77 x 30001 of 768 9.7 us by 64 x 128 tiles, two a CU.
+// Sums to results.  With it the product 4096 x 4096 of 4096 takes 61 us, 2250 TOPS (the library's large
+// products 2430; in a card's first calls 67 us, and 2090); 77 x 30001 of 768 9.3 us by 64 x 128 tiles, two a CU.
 template <class T>
 struct Scaled : Plainly {
     const float *a_scale, *b_scale;
@@ -189,7 +189,7 @@ struct Shares : Plainly {
 // Up to FEW short rows x against many rows of b in whole numbers, in one launch.  The blocks stay: a wave
 // brings a row of x to whole numbers in LDS, while its first chunks of b are under way, and then
 // takes 64 rows of b at a time, past LDS and without barriers.  4 x 384 against 1000 rows 6.4 us, in two
-// launches 7.1; 100000 rows 10.6 and 11.9; 1000000 rows 94 and 87.  With longer rows the first step costs
+// launches 7.1; 100000 rows 10.5 and 11.9; 1000000 rows 94 and 87.  With longer rows the first step costs
 // more than the launch: 1 x 1536 against 1000 rows 14.7 and 9.8.
 constexpr uint32_t FEW = 4, FEW_LONG = 512, FEW_TABLE = 200000;
 static_assert(FEW_LONG == 4 * CHUNK, "a row is two loads of two chunks");

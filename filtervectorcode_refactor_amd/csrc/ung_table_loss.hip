@@ -47,10 +47,10 @@ __device__ inline Part joined(Part a, Part b)
 
 // Of a tile of scores (rows of x, columns: rows of the table): every row's part, and the
 // target's score where the tile holds it.  A lane makes a part of its 16 columns; the block joins them.
-//   Matrix instructions bound it where rows are long (2000 x 50001 of 1024 bf16 222 us a call, 920 TFLOP/s;
-// seven rounds of tiles, the last an eighth full), a tile's end beside them where they are short (4096 x
-// 100000 of 384 370 to 390 us, 800 to 850): its exponentials and the join, when no wave of the block
-// has products left.
+//   A tile's begin and end bound it, when no wave of the CU's one block has products under way: its first
+// loads, its exponentials and the join (4096 x 100000 of 384 bf16 359 us, 880 TFLOP/s, matrix instructions
+// busy in 36 % of the cycles; 2000 x 50001 of 1024 216 us, 950 and 39 %, seven rounds of tiles, the last an
+// eighth full; the library's large products 1610).
 struct LogSum : Plainly {
     const int32_t *ids, *without;
     float *target; // [n]
@@ -309,8 +309,8 @@ struct Weights : Plainly {
 // Where the rows are long and tiles of scores too few for the chip, the tiles' sums are made in shares
 // (Sums), and these kernels take LogSum's and Weights' place: a wave four columns a lane of a row's 256,
 // the shares added in order.  They cost a pass over the sums.  Both passes, us, with shares and
-// without: 613 x 3520 of 4096 float32 691 and 855, 983 x 859 298 and 439; 3 x 145 of 1984 36 and 115;
-// bf16 225 x 1269 of 4096 62 and 104, 3 x 5269 71 and 112.
+// without: 613 x 3520 of 4096 float32 679 and 851, 983 x 859 296 and 437; 3 x 145 of 1984 34 and 116;
+// bf16 225 x 1269 of 4096 61 and 103, 3 x 5269 63 and 105.
 __device__ inline f32x4 shares_sum(const float *part, uint32_t splits, uint64_t n, uint64_t stride, uint64_t row, uint64_t col)
 {
     f32x4 s = {0.0f, 0.0f, 0.0f, 0.0f};
@@ -411,8 +411,8 @@ struct Rest {
 // The same for dT = G^T X: row i of x times its rest joins row id of dT.  So G has a second part with one
 // element a row, of 16 bits too: what is left then is 2^-17 of a weight in bf16, 2^-22 in fp16.  A wave
 // looks at 64 ids a chunk, and makes fragments of the second part for the halves of groups of 16 rows that
-// hold some.  The backward pass with it and without, us: 4096 x 100000 of 384 bf16 1196 and 1181, 2000 x 2000
-// of 768 64 and 57, 8192 x 1000 of 256 61 and 55.
+// hold some.  The backward pass with it and without, us: 4096 x 100000 of 384 bf16 1187 and 1181, 2000 x 2000
+// of 768 58 and 52; where every chunk has targets, 4366 x 201 of 4096, 107 and 87.
 template <class E>
 struct Targets {
     static constexpr uint32_t MORE = 64 * 4; // of the chunk's rows: place among the wave's rows, and the rest
@@ -518,8 +518,9 @@ struct Whole : Plainly, More {
 };
 
 // Sums of a share of the inner length in 32 bits, from 0 or (ADD) from an earlier piece's: dX, whose tiles
-// are few and whose inner length is the table's.  4096 x 384 of 20224 bf16, 5 shares, 73 us (870 TFLOP/s),
-// 77 onto an earlier piece's; 2048 x 768 of 32768 fp16 112 us (920).
+// are few and whose inner length is the table's.  4096 x 384 of 20224 bf16, 5 shares, 68 us (930 TFLOP/s),
+// 72 onto an earlier piece's; 2048 x 768 of 32768 fp16 108 us (960): matrix instructions busy in 35 to 42 % of
+// the cycles, a third of the LDS cycles bank conflicts of the transposing reads.
 template <bool ADD, class More = NoTargets>
 struct Sums : More {
     float *part;
@@ -611,9 +612,8 @@ struct Weight {
     double alone, shared, ends;
 };
 // Tiles of 128 x 64 are for few columns: the backward pass of 1044 x 185304 of 64
-// float32 987 us (1300 by 128 columns), 2000 x 20000 of 64 bf16 74 (77), the
-// forward pass of 6565 x 53 of 4096 float32 92 (180); 3000 x 50000 of 192 bf16 355 by
-// three of them, 332 by two of 128 (a line of 64 elements meets the same banks twice).
+// float32 1000 us (1304 by 128 columns), 2000 x 20000 of 64 bf16 78 (82), 3000 x 50000 of 192
+// 339 (351), both passes of 6565 x 53 of 4096 float32 240 (283).
 constexpr Weight WEIGHTS_16[] = {{BIG, BIG, 1, 1.75, 1.75, 5.0}, {128, 128, 2, 0.6, 0.52, 3.5}, {64, 128, 3, 0.55, 0.33, 3.0},
                                  {32, 128, 3, 0.5, 0.25, 2.5}, {128, 64, 3, 0.6, 0.40, 3.0}};
 constexpr Weight WEIGHTS_32[] = {{128, 128, 2, 2.0, 1.95, 4.0}, {64, 128, 3, 1.1, 0.98, 3.0}, {32, 128, 3, 2.2, 0.8, 2.5},
@@ -675,9 +675,9 @@ Shape shape_of(uint64_t m, uint64_t n, uint64_t k, int type, bool shares, uint32
 
 // dT and dX in one launch: the shape of dX, of whose height dT's tiles are too; us is 0 where two launches
 // are faster.  Each alone leaves a part of the chip idle in its last or only round, and the second waits
-// for the first's last tile.  The backward pass, us, by one launch and by two: 16 x 1000 of 64 bf16 12.5
-// and 15.6, 500 x 10001 of 100 float32 62 and 74, 2000 x 2000 of 768 bf16 52 and 72, 300 x 20000 of 512 bf16
-// 53 and 62.
+// for the first's last tile.  The backward pass, us, by one launch and by two: 16 x 1000 of 64 bf16 12.7
+// and 16.1, 500 x 10001 of 100 float32 62 and 72, 2000 x 2000 of 768 bf16 58 and 75, 300 x 20000 of 512 bf16
+// 52 and 58.
 Shape together_of(uint64_t n, uint64_t v, uint64_t d, int type, double two_us)
 {
     const uint64_t cus = cu_count();

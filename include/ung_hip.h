@@ -368,7 +368,8 @@ int ung_hip_int8_quantize(const void *x, int type, uint64_t rows, uint64_t cols,
 /* c [m x n] = a b^T of such rows of length kp (a multiple of UNG_HIP_INT8_CHUNK):
  * c[i][j] = (float)(sum_k a[i][k] * b[j][k]) * (a_scale[i] * b_scale[j]), the sum a whole number in
  * 32 bits, exact for every number of 8 bits up to the largest kp; then rounded to `type`.  Rows of
- * c may have any stride and alignment; at 4-byte boundaries they are written fastest. */
+ * c may have any stride and alignment; at 4-byte boundaries they are written fastest.  m x n up to about
+ * 6.8e10 (2^24 tiles of 32 x 128). */
 #define UNG_HIP_INT8_LONGEST 130944
 int ung_hip_int8_matmul_workspace(uint64_t m, uint64_t n, uint64_t kp, int type, uint64_t *bytes);
 int ung_hip_int8_matmul(const int8_t *a, const float *a_scale, const int8_t *b, const float *b_scale, uint64_t m,
