@@ -575,7 +575,8 @@ def _against(x, table, ids, without):
 def table_loss_forward(x, table, ids, without=None, temperature=1.0):
     """(loss [n], lse [n]) float32: cross entropy of each row of ``x`` with row ``ids`` of the table
     as its target, scores being x table^T / temperature, and the log-sum-exp of all its scores,
-    which table_loss_backward needs.  A large batch's scores are never in memory.
+    which table_loss_backward needs.  A large batch's scores are never in memory.  Rows of x times rows of
+    the table may be up to about 2.7e11 in float32, 5.4e11 in 16 bits; more are refused.
 
     ``without`` names one row of the table that each row of x leaves out (its own entry; -1: none).
     A row whose id is outside the table, or the one left out, has no target: its loss is 0."""
@@ -594,7 +595,7 @@ def table_loss_backward(weight, x, table, ids, lse, without=None, temperature=1.
     """Gradients of sum(weight * loss) by x and by the table, in their type; the arguments are those
     of the forward call and its log-sum-exp.  ``need``: which of the two to make (the other is
     None).  All weights of a row are off together by lse's one rounding: half its step, 1e-6 of
-    themselves at scores of 20, 3e-5 at 1000.  Rows without a target are not read: padding of any value, NaN too, may stand there."""
+    themselves at scores of 20, 3e-5 at 1000 (and all of them past 1e7).  Rows without a target are not read: padding of any value, NaN too, may stand there."""
     sizes, ids, without = _against(x, table, ids, without)
     n, device = x.shape[0], x.device
     lse = _vector("lse", lse, n, x)

@@ -396,7 +396,8 @@ int ung_hip_int8_linear(const void *x, int type, uint64_t rows, uint64_t cols, u
  * between its two products, but for the target's weight, of which it keeps what the rounding takes.  A row whose id is outside 0..table_rows-1 or the row left out has no
  * target: its loss and gradient are 0, and its x (padding, of any value) does not reach dtable.  A
  * row left out counts in dx with the factor 0.  lse is rounded once, and all weights of a row are off
- * together by that: half a step of lse, 1e-6 of themselves at 20, 3e-5 at 1000, 0.4 % at 80000.  The temperature is as below, at
+ * together by that: half a step of lse, 1e-6 of themselves at 20, 3e-5 at 1000, 0.4 % at 80000, and all of
+ * them past 1e7, where scores are too large for gradients.  The temperature is as below, at
  * UNG_HIP_TOP_SCORES_MAX.  Rows at 16-byte boundaries of whole 16-byte vectors are read where they
  * lie; others are copied to the workspace first, but not by the forward pass of 32 rows or fewer.
  * Up to 2^27 rows of up to 2^20 columns, and as many tiles of scores as a launch takes: rows x
